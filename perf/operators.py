@@ -1,0 +1,484 @@
+"""Cases, plain forms and 64-bit values of the operators around a KV cache held in 4 bits.
+
+A serving loop keeps K and V rows in 4 bits (append), attends over them with one token, a few
+drafted tokens or a whole prompt (attention), checks drafted tokens against the model's
+probabilities (verify) and drops the rows that drew the least attention when a cache is full
+(evict). Shapes are those of the BaseLM backbone (16 query heads of 128 on 2 KV heads, 28 layers,
+a vocabulary of 73448, contexts of 64 to 4096 for 16 streams and up to 32768 for one) and of the
+one-layer model with heads of 64.
+
+The cache, per sequence and KV head, is a run of tiles of 64 rows. A tile holds, one after the
+other, the K codes (64 rows of head_dim / 2 bytes), the V codes, the K scales (64 rows of
+head_dim / 32 fp16 values) and the V scales. A code is a nibble, channel 2j in the low half of
+byte j, and stands for (nibble - 8) * scale of its block of 32 channels. A scale has 7 significant
+bits, so every value in the cache is an exact fp16 number.
+
+``state`` is int32 [sequences][4]: rows held, the next position, status bits, a counter that the
+kernels leave at 0.
+"""
+import math
+
+import torch
+
+own = False
+
+BLOCK = 32      # channels that share a scale
+TILE = 64       # rows of a tile
+LARGEST = 65024.0   # 8 * 127 * 64: the largest magnitude a code and a scale can stand for
+SMALLEST = 2.0 ** -18
+FIXED = 2.0 ** 38   # probabilities are summed as multiples of 2^-38, so no order of summation changes them
+DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+# --------------------------------------------------------------------------------------------
+# cases
+# --------------------------------------------------------------------------------------------
+def listed():
+    backbone = {"heads": 16, "kv_heads": 2, "head_dim": 128}
+    return [
+        # one new row for each of 16 streams: the store of a batched decode step (latency)
+        {"name": "append_step", "op": "append", "seqs": 16, "tokens": 1, "kv_heads": 2, "head_dim": 128, "at": 1000,
+         "dtype": "f32"},
+        # a whole session's fp16 cache (28 layers of 4096 rows) put into 4 bits and read back
+        {"name": "append_session", "op": "append", "seqs": 28, "tokens": 4096, "kv_heads": 2, "head_dim": 128, "at": 0,
+         "dtype": "f16"},
+        # the one-layer model's single token after 512 cached rows: the smallest call (latency)
+        {"name": "attend_one", "op": "attend", "seqs": 1, "tokens": 1, "heads": 16, "kv_heads": 2, "head_dim": 64,
+         "low": 513, "high": 513, "dtype": "f32", "track": False},
+        # a decode step of 16 streams at ragged contexts
+        {"name": "attend_streams", "op": "attend", "seqs": 16, "tokens": 1, **backbone, "low": 64, "high": 4096,
+         "dtype": "f32", "track": False},
+        # a decode step of 16 streams deep in long contexts, 16-bit activations
+        {"name": "attend_long", "op": "attend", "seqs": 16, "tokens": 1, **backbone, "low": 24001, "high": 32768,
+         "dtype": "bf16", "track": False},
+        # 5 drafted tokens of 16 streams in one pass, with the attention that each row draws recorded
+        {"name": "attend_draft", "op": "attend", "seqs": 16, "tokens": 5, **backbone, "low": 64, "high": 4096,
+         "dtype": "f16", "track": True},
+        # a 512-token prompt at the backbone's shape, 32-bit activations
+        {"name": "attend_prompt", "op": "attend", "seqs": 1, "tokens": 512, **backbone, "low": 512, "high": 512,
+         "dtype": "f32", "track": False},
+        # a long prompt's last 4096 tokens over a context of 32768
+        {"name": "attend_prompt_long", "op": "attend", "seqs": 1, "tokens": 4096, **backbone, "low": 32768,
+         "high": 32768, "dtype": "f16", "track": False},
+        # one row more than the budget in each of 16 streams: the eviction of a decode step
+        {"name": "evict_step", "op": "evict", "seqs": 16, "kv_heads": 2, "head_dim": 128, "rows": 2049,
+         "budget": 2048, "recent": 256, "sinks": 4},
+        # 8 sessions of 28 layers cut from 4096 to 1024 rows
+        {"name": "evict_sessions", "op": "evict", "seqs": 224, "kv_heads": 2, "head_dim": 128, "rows": 4096,
+         "budget": 1024, "recent": 256, "sinks": 4},
+        # 4 drafted tokens of one stream (latency)
+        {"name": "verify_one", "op": "verify", "seqs": 1, "tokens": 4, "vocab": 73448},
+        # 8 drafted tokens of 32 streams
+        {"name": "verify_streams", "op": "verify", "seqs": 32, "tokens": 8, "vocab": 73448},
+    ]
+
+
+def _log(rng, low, high):
+    return min(high, max(low, int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))))
+
+
+def draw(rng):
+    op = rng.choice(["append", "attend", "attend", "attend", "evict", "verify"])
+    if op == "append":
+        while True:
+            c = {"op": op, "seqs": _log(rng, 1, 32), "tokens": _log(rng, 1, 4096), "kv_heads": rng.choice([1, 2, 3, 8]),
+                 "head_dim": rng.choice([64, 128]), "at": rng.choice([0, 1, rng.randrange(2, 2000)]),
+                 "dtype": rng.choice(list(DTYPES))}
+            if c["seqs"] * c["tokens"] * c["kv_heads"] * c["head_dim"] <= 28 * 4096 * 256:
+                return c
+    if op == "attend":
+        while True:
+            heads, kv_heads = rng.choice([(16, 2), (8, 2), (2, 1), (12, 2), (8, 8), (32, 2), (6, 3)])
+            prompt = rng.random() < 0.4
+            tokens = _log(rng, 17, 4096) if prompt else rng.choice([1, 1, _log(rng, 2, 16)])
+            high = _log(rng, max(64, tokens), 32768)
+            c = {"op": op, "seqs": _log(rng, 1, 4 if prompt else 24), "tokens": tokens, "heads": heads,
+                 "kv_heads": kv_heads, "head_dim": rng.choice([64, 128, 128]),
+                 "low": rng.randrange(tokens, high + 1), "high": high, "dtype": rng.choice(list(DTYPES)),
+                 "track": rng.random() < 0.25}
+            w = work(c)
+            scores = c["seqs"] * heads * tokens * _capacity(c)
+            if w["flops"] <= 6e11 and w["bytes"] <= 1.4e8 and scores <= 1 << 31:
+                return c
+    if op == "evict":
+        while True:
+            rows = _log(rng, 65, 8192)
+            budget = rng.choice([rows - 1, rng.randrange(32, rows)])
+            recent = rng.randrange(0, max(1, budget // 2))
+            c = {"op": op, "seqs": _log(rng, 1, 224), "kv_heads": rng.choice([1, 2, 3, 8]),
+                 "head_dim": rng.choice([64, 128]), "rows": rows, "budget": budget, "recent": recent,
+                 "sinks": min(rng.randrange(0, 9), budget - recent)}
+            if c["seqs"] * c["kv_heads"] * rows * c["head_dim"] <= 224 * 2 * 4096 * 128:
+                return c
+    return {"op": op, "seqs": _log(rng, 1, 32), "tokens": rng.randrange(1, 9),
+            "vocab": rng.choice([73448 - rng.randrange(1, 256), _log(rng, 96, 73448), _log(rng, 96, 73448)])}
+
+
+def _lengths(case):
+    """Rows held by each sequence once its new tokens are in: spread over [low, high], in a mixed order."""
+    n, low, high = case["seqs"], case["low"], case["high"]
+    if n == 1:
+        return [high]
+    step = next(k for k in range(max(1, n * 5 // 8), n + 2) if math.gcd(k, n) == 1)
+    return [low + (high - low) * (i * step % n) // (n - 1) for i in range(n)]
+
+
+def _capacity(case):
+    """Rows that a sequence of the case has room for."""
+    if case["op"] == "append":
+        return case["at"] + case["tokens"] + 64
+    return case["rows"] if case["op"] == "evict" else case["high"]
+
+
+def _row_bytes(head_dim):
+    return head_dim // 2 + head_dim // BLOCK * 2
+
+
+def work(case):
+    if case["op"] == "append":
+        values = 2 * case["seqs"] * case["tokens"] * case["kv_heads"] * case["head_dim"]
+        size = torch.empty(0, dtype=DTYPES[case["dtype"]]).element_size()
+        held = values // case["head_dim"] * _row_bytes(case["head_dim"])
+        # the rows in, the codes out; the codes back in, the fp16 values out
+        return {"bytes": values * size + 2 * held + 2 * values, "flops": 4 * values}
+    if case["op"] == "attend":
+        n, t = _lengths(case), case["tokens"]
+        rows = sum(n)
+        pairs = sum(t * (m - t) + t * (t + 1) // 2 for m in n) * case["heads"]
+        size = torch.empty(0, dtype=DTYPES[case["dtype"]]).element_size()
+        read = rows * case["kv_heads"] * 2 * _row_bytes(case["head_dim"])
+        q = case["seqs"] * t * case["heads"] * case["head_dim"] * size
+        drawn = rows * case["kv_heads"] * 8 if case["track"] else 0
+        return {"bytes": read + 2 * q + drawn, "flops": 4 * pairs * case["head_dim"]}
+    if case["op"] == "evict":
+        lanes = case["seqs"] * case["kv_heads"]
+        # weights and positions read and the kept ones written; about the share of kept rows that lie past
+        # the budget is read and written once
+        moved = case["budget"] * (case["rows"] - case["budget"]) / case["rows"]
+        return {"bytes": lanes * (8 * case["rows"] + 8 * case["budget"] + 4 * moved * _row_bytes(case["head_dim"])),
+                "flops": lanes * case["rows"]}
+    # the drafted tokens' two probabilities, then one row of each distribution
+    n, t, v = case["seqs"], case["tokens"], case["vocab"]
+    return {"bytes": n * (t * 16 + 8 * v), "flops": 3 * n * v}
+
+
+# --------------------------------------------------------------------------------------------
+# inputs
+# --------------------------------------------------------------------------------------------
+def _generator(seed):
+    return torch.Generator(device="cuda").manual_seed(seed & 0x7FFFFFFF)
+
+
+def _normal(g, *shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=g, device="cuda").to(dtype)
+
+
+def _tiles(capacity):
+    return -(-capacity // TILE)
+
+
+def _parts(data, head_dim):
+    """K codes, V codes, K scales and V scales as views of the cache, each [seqs, kv_heads, tiles, TILE, ...]."""
+    s, h, t, _ = data.shape
+    c, e = TILE * head_dim // 2, TILE * head_dim // BLOCK * 2
+    codes = [data[..., i * c:(i + 1) * c].unflatten(-1, (TILE, head_dim // 2)) for i in (0, 1)]
+    scales = [data[..., 2 * c + i * e:2 * c + (i + 1) * e].unflatten(-1, (TILE, head_dim // BLOCK * 2)) for i in (0, 1)]
+    return codes + scales
+
+
+def _codes(x):
+    """Nibbles (0 to 15) and fp32 scales of rows [..., head_dim], quantised in 32 bits."""
+    x = torch.nan_to_num(x.float(), nan=0.0, posinf=LARGEST, neginf=-LARGEST).clamp(-LARGEST, LARGEST)
+    b = x.unflatten(-1, (-1, BLOCK))
+    high, low = b.amax(-1), b.amin(-1)
+    d = torch.where(high >= -low, high, low) * -0.125
+    bits = d.view(torch.int32)
+    d = ((bits + 0xFFFF + ((bits >> 17) & 1)) & ~0x1FFFF).view(torch.float32)   # 7 significant bits, ties to even
+    d = torch.where(d.abs() < SMALLEST, 0.0, d)
+    inverse = torch.where(d == 0, 0.0, 1.0 / d)
+    n = (b * inverse.unsqueeze(-1)).round().clamp(-8, 7) + 8
+    return n.flatten(-2), d
+
+
+def _pack(n):
+    """Two nibbles a byte, the even channel in the low half."""
+    n = n.to(torch.uint8).unflatten(-1, (-1, 2))
+    return n[..., 0] | n[..., 1] << 4
+
+
+def _fill(g, codes, scales, head_dim):
+    n, d = _codes(torch.randn(*codes.shape[:-1], head_dim, generator=g, device="cuda"))
+    codes.copy_(_pack(n))
+    scales.copy_(d.half().view(torch.uint8))
+
+
+def _filled(g, seqs, kv_heads, head_dim, capacity):
+    """A cache whose rows hold quantised normal values."""
+    data = torch.empty(seqs, kv_heads, _tiles(capacity), TILE * 2 * _row_bytes(head_dim), dtype=torch.uint8, device="cuda")
+    kc, vc, ks, vs = _parts(data, head_dim)
+    _fill(g, kc, ks, head_dim)
+    _fill(g, vc, vs, head_dim)
+    return data
+
+
+def _state(lengths):
+    state = torch.zeros(len(lengths), 4, dtype=torch.int32)
+    state[:, 0] = torch.tensor(lengths, dtype=torch.int32)
+    state[:, 1] = state[:, 0]
+    return state.cuda()
+
+
+def prepare(case, seed):
+    g = _generator(seed)
+    s = dict(case)
+    if case["op"] == "append":
+        shape = case["seqs"], case["tokens"], case["kv_heads"], case["head_dim"]
+        s["k"], s["v"] = (_normal(g, *shape, dtype=DTYPES[case["dtype"]]) for _ in "kv")
+        cap = s["capacity"] = _capacity(case)
+        s["data"] = torch.zeros(case["seqs"], case["kv_heads"], _tiles(cap), TILE * 2 * _row_bytes(case["head_dim"]),
+                                dtype=torch.uint8, device="cuda")
+        s["state"] = _state([case["at"]] * case["seqs"])
+        s["at"] = torch.full((case["seqs"],), case["at"], dtype=torch.int32, device="cuda")
+    elif case["op"] == "attend":
+        cap = s["capacity"] = _capacity(case)
+        s["data"] = _filled(g, case["seqs"], case["kv_heads"], case["head_dim"], cap)
+        s["state"] = _state(_lengths(case))
+        s["q"] = _normal(g, case["seqs"], case["tokens"], case["heads"], case["head_dim"]).mul(1.5).to(DTYPES[case["dtype"]])
+        s["weights"] = s["positions"] = None
+        if case["track"]:
+            shape = case["seqs"], case["kv_heads"], cap
+            s["weights"] = torch.rand(*shape, generator=g, device="cuda")
+            s["positions"] = torch.arange(cap, dtype=torch.int32, device="cuda").expand(shape).contiguous()
+    elif case["op"] == "evict":
+        n = s["capacity"] = case["rows"]
+        shape = case["seqs"], case["kv_heads"], n
+        # any bytes will do: rows are moved, not computed with
+        s["data"] = torch.randint(0, 256, (*shape[:2], _tiles(n), TILE * 2 * _row_bytes(case["head_dim"])), generator=g,
+                                  dtype=torch.uint8, device="cuda")
+        s["state"] = _state([n] * case["seqs"])
+        s["state"][:, 1] = 2 * n
+        # attention is heavy-tailed; one row in ten drew the same little, so that there are ties
+        w = torch.randn(*shape, generator=g, device="cuda").mul(2).exp()
+        s["weights"] = torch.where(torch.rand(*shape, generator=g, device="cuda") < 0.1, 0.125, w)
+        # rows have been moved before: any n of the 2n positions seen, in any order
+        s["positions"] = torch.rand(*shape[:2], 2 * n, generator=g, device="cuda").argsort(-1)[..., :n].int().contiguous()
+        s["after"] = [torch.full_like(s[k], -1) for k in ("state", "weights", "positions")]
+    else:
+        n, t, v = case["seqs"], case["tokens"], case["vocab"]
+        logits = _normal(g, n, t + 1, v).mul_(2.5)
+        s["target"] = logits.softmax(-1)
+        near = logits[:, :t].add_(_normal(g, n, t, v).mul_(0.7))
+        s["draft"] = near.softmax(-1)
+        gumbel = -(torch.rand(n, t, v, generator=g, device="cuda").clamp_min_(1e-20).log_().neg_().log_())
+        s["tokens_in"] = near.add_(gumbel).argmax(-1).int()
+        s["u_accept"] = torch.rand(n, t, generator=g, device="cuda")
+        s["u_sample"] = torch.rand(n, generator=g, device="cuda")
+    return s
+
+
+# --------------------------------------------------------------------------------------------
+# the framework's operators
+# --------------------------------------------------------------------------------------------
+def _cache(s):
+    """The session's cache object over the buffers in hand, kept as a program keeps it."""
+    if "cache" not in s:
+        from voxgen_b200.kv4 import Kv4Cache
+        s["cache"] = Kv4Cache(s["seqs"], s["kv_heads"], s["head_dim"], s["capacity"], data=s["data"], state=s["state"],
+                              weights=s.get("weights"), positions=s.get("positions"))
+        if s["op"] == "evict":
+            s["into"] = Kv4Cache(s["seqs"], s["kv_heads"], s["head_dim"], s["capacity"], data=s["data"],
+                                 state=s["after"][0], weights=s["after"][1], positions=s["after"][2])
+    return s["cache"]
+
+
+def _run_own(s):
+    if s["op"] == "append":
+        cache = _cache(s)
+        cache.append(s["k"], s["v"], at=s["at"])
+        k, v = cache.read(s["tokens"], first=s["at"])
+        return {"k": k, "v": v, "state": s["state"]}
+    if s["op"] == "attend":
+        out = _cache(s).attention(s["q"])
+        return {"out": out, "weights": s["weights"]} if s["track"] else {"out": out}
+    if s["op"] == "evict":
+        _cache(s).evict(s["budget"], s["recent"], s["sinks"], into=s.get("into"))
+        return {"data": s["data"], "state": s["after"][0], "weights": s["after"][1], "positions": s["after"][2]}
+    from voxgen_b200 import kv4
+    accepted, token = kv4.verify_draft(s["tokens_in"], s["draft"], s["target"], s["u_accept"], s["u_sample"])
+    return {"accepted": accepted, "next": token}
+
+
+# --------------------------------------------------------------------------------------------
+# plain forms
+# --------------------------------------------------------------------------------------------
+def _values(codes, scales):
+    """fp32 values [seqs, kv_heads, rows, head_dim] that codes and scales stand for."""
+    n = torch.stack((codes & 15, codes >> 4), -1).flatten(-2)
+    d = scales.contiguous().view(torch.float16).float()
+    x = (n.float() - 8).unflatten(-1, (-1, BLOCK)) * d.unsqueeze(-1)
+    return x.flatten(-2).flatten(2, 3)
+
+
+def _store(rows, codes, scales, at):
+    """Puts rows [seqs, tokens, kv_heads, head_dim] into the cache; returns the values that it then holds."""
+    n, d = _codes(rows)
+    codes[at] = _pack(n)
+    scales[at] = d.half().view(torch.uint8)
+    held = _values(codes[at].transpose(1, 2)[:, :, None], scales[at].transpose(1, 2)[:, :, None])
+    return held.transpose(1, 2).half()
+
+
+def _append(s):
+    t = s["tokens"]
+    row = s["at"].long()[:, None] + torch.arange(t, device="cuda")
+    at = torch.arange(s["seqs"], device="cuda")[:, None], slice(None), row // TILE, row % TILE
+    kc, vc, ks, vs = _parts(s["data"], s["head_dim"])
+    k, v = _store(s["k"], kc, ks, at), _store(s["v"], vc, vs, at)
+    s["state"][:, 1] += s["at"] + t - s["state"][:, 0]
+    s["state"][:, 0] = s["at"] + t
+    return {"k": k, "v": v, "state": s["state"]}
+
+
+def _attend(s):
+    t, group, cap = s["tokens"], s["heads"] // s["kv_heads"], s["capacity"]
+    kc, vc, ks, vs = _parts(s["data"], s["head_dim"])
+    k, v = (_values(c, e)[:, :, :cap] for c, e in ((kc, ks), (vc, vs)))
+    q = s["q"].float().unflatten(2, (s["kv_heads"], group)).permute(0, 2, 1, 3, 4).flatten(2, 3)  # rows: token, then head
+    score = (q / math.sqrt(s["head_dim"])) @ k.transpose(-1, -2)
+    seen = s["state"][:, :1] - t + 1 + torch.arange(t, device="cuda")   # rows that each token sees
+    hidden = torch.arange(cap, device="cuda") >= seen[..., None]
+    score = score.unflatten(2, (t, group)).masked_fill_(hidden[:, None, :, None], -math.inf)
+    p = (score - score.amax(-1, keepdim=True)).exp_()
+    p = p / p.sum(-1, keepdim=True)
+    out = (p.flatten(2, 3) @ v).unflatten(2, (t, group)).permute(0, 2, 1, 3, 4).flatten(2, 3)
+    out = out.to(s["q"].dtype)
+    if not s["track"]:
+        return {"out": out}
+    s["weights"] += p.sum((2, 3))
+    return {"out": out, "weights": s["weights"]}
+
+
+def _move(part, source, budget):
+    """Rows [0, budget) of a part of the cache become the rows `source` names."""
+    rows = part.flatten(2, 3)
+    moved = rows.gather(2, source[..., None].expand(*source.shape, rows.shape[-1]))
+    end = -(-budget // TILE)
+    part[:, :, :end] = torch.cat((moved, rows[:, :, budget:end * TILE]), 2).unflatten(2, (-1, TILE))
+
+
+def _evict(s):
+    n, budget = s["rows"], s["budget"]
+    row = torch.arange(n, device="cuda")
+    kept_by_place = (s["positions"] >= s["state"][:, 1, None, None] - s["recent"]) | (s["positions"] < s["sinks"])
+    key = torch.where(kept_by_place, math.inf, s["weights"])
+    key = torch.where(row < s["state"][:, :1, None], key, -math.inf)
+    order = key.argsort(dim=-1, descending=True, stable=True)
+    keep = torch.zeros_like(key, dtype=torch.bool).scatter_(-1, order[..., :budget], True)
+    # kept rows past the budget fill, in order, the places of the others
+    late = torch.where(keep & (row >= budget), row, n).sort(-1).values
+    hole = ~keep[..., :budget]
+    source = torch.where(hole, late.gather(-1, (hole.cumsum(-1) - 1).clamp_min(0)), row[:budget])
+    kc, vc, ks, vs = _parts(s["data"], s["head_dim"])
+    _move(kc, source, budget)
+    _move(vc, source, budget)
+    _move(ks, source, budget)
+    _move(vs, source, budget)
+    state, weights, positions = s["after"]
+    state.copy_(s["state"])
+    state[:, 0].clamp_(max=budget)
+    weights[..., :budget] = s["weights"].gather(-1, source)
+    positions[..., :budget] = s["positions"].gather(-1, source)
+    return {"data": s["data"], "state": state, "weights": weights, "positions": positions}
+
+
+def _verify(s):
+    n, t = s["seqs"], s["tokens"]
+    token = s["tokens_in"].long()[..., None]
+    p = s["target"][:, :t].gather(-1, token)[..., 0]
+    q = s["draft"].gather(-1, token)[..., 0]
+    accepted = (s["u_accept"] * q < p).int().cumprod(-1).sum(-1)
+    at = torch.arange(n, device="cuda"), accepted
+    target = s["target"][at]
+    draft = torch.where((accepted == t)[:, None], 0.0, s["draft"][at[0], accepted.clamp_max(t - 1)])
+    rest = (target - draft).clamp(0, 1)
+    rest = torch.where((rest > 0).any(-1, keepdim=True), rest, target)
+    total = (rest * FIXED).long().cumsum(-1)
+    point = (s["u_sample"] * 2.0 ** 24).long() * total[:, -1] >> 24
+    return {"accepted": accepted.int(), "next": (total <= point[:, None]).sum(-1).int()}
+
+
+def run(state):
+    if own:
+        return _run_own(state)
+    return {"append": _append, "attend": _attend, "evict": _evict, "verify": _verify}[state["op"]](state)
+
+
+# --------------------------------------------------------------------------------------------
+# 64-bit values
+# --------------------------------------------------------------------------------------------
+def _nearest(x):
+    """What the cache stands for after rows x [rows, head_dim] of ordinary values, in 64 bits."""
+    x = x.double().clamp(-LARGEST, LARGEST).reshape(-1, BLOCK)
+    scale = torch.where(x.max(1, keepdim=True)[0] < x.neg().max(1, keepdim=True)[0], -x.min(1, keepdim=True)[0],
+                        -x.max(1, keepdim=True)[0]) / 8
+    m, e = torch.frexp(scale)
+    scale = torch.ldexp((m * 128).round() / 128, e)
+    scale[scale.abs() < SMALLEST] = 0
+    n = torch.where(scale == 0, 0, x / scale).round().clamp(-8, 7)
+    return n * scale
+
+
+def _unpacked(tile, head_dim):
+    """K and V in 64 bits of one sequence's and head's tiles, [rows, head_dim] each."""
+    size = TILE * head_dim // 2
+
+    def one(i):
+        b = tile[:, i * size:(i + 1) * size].reshape(-1, head_dim // 2).to(torch.int64)
+        n = torch.empty(b.shape[0], head_dim, dtype=torch.float64, device="cuda")
+        n[:, 0::2], n[:, 1::2] = b % 16 - 8, b // 16 - 8
+        e = tile[:, 2 * size + i * size // 8:2 * size + (i + 1) * size // 8].contiguous().view(torch.float16)
+        return n * e.reshape(-1, head_dim // BLOCK).double().repeat_interleave(BLOCK, 1)
+
+    return one(0), one(1)
+
+
+def exact(case, seed):
+    if case["op"] == "verify":
+        return None
+    s = prepare(case, seed)
+    if case["op"] == "append":
+        rows = {c: torch.empty(s[c].shape, dtype=torch.float64, device="cuda") for c in "kv"}
+        for c in "kv":
+            for i in range(case["seqs"]):
+                rows[c][i] = _nearest(s[c][i]).view_as(rows[c][i])
+        return {**rows, "state": None}
+    if case["op"] == "evict":
+        w = s["weights"].double().cpu().numpy()
+        pos = s["positions"].cpu().numpy()
+        after = s["after"][1].double().cpu().numpy()
+        n, b = case["rows"], case["budget"]
+        for i in range(case["seqs"]):
+            for h in range(case["kv_heads"]):
+                place = [-1.0 if p < case["sinks"] or p >= 2 * n - case["recent"] else 0.0 for p in pos[i, h].tolist()]
+                rank = sorted(range(n), key=lambda r: (place[r], 0.0 if place[r] else -w[i, h, r], r))[:b]
+                kept, late = set(rank), iter(sorted(r for r in rank if r >= b))
+                after[i, h, :b] = [w[i, h, r if r in kept else next(late)] for r in range(b)]
+        return {"data": None, "state": None, "weights": torch.from_numpy(after), "positions": None}
+    t, group, d = case["tokens"], case["heads"] // case["kv_heads"], case["head_dim"]
+    if 2 * work(case)["flops"] > 6e12:
+        return None
+    out = torch.empty(s["q"].shape, dtype=torch.float64, device="cuda")
+    drawn = s["weights"].double() if case["track"] else None
+    for i, n in enumerate(_lengths(case)):
+        for h in range(case["kv_heads"]):
+            k, v = (x[:n] for x in _unpacked(s["data"][i, h], d))
+            for a in range(0, t, 512):
+                b = min(t, a + 512)
+                late = torch.arange(n, device="cuda")[None] > torch.arange(n - t + a, n - t + b, device="cuda")[:, None]
+                for j in range(h * group, (h + 1) * group):
+                    e = s["q"][i, a:b, j].double() @ k.T * d ** -0.5
+                    p = e.masked_fill_(late, -math.inf).softmax(-1)
+                    out[i, a:b, j] = p @ v
+                    if drawn is not None:
+                        drawn[i, h, :n] += p.sum(0)
+    return {"out": out, "weights": drawn} if case["track"] else {"out": out}
