@@ -24,7 +24,7 @@ own = False
 
 BLOCK = 32      # channels that share a scale
 TILE = 64       # rows of a tile
-LARGEST = 65024.0   # 8 * 127 * 64: the largest magnitude a code and a scale can stand for
+LARGEST = 7168.0    # 8 * 896: the largest magnitude a code and a scale stand for
 SMALLEST = 2.0 ** -18
 FIXED = 2.0 ** 38   # probabilities are summed as multiples of 2^-38, so no order of summation changes them
 DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
