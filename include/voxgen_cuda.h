@@ -374,6 +374,111 @@ int vg_k_attention_noalloc(const float *q, const uint16_t *k_cache,
                            uint32_t kv_heads, uint32_t head_dim, uint32_t ctx,
                            uint32_t position, float *out, void *cuda_stream);
 
+/* ---- a KV cache held in 4 bits ---------------------------------------------
+ * No reference counterpart: the reference keeps K and V in fp16
+ * (store_kv.comp:21). Entry points on the caller's device buffers and stream,
+ * like the kernel-level ones above. A caller keeps many sessions (or the layers
+ * of one) as the sequences of a cache, and runs
+ *   append -> attention -> verify_draft -> append at the accepted row -> evict.
+ *
+ * Values. A block is 32 consecutive channels of a row: 32 codes in [-8, 7] and
+ * one scale of 7 significant bits, 4.5 bits a value. The scale is -b/8, b being
+ * the block's value of largest magnitude (the positive one where two tie); a
+ * code is rint(x * (1/scale)), clamped. Values are clamped to +-7168 and a NaN
+ * is held as 0 (VG_KV4_NONFINITE reports both), so a cache is always finite;
+ * blocks whose largest magnitude is below 2^-15 are held as zeros. Every value
+ * that the cache stands for is an exact fp16 number.
+ *
+ * data: vg_k_kv4_bytes() bytes, 16-byte aligned: per (sequence, KV head) tiles
+ * of 64 rows, each K codes [64][head_dim/2], V codes, K scales fp16
+ * [64][head_dim/32], V scales; channel 2j is the low nibble of byte j and a
+ * nibble is the code plus 8. head_dim is 64 or 128.
+ * state: per sequence {rows held, next position, VG_KV4_* status bits, 0}, 16-byte
+ * aligned, zeros for an empty cache. It lives on the device and only the calls
+ * below advance it, so no call waits for the host.
+ * weights, positions: [seqs][kv_heads][capacity], the attention that each row
+ * has drawn and the position it holds; NULL unless rows are to be evicted.
+ *
+ * A cache is used by one stream at a time. */
+#define VG_DTYPE_F32 0
+#define VG_DTYPE_F16 1
+#define VG_DTYPE_BF16 30
+#define VG_KV4_FULL 1       /* an append would have passed the capacity            */
+#define VG_KV4_BAD_ROW 2    /* an append's first row or count was out of range     */
+#define VG_KV4_NONFINITE 4  /* an append met a NaN or an infinity                  */
+typedef struct vg_kv4_cache {
+  void *data;
+  int32_t *state;
+  float *weights;
+  int32_t *positions;
+  uint32_t seqs;
+  uint32_t kv_heads;
+  uint32_t head_dim;
+  uint32_t capacity;
+} vg_kv4_cache;
+
+/* Bytes of vg_kv4_cache.data. Host only. */
+int vg_k_kv4_bytes(uint32_t seqs, uint32_t kv_heads, uint32_t head_dim,
+                   uint32_t capacity, uint64_t *bytes);
+/* Stores `tokens` new K and V rows of every sequence from row at[s] on (NULL:
+ * after the rows held) and sets the rows held to at[s] + tokens; at[s] below
+ * the rows held drops what was appended since, such as rejected draft tokens.
+ * counts[s] <= tokens (NULL: tokens) is how many of them sequence s has. k and v
+ * are of type dtype with element strides {sequence, token, head} (host arrays;
+ * NULL: [seqs][tokens][kv_heads][head_dim]) and contiguous channels. New rows
+ * take the positions that follow and a weight of 0. A sequence whose append is
+ * out of range or would not fit is left as it was and says so in its status. */
+int vg_k_kv4_append(const vg_kv4_cache *cache, const void *k, const void *v, int dtype,
+                    uint32_t tokens, const int64_t *k_strides, const int64_t *v_strides,
+                    const int32_t *at, const int32_t *counts, void *cuda_stream);
+/* The values of rows first[s] .. first[s] + tokens - 1 (NULL: from row 0) as
+ * [seqs][tokens][kv_heads][head_dim] of type dtype (fp16 and fp32 are exact);
+ * rows that a sequence does not hold read as 0. */
+int vg_k_kv4_read(const vg_kv4_cache *cache, const int32_t *first, uint32_t tokens,
+                  int dtype, void *k, void *v, void *cuda_stream);
+/* Causal grouped-query attention of the last `tokens` rows of every sequence
+ * (already appended): with c = counts[s] (NULL: tokens), query token t < c of
+ * sequence s attends rows 0 .. rows - c + t, so one token attends every row.
+ * out is [seqs][tokens][heads][head_dim] of q's type; a query that sees no row, and
+ * tokens past the count, give zeros. scale multiplies the scores (usually
+ * 1/sqrt(head_dim)). With track, the attention that each row draws, summed over
+ * the call's tokens and the heads that share the row, is added to the cache's
+ * weights. Results do not depend on timing: every sum has a fixed order.
+ *
+ * workspace: vg_k_kv4_attention_bytes() bytes, 16-byte aligned, zero-filled
+ * once before its first use; calls leave it ready for the next call of any
+ * shape it is large enough for. */
+int vg_k_kv4_attention_bytes(const vg_kv4_cache *cache, uint32_t heads, uint32_t tokens,
+                             uint64_t *bytes);
+int vg_k_kv4_attention(const vg_kv4_cache *cache, const void *q, int dtype, uint32_t heads,
+                       uint32_t tokens, const int64_t *q_strides, const int32_t *counts,
+                       float scale, int track, void *out, void *workspace,
+                       uint64_t workspace_bytes, void *cuda_stream);
+/* Cuts every sequence that holds more than `budget` rows to `budget`, head by
+ * head: rows of the last `recent` positions and of the first `sinks` positions
+ * stay, and of the others those with the largest weights (equal weights: the
+ * lowest row; a NaN weight goes first). Kept rows past the budget move, in order,
+ * into the places of dropped rows; all others stay where they are, and rows past
+ * the budget are not written. recent + sinks <= budget; capacity <= 65536.
+ * into, when not NULL, is a cache of the same shape and data whose state,
+ * weights and positions receive the result, and the first cache's are left. */
+int vg_k_kv4_evict(const vg_kv4_cache *cache, uint32_t budget, uint32_t recent,
+                   uint32_t sinks, const vg_kv4_cache *into, void *cuda_stream);
+
+/* Verification of drafted tokens from given random numbers in [0, 1). draft is
+ * [seqs][drafted][vocab], target [seqs][drafted + 1][vocab]: the probabilities
+ * from which the tokens were drafted and those of the model. Token t is accepted
+ * while u_accept[t] * draft(token) < target(token); next is drawn from
+ * max(target - draft, 0) at the first token that is not, or from the target after
+ * the last one, as the first id whose cumulative sum exceeds u_sample times the
+ * total. Probabilities are summed as multiples of 2^-38, so the result is exact
+ * and the same for every order of summation. counts[s] <= drafted (NULL: drafted).
+ * A token outside the vocabulary is not accepted. */
+int vg_k_verify_draft(const int32_t *tokens, const float *draft, const float *target,
+                      const float *u_accept, const float *u_sample, const int32_t *counts,
+                      uint32_t seqs, uint32_t drafted, uint32_t vocab, int32_t *accepted,
+                      int32_t *next, void *cuda_stream);
+
 /* ---- failure-detection test hooks (no reference counterpart) -------------- */
 /* One token step (like vg_decode_token without logits) in which every grid-
  * barrier target is one arrival beyond what the grid provides, so the first

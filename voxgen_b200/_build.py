@@ -15,7 +15,7 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libvoxgen_b200.so"
-SOURCES = [CSRC / "engine.cu", CSRC / "gguf_loader.cpp"]
+SOURCES = [CSRC / "engine.cu", CSRC / "kv4.cu", CSRC / "gguf_loader.cpp"]
 HEADERS = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + sorted((ROOT / "include").glob("*.h"))
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -40,6 +40,8 @@ EXPORTS = [
     "vg_residual_load_gguf", "vg_residual_step", "vg_residual_step_host", "vg_residual_state",
     "vg_residual_copy_state", "vg_stream_seek", "vg_stream_set_wait_limit", "vg_test_stalled_step",
     "vg_test_fake_event_status", "vg_model_batch_columns",
+    "vg_k_kv4_bytes", "vg_k_kv4_append", "vg_k_kv4_read", "vg_k_kv4_attention_bytes", "vg_k_kv4_attention",
+    "vg_k_kv4_evict", "vg_k_verify_draft",
 ]
 
 # which buffer vg_residual_state / vg_residual_copy_state return
@@ -75,6 +77,12 @@ class TopLogitPy:
 
 class TopLogit(C.Structure):
     _fields_ = [("token_id", C.c_uint32), ("logit", C.c_float)]
+
+
+class Kv4CacheDesc(C.Structure):
+    """vg_kv4_cache: the device buffers and the shape of a cache held in 4 bits."""
+    _fields_ = [(n, C.c_void_p) for n in ("data", "state", "weights", "positions")] + \
+        [(n, C.c_uint32) for n in ("seqs", "kv_heads", "head_dim", "capacity")]
 
 
 class KernelTime(C.Structure):
@@ -143,6 +151,13 @@ def lib() -> C.CDLL:
         "vg_test_stalled_step": ([P, U32], I),
         "vg_test_fake_event_status": ([I], I),
         "vg_model_batch_columns": ([P, C.POINTER(U32)], I),
+        "vg_k_kv4_bytes": ([U32, U32, U32, U32, C.POINTER(U64)], I),
+        "vg_k_kv4_append": ([P, P, P, I, U32, P, P, P, P, P], I),
+        "vg_k_kv4_read": ([P, P, U32, I, P, P, P], I),
+        "vg_k_kv4_attention_bytes": ([P, U32, U32, C.POINTER(U64)], I),
+        "vg_k_kv4_attention": ([P, P, I, U32, U32, P, P, F, I, P, P, U64, P], I),
+        "vg_k_kv4_evict": ([P, U32, U32, U32, P, P], I),
+        "vg_k_verify_draft": ([P, P, P, P, P, P, U32, U32, U32, P, P, P], I),
     }
     for name, (args, res) in sig.items():
         f = getattr(L, name)

@@ -1,0 +1,252 @@
+// C entry points of the 4-bit KV cache and of draft verification
+// (include/voxgen_cuda.h). They work on the caller's device buffers, enqueue on
+// the caller's stream and return after the launch; no C++ exception is thrown.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "../../include/voxgen_cuda.h"
+#include "kv4_attention.cuh"
+#include "kv4_rows.cuh"
+#include "verify_kernel.cuh"
+
+using namespace vg;
+
+namespace {
+
+constexpr uint64_t kMaxGrid = 0x7FFFFFFFu;
+
+bool aligned(const void *p, size_t a) { return (uintptr_t)p % a == 0; }
+
+int launched() {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? VG_OK : e == cudaErrorMemoryAllocation ? VG_ENOMEM : VG_ECUDA;
+}
+
+int shape_status(uint64_t seqs, uint64_t kv_heads, uint32_t head_dim, uint32_t capacity) {
+  if (!seqs || !kv_heads || !capacity) return VG_EINVAL;
+  if (head_dim != 64 && head_dim != 128) return VG_EUNSUPPORTED;
+  if (capacity > 0x40000000u || seqs * kv_heads > kMaxGrid) return VG_ERANGE;
+  return VG_OK;
+}
+
+int view_of(const vg_kv4_cache *c, Kv4View *v) {
+  if (!c || !c->data || !c->state) return VG_EINVAL;
+  if (!aligned(c->data, 16) || !aligned(c->state, 16) || !aligned(c->weights, 4) || !aligned(c->positions, 4))
+    return VG_EINVAL;
+  const int rc = shape_status(c->seqs, c->kv_heads, c->head_dim, c->capacity);
+  if (rc) return rc;
+  *v = Kv4View{(uint8_t *)c->data, (Kv4Seq *)c->state, c->weights, c->positions,
+               c->seqs,            c->kv_heads,        c->capacity, kv4_tiles(c->capacity)};
+  return VG_OK;
+}
+
+size_t type_size(int dtype) {
+  return dtype == VG_DTYPE_F32 ? 4 : dtype == VG_DTYPE_F16 || dtype == VG_DTYPE_BF16 ? 2 : 0;
+}
+
+// Strides in elements {sequence, token, head}; NULL: [seqs][tokens][heads][head_dim].
+Strides strides_of(const int64_t *s, uint32_t tokens, uint32_t heads, uint32_t head_dim) {
+  const int64_t row = (int64_t)heads * head_dim;
+  return s ? Strides{s[0], s[1], s[2]} : Strides{row * tokens, row, (int64_t)head_dim};
+}
+
+// 16-byte loads need the base and every row on a 16-byte boundary.
+bool wide(const void *p, const Strides &s, size_t size) {
+  const int64_t n = (int64_t)(16 / size);
+  return aligned(p, 16) && s.seq % n == 0 && s.token % n == 0 && s.head % n == 0;
+}
+
+template <typename F>
+int by_type(int dtype, F &&f) {
+  switch (dtype) {
+    case VG_DTYPE_F32: return f(float{});
+    case VG_DTYPE_F16: return f(__half{});
+    case VG_DTYPE_BF16: return f(__nv_bfloat16{});
+  }
+  return VG_EUNSUPPORTED;
+}
+
+template <int D>
+struct Dim {
+  static constexpr int value = D;
+};
+template <typename F>
+int by_dim(uint32_t head_dim, F &&f) {
+  return head_dim == 64 ? f(Dim<64>{}) : f(Dim<128>{});
+}
+
+int allow_smem(const void *fn, size_t bytes) {
+  if (bytes <= 48 * 1024) return VG_OK;
+  return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess ? VG_OK
+                                                                                                          : VG_ECUDA;
+}
+
+}  // namespace
+
+extern "C" {
+
+int vg_k_kv4_bytes(uint32_t seqs, uint32_t kv_heads, uint32_t head_dim, uint32_t capacity, uint64_t *bytes) {
+  if (!bytes) return VG_EINVAL;
+  const int rc = shape_status(seqs, kv_heads, head_dim, capacity);
+  if (rc) return rc;
+  const uint64_t tile = head_dim == 64 ? Kv4<64>::kTileBytes : Kv4<128>::kTileBytes;
+  *bytes = (uint64_t)seqs * kv_heads * kv4_tiles(capacity) * tile;
+  return VG_OK;
+}
+
+int vg_k_kv4_append(const vg_kv4_cache *cache, const void *k, const void *v, int dtype, uint32_t tokens,
+                    const int64_t *k_strides, const int64_t *v_strides, const int32_t *at, const int32_t *counts,
+                    void *cuda_stream) {
+  AppendParams p{};
+  const int rc = view_of(cache, &p.c);
+  if (rc) return rc;
+  const size_t size = type_size(dtype);
+  if (!size) return VG_EUNSUPPORTED;
+  if (!k || !v || !tokens || !aligned(k, size) || !aligned(v, size) || !aligned(at, 4) || !aligned(counts, 4))
+    return VG_EINVAL;
+  if (tokens > cache->capacity) return VG_EFULL;
+  p.k = k;
+  p.v = v;
+  p.ks = strides_of(k_strides, tokens, cache->kv_heads, cache->head_dim);
+  p.vs = strides_of(v_strides, tokens, cache->kv_heads, cache->head_dim);
+  p.at = at;
+  p.counts = counts;
+  p.tokens = tokens;
+  const uint64_t items = (uint64_t)tokens * cache->kv_heads;
+  const uint32_t per_block = kRowThreads / (cache->head_dim / 8);
+  const uint64_t blocks = (items + per_block - 1) / per_block;
+  if (items > 0xFFFFFFFFull || blocks * cache->seqs > kMaxGrid) return VG_ERANGE;
+  p.blocks = (uint32_t)blocks;
+  const bool vec = wide(k, p.ks, size) && wide(v, p.vs, size);
+  const dim3 grid((uint32_t)(blocks * cache->seqs));
+  const cudaStream_t st = (cudaStream_t)cuda_stream;
+  return by_dim(cache->head_dim, [&](auto d) {
+    return by_type(dtype, [&](auto t) {
+      using T = decltype(t);
+      if (vec) kv4_append_kernel<decltype(d)::value, T, true><<<grid, kRowThreads, 0, st>>>(p);
+      else kv4_append_kernel<decltype(d)::value, T, false><<<grid, kRowThreads, 0, st>>>(p);
+      return launched();
+    });
+  });
+}
+
+int vg_k_kv4_read(const vg_kv4_cache *cache, const int32_t *first, uint32_t tokens, int dtype, void *k, void *v,
+                  void *cuda_stream) {
+  ReadParams p{};
+  const int rc = view_of(cache, &p.c);
+  if (rc) return rc;
+  if (!type_size(dtype)) return VG_EUNSUPPORTED;
+  if (!k || !v || !tokens || !aligned(k, 16) || !aligned(v, 16) || !aligned(first, 4)) return VG_EINVAL;
+  p.k = k;
+  p.v = v;
+  p.first = first;
+  p.tokens = tokens;
+  const uint32_t per_block = kRowThreads / (cache->head_dim / 8);
+  const uint64_t lanes = (uint64_t)cache->seqs * cache->kv_heads;
+  if (tokens > (kMaxGrid * per_block) / lanes) return VG_ERANGE;
+  const dim3 grid((uint32_t)((lanes * tokens + per_block - 1) / per_block));
+  return by_dim(cache->head_dim, [&](auto d) {
+    return by_type(dtype, [&](auto t) {
+      kv4_read_kernel<decltype(d)::value, decltype(t)><<<grid, kRowThreads, 0, (cudaStream_t)cuda_stream>>>(p);
+      return launched();
+    });
+  });
+}
+
+int vg_k_kv4_attention_bytes(const vg_kv4_cache *cache, uint32_t heads, uint32_t tokens, uint64_t *bytes) {
+  Kv4View v;
+  const int rc = view_of(cache, &v);
+  if (rc) return rc;
+  if (!bytes || !heads || !tokens || heads % cache->kv_heads) return VG_EINVAL;
+  if ((uint64_t)heads * tokens > kMaxGrid / cache->seqs) return VG_ERANGE;
+  *bytes = (uint64_t)cache->seqs * tokens * heads * 4;
+  return VG_OK;
+}
+
+int vg_k_kv4_attention(const vg_kv4_cache *cache, const void *q, int dtype, uint32_t heads, uint32_t tokens,
+                       const int64_t *q_strides, const int32_t *counts, float scale, int track, void *out,
+                       void *workspace, uint64_t workspace_bytes, void *cuda_stream) {
+  Kv4AttnParams p{};
+  uint64_t need = 0;
+  int rc = vg_k_kv4_attention_bytes(cache, heads, tokens, &need);
+  if (rc) return rc;
+  if ((rc = view_of(cache, &p.c))) return rc;
+  const size_t size = type_size(dtype);
+  if (!size) return VG_EUNSUPPORTED;
+  if (!q || !out || !workspace || workspace_bytes < need || !aligned(q, size) || !aligned(out, 16) ||
+      !aligned(workspace, 16) || !aligned(counts, 4) || (track && !cache->weights) || !(scale > 0.f) ||
+      !(scale < __builtin_huge_valf()))
+    return VG_EINVAL;
+  p.q = q;
+  p.out = out;
+  p.lse = track ? (float *)workspace : nullptr;
+  p.qs = strides_of(q_strides, tokens, heads, cache->head_dim);
+  p.counts = counts;
+  p.tokens = tokens;
+  p.heads = heads;
+  p.group = heads / cache->kv_heads;
+  p.scale = scale * 1.44269504088896340736f;
+  const uint64_t blocks = ((uint64_t)cache->capacity + kAttnWarps - 1) / kAttnWarps * cache->seqs * cache->kv_heads;
+  if (track && blocks > kMaxGrid) return VG_ERANGE;
+  const cudaStream_t st = (cudaStream_t)cuda_stream;
+  return by_dim(cache->head_dim, [&](auto d) {
+    return by_type(dtype, [&](auto t) {
+      using T = decltype(t);
+      kv4_attention_kernel<decltype(d)::value, T><<<cache->seqs * tokens * heads, kAttnWarps * 32, 0, st>>>(p);
+      if (track) kv4_weights_kernel<decltype(d)::value, T><<<(uint32_t)blocks, kAttnWarps * 32, 0, st>>>(p);
+      return launched();
+    });
+  });
+}
+
+int vg_k_kv4_evict(const vg_kv4_cache *cache, uint32_t budget, uint32_t recent, uint32_t sinks,
+                   const vg_kv4_cache *into, void *cuda_stream) {
+  EvictParams p{};
+  int rc = view_of(cache, &p.c);
+  if (rc) return rc;
+  if (!cache->weights || !cache->positions || !budget) return VG_EINVAL;
+  if (budget > cache->capacity || (uint64_t)recent + sinks > budget) return VG_ERANGE;
+  if (cache->capacity > 65536) return VG_ERANGE;
+  if (into) {
+    Kv4View o;
+    if ((rc = view_of(into, &o))) return rc;
+    if (!into->weights || !into->positions || into->data != cache->data || into->seqs != cache->seqs ||
+        into->kv_heads != cache->kv_heads || into->head_dim != cache->head_dim || into->capacity != cache->capacity)
+      return VG_EINVAL;
+    const int same = (into->state == cache->state) + (into->weights == cache->weights) + (into->positions == cache->positions);
+    if (same != 0 && same != 3) return VG_EINVAL;
+  }
+  const vg_kv4_cache *o = into ? into : cache;
+  p.state_out = (Kv4Seq *)o->state;
+  p.weights_out = o->weights;
+  p.positions_out = o->positions;
+  p.budget = budget;
+  p.recent = recent;
+  p.sinks = sinks;
+  p.list = std::min(budget, cache->capacity - budget);
+  const size_t smem = (size_t)p.list * 4;
+  return by_dim(cache->head_dim, [&](auto d) {
+    const auto fn = kv4_evict_kernel<decltype(d)::value>;
+    const int e = allow_smem((const void *)fn, smem);
+    if (e) return e;
+    fn<<<cache->seqs * cache->kv_heads, kEvictThreads, smem, (cudaStream_t)cuda_stream>>>(p);
+    return launched();
+  });
+}
+
+int vg_k_verify_draft(const int32_t *tokens, const float *draft, const float *target, const float *u_accept,
+                      const float *u_sample, const int32_t *counts, uint32_t seqs, uint32_t drafted, uint32_t vocab,
+                      int32_t *accepted, int32_t *next, void *cuda_stream) {
+  if (!tokens || !draft || !target || !u_accept || !u_sample || !accepted || !next || !seqs || !drafted || !vocab)
+    return VG_EINVAL;
+  for (const void *q : {(const void *)tokens, (const void *)draft, (const void *)target, (const void *)u_accept,
+                        (const void *)u_sample, (const void *)counts, (const void *)accepted, (const void *)next})
+    if (!aligned(q, 4)) return VG_EINVAL;
+  if (seqs > kMaxGrid || vocab > 0x1000000u || drafted > 0x100000u) return VG_ERANGE;
+  const VerifyParams p{tokens, draft, target, u_accept, u_sample, counts, accepted, next, drafted, vocab};
+  verify_draft_kernel<<<seqs, kVerifyThreads, 0, (cudaStream_t)cuda_stream>>>(p);
+  return launched();
+}
+
+}  // extern "C"

@@ -1,0 +1,262 @@
+"""Sessions on a KV cache held in 4 bits, over the ``vg_k_kv4_*`` entry points.
+
+:class:`Kv4Cache` holds the rows of one or many sequences (streams, or the layers of a session)
+on the device, 4.5 bits a value. The calls of a serving loop take and return torch tensors on the
+cache's device, run on the current CUDA stream (or ``stream``), and do not wait for the host:
+how many rows a sequence holds lives in ``cache.state`` on the device::
+
+    cache = Kv4Cache(seqs=16, kv_heads=2, head_dim=128, capacity=4096, track=True)
+    cache.append(k, v)                  # [16, new, 2, 128], any strides with contiguous channels
+    out = cache.attention(q)            # [16, new, 16, 128], causal within the new tokens
+    accepted, token = verify_draft(drafted, draft_probs, target_probs, u_accept, u_sample)
+    cache.append(k, v, at=rows)         # overwrites what was appended past rows[s]
+    cache.evict(budget=2048, recent=256, sinks=4)
+
+A cache is used by one stream at a time; a program that changes streams orders them itself, as for
+any tensor. Errors raise :class:`~voxgen_b200.api.VoxGenError`; what only the device can know (an
+append past the capacity, a NaN among the rows) is in ``cache.status()``.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from . import api
+from .api import VoxGenError
+
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
+STATUS_FULL, STATUS_BAD_ROW, STATUS_NONFINITE = 1, 2, 4
+
+
+def _check(rc: int, what: str) -> None:
+    if rc:
+        raise VoxGenError(rc, what)
+
+
+def _invalid(what: str) -> VoxGenError:
+    return VoxGenError(-1, what)
+
+
+def _stream(stream, device) -> int:
+    if stream is None:
+        stream = torch.cuda.current_stream(device)
+    return stream if isinstance(stream, int) else stream.cuda_stream
+
+
+def _ints(x: Optional[torch.Tensor], n: int, device, what: str) -> Optional[int]:
+    """Device address of an int32 tensor with one value per sequence."""
+    if x is None:
+        return None
+    if x.dtype != torch.int32 or x.shape != (n,) or x.device != device or not x.is_contiguous():
+        raise _invalid(f"{what} must be {n} contiguous int32 values on {device}")
+    return x.data_ptr()
+
+
+def _strides(x: torch.Tensor):
+    """Element strides of [seqs, tokens, heads, head_dim] for the C ABI; None when contiguous."""
+    if x.is_contiguous():
+        return None
+    if x.shape[3] > 1 and x.stride(3) != 1:
+        raise _invalid("channels must be contiguous")
+    return (C.c_int64 * 3)(*x.stride()[:3])
+
+
+class Kv4Cache:
+    """K and V rows of ``seqs`` sequences in 4 bits, ``capacity`` rows each.
+
+    ``track`` keeps the attention that each row draws and the position it holds, which
+    :meth:`evict` needs. ``data``, ``state``, ``weights`` and ``positions`` may be given instead
+    of allocated: uint8 of :func:`cache_bytes` bytes, int32 ``[seqs, 4]`` (rows held, next
+    position, status bits, 0), fp32 and int32 ``[seqs, kv_heads, capacity]``.
+    """
+
+    def __init__(self, seqs: int, kv_heads: int, head_dim: int, capacity: int, *, track: bool = False, device=None,
+                 data: Optional[torch.Tensor] = None, state: Optional[torch.Tensor] = None,
+                 weights: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None):
+        nbytes = cache_bytes(seqs, kv_heads, head_dim, capacity)
+        if device is None:
+            device = data.device if data is not None else torch.device("cuda", torch.cuda.current_device())
+        self.device = device = torch.device(device)
+        if device.type != "cuda":
+            raise _invalid("a 4-bit cache lives on a CUDA device")
+        if device.index is None:
+            self.device = device = torch.device("cuda", torch.cuda.current_device())
+        rows = (seqs, kv_heads, capacity)
+        if data is None:
+            data = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        if state is None:
+            state = torch.zeros(seqs, 4, dtype=torch.int32, device=device)
+        if track and weights is None:
+            weights = torch.zeros(rows, dtype=torch.float32, device=device)
+        if track and positions is None:
+            positions = torch.zeros(rows, dtype=torch.int32, device=device)
+        for x, dtype, shape, what in ((data, torch.uint8, None, "data"), (state, torch.int32, (seqs, 4), "state"),
+                                      (weights, torch.float32, rows, "weights"),
+                                      (positions, torch.int32, rows, "positions")):
+            if x is None:
+                continue
+            if x.dtype != dtype or x.device != device or not x.is_contiguous() or (shape and tuple(x.shape) != shape) \
+                    or (shape is None and x.numel() < nbytes):
+                raise _invalid(f"{what}: expected contiguous {dtype} of {shape or nbytes} on {device}")
+        self.seqs, self.kv_heads, self.head_dim, self.capacity = seqs, kv_heads, head_dim, capacity
+        self.data, self.state, self.weights, self.positions = data, state, weights, positions
+        address = [None if x is None else x.data_ptr() for x in (data, state, weights, positions)]
+        self.desc = api.Kv4CacheDesc(*address, seqs, kv_heads, head_dim, capacity)
+        self._ref = C.byref(self.desc)
+        self._need = {}
+        self._workspace = None
+        self._lib = api.lib()
+
+    # -- rows -------------------------------------------------------------------------------
+    def rows(self) -> torch.Tensor:
+        """Rows held by each sequence (a view of the device state)."""
+        return self.state[:, 0]
+
+    def status(self) -> list:
+        """Status bits of each sequence (STATUS_FULL, STATUS_BAD_ROW, STATUS_NONFINITE). Waits for the device."""
+        return self.state[:, 2].tolist()
+
+    def reset(self) -> None:
+        """Empties every sequence and clears its status."""
+        self.state.zero_()
+
+    def _rows_of(self, x: torch.Tensor, heads: int, what: str) -> int:
+        if x.dim() != 4 or x.shape[0] != self.seqs or x.shape[2] != heads or x.shape[3] != self.head_dim \
+                or x.device != self.device:
+            raise _invalid(f"{what}: expected [{self.seqs}, tokens, {heads}, {self.head_dim}] on {self.device}, "
+                           f"got {list(x.shape)} on {x.device}")
+        dtype = DTYPES.get(x.dtype)
+        if dtype is None:
+            raise VoxGenError(-4, f"{what}: {x.dtype} is not supported")
+        return dtype
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, *, at: Optional[torch.Tensor] = None,
+               counts: Optional[torch.Tensor] = None, stream=None) -> None:
+        """Stores new K and V rows ``[seqs, tokens, kv_heads, head_dim]`` from row ``at[s]`` on (default: after
+        the rows held); ``counts[s]`` says how many of them a sequence has (default: all)."""
+        dtype = self._rows_of(k, self.kv_heads, "k")
+        if self._rows_of(v, self.kv_heads, "v") != dtype or v.shape != k.shape:
+            raise _invalid("k and v must agree in shape and type")
+        with torch.cuda.device(self.device):
+            _check(self._lib.vg_k_kv4_append(
+                self._ref, k.data_ptr(), v.data_ptr(), dtype, k.shape[1], _strides(k), _strides(v),
+                _ints(at, self.seqs, self.device, "at"), _ints(counts, self.seqs, self.device, "counts"),
+                _stream(stream, self.device)), f"append of {k.shape[1]} rows to a cache of {self.capacity}")
+
+    def read(self, tokens: int, *, first: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.float16,
+             stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Values of rows ``first[s] .. first[s] + tokens - 1`` (default: from row 0), K and V; rows that are not
+        held read as 0."""
+        if dtype not in DTYPES:
+            raise VoxGenError(-4, f"{dtype} is not supported")
+        shape = self.seqs, tokens, self.kv_heads, self.head_dim
+        k, v = (torch.empty(shape, dtype=dtype, device=self.device) for _ in "kv")
+        with torch.cuda.device(self.device):
+            _check(self._lib.vg_k_kv4_read(self._ref, _ints(first, self.seqs, self.device, "first"), tokens,
+                                           DTYPES[dtype], k.data_ptr(), v.data_ptr(), _stream(stream, self.device)),
+                   f"read of {tokens} rows")
+        return k, v
+
+    # -- attention --------------------------------------------------------------------------
+    def _work(self, heads: int, tokens: int) -> torch.Tensor:
+        need = self._need.get((heads, tokens))
+        if need is None:
+            n = C.c_uint64()
+            _check(self._lib.vg_k_kv4_attention_bytes(self._ref, heads, tokens, C.byref(n)),
+                   f"attention of {heads} heads over {self.kv_heads} KV heads, {tokens} tokens")
+            need = self._need[heads, tokens] = n.value
+        ws = self._workspace
+        if ws is None or ws.numel() < need:
+            if ws is not None:
+                ws.record_stream(torch.cuda.current_stream(self.device))
+            ws = self._workspace = torch.zeros(need, dtype=torch.uint8, device=self.device)
+        return ws
+
+    def attention(self, q: torch.Tensor, *, counts: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                  track: Optional[bool] = None, out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+        """Attention of the last ``tokens`` rows' queries ``[seqs, tokens, heads, head_dim]``, causal within them.
+
+        Adds the attention that each row draws to ``weights`` when the cache tracks it (``track=False`` leaves
+        them). ``scale`` is 1/sqrt(head_dim) by default."""
+        if q.dim() != 4:
+            raise _invalid("q: expected [seqs, tokens, heads, head_dim]")
+        heads, tokens = q.shape[2], q.shape[1]
+        dtype = self._rows_of(q, heads, "q")
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != self.device or not out.is_contiguous():
+            raise _invalid("out must be contiguous and like q")
+        if track is None:
+            track = self.weights is not None
+        elif track and self.weights is None:
+            raise _invalid("this cache does not track attention")
+        with torch.cuda.device(self.device):
+            raw = _stream(stream, self.device)
+            if stream is not None and self._workspace is None:
+                with torch.cuda.stream(torch.cuda.ExternalStream(raw, device=self.device)):
+                    ws = self._work(heads, tokens)
+            else:
+                ws = self._work(heads, tokens)
+            _check(self._lib.vg_k_kv4_attention(
+                self._ref, q.data_ptr(), dtype, heads, tokens, _strides(q),
+                _ints(counts, self.seqs, self.device, "counts"),
+                1.0 / math.sqrt(self.head_dim) if scale is None else scale, int(track), out.data_ptr(),
+                ws.data_ptr(), ws.numel(), raw), f"attention of {tokens} tokens, {heads} heads")
+        return out
+
+    # -- eviction ---------------------------------------------------------------------------
+    def evict(self, budget: int, recent: int = 0, sinks: int = 0, *, into: Optional["Kv4Cache"] = None,
+              stream=None) -> None:
+        """Cuts sequences that hold more than ``budget`` rows to it: the last ``recent`` and first ``sinks``
+        positions stay, and the rest that drew the most attention. ``into``: a cache over the same ``data``
+        whose state, weights and positions receive the result instead."""
+        with torch.cuda.device(self.device):
+            _check(self._lib.vg_k_kv4_evict(self._ref, budget, recent, sinks, into._ref if into is not None else None,
+                                            _stream(stream, self.device)),
+                   f"eviction to {budget} rows ({recent} recent, {sinks} sinks) of a cache of {self.capacity}"
+                   + ("" if self.weights is not None else " that does not track attention"))
+
+
+def cache_bytes(seqs: int, kv_heads: int, head_dim: int, capacity: int) -> int:
+    """Device bytes of a cache's rows. Needs no GPU."""
+    n = C.c_uint64()
+    for x in (seqs, kv_heads, head_dim, capacity):
+        if not 0 <= x < 1 << 32:
+            raise _invalid(f"{x} is not a size")
+    _check(api.lib().vg_k_kv4_bytes(seqs, kv_heads, head_dim, capacity, C.byref(n)),
+           f"a 4-bit cache of {seqs} sequences, {kv_heads} KV heads of {head_dim}, {capacity} rows")
+    return n.value
+
+
+def verify_draft(tokens: torch.Tensor, draft: torch.Tensor, target: torch.Tensor, u_accept: torch.Tensor,
+                 u_sample: torch.Tensor, *, counts: Optional[torch.Tensor] = None,
+                 stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Accepts drafted tokens and draws the token after them, from given random numbers in [0, 1).
+
+    ``tokens`` int32 ``[seqs, drafted]``, ``draft`` ``[seqs, drafted, vocab]`` and ``target``
+    ``[seqs, drafted + 1, vocab]`` fp32 probabilities, ``u_accept`` ``[seqs, drafted]``, ``u_sample``
+    ``[seqs]``. Returns int32 ``accepted`` and ``next``, one of each per sequence."""
+    if tokens.dim() != 2 or draft.dim() != 3:
+        raise _invalid("verify_draft: expected tokens [seqs, drafted] and draft [seqs, drafted, vocab]")
+    seqs, drafted = tokens.shape
+    vocab = draft.shape[2]
+    device = tokens.device
+    for x, dtype, shape, what in ((tokens, torch.int32, (seqs, drafted), "tokens"),
+                                  (draft, torch.float32, (seqs, drafted, vocab), "draft"),
+                                  (target, torch.float32, (seqs, drafted + 1, vocab), "target"),
+                                  (u_accept, torch.float32, (seqs, drafted), "u_accept"),
+                                  (u_sample, torch.float32, (seqs,), "u_sample")):
+        if x.dtype != dtype or x.shape != shape or x.device != device or not x.is_contiguous():
+            raise _invalid(f"verify_draft: {what} must be contiguous {dtype} {list(shape)} on {device}")
+    if device.type != "cuda":
+        raise _invalid("verify_draft runs on a CUDA device")
+    accepted, token = torch.empty(2, seqs, dtype=torch.int32, device=device)
+    with torch.cuda.device(device):
+        _check(api.lib().vg_k_verify_draft(
+            tokens.data_ptr(), draft.data_ptr(), target.data_ptr(), u_accept.data_ptr(), u_sample.data_ptr(),
+            _ints(counts, seqs, device, "counts"), seqs, drafted, vocab, accepted.data_ptr(), token.data_ptr(),
+            _stream(stream, device)), f"verification of {drafted} tokens of a vocabulary of {vocab}")
+    return accepted, token
