@@ -406,6 +406,7 @@ int vg_k_attention_noalloc(const float *q, const uint16_t *k_cache,
 #define VG_KV4_FULL 1       /* an append would have passed the capacity            */
 #define VG_KV4_BAD_ROW 2    /* an append's first row or count was out of range     */
 #define VG_KV4_NONFINITE 4  /* an append met a NaN or an infinity                  */
+#define VG_KV4_TIMEOUT 8    /* a bounded wait of an attention ran out (sequence 0)  */
 typedef struct vg_kv4_cache {
   void *data;
   int32_t *state;

@@ -6,8 +6,9 @@
 #include <algorithm>
 
 #include "../../include/voxgen_cuda.h"
-#include "kv4_attention.cuh"
 #include "kv4_rows.cuh"
+#include "kv4_rows_attention.cuh"
+#include "kv4_weights.cuh"
 #include "verify_kernel.cuh"
 
 using namespace vg;
@@ -81,6 +82,12 @@ int allow_smem(const void *fn, size_t bytes) {
   return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess ? VG_OK
                                                                                                           : VG_ECUDA;
 }
+
+// Attention workspace: counters (zero between calls, at the same place for every
+// shape), partial results of the CTAs, then the softmax denominators.
+constexpr uint32_t kCtas = 148;   // one per SM
+constexpr uint64_t kTicketBytes = 1024;
+uint64_t part_bytes(uint32_t head_dim) { return (uint64_t)2 * kCtas * 16 * (head_dim + 2) * 4; }
 
 }  // namespace
 
@@ -160,7 +167,7 @@ int vg_k_kv4_attention_bytes(const vg_kv4_cache *cache, uint32_t heads, uint32_t
   if (rc) return rc;
   if (!bytes || !heads || !tokens || heads % cache->kv_heads) return VG_EINVAL;
   if ((uint64_t)heads * tokens > kMaxGrid / cache->seqs) return VG_ERANGE;
-  *bytes = (uint64_t)cache->seqs * tokens * heads * 4;
+  *bytes = kTicketBytes + part_bytes(cache->head_dim) + (uint64_t)cache->seqs * tokens * heads * 4;
   return VG_OK;
 }
 
@@ -178,23 +185,33 @@ int vg_k_kv4_attention(const vg_kv4_cache *cache, const void *q, int dtype, uint
       !aligned(workspace, 16) || !aligned(counts, 4) || (track && !cache->weights) || !(scale > 0.f) ||
       !(scale < __builtin_huge_valf()))
     return VG_EINVAL;
+  uint8_t *ws = (uint8_t *)workspace;
   p.q = q;
   p.out = out;
-  p.lse = track ? (float *)workspace : nullptr;
+  p.tickets = (uint32_t *)ws;
+  p.parts = (float *)(ws + kTicketBytes);
+  p.lse = track ? (float *)(ws + kTicketBytes + part_bytes(cache->head_dim)) : nullptr;
   p.qs = strides_of(q_strides, tokens, heads, cache->head_dim);
+  p.wide = wide(q, p.qs, size);
   p.counts = counts;
   p.tokens = tokens;
   p.heads = heads;
   p.group = heads / cache->kv_heads;
   p.scale = scale * 1.44269504088896340736f;
-  const uint64_t blocks = ((uint64_t)cache->capacity + kAttnWarps - 1) / kAttnWarps * cache->seqs * cache->kv_heads;
+  const uint32_t tile = size == 4 ? 8 : 16;
+  p.row_tiles = (tokens * p.group + tile - 1) / tile;
+  const uint64_t blocks = ((uint64_t)cache->capacity + kWeightWarps - 1) / kWeightWarps * cache->seqs * cache->kv_heads;
   if (track && blocks > kMaxGrid) return VG_ERANGE;
   const cudaStream_t st = (cudaStream_t)cuda_stream;
   return by_dim(cache->head_dim, [&](auto d) {
     return by_type(dtype, [&](auto t) {
       using T = decltype(t);
-      kv4_attention_kernel<decltype(d)::value, T><<<cache->seqs * tokens * heads, kAttnWarps * 32, 0, st>>>(p);
-      if (track) kv4_weights_kernel<decltype(d)::value, T><<<(uint32_t)blocks, kAttnWarps * 32, 0, st>>>(p);
+      constexpr int D = decltype(d)::value;
+      const auto fn = kv4_rows_kernel<D, T>;
+      const int e = allow_smem((const void *)fn, RowsSmem<D>::kBytes);
+      if (e) return e;
+      fn<<<kCtas, kRowsThreads, RowsSmem<D>::kBytes, st>>>(p);
+      if (track) kv4_weights_kernel<D, T><<<(uint32_t)blocks, kWeightWarps * 32, 0, st>>>(p);
       return launched();
     });
   });

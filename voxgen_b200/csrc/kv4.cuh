@@ -64,6 +64,7 @@ enum : int32_t {
   kKv4Full = 1,       // an append went past the capacity
   kKv4BadRow = 2,     // an append started past the rows held, or its count is out of range
   kKv4NonFinite = 4,  // an append met a NaN or an infinity
+  kKv4Timeout = 8,    // a bounded wait inside attention ran out (sequence 0's word)
 };
 
 // d of a block from its extremes.

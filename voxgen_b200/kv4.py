@@ -28,7 +28,7 @@ from . import api
 from .api import VoxGenError
 
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
-STATUS_FULL, STATUS_BAD_ROW, STATUS_NONFINITE = 1, 2, 4
+STATUS_FULL, STATUS_BAD_ROW, STATUS_NONFINITE, STATUS_TIMEOUT = 1, 2, 4, 8
 
 
 def _check(rc: int, what: str) -> None:
@@ -116,7 +116,8 @@ class Kv4Cache:
         return self.state[:, 0]
 
     def status(self) -> list:
-        """Status bits of each sequence (STATUS_FULL, STATUS_BAD_ROW, STATUS_NONFINITE). Waits for the device."""
+        """Status bits of each sequence (STATUS_FULL, STATUS_BAD_ROW, STATUS_NONFINITE,
+        STATUS_TIMEOUT). Waits for the device."""
         return self.state[:, 2].tolist()
 
     def reset(self) -> None:
