@@ -474,7 +474,8 @@ int vg_k_kv4_evict(const vg_kv4_cache *cache, uint32_t budget, uint32_t recent,
  * the last one, as the first id whose cumulative sum exceeds u_sample times the
  * total. Probabilities are summed as multiples of 2^-38, so the result is exact
  * and the same for every order of summation. counts[s] <= drafted (NULL: drafted).
- * A token outside the vocabulary is not accepted. */
+ * A token outside the vocabulary is not accepted. vocab <= 2^20; where the total
+ * is 0 (no probability above 2^-38), next is vocab - 1. */
 int vg_k_verify_draft(const int32_t *tokens, const float *draft, const float *target,
                       const float *u_accept, const float *u_sample, const int32_t *counts,
                       uint32_t seqs, uint32_t drafted, uint32_t vocab, int32_t *accepted,

@@ -260,9 +260,13 @@ int vg_k_verify_draft(const int32_t *tokens, const float *draft, const float *ta
   for (const void *q : {(const void *)tokens, (const void *)draft, (const void *)target, (const void *)u_accept,
                         (const void *)u_sample, (const void *)counts, (const void *)accepted, (const void *)next})
     if (!aligned(q, 4)) return VG_EINVAL;
-  if (seqs > kMaxGrid || vocab > 0x1000000u || drafted > 0x100000u) return VG_ERANGE;
+  if (seqs > kMaxGrid / kVerifyCtas || vocab > kVerifyVocab || drafted > 0x100000u) return VG_ERANGE;
   const VerifyParams p{tokens, draft, target, u_accept, u_sample, counts, accepted, next, drafted, vocab};
-  verify_draft_kernel<<<seqs, kVerifyThreads, 0, (cudaStream_t)cuda_stream>>>(p);
+  const cudaStream_t st = (cudaStream_t)cuda_stream;
+  if (vocab % 4 == 0 && aligned(draft, 16) && aligned(target, 16))
+    verify_draft_kernel<true><<<seqs * kVerifyCtas, kVerifyThreads, 0, st>>>(p);
+  else
+    verify_draft_kernel<false><<<seqs * kVerifyCtas, kVerifyThreads, 0, st>>>(p);
   return launched();
 }
 
