@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "../../include/voxgen_cuda.h"
 #include "kv4_rows.cuh"
@@ -77,10 +78,24 @@ int by_dim(uint32_t head_dim, F &&f) {
   return head_dim == 64 ? f(Dim<64>{}) : f(Dim<128>{});
 }
 
-int allow_smem(const void *fn, size_t bytes) {
+// Lets fn use up to `bytes` of dynamic shared memory on the current device. `done`
+// belongs to fn: the devices (up to 64) on which that has been set.
+int allow_smem(const void *fn, size_t bytes, std::atomic<uint64_t> &done) {
   if (bytes <= 48 * 1024) return VG_OK;
-  return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess ? VG_OK
-                                                                                                          : VG_ECUDA;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return VG_ECUDA;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (bit && done.load(std::memory_order_acquire) & bit) return VG_OK;
+  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return VG_ECUDA;
+  done.fetch_or(bit, std::memory_order_release);
+  return VG_OK;
+}
+
+// Blocks of a sequence for `items` (token, head) pairs: enough for every SM to be
+// full (8 blocks each), no more than have two passes to make.
+uint32_t row_blocks(uint64_t items, uint32_t per_block, uint32_t seqs) {
+  const uint64_t most = (items + 2 * per_block - 1) / (2 * per_block), full = (148 * 8 + seqs - 1) / seqs;
+  return (uint32_t)std::min(most, full);
 }
 
 // Attention workspace: counters (zero between calls, at the same place for every
@@ -122,11 +137,10 @@ int vg_k_kv4_append(const vg_kv4_cache *cache, const void *k, const void *v, int
   p.tokens = tokens;
   const uint64_t items = (uint64_t)tokens * cache->kv_heads;
   const uint32_t per_block = kRowThreads / (cache->head_dim / 8);
-  const uint64_t blocks = (items + per_block - 1) / per_block;
-  if (items > 0xFFFFFFFFull || blocks * cache->seqs > kMaxGrid) return VG_ERANGE;
-  p.blocks = (uint32_t)blocks;
+  if (items > kMaxGrid) return VG_ERANGE;
+  p.blocks = row_blocks(items, per_block, cache->seqs);
   const bool vec = wide(k, p.ks, size) && wide(v, p.vs, size);
-  const dim3 grid((uint32_t)(blocks * cache->seqs));
+  const dim3 grid(p.blocks * cache->seqs);
   const cudaStream_t st = (cudaStream_t)cuda_stream;
   return by_dim(cache->head_dim, [&](auto d) {
     return by_type(dtype, [&](auto t) {
@@ -150,9 +164,10 @@ int vg_k_kv4_read(const vg_kv4_cache *cache, const int32_t *first, uint32_t toke
   p.first = first;
   p.tokens = tokens;
   const uint32_t per_block = kRowThreads / (cache->head_dim / 8);
-  const uint64_t lanes = (uint64_t)cache->seqs * cache->kv_heads;
-  if (tokens > (kMaxGrid * per_block) / lanes) return VG_ERANGE;
-  const dim3 grid((uint32_t)((lanes * tokens + per_block - 1) / per_block));
+  const uint64_t items = (uint64_t)tokens * cache->kv_heads;
+  if (items > kMaxGrid) return VG_ERANGE;
+  p.blocks = row_blocks(items, per_block, cache->seqs);
+  const dim3 grid(p.blocks * cache->seqs);
   return by_dim(cache->head_dim, [&](auto d) {
     return by_type(dtype, [&](auto t) {
       kv4_read_kernel<decltype(d)::value, decltype(t)><<<grid, kRowThreads, 0, (cudaStream_t)cuda_stream>>>(p);
@@ -208,7 +223,8 @@ int vg_k_kv4_attention(const vg_kv4_cache *cache, const void *q, int dtype, uint
       using T = decltype(t);
       constexpr int D = decltype(d)::value;
       const auto fn = kv4_rows_kernel<D, T>;
-      const int e = allow_smem((const void *)fn, RowsSmem<D>::kBytes);
+      static std::atomic<uint64_t> done{0};
+      const int e = allow_smem((const void *)fn, RowsSmem<D>::kBytes, done);
       if (e) return e;
       fn<<<kCtas, kRowsThreads, RowsSmem<D>::kBytes, st>>>(p);
       if (track) kv4_weights_kernel<D, T><<<(uint32_t)blocks, kWeightWarps * 32, 0, st>>>(p);
@@ -242,13 +258,18 @@ int vg_k_kv4_evict(const vg_kv4_cache *cache, uint32_t budget, uint32_t recent, 
   p.recent = recent;
   p.sinks = sinks;
   p.list = std::min(budget, cache->capacity - budget);
-  const size_t smem = (size_t)p.list * 4;
+  const size_t rest = kEvictBins * 4 + (size_t)p.list * 4, with_keys = rest + (size_t)cache->capacity * 4;
+  const bool keys = with_keys <= kEvictSmem;
   return by_dim(cache->head_dim, [&](auto d) {
-    const auto fn = kv4_evict_kernel<decltype(d)::value>;
-    const int e = allow_smem((const void *)fn, smem);
-    if (e) return e;
-    fn<<<cache->seqs * cache->kv_heads, kEvictThreads, smem, (cudaStream_t)cuda_stream>>>(p);
-    return launched();
+    constexpr int D = decltype(d)::value;
+    const auto go = [&](auto fn, std::atomic<uint64_t> &done) {
+      const int e = allow_smem((const void *)fn, kEvictSmem, done);
+      if (e) return e;
+      fn<<<cache->seqs * cache->kv_heads, kEvictThreads, keys ? with_keys : rest, (cudaStream_t)cuda_stream>>>(p);
+      return launched();
+    };
+    static std::atomic<uint64_t> done[2];
+    return keys ? go(kv4_evict_kernel<D, true>, done[0]) : go(kv4_evict_kernel<D, false>, done[1]);
   });
 }
 

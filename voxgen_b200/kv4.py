@@ -19,6 +19,7 @@ append past the capacity, a NaN among the rows) is in ``cache.status()``.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -40,10 +41,25 @@ def _invalid(what: str) -> VoxGenError:
     return VoxGenError(-1, what)
 
 
-def _stream(stream, device) -> int:
+# The current stream's address without building a Stream object, which takes as long as a small kernel.
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _stream(stream, index: int) -> int:
     if stream is None:
-        stream = torch.cuda.current_stream(device)
+        return _current_stream(index)
     return stream if isinstance(stream, int) else stream.cuda_stream
+
+
+def _on_its_device(call):
+    """Runs a method with the cache's device as the current one."""
+    def run(self, *args, **kwargs):
+        if torch.cuda.current_device() == self._index:
+            return call(self, *args, **kwargs)
+        with torch.cuda.device(self._index):
+            return call(self, *args, **kwargs)
+    return functools.wraps(call)(run)
 
 
 def _ints(x: Optional[torch.Tensor], n: int, device, what: str) -> Optional[int]:
@@ -102,6 +118,8 @@ class Kv4Cache:
                     or (shape is None and x.numel() < nbytes):
                 raise _invalid(f"{what}: expected contiguous {dtype} of {shape or nbytes} on {device}")
         self.seqs, self.kv_heads, self.head_dim, self.capacity = seqs, kv_heads, head_dim, capacity
+        self._index = device.index
+        self._scale = 1.0 / math.sqrt(head_dim)
         self.data, self.state, self.weights, self.positions = data, state, weights, positions
         address = [None if x is None else x.data_ptr() for x in (data, state, weights, positions)]
         self.desc = api.Kv4CacheDesc(*address, seqs, kv_heads, head_dim, capacity)
@@ -125,15 +143,17 @@ class Kv4Cache:
         self.state.zero_()
 
     def _rows_of(self, x: torch.Tensor, heads: int, what: str) -> int:
-        if x.dim() != 4 or x.shape[0] != self.seqs or x.shape[2] != heads or x.shape[3] != self.head_dim \
+        shape = x.shape
+        if len(shape) != 4 or shape[0] != self.seqs or shape[2] != heads or shape[3] != self.head_dim \
                 or x.device != self.device:
             raise _invalid(f"{what}: expected [{self.seqs}, tokens, {heads}, {self.head_dim}] on {self.device}, "
-                           f"got {list(x.shape)} on {x.device}")
+                           f"got {list(shape)} on {x.device}")
         dtype = DTYPES.get(x.dtype)
         if dtype is None:
             raise VoxGenError(-4, f"{what}: {x.dtype} is not supported")
         return dtype
 
+    @_on_its_device
     def append(self, k: torch.Tensor, v: torch.Tensor, *, at: Optional[torch.Tensor] = None,
                counts: Optional[torch.Tensor] = None, stream=None) -> None:
         """Stores new K and V rows ``[seqs, tokens, kv_heads, head_dim]`` from row ``at[s]`` on (default: after
@@ -141,12 +161,15 @@ class Kv4Cache:
         dtype = self._rows_of(k, self.kv_heads, "k")
         if self._rows_of(v, self.kv_heads, "v") != dtype or v.shape != k.shape:
             raise _invalid("k and v must agree in shape and type")
-        with torch.cuda.device(self.device):
-            _check(self._lib.vg_k_kv4_append(
-                self._ref, k.data_ptr(), v.data_ptr(), dtype, k.shape[1], _strides(k), _strides(v),
-                _ints(at, self.seqs, self.device, "at"), _ints(counts, self.seqs, self.device, "counts"),
-                _stream(stream, self.device)), f"append of {k.shape[1]} rows to a cache of {self.capacity}")
+        tokens = k.shape[1]
+        rc = self._lib.vg_k_kv4_append(
+            self._ref, k.data_ptr(), v.data_ptr(), dtype, tokens, _strides(k), _strides(v),
+            _ints(at, self.seqs, self.device, "at"), _ints(counts, self.seqs, self.device, "counts"),
+            _stream(stream, self._index))
+        if rc:
+            raise VoxGenError(rc, f"append of {tokens} rows to a cache of {self.capacity}")
 
+    @_on_its_device
     def read(self, tokens: int, *, first: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.float16,
              stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
         """Values of rows ``first[s] .. first[s] + tokens - 1`` (default: from row 0), K and V; rows that are not
@@ -154,15 +177,16 @@ class Kv4Cache:
         if dtype not in DTYPES:
             raise VoxGenError(-4, f"{dtype} is not supported")
         shape = self.seqs, tokens, self.kv_heads, self.head_dim
-        k, v = (torch.empty(shape, dtype=dtype, device=self.device) for _ in "kv")
-        with torch.cuda.device(self.device):
-            _check(self._lib.vg_k_kv4_read(self._ref, _ints(first, self.seqs, self.device, "first"), tokens,
-                                           DTYPES[dtype], k.data_ptr(), v.data_ptr(), _stream(stream, self.device)),
-                   f"read of {tokens} rows")
+        k, v = self.data.new_empty(shape, dtype=dtype), self.data.new_empty(shape, dtype=dtype)
+        rc = self._lib.vg_k_kv4_read(self._ref, _ints(first, self.seqs, self.device, "first"), tokens, DTYPES[dtype],
+                                     k.data_ptr(), v.data_ptr(), _stream(stream, self._index))
+        if rc:
+            raise VoxGenError(rc, f"read of {tokens} rows")
         return k, v
 
     # -- attention --------------------------------------------------------------------------
-    def _work(self, heads: int, tokens: int) -> torch.Tensor:
+    def _work(self, heads: int, tokens: int, stream) -> torch.Tensor:
+        """The workspace, large enough for the call; zeroed on the stream that is to use it."""
         need = self._need.get((heads, tokens))
         if need is None:
             n = C.c_uint64()
@@ -170,12 +194,18 @@ class Kv4Cache:
                    f"attention of {heads} heads over {self.kv_heads} KV heads, {tokens} tokens")
             need = self._need[heads, tokens] = n.value
         ws = self._workspace
-        if ws is None or ws.numel() < need:
-            if ws is not None:
-                ws.record_stream(torch.cuda.current_stream(self.device))
-            ws = self._workspace = torch.zeros(need, dtype=torch.uint8, device=self.device)
-        return ws
+        if ws is not None and ws.numel() >= need:
+            return ws
+        on = torch.cuda.current_stream(self._index)
+        if stream is not None:
+            on = torch.cuda.ExternalStream(_stream(stream, self._index), device=self.device)
+        if ws is not None:
+            ws.record_stream(on)
+        with torch.cuda.stream(on):
+            self._workspace = torch.zeros(need, dtype=torch.uint8, device=self.device)
+        return self._workspace
 
+    @_on_its_device
     def attention(self, q: torch.Tensor, *, counts: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                   track: Optional[bool] = None, out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
         """Attention of the last ``tokens`` rows' queries ``[seqs, tokens, heads, head_dim]``, causal within them.
@@ -184,41 +214,37 @@ class Kv4Cache:
         them). ``scale`` is 1/sqrt(head_dim) by default."""
         if q.dim() != 4:
             raise _invalid("q: expected [seqs, tokens, heads, head_dim]")
-        heads, tokens = q.shape[2], q.shape[1]
+        _, tokens, heads, _ = q.shape
         dtype = self._rows_of(q, heads, "q")
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != self.device or not out.is_contiguous():
             raise _invalid("out must be contiguous and like q")
         if track is None:
             track = self.weights is not None
         elif track and self.weights is None:
             raise _invalid("this cache does not track attention")
-        with torch.cuda.device(self.device):
-            raw = _stream(stream, self.device)
-            if stream is not None and self._workspace is None:
-                with torch.cuda.stream(torch.cuda.ExternalStream(raw, device=self.device)):
-                    ws = self._work(heads, tokens)
-            else:
-                ws = self._work(heads, tokens)
-            _check(self._lib.vg_k_kv4_attention(
-                self._ref, q.data_ptr(), dtype, heads, tokens, _strides(q),
-                _ints(counts, self.seqs, self.device, "counts"),
-                1.0 / math.sqrt(self.head_dim) if scale is None else scale, int(track), out.data_ptr(),
-                ws.data_ptr(), ws.numel(), raw), f"attention of {tokens} tokens, {heads} heads")
+        ws = self._work(heads, tokens, stream)
+        rc = self._lib.vg_k_kv4_attention(
+            self._ref, q.data_ptr(), dtype, heads, tokens, _strides(q),
+            _ints(counts, self.seqs, self.device, "counts"), self._scale if scale is None else scale, track,
+            out.data_ptr(), ws.data_ptr(), ws.numel(), _stream(stream, self._index))
+        if rc:
+            raise VoxGenError(rc, f"attention of {tokens} tokens, {heads} heads")
         return out
 
     # -- eviction ---------------------------------------------------------------------------
+    @_on_its_device
     def evict(self, budget: int, recent: int = 0, sinks: int = 0, *, into: Optional["Kv4Cache"] = None,
               stream=None) -> None:
         """Cuts sequences that hold more than ``budget`` rows to it: the last ``recent`` and first ``sinks``
         positions stay, and the rest that drew the most attention. ``into``: a cache over the same ``data``
         whose state, weights and positions receive the result instead."""
-        with torch.cuda.device(self.device):
-            _check(self._lib.vg_k_kv4_evict(self._ref, budget, recent, sinks, into._ref if into is not None else None,
-                                            _stream(stream, self.device)),
-                   f"eviction to {budget} rows ({recent} recent, {sinks} sinks) of a cache of {self.capacity}"
-                   + ("" if self.weights is not None else " that does not track attention"))
+        rc = self._lib.vg_k_kv4_evict(self._ref, budget, recent, sinks, None if into is None else into._ref,
+                                      _stream(stream, self._index))
+        if rc:
+            raise VoxGenError(rc, f"eviction to {budget} rows ({recent} recent, {sinks} sinks) of a cache of "
+                              f"{self.capacity}" + ("" if self.weights is not None else " that does not track attention"))
 
 
 def cache_bytes(seqs: int, kv_heads: int, head_dim: int, capacity: int) -> int:
@@ -254,10 +280,14 @@ def verify_draft(tokens: torch.Tensor, draft: torch.Tensor, target: torch.Tensor
             raise _invalid(f"verify_draft: {what} must be contiguous {dtype} {list(shape)} on {device}")
     if device.type != "cuda":
         raise _invalid("verify_draft runs on a CUDA device")
-    accepted, token = torch.empty(2, seqs, dtype=torch.int32, device=device)
-    with torch.cuda.device(device):
-        _check(api.lib().vg_k_verify_draft(
-            tokens.data_ptr(), draft.data_ptr(), target.data_ptr(), u_accept.data_ptr(), u_sample.data_ptr(),
-            _ints(counts, seqs, device, "counts"), seqs, drafted, vocab, accepted.data_ptr(), token.data_ptr(),
-            _stream(stream, device)), f"verification of {drafted} tokens of a vocabulary of {vocab}")
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            return verify_draft(tokens, draft, target, u_accept, u_sample, counts=counts, stream=stream)
+    accepted, token = tokens.new_empty(seqs), tokens.new_empty(seqs)
+    rc = api.lib().vg_k_verify_draft(
+        tokens.data_ptr(), draft.data_ptr(), target.data_ptr(), u_accept.data_ptr(), u_sample.data_ptr(),
+        _ints(counts, seqs, device, "counts"), seqs, drafted, vocab, accepted.data_ptr(), token.data_ptr(),
+        _stream(stream, device.index))
+    if rc:
+        raise VoxGenError(rc, f"verification of {drafted} tokens of a vocabulary of {vocab}")
     return accepted, token
