@@ -99,10 +99,15 @@ uint32_t row_blocks(uint64_t items, uint32_t per_block, uint32_t seqs) {
 }
 
 // Attention workspace: counters (zero between calls, at the same place for every
-// shape), partial results of the CTAs, then the softmax denominators.
-constexpr uint32_t kCtas = 148;   // one per SM
-constexpr uint64_t kTicketBytes = 1024;
-uint64_t part_bytes(uint32_t head_dim) { return (uint64_t)2 * kCtas * 16 * (head_dim + 2) * 4; }
+// shape), partial results, then the softmax denominators.
+constexpr uint64_t kTicketBytes = kMostTickets * 4;
+uint64_t segments_of(const vg_kv4_cache *c, uint32_t heads, uint32_t tokens) {
+  const uint64_t rows = (uint64_t)tokens * (heads / c->kv_heads);
+  return (rows + kTileRows - 1) / kTileRows * c->kv_heads * c->seqs;
+}
+uint64_t part_bytes(const vg_kv4_cache *c, uint32_t heads, uint32_t tokens) {
+  return most_pieces(segments_of(c, heads, tokens)) * kTileRows * (c->head_dim + 2) * 4;
+}
 
 }  // namespace
 
@@ -182,7 +187,8 @@ int vg_k_kv4_attention_bytes(const vg_kv4_cache *cache, uint32_t heads, uint32_t
   if (rc) return rc;
   if (!bytes || !heads || !tokens || heads % cache->kv_heads) return VG_EINVAL;
   if ((uint64_t)heads * tokens > kMaxGrid / cache->seqs) return VG_ERANGE;
-  *bytes = kTicketBytes + part_bytes(cache->head_dim) + (uint64_t)cache->seqs * tokens * heads * 4;
+  if (segments_of(cache, heads, tokens) * ((cache->capacity + kUnit - 1) / kUnit) > kMaxGrid) return VG_ERANGE;
+  *bytes = kTicketBytes + part_bytes(cache, heads, tokens) + (uint64_t)cache->seqs * tokens * heads * 4;
   return VG_OK;
 }
 
@@ -205,16 +211,14 @@ int vg_k_kv4_attention(const vg_kv4_cache *cache, const void *q, int dtype, uint
   p.out = out;
   p.tickets = (uint32_t *)ws;
   p.parts = (float *)(ws + kTicketBytes);
-  p.lse = track ? (float *)(ws + kTicketBytes + part_bytes(cache->head_dim)) : nullptr;
+  p.lse = track ? (float *)(ws + kTicketBytes + part_bytes(cache, heads, tokens)) : nullptr;
   p.qs = strides_of(q_strides, tokens, heads, cache->head_dim);
-  p.wide = wide(q, p.qs, size);
   p.counts = counts;
   p.tokens = tokens;
   p.heads = heads;
   p.group = heads / cache->kv_heads;
   p.scale = scale * 1.44269504088896340736f;
-  const uint32_t tile = size == 4 ? 8 : 16;
-  p.row_tiles = (tokens * p.group + tile - 1) / tile;
+  p.row_tiles = (tokens * p.group + kTileRows - 1) / kTileRows;
   const uint64_t blocks = ((uint64_t)cache->capacity + kWeightWarps - 1) / kWeightWarps * cache->seqs * cache->kv_heads;
   if (track && blocks > kMaxGrid) return VG_ERANGE;
   const cudaStream_t st = (cudaStream_t)cuda_stream;
@@ -226,7 +230,7 @@ int vg_k_kv4_attention(const vg_kv4_cache *cache, const void *q, int dtype, uint
       static std::atomic<uint64_t> done{0};
       const int e = allow_smem((const void *)fn, RowsSmem<D>::kBytes, done);
       if (e) return e;
-      fn<<<kCtas, kRowsThreads, RowsSmem<D>::kBytes, st>>>(p);
+      fn<<<kRowsCtas, kRowsThreads, RowsSmem<D>::kBytes, st>>>(p);
       if (track) kv4_weights_kernel<D, T><<<(uint32_t)blocks, kWeightWarps * 32, 0, st>>>(p);
       return launched();
     });

@@ -1,30 +1,37 @@
 // Attention of few query rows over a 4-bit cache: single tokens and short drafts.
 //
 // The mathematics. The query rows of a (sequence, KV head) are packed: row
-// r = token * group + head of the group. A tile is 16 rows of one m16n8k16 MMA
-// A operand; fp32 queries are split into fp16 hi + lo, which takes two rows, so
-// a tile is then 8 query rows and C row g + C row g + 8 is the score. Scores are
-// Q K^T with the cache's K rows as the B operand, and the output P V with its V
-// rows as B: both come out of the codes with one shift, one lop3 and one fused
-// multiply-add a pair (kv4.cuh), exactly. P is kept as hi + lo for fp32 queries
-// and rounded to fp16 (11 bits) for 16-bit ones, where the output's rounding is
-// as large. Softmax statistics and sums are fp32.
+// r = token * group + head of the group. A tile is 8 of them, the columns of an
+// m16n8k16 MMA: scores are S^T = K Q^T and the output O^T = V^T P^T, with the
+// cache as the A operand. Both K and V come out of the codes with one shift, one
+// lop3 and one fused multiply-add a pair (kv4.cuh), exactly. fp32 queries are
+// fp16 hi + lo, and so is their P, accumulated by a second MMA; 16-bit queries
+// are exact in fp16 (times a power of two) and their P is rounded to 11 bits,
+// like the output. Softmax statistics and sums are fp32.
 //
 // The contraction over channels may run in any order as long as both operands
-// agree, so lane (g, t) takes channels [t*D/4, (t+1)*D/4) of K row g: one wide
-// load, and at head_dim 128 one scale. The scores' C fragment (rows = heads,
-// columns = cache rows) is the A fragment of P without a shuffle, when lane t's
-// V rows are those of its score columns. V needs pairs along rows: two bytes
-// permutes put the nibbles of two rows side by side.
+// agree, so lane (g, t) takes channels [t*D/4, (t+1)*D/4) of its K rows: one wide
+// load, and at head_dim 128 one scale. An 8x8 transpose (movmatrix) turns the
+// scores' C fragment into the B fragment of P^T. V needs pairs along rows: two
+// byte permutes put the nibbles of two rows side by side. Row order within a
+// tile is free too; kPerm's keeps K's 16-byte loads and V's 8-byte loads to the
+// fewest bank conflicts (none, and 2-way).
 //
-// The split. All (sequence, KV head, row tile) segments are cut into units of
-// 32 cache rows, and the units of all segments are dealt out evenly to one CTA
-// per SM, in order: ragged lengths balance by themselves. A warp takes every
-// kWarps-th unit of its CTA's range through a private ring of bulk copies (no
-// CTA barrier while it streams), keeps its own softmax state, and the warps
-// meet when a segment ends. A segment that spans CTAs leaves one partial result
-// per CTA; the last CTA to arrive (a counter, left at zero) adds them in CTA
-// order. Sums therefore never depend on timing.
+// The split. A segment is a (sequence, KV head, row tile); its cache rows are cut
+// into units of 32. Segments are cut into pieces of at most U units, with U such
+// that there is about one piece for each of the 148 CTAs (4, where segments are
+// many), so ragged lengths share the SMs evenly and a CTA seldom changes
+// segments, which costs about as much as 16 units (q, the merge). A warp takes
+// every 16th unit of the piece through a private ring of bulk copies (no CTA
+// barrier while it streams) and keeps its own softmax state; the warps meet when
+// the piece ends. A segment of several pieces leaves a partial result for each,
+// and the CTA that finishes last (a counter, left at zero) adds them in order:
+// sums never depend on timing.
+//
+// What one call pays once is mostly instruction fetch: code that runs once costs
+// about 5 cycles an instruction here. So the loop body covers 16 cache rows and
+// not 32, q becomes fragments once per CTA and not per warp, and divisions are
+// 32-bit.
 #pragma once
 #include "kv4_rows.cuh"
 #include "ptx.cuh"
@@ -40,10 +47,9 @@ struct Kv4AttnParams {
   const int32_t *counts;    // new tokens of each sequence, may be null
   uint32_t tokens, heads, group;
   float scale;              // of the scores, times log2(e)
-  uint32_t wide;            // 16-byte loads of q are aligned
   uint32_t row_tiles;       // tiles of a (sequence, KV head)'s query rows
-  uint32_t *tickets;        // [CTAs], zero between calls
-  float *parts;             // [2 * CTAs][rows of a tile][D + 2]
+  uint32_t *tickets;        // [segments], zero between calls
+  float *parts;             // [pieces] partial results
 };
 
 __device__ __forceinline__ uint32_t kv4_held(const Kv4View &c, uint32_t seq) {
@@ -53,11 +59,22 @@ __device__ __forceinline__ int32_t kv4_count(const Kv4AttnParams &p, uint32_t se
   return p.counts ? min(max(p.counts[seq], 0), (int32_t)p.tokens) : (int32_t)p.tokens;
 }
 
-__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+// Transpose of an 8x8 matrix of halves held as one pair a lane.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// 2^x to within 2 units of the 22nd bit; results below 2^-126 are 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
@@ -78,11 +95,18 @@ __device__ __forceinline__ float row_power(float top, float &inverse) {
   return __uint_as_float((uint32_t)(127 + k) << 23);
 }
 
-constexpr uint32_t kUnit = 32;      // cache rows of a unit
-constexpr uint32_t kRowsWarps = 12;
-constexpr uint32_t kRowsStages = 3;
+constexpr uint32_t kUnit = 32;        // cache rows of a unit
+constexpr uint32_t kRowsWarps = 16;
+constexpr uint32_t kRowsStages = 2;
+constexpr uint32_t kTileRows = 8;     // query rows of a tile
 constexpr uint32_t kRowsThreads = kRowsWarps * 32;
-constexpr float kPScale = 14.f;     // P is held times 2^14: fp16's smallest numbers then lie 2^38 below the largest
+constexpr uint32_t kRowsCtas = 148;   // one per SM
+constexpr uint32_t kLeastUnits = 16;  // of a piece: one round of the warps
+constexpr uint32_t kMostTickets = 1u << 14;   // segments that may be cut
+constexpr float kPScale = 14.f;       // P is held times 2^14: fp16's smallest numbers then lie 2^38 below the largest
+
+template <int D>
+constexpr uint32_t kPart = kTileRows * (D + 2);   // floats of a partial result: values, maxima, denominators
 
 template <int D>
 struct RowsSmem {
@@ -90,69 +114,107 @@ struct RowsSmem {
   static constexpr uint32_t kScales = kUnit * D / 16;
   static constexpr uint32_t kStage = 2 * (kCodes + kScales);
   static constexpr uint32_t kRing = kRowsWarps * kRowsStages * kStage;
-  static constexpr uint32_t kMerge = kRowsWarps * 8 * D * 4;
+  static constexpr uint32_t kMerge = kRowsWarps * kTileRows * D * 4;
   static constexpr uint32_t kBytes = kRing + kMerge;
 };
 
-// Position in the dealt-out order of units.
-struct UnitCursor {
-  uint32_t seq, lane, unit, units;  // lane: (KV head, row tile) of the sequence
-};
+// Pieces that a call may be cut into: `segments` plus what the target allows.
+__host__ __device__ __forceinline__ uint32_t target_pieces(uint32_t segments) {
+  return kRowsCtas * (segments * 4 <= kRowsCtas * 3 ? 1 : 4);
+}
+__host__ __device__ __forceinline__ uint64_t most_pieces(uint64_t segments) {
+  return segments > kMostTickets ? 0 : segments + target_pieces((uint32_t)segments);
+}
 
 __device__ __forceinline__ uint32_t units_of(uint32_t rows) { return max(1u, (rows + kUnit - 1) / kUnit); }
 
-// Total units of all sequences times lanes, and where unit `x` lies. Every warp
-// computes them for itself.
-__device__ __forceinline__ uint64_t total_units(const Kv4View &c, uint32_t lanes) {
-  uint64_t n = 0;
-  for (uint32_t s = threadIdx.x % 32; s < c.seqs; s += 32) n += units_of(kv4_held(c, s));
-#pragma unroll
-  for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(~0u, n, o);
-  return n * lanes;
+// How segments are cut: `lanes` segments a sequence, pieces of `size` units, and
+// how many pieces there are. Every warp plans for itself.
+struct Plan {
+  uint32_t lanes, size, pieces;
+};
+__device__ __forceinline__ uint32_t pieces_of(const Kv4View &c, uint32_t s, uint32_t size) {
+  return s < c.seqs ? (units_of(kv4_held(c, s)) + size - 1) / size : 0u;
 }
-__device__ __forceinline__ UnitCursor find_unit(const Kv4View &c, uint32_t lanes, uint64_t x) {
+__device__ __forceinline__ Plan make_plan(const Kv4View &c, uint32_t lanes) {
+  const uint32_t lane = threadIdx.x % 32, segments = c.seqs * lanes;
+  Plan p{lanes, 1u << 30, segments};   // one piece a segment
+  if (segments > kMostTickets) return p;
+  uint32_t total = 0;
+#pragma unroll 1
+  for (uint32_t s = lane; s < c.seqs; s += 32) total += units_of(kv4_held(c, s));
+  total = __reduce_add_sync(~0u, total) * lanes;   // the host keeps it below 2^31
+  const uint32_t target = target_pieces(segments);
+  p.size = max(kLeastUnits, (total + target - 1) / target);
+#pragma unroll 1
+  for (int i = 0;; ++i) {
+    uint32_t n = 0;
+#pragma unroll 1
+    for (uint32_t s = lane; s < c.seqs; s += 32) n += pieces_of(c, s, p.size);
+    p.pieces = __reduce_add_sync(~0u, n) * lanes;
+    if (p.pieces <= target || i == 3) return p;
+    p.size = max(p.size + 1, (uint32_t)((uint64_t)p.size * p.pieces / target));
+  }
+}
+
+struct Piece {
+  uint32_t seq, lane;          // lane: (KV head, row tile) of the sequence
+  uint32_t part, parts;        // of the segment
+  uint32_t first, units;       // of the piece, in the segment
+};
+__device__ __forceinline__ Piece find_piece(const Kv4View &c, const Plan &p, uint32_t index) {
   const uint32_t lane = threadIdx.x % 32;
-  uint64_t before = 0;
+  uint32_t before = 0;
+#pragma unroll 1
   for (uint32_t base = 0; base < c.seqs; base += 32) {
-    const uint32_t s = base + lane;
-    const uint32_t u = s < c.seqs ? units_of(kv4_held(c, s)) : 0;
-    uint64_t sum = (uint64_t)u * lanes;
+    const uint32_t n = pieces_of(c, base + lane, p.size);
+    uint32_t sum = n * p.lanes;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t up = __shfl_up_sync(~0u, sum, o);
+      const uint32_t up = __shfl_up_sync(~0u, sum, o);
       if (lane >= (uint32_t)o) sum += up;
     }
-    const uint32_t past = __ballot_sync(~0u, before + sum > x);
+    const uint32_t past = __ballot_sync(~0u, before + sum > index);
     if (past) {
       const int at = __ffs(past) - 1;
-      const uint32_t units = __shfl_sync(~0u, u, at);
-      const uint64_t into = x - before - (__shfl_sync(~0u, sum, at) - (uint64_t)units * lanes);
-      return UnitCursor{base + at, (uint32_t)(into / units), (uint32_t)(into % units), units};
+      const uint32_t parts = __shfl_sync(~0u, n, at);
+      const uint32_t into = index - before - (__shfl_sync(~0u, sum, at) - parts * p.lanes);
+      Piece x;
+      x.seq = base + at;
+      x.lane = into / parts;
+      x.part = into - x.lane * parts;
+      x.parts = parts;
+      x.first = x.part * p.size;
+      x.units = parts == 1 ? units_of(kv4_held(c, x.seq)) : min(p.size, units_of(kv4_held(c, x.seq)) - x.first);
+      return x;
     }
     before += __shfl_sync(~0u, sum, 31);
   }
-  return UnitCursor{c.seqs, 0, 0, 1};
+  return Piece{0, 0, 0, 1, 0, 0};   // past the last piece
 }
 
-// T: type of q and out. fp32 queries take two MMA rows each.
+// Cache row of a 16-row tile that MMA row i is (in both halves of the tile).
+__device__ __forceinline__ uint32_t perm8(uint32_t i) { return i % 2 ? 4 + (i / 2 ^ 1) : i / 2; }
+
+// T: type of q and out; fp32 operands are hi + lo.
 template <int D, typename T>
 __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4AttnParams p) {
   using S = RowsSmem<D>;
   constexpr bool kSplit = sizeof(T) == 4;
-  constexpr uint32_t kRows = kSplit ? 8 : 16;   // query rows of a tile
-  constexpr int kSteps = D / 16;                // MMAs of a score, and n-tiles of the output (D / 8) / 2
-  constexpr uint32_t kLaneChannels = D / 4;
+  constexpr int kSteps = D / 16;                // k-steps of a score, and m-tiles of the output
+  constexpr uint32_t kLaneChannels = D / 4;     // of K
+  constexpr uint32_t kLaneValues = D / 8;       // channels of V
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t bars[kRowsWarps][kRowsStages];
-  __shared__ float w_max[kRowsWarps][16], w_sum[kRowsWarps][16];
-  __shared__ float f_max[16], f_sum[16];
+  __shared__ __align__(8) float w_max[kRowsWarps][kTileRows], w_sum[kRowsWarps][kTileRows];
+  __shared__ float f_max[kTileRows], f_sum[kTileRows];
   __shared__ uint32_t last;
+  __shared__ __align__(8) uint32_t q_frag[kSplit ? 2 : 1][kSteps][32][2];   // B fragments: hi, lo
+  __shared__ __align__(8) float factors[kTileRows];
+  __shared__ __align__(8) uint32_t seens[kTileRows];
   const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
-  const uint32_t lanes = p.c.kv_heads * p.row_tiles, rows = p.tokens * p.group;
-  const uint64_t total = total_units(p.c, lanes);
-  const uint32_t ctas = (uint32_t)min((uint64_t)gridDim.x, total);   // every one of them has a unit
-  if (blockIdx.x >= ctas) return;
-  const uint64_t begin = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1) / ctas;
+  const Plan plan = make_plan(p.c, p.c.kv_heads * p.row_tiles);
+  if (blockIdx.x >= plan.pieces) return;
   const size_t run_bytes = (size_t)p.c.tiles * Kv4<D>::kTileBytes;
   uint8_t *ring = smem + warp * kRowsStages * S::kStage;
   float *merge = (float *)(smem + S::kRing);
@@ -162,333 +224,362 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
   fence_mbar_init();
   __syncwarp();
 
-  UnitCursor seg = find_unit(p.c, lanes, begin);   // segment being worked on (the same in every warp)
-  UnitCursor ahead = seg;                          // next unit of this warp to fetch
-  uint64_t fetch = begin + warp;
-  uint32_t fetched = 0;
-  auto advance = [&](UnitCursor &u, uint32_t by) {
-    u.unit += by;
-    while (u.unit >= u.units && u.seq < p.c.seqs) {
-      u.unit -= u.units;
-      if (++u.lane == lanes) {
-        u.lane = 0;
-        if (++u.seq < p.c.seqs) u.units = units_of(kv4_held(p.c, u.seq));
-      }
-    }
-  };
-  advance(ahead, warp);
-  auto fetch_next = [&]() {  // one lane
-    if (fetch >= end) return;
-    const uint32_t stage = fetched % kRowsStages;
-    uint8_t *dst = ring + stage * S::kStage;
-    const uint32_t row = ahead.unit * kUnit;
-    const uint8_t *run = p.c.data + ((size_t)ahead.seq * p.c.kv_heads + ahead.lane / p.row_tiles) * run_bytes;
-    uint64_t *bar = &bars[warp][stage];
-    mbar_arrive_expect_tx(bar, S::kStage);
-    bulk_g2s(dst, run + Kv4<D>::codes(row, 0), S::kCodes, bar);
-    bulk_g2s(dst + S::kCodes, run + Kv4<D>::codes(row, 1), S::kCodes, bar);
-    bulk_g2s(dst + 2 * S::kCodes, run + Kv4<D>::scales(row, 0), S::kScales, bar);
-    bulk_g2s(dst + 2 * S::kCodes + S::kScales, run + Kv4<D>::scales(row, 1), S::kScales, bar);
-    ++fetched;
-    fetch += kRowsWarps;
-    advance(ahead, kRowsWarps);
-  };
-  if (lane == 0)
-    for (uint32_t i = 0; i < kRowsStages; ++i) fetch_next();
-
-  uint32_t used = 0;            // units taken by this warp
-  uint64_t mine = begin + warp; // its next unit
+  uint32_t stage = 0, parity = 0, fetch_stage = 0;
   bool timed_out = false;
-  for (uint64_t at = begin; at < end;) {
-    const uint64_t seg_end = min(end, at + (seg.units - seg.unit));
-    const bool whole = seg.unit == 0 && at + seg.units <= end;
-    const uint32_t kv = seg.lane / p.row_tiles, row0 = seg.lane % p.row_tiles * kRows;
+  // this lane's places in a stage
+  const uint32_t k_codes = perm8(g) * (D / 2) + t * (D / 8);
+  const uint32_t k_scale = 2 * S::kCodes + perm8(g) * (D / 16) + t * kLaneChannels / 32 * 2;
+  const uint32_t v_row[2] = {perm8(2 * t), perm8(2 * t + 1)};
+  const uint32_t v_codes = S::kCodes + g * (D / 16), v_scale = 2 * S::kCodes + S::kScales + g * kLaneValues / 32 * 2;
+
+  // units of a piece from this warp's `unit` on, one each call, into the next stage of the ring
+  auto fetch = [&](const Piece &x, uint32_t unit) {
+    if (lane == 0) {
+      uint8_t *dst = ring + fetch_stage * S::kStage;
+      const uint32_t row = (x.first + unit) * kUnit;
+      const uint8_t *run = p.c.data + ((size_t)x.seq * p.c.kv_heads + x.lane / p.row_tiles) * run_bytes;
+      uint64_t *bar = &bars[warp][fetch_stage];
+      mbar_arrive_expect_tx(bar, S::kStage);
+      bulk_g2s(dst, run + Kv4<D>::codes(row, 0), S::kCodes, bar);
+      bulk_g2s(dst + S::kCodes, run + Kv4<D>::codes(row, 1), S::kCodes, bar);
+      bulk_g2s(dst + 2 * S::kCodes, run + Kv4<D>::scales(row, 0), S::kScales, bar);
+      bulk_g2s(dst + 2 * S::kCodes + S::kScales, run + Kv4<D>::scales(row, 1), S::kScales, bar);
+    }
+    fetch_stage = fetch_stage + 1 == kRowsStages ? 0 : fetch_stage + 1;
+  };
+
+  Piece seg = find_piece(p.c, plan, blockIdx.x);
+  uint32_t ahead = warp;    // next unit of the piece to fetch
+#pragma unroll 1
+  for (uint32_t i = 0; i < kRowsStages && ahead < seg.units; ++i, ahead += kRowsWarps) fetch(seg, ahead);
+
+#pragma unroll 1
+  for (uint32_t index = blockIdx.x; index < plan.pieces; index += gridDim.x) {
+    const Piece next = index + gridDim.x < plan.pieces ? find_piece(p.c, plan, index + gridDim.x) : Piece{0, 0, 0, 1, 0, 0};
+    uint32_t next_ahead = warp;
+    const bool whole = seg.parts == 1;
+    const uint32_t kv = seg.lane / p.row_tiles, row0 = (seg.lane - kv * p.row_tiles) * kTileRows;
+    const uint32_t rows = p.tokens * p.group, tile_rows = min(kTileRows, rows - row0);
     const uint32_t held = kv4_held(p.c, seg.seq);
-    const int32_t count = kv4_count(p, seg.seq);
-    // cache rows that this lane's query rows (g, and g + 8) see, and the fewest of the tile
-    uint32_t seen[2] = {0, 0};
-    float factor[2] = {0.f, 0.f};
-    uint32_t qa[kSteps][4];
+    // ---- the queries as B fragments, a warp a row: column `warp` of the MMA is query row row0 + warp ----
+    if (warp < kTileRows) {
+      constexpr uint32_t N = D / 32;    // channels of a lane
+      const uint32_t r = row0 + warp, tok = r / p.group;
+      float x[N];
 #pragma unroll
-    for (int h = 0; h < (kSplit ? 1 : 2); ++h) {
-      const uint32_t r = row0 + g + 8 * h;
-      float x[kLaneChannels], top = 0.f;
+      for (uint32_t i = 0; i < N; ++i) x[i] = 0.f;
+      uint32_t seen = 0;
       if (r < rows) {
-        const uint32_t tok = r / p.group, head = kv * p.group + r % p.group;
-        const int32_t n = (int32_t)held - count + (int32_t)tok + 1;
-        seen[h] = (int32_t)tok < count && n > 0 ? (uint32_t)n : 0u;
+        const int32_t count = kv4_count(p, seg.seq), n = (int32_t)held - count + (int32_t)tok + 1;
+        seen = (int32_t)tok < count && n > 0 ? (uint32_t)n : 0u;
         const T *q = (const T *)p.q + (int64_t)seg.seq * p.qs.seq + (int64_t)tok * p.qs.token +
-                     (int64_t)head * p.qs.head + t * kLaneChannels;
+                     (int64_t)(kv * p.group + r - tok * p.group) * p.qs.head + lane * N;
 #pragma unroll
-        for (uint32_t i = 0; i < kLaneChannels; i += 8) {
-          if (p.wide) load8<T, true>(q + i, *(float(*)[8])(x + i));
-          else load8<T, false>(q + i, *(float(*)[8])(x + i));
-        }
-      } else {
-#pragma unroll
-        for (uint32_t i = 0; i < kLaneChannels; ++i) x[i] = 0.f;
+        for (uint32_t i = 0; i < N; ++i) x[i] = (float)q[i];
       }
+      uint32_t top = 0;
 #pragma unroll
-      for (uint32_t i = 0; i < kLaneChannels; ++i) top = fmaxf(top, fabsf(x[i]));
-      top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+      for (uint32_t i = 0; i < N; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+      top = __reduce_max_sync(~0u, top);
       float inverse;
-      const float power = row_power(top, inverse);
-      factor[h] = p.scale * inverse;
-      // step s = word s/2 of the lane's channels, pairs (i, i + 4) with i = 2 * (s % 2) and the next
+      const float power = row_power(__uint_as_float(top), inverse);
+      if (lane == 0) factors[warp] = fmaxf(p.scale * inverse, 0x1p-126f), seens[warp] = seen;
+      // channel c: lane t = c / (D/4) of row g, word (c % (D/4)) / 8, and within the word i = c % 8: pair i % 4 (half
+      // i / 4), two pairs a step
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const int c = s / 2 * 8 + s % 2 * 2;
-        if constexpr (kSplit) {
-          split2(x[c] * power, x[c + 4] * power, qa[s][0], qa[s][1]);
-          split2(x[c + 1] * power, x[c + 5] * power, qa[s][2], qa[s][3]);
-        } else {
-          qa[s][h] = half2_bits(__floats2half2_rn(x[c] * power, x[c + 4] * power));
-          qa[s][2 + h] = half2_bits(__floats2half2_rn(x[c + 1] * power, x[c + 5] * power));
-        }
+      for (uint32_t i = 0; i < N; ++i) {
+        const uint32_t c = lane * N + i, in = c % kLaneChannels, y = c % 4;
+        const uint32_t step = in / 8 * 2 + y / 2, half = c % 8 / 4;
+        const float v = x[i] * power;
+        const __half hi = __float2half_rn(v);
+        ((__half *)&q_frag[0][step][warp * 4 + c / kLaneChannels][y % 2])[half] = hi;
+        if constexpr (kSplit)
+          ((__half *)&q_frag[1][step][warp * 4 + c / kLaneChannels][y % 2])[half] = __float2half_rn(v - __half2float(hi));
       }
     }
-    uint32_t least = held;
-    if (row0 + g < rows) least = min(least, seen[0]);
-    if (!kSplit && row0 + g + 8 < rows) least = min(least, seen[1]);
+    __syncthreads();
+    uint32_t q_hi[kSteps][2], q_lo[kSplit ? kSteps : 1][2];
 #pragma unroll
-    for (int o = 4; o < 32; o <<= 1) least = min(least, __shfl_xor_sync(~0u, least, o));
+    for (int i = 0; i < kSteps; ++i) {
+      *(uint2 *)q_hi[i] = *(const uint2 *)q_frag[0][i][lane];
+      if constexpr (kSplit) *(uint2 *)q_lo[i] = *(const uint2 *)q_frag[1][i][lane];
+    }
+    // scores of query rows 2t and 2t + 1 are this lane's
+    const float f0 = factors[2 * t], f1 = factors[2 * t + 1];
+    const uint32_t seen0 = seens[2 * t], seen1 = seens[2 * t + 1];
+    const uint32_t least = min(seens[0], seens[tile_rows - 1]);   // every row sees these
 
-    float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float o[kSteps][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    for (int j = 0; j < kSteps; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 
-    for (; mine < seg_end; mine += kRowsWarps, ++used) {
-      const uint32_t stage = used % kRowsStages;
-      const uint8_t *st = ring + stage * S::kStage;
-      const uint32_t first = (seg.unit + (uint32_t)(mine - at)) * kUnit;   // its first cache row
-      if (!mbar_wait_bounded(&bars[warp][stage], used / kRowsStages & 1)) timed_out = true;
-      const bool tail = first + kUnit > least;
-      // ---- scores: columns of n-tile i are cache rows 8i + {t, 4 + (t^1)} ----
-      float c[kUnit / 8][4];
-      const uint32_t krow = g % 2 ? 4 + (g / 2 ^ 1) : g / 2;
+#pragma unroll 1
+    for (uint32_t unit = warp; unit < seg.units; unit += kRowsWarps) {
+      if (!mbar_wait_bounded(&bars[warp][stage], parity)) timed_out = true;
+      const uint32_t unit_row = (seg.first + unit) * kUnit;
+#pragma unroll 1
+      for (uint32_t half = 0; half < kUnit; half += 16) {
+        const uint8_t *st = ring + stage * S::kStage + half * (D / 2);            // codes
+        const uint8_t *sc = ring + stage * S::kStage + half * (D / 16);           // scales
+        const uint32_t first = unit_row + half;   // the first of 16 cache rows
+        const bool tail = first + 16 > least;
+        // ---- scores ----
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
+        {
+          uint32_t w[2][kSteps / 2];
+          __half2 d[2], d72[2];
 #pragma unroll
-      for (int i = 0; i < (int)kUnit / 8; ++i) {
-        const uint32_t r = 8 * i + krow;
-        uint32_t w[kSteps / 2];
-        if constexpr (D == 128) {
-          const uint4 v = *(const uint4 *)(st + r * (D / 2) + t * 16);
-          w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-        } else {
-          const uint2 v = *(const uint2 *)(st + r * (D / 2) + t * 8);
-          w[0] = v.x, w[1] = v.y;
-        }
-        const __half2 d = __half2half2(*(const __half *)(st + 2 * S::kCodes + r * (D / 16) + t * kLaneChannels / 32 * 2));
-        const __half2 d72 = minus72(d);
-        c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.f;
+          for (int y = 0; y < 2; ++y) {
+            const uint8_t *b = st + k_codes + 8 * y * (D / 2);
+            if constexpr (D == 128) {
+              const uint4 v = *(const uint4 *)b;
+              w[y][0] = v.x, w[y][1] = v.y, w[y][2] = v.z, w[y][3] = v.w;
+            } else {
+              const uint2 v = *(const uint2 *)b;
+              w[y][0] = v.x, w[y][1] = v.y;
+            }
+            d[y] = __half2half2(*(const __half *)(sc + k_scale + 8 * y * (D / 16)));
+            d72[y] = minus72(d[y]);
+          }
 #pragma unroll
-        for (int k = 0; k < kSteps / 2; ++k) {
-          __half2 h[4];
-          unpack8(w[k], d, d72, h);
-          mma_f16(c[i], qa[2 * k], half2_bits(h[0]), half2_bits(h[1]));
-          mma_f16(c[i], qa[2 * k + 1], half2_bits(h[2]), half2_bits(h[3]));
-        }
-      }
-      // ---- softmax ----
-      float s[2][kUnit / 4], top[2] = {m[0], m[1]};
+          for (int k = 0; k < kSteps / 2; ++k) {
+            __half2 a[4], b[4];
+            unpack8(w[0][k], d[0], d72[0], a);
+            unpack8(w[1][k], d[1], d72[1], b);
 #pragma unroll
-      for (int i = 0; i < (int)kUnit / 8; ++i) {
-        if constexpr (kSplit) {
-          s[0][2 * i] = (c[i][0] + c[i][2]) * factor[0];
-          s[0][2 * i + 1] = (c[i][1] + c[i][3]) * factor[0];
-        } else {
-          s[0][2 * i] = c[i][0] * factor[0], s[0][2 * i + 1] = c[i][1] * factor[0];
-          s[1][2 * i] = c[i][2] * factor[1], s[1][2 * i + 1] = c[i][3] * factor[1];
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < (kSplit ? 1 : 2); ++h) {
-        if (tail) {
-#pragma unroll
-          for (int i = 0; i < (int)kUnit / 4; ++i) {
-            const uint32_t r = first + i / 2 * 8 + (i % 2 ? 4 + (t ^ 1) : t);
-            if (r >= seen[h]) s[h][i] = -INFINITY;
+            for (int y = 0; y < 2; ++y) {
+              const uint32_t x[4] = {half2_bits(a[2 * y]), half2_bits(b[2 * y]), half2_bits(a[2 * y + 1]), half2_bits(b[2 * y + 1])};
+              mma_f16(c, x, q_hi[2 * k + y]);
+              if constexpr (kSplit) mma_f16(c, x, q_lo[2 * k + y]);
+            }
           }
         }
+        // ---- softmax: c[2y + z] is cache row 8y + perm8(g), query row 2t + z ----
+        if (tail) {
 #pragma unroll
-        for (int i = 0; i < (int)kUnit / 4; ++i) top[h] = fmaxf(top[h], s[h][i]);
-        top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 1));
-        top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 2));
-      }
-      if (__any_sync(~0u, top[0] > m[0] || top[1] > m[1])) {
-        const float f0 = m[0] == top[0] ? 1.f : exp2f(m[0] - top[0]), f1 = m[1] == top[1] ? 1.f : exp2f(m[1] - top[1]);
-        l[0] *= f0, l[1] *= f1;
-        m[0] = top[0], m[1] = top[1];
-#pragma unroll
-        for (int j = 0; j < D / 8; ++j) {
-          o[j][0] *= f0, o[j][1] *= f0;
-          o[j][2] *= kSplit ? f0 : f1, o[j][3] *= kSplit ? f0 : f1;
+          for (int y = 0; y < 2; ++y) {
+            const uint32_t r = first + 8 * y + perm8(g);
+            if (r >= seen0) c[2 * y] = -INFINITY;
+            if (r >= seen1) c[2 * y + 1] = -INFINITY;
+          }
         }
-      }
-      uint32_t pa[kUnit / 16][4];
+        float top0 = fmaxf(c[0], c[2]) * f0, top1 = fmaxf(c[1], c[3]) * f1;
+        if (__any_sync(~0u, top0 > m0 || top1 > m1)) {   // few raise a maximum
 #pragma unroll
-      for (int h = 0; h < (kSplit ? 1 : 2); ++h) {
-        const float base = kPScale - (m[h] == -INFINITY ? 0.f : m[h]);
+          for (int x = 4; x < 32; x <<= 1) {
+            top0 = fmaxf(top0, __shfl_xor_sync(~0u, top0, x));
+            top1 = fmaxf(top1, __shfl_xor_sync(~0u, top1, x));
+          }
+          top0 = fmaxf(top0, m0), top1 = fmaxf(top1, m1);
+          const float r0 = top0 == m0 ? 1.f : exp2_fast(m0 - top0), r1 = top1 == m1 ? 1.f : exp2_fast(m1 - top1);
+          m0 = top0, m1 = top1;
+          l0 *= r0, l1 *= r1;
 #pragma unroll
-        for (int i = 0; i < (int)kUnit / 4; ++i) {
-          s[h][i] = exp2f(s[h][i] + base);
-          l[h] += s[h][i];
+          for (int j = 0; j < kSteps; ++j) o[j][0] *= r0, o[j][1] *= r1, o[j][2] *= r0, o[j][3] *= r1;
         }
+        const float base0 = kPScale - (m0 == -INFINITY ? 0.f : m0), base1 = kPScale - (m1 == -INFINITY ? 0.f : m1);
+        uint32_t p_hi[2], p_lo[2];
 #pragma unroll
-        for (int i = 0; i < (int)kUnit / 8; ++i) {
-          if constexpr (kSplit) split2(s[0][2 * i], s[0][2 * i + 1], pa[i / 2][i % 2 * 2], pa[i / 2][i % 2 * 2 + 1]);
-          else pa[i / 2][i % 2 * 2 + h] = half2_bits(__floats2half2_rn(s[h][2 * i], s[h][2 * i + 1]));
+        for (int y = 0; y < 2; ++y) {
+          const float x0 = exp2_fast(fmaf(c[2 * y], f0, base0)), x1 = exp2_fast(fmaf(c[2 * y + 1], f1, base1));
+          l0 += x0, l1 += x1;
+          if constexpr (kSplit) {
+            split2(x0, x1, p_hi[y], p_lo[y]);
+            p_lo[y] = transpose8(p_lo[y]);
+          } else {
+            p_hi[y] = half2_bits(__floats2half2_rn(x0, x1));
+          }
+          p_hi[y] = transpose8(p_hi[y]);
         }
-      }
-      // ---- values: lane t's rows are its score columns; its channels [g*D/8, (g+1)*D/8), n-tile j the j-th ----
-#pragma unroll
-      for (int k = 0; k < (int)kUnit / 16; ++k) {
+        // ---- values: m-tile j is channels g*D/8 + 2j (row g) and the next (row g + 8) ----
         uint32_t w[4][D / 64];
         __half d[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t r = 16 * k + i / 2 * 8 + (i % 2 ? 4 + (t ^ 1) : t);
-          const uint8_t *b = st + S::kCodes + r * (D / 2) + g * (D / 16);
+        for (int y = 0; y < 4; ++y) {
+          const uint32_t r = y / 2 * 8 + v_row[y % 2];
+          const uint8_t *b = st + v_codes + r * (D / 2);
           if constexpr (D == 128) {
             const uint2 v = *(const uint2 *)b;
-            w[i][0] = v.x, w[i][1] = v.y;
+            w[y][0] = v.x, w[y][1] = v.y;
           } else {
-            w[i][0] = *(const uint32_t *)b;
+            w[y][0] = *(const uint32_t *)b;
           }
-          d[i] = *(const __half *)(st + 2 * S::kCodes + S::kScales + r * (D / 16) + g * (D / 8) / 32 * 2);
-          if (tail && first + r >= held) d[i] = __half(0.f);   // bytes past the rows held may be anything
+          d[y] = *(const __half *)(sc + v_scale + r * (D / 16));
+          if (tail && first + r >= held) d[y] = __half(0.f);   // bytes past the rows held may be anything
         }
         const __half2 da = __halves2half2(d[0], d[1]), db = __halves2half2(d[2], d[3]);
         const __half2 da72 = minus72(da), db72 = minus72(db);
 #pragma unroll
         for (int j = 0; j < D / 64; ++j) {
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {   // channels 0-3, 4-7 of the word
-            const uint32_t sel = x ? 0x7632 : 0x5410;
+          for (int y = 0; y < 2; ++y) {   // channels 0-3, 4-7 of the word
+            const uint32_t sel = y ? 0x7632 : 0x5410;
             __half2 a[4], b[4];
             unpack8(__byte_perm(w[0][j], w[1][j], sel), da, da72, a);
             unpack8(__byte_perm(w[2][j], w[3][j], sel), db, db72, b);
 #pragma unroll
-            for (int y = 0; y < 4; ++y) mma_f16(o[j * 8 + x * 4 + y], pa[k], half2_bits(a[y]), half2_bits(b[y]));
+            for (int z = 0; z < 2; ++z) {
+              const uint32_t x[4] = {half2_bits(a[2 * z]), half2_bits(a[2 * z + 1]), half2_bits(b[2 * z]), half2_bits(b[2 * z + 1])};
+              mma_f16(o[j * 4 + y * 2 + z], x, p_hi);
+              if constexpr (kSplit) mma_f16(o[j * 4 + y * 2 + z], x, p_lo);
+            }
           }
         }
       }
       __syncwarp();
-      if (lane == 0) fetch_next();
+      if (ahead < seg.units) fetch(seg, ahead), ahead += kRowsWarps;
+      else if (next_ahead < next.units) fetch(next, next_ahead), next_ahead += kRowsWarps;
+      if (++stage == kRowsStages) stage = 0, parity ^= 1;
     }
 
     // ---- the warps' results meet ----
 #pragma unroll
-    for (int h = 0; h < (kSplit ? 1 : 2); ++h) {
-      l[h] += __shfl_xor_sync(~0u, l[h], 1);
-      l[h] += __shfl_xor_sync(~0u, l[h], 2);
-      if (t == 0) w_max[warp][g + 8 * h] = m[h], w_sum[warp][g + 8 * h] = l[h];
+    for (int x = 4; x < 32; x <<= 1) {
+      l0 += __shfl_xor_sync(~0u, l0, x);
+      l1 += __shfl_xor_sync(~0u, l1, x);
+    }
+    if (g == 0) {
+      *(float2 *)&w_max[warp][2 * t] = make_float2(m0, m1);
+      *(float2 *)&w_sum[warp][2 * t] = make_float2(l0, l1);
     }
     __syncthreads();
-    const uint32_t tile_rows = min(kRows, rows - row0);
-    if (threadIdx.x < kRows) {
-      float top = -INFINITY, all = 0.f;
-      for (uint32_t w = 0; w < kRowsWarps; ++w) top = fmaxf(top, w_max[w][threadIdx.x]);
-      for (uint32_t w = 0; w < kRowsWarps; ++w) {
-        const float wm = w_max[w][threadIdx.x];
-        all += w_sum[w][threadIdx.x] * (wm == -INFINITY ? 0.f : exp2f(wm - top));
+    float top0 = -INFINITY, top1 = -INFINITY;
+#pragma unroll
+    for (uint32_t w = 0; w < kRowsWarps; ++w) {
+      const float2 x = *(const float2 *)&w_max[w][2 * t];
+      top0 = fmaxf(top0, x.x), top1 = fmaxf(top1, x.y);
+    }
+    // [warp][query row][channel], 16-byte chunks of a lane's channels turned by its query rows: no bank conflicts
+    constexpr uint32_t kChunks = kLaneValues / 4;
+    {
+      const float e0 = m0 == -INFINITY ? 0.f : exp2_fast(m0 - top0), e1 = m1 == -INFINITY ? 0.f : exp2_fast(m1 - top1);
+      float4 *dst = (float4 *)(merge + (warp * kTileRows + 2 * t) * D + g * kLaneValues);
+#pragma unroll
+      for (uint32_t i = 0; i < kChunks; ++i) {
+        dst[i ^ (t % kChunks)] = make_float4(e0 * o[2 * i][0], e0 * o[2 * i][2], e0 * o[2 * i + 1][0], e0 * o[2 * i + 1][2]);
+        dst[D / 4 + (i ^ (t % kChunks))] =
+            make_float4(e1 * o[2 * i][1], e1 * o[2 * i][3], e1 * o[2 * i + 1][1], e1 * o[2 * i + 1][3]);
       }
-      f_max[threadIdx.x] = top;
-      f_sum[threadIdx.x] = all;
+    }
+    if (warp == 0 && g < 2) {   // lanes of g = 0 and 1: the denominators of rows 2t and 2t + 1
+      const float top = g ? top1 : top0;
+      float all = 0.f;
+#pragma unroll
+      for (uint32_t w = 0; w < kRowsWarps; ++w) {
+        const float wm = w_max[w][2 * t + g];
+        all += w_sum[w][2 * t + g] * (wm == -INFINITY ? 0.f : exp2_fast(wm - top));
+      }
+      f_max[2 * t + g] = top;
+      f_sum[2 * t + g] = all;
     }
     __syncthreads();
-    // partial results: this CTA's piece of a segment begun before it is slot 0, else slot 1
-    const uint32_t slot = blockIdx.x * 2 + (seg.unit == 0);
-    float *part = p.parts + (size_t)slot * kRows * (D + 2);
-    auto emit = [&](uint32_t r, uint32_t ch, float x, float sum) {   // a finished output value
+    auto place = [&](uint32_t r) {   // of a query row in out and lse
       const uint32_t tok = (row0 + r) / p.group, head = kv * p.group + (row0 + r) % p.group;
-      const size_t i = ((size_t)seg.seq * p.tokens + tok) * p.heads + head;
-      ((T *)p.out)[i * D + ch] = from_float<T>(sum == 0.f ? 0.f : x / sum);
+      return ((size_t)seg.seq * p.tokens + tok) * p.heads + head;
+    };
+    auto emit = [&](uint32_t r, uint32_t ch, float4 x, float sum) {   // finished output values
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      T y[4] = {from_float<T>(x.x * inv), from_float<T>(x.y * inv), from_float<T>(x.z * inv), from_float<T>(x.w * inv)};
+      T *dst = (T *)p.out + place(r) * D + ch;
+      if constexpr (sizeof(T) == 4) *(float4 *)dst = *(const float4 *)y;
+      else *(uint2 *)dst = *(const uint2 *)y;
     };
     auto emit_lse = [&](uint32_t r, float top, float sum) {
-      const uint32_t tok = (row0 + r) / p.group, head = kv * p.group + (row0 + r) % p.group;
-      p.lse[((size_t)seg.seq * p.tokens + tok) * p.heads + head] = sum == 0.f ? INFINITY : top + log2f(sum) - kPScale;
+      p.lse[place(r)] = sum == 0.f ? INFINITY : top + log2f(sum) - kPScale;
     };
+    float *part = p.parts + (size_t)index * kPart<D>;
+    if (threadIdx.x < tile_rows * (D / 4)) {
+      const uint32_t r = threadIdx.x / (D / 4), ch = threadIdx.x % (D / 4) * 4;
+      const float *src = merge + r * D + ch / kLaneValues * kLaneValues + (ch / 4 % kChunks ^ (r / 2 % kChunks)) * 4;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (uint32_t h = 0; h < (kSplit ? 1 : 2); ++h) {
-      if (h * 8 >= tile_rows) break;
-      const float top = f_max[g + 8 * h], f = m[h] == -INFINITY ? 0.f : exp2f(m[h] - top);
-      float *dst = merge + warp * 8 * D + lane * kLaneChannels;   // row g, channels [t*D/4, (t+1)*D/4)
-      // column 2t of n-tile j is channel 2t*D/8 + j, column 2t + 1 the one D/8 on
-#pragma unroll
-      for (int j = 0; j < D / 8; j += 4) {
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          float4 v;
-          float *e = (float *)&v;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) e[i] = f * (kSplit ? o[j + i][y] + o[j + i][y + 2] : o[j + i][y + 2 * h]);
-          const uint32_t chunk = y * (D / 32) + j / 4;
-          ((float4 *)dst)[chunk ^ (lane % (D / 16))] = v;
-        }
+      for (uint32_t w = 0; w < kRowsWarps; ++w) {
+        const float4 y = *(const float4 *)(src + w * kTileRows * D);
+        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
       }
-      __syncthreads();
-      const uint32_t n = min(8u, tile_rows - 8 * h) * D;
-      for (uint32_t e = threadIdx.x; e < n; e += kRowsThreads) {
-        const uint32_t r = e / D, ch = e % D, ln = r * 4 + ch / kLaneChannels, in = ch % kLaneChannels;
-        const uint32_t at4 = ln * kLaneChannels + (((in / 4) ^ (ln % (D / 16))) * 4 + in % 4);
-        float x = 0.f;
-#pragma unroll
-        for (uint32_t w = 0; w < kRowsWarps; ++w) x += merge[w * 8 * D + at4];
-        if (whole) emit(r + 8 * h, ch, x, f_sum[r + 8 * h]);
-        else part[(r + 8 * h) * (D + 2) + ch] = x;
-      }
-      __syncthreads();
+      if (whole) emit(r, ch, x, f_sum[r]);
+      else *(float4 *)(part + r * D + ch) = x;
     }
     if (threadIdx.x < tile_rows) {
-      if (whole) {
-        if (p.lse) emit_lse(threadIdx.x, f_max[threadIdx.x], f_sum[threadIdx.x]);
-      } else {
-        part[threadIdx.x * (D + 2) + D] = f_max[threadIdx.x];
-        part[threadIdx.x * (D + 2) + D + 1] = f_sum[threadIdx.x];
+      if (!whole) {
+        part[kTileRows * D + threadIdx.x] = f_max[threadIdx.x];
+        part[kTileRows * (D + 1) + threadIdx.x] = f_sum[threadIdx.x];
+      } else if (p.lse) {
+        emit_lse(threadIdx.x, f_max[threadIdx.x], f_sum[threadIdx.x]);
       }
     }
+    __syncthreads();
     if (!whole) {
-      // CTAs that share the segment: those that hold its first and its last unit, and all between
-      const uint64_t seg_first = at - seg.unit, seg_last = seg_first + seg.units - 1;
-      const uint32_t c0 = (uint32_t)(((seg_first + 1) * ctas - 1) / total);
-      const uint32_t c1 = (uint32_t)(((seg_last + 1) * ctas - 1) / total);
-      const uint32_t pieces = c1 - c0 + 1;
-      uint32_t *ticket = p.tickets + c0;   // a CTA begins at most one segment that others finish
-      __syncthreads();
+      const uint32_t pieces = seg.parts;
+      const float *others = p.parts + (size_t)(index - seg.part) * kPart<D>;
+      uint32_t *ticket = p.tickets + seg.seq * plan.lanes + seg.lane;
       if (threadIdx.x == 0) last = atomic_add_acq_rel(ticket, 1u) == pieces - 1;
       __syncthreads();
       if (last) {
         if (threadIdx.x == 0) *ticket = 0;
-        float *weight = merge;   // [pieces][kRows]: at most 148 * 16 floats
-        auto piece = [&](uint32_t i) { return p.parts + (size_t)((c0 + i) * 2 + (i == 0)) * kRows * (D + 2); };
-        for (uint32_t i = threadIdx.x; i < pieces * tile_rows; i += kRowsThreads)
-          weight[i] = __ldcg(piece(i / tile_rows) + i % tile_rows * (D + 2) + D);
-        __syncthreads();
-        if (threadIdx.x < tile_rows) {
-          const uint32_t r = threadIdx.x;
+        float *weight = merge;   // [pieces][kTileRows]
+        auto piece = [&](uint32_t i) { return others + (size_t)i * kPart<D>; };
+        if (warp < tile_rows) {   // a warp a query row, its lanes the pieces
           float top = -INFINITY, all = 0.f;
-          for (uint32_t i = 0; i < pieces; ++i) top = fmaxf(top, weight[i * tile_rows + r]);
-          for (uint32_t i = 0; i < pieces; ++i) {
-            const float wm = weight[i * tile_rows + r], w = wm == -INFINITY ? 0.f : exp2f(wm - top);
-            weight[i * tile_rows + r] = w;
-            all += w * __ldcg(piece(i) + r * (D + 2) + D + 1);
+#pragma unroll 1
+          for (uint32_t i = lane; i < pieces; i += 32) {
+            const float m = __ldcg(piece(i) + kTileRows * D + warp);
+            weight[i * kTileRows + warp] = m;
+            top = fmaxf(top, m);
           }
-          f_sum[r] = all;
-          if (p.lse) emit_lse(r, top, all);
+#pragma unroll
+          for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+#pragma unroll 1
+          for (uint32_t i = lane; i < pieces; i += 32) {
+            const float m = weight[i * kTileRows + warp], sum = __ldcg(piece(i) + kTileRows * (D + 1) + warp);
+            const float w = m == -INFINITY ? 0.f : exp2_fast(m - top);
+            all += w * sum;
+            weight[i * kTileRows + warp] = w;
+          }
+#pragma unroll
+          for (int x = 16; x; x >>= 1) all += __shfl_xor_sync(~0u, all, x);
+          if (lane == 0) {
+            f_sum[warp] = all;
+            if (p.lse) emit_lse(warp, top, all);
+          }
         }
         __syncthreads();
-        for (uint32_t e = threadIdx.x; e < tile_rows * D; e += kRowsThreads) {
-          const uint32_t r = e / D, ch = e % D;
-          float x = 0.f;
-          for (uint32_t i = 0; i < pieces; ++i) x += weight[i * tile_rows + r] * __ldcg(piece(i) + r * (D + 2) + ch);
+        // threads are [share of the pieces][query row][4 channels]
+        constexpr uint32_t kItems = kTileRows * (D / 4), kShares = kRowsThreads / kItems;
+        const uint32_t item = threadIdx.x % kItems, share = threadIdx.x / kItems;
+        const uint32_t r = item / (D / 4), ch = item % (D / 4) * 4;
+        float4 *shared = (float4 *)(merge + S::kMerge / 4 - kRowsThreads * 4);   // [kShares][kItems]
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < tile_rows) {
+#pragma unroll 8
+          for (uint32_t i = share; i < pieces; i += kShares) {
+            const float w = weight[i * kTileRows + r];
+            const float4 y = __ldcg((const float4 *)(piece(i) + r * D + ch));
+            x.x = fmaf(w, y.x, x.x), x.y = fmaf(w, y.y, x.y), x.z = fmaf(w, y.z, x.z), x.w = fmaf(w, y.w, x.w);
+          }
+        }
+        shared[share * kItems + item] = x;
+        __syncthreads();
+        if (share == 0 && r < tile_rows) {
+#pragma unroll
+          for (uint32_t i = 1; i < kShares; ++i) {
+            const float4 y = shared[i * kItems + item];
+            x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+          }
           emit(r, ch, x, f_sum[r]);
         }
         __syncthreads();
       }
     }
-    advance(seg, (uint32_t)(seg_end - at));
-    at = seg_end;
+    // what of the next piece no unit of this one made room for
+    if (index + gridDim.x < plan.pieces) {
+      const uint32_t had = (seg.units + kRowsWarps - 1 - warp) / kRowsWarps;   // units that this warp took
+#pragma unroll 1
+      for (uint32_t i = had; i < kRowsStages; ++i)
+        if (next_ahead < next.units) fetch(next, next_ahead), next_ahead += kRowsWarps;
+    }
+    seg = next;
+    ahead = next_ahead;
   }
   if (timed_out && lane == 0) atomicOr(&p.c.state[0].status, kKv4Timeout);
 }
