@@ -103,7 +103,10 @@ constexpr uint32_t kRowsThreads = kRowsWarps * 32;
 constexpr uint32_t kRowsCtas = 148;   // one per SM
 constexpr uint32_t kLeastUnits = 16;  // of a piece: one round of the warps
 constexpr uint32_t kMostTickets = 1u << 14;   // segments that may be cut
-constexpr float kPScale = 14.f;       // P is held times 2^14: fp16's smallest numbers then lie 2^38 below the largest
+// P is held times 2^6 relative to a maximum that is only raised once a score passes it by 2^8: raising costs as much as
+// a quarter of a step and a new maximum, however small its lead, is common. P stays below 2^14, and fp16's smallest
+// numbers lie 2^30 below a weight of 1.
+constexpr float kPScale = 6.f, kLead = 8.f;
 
 template <int D>
 constexpr uint32_t kPart = kTileRows * (D + 2);   // floats of a partial result: values, maxima, denominators
@@ -364,7 +367,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
           }
         }
         float top0 = fmaxf(c[0], c[2]) * f0, top1 = fmaxf(c[1], c[3]) * f1;
-        if (__any_sync(~0u, top0 > m0 || top1 > m1)) {   // few raise a maximum
+        if (__any_sync(~0u, top0 > m0 + kLead || top1 > m1 + kLead)) {
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) {
             top0 = fmaxf(top0, __shfl_xor_sync(~0u, top0, x));
