@@ -9,6 +9,7 @@
 #include "../../include/voxgen_cuda.h"
 #include "kv4_rows.cuh"
 #include "kv4_rows_attention.cuh"
+#include "kv4_tile_attention.cuh"
 #include "kv4_weights.cuh"
 #include "verify_kernel.cuh"
 
@@ -105,7 +106,13 @@ uint64_t segments_of(const vg_kv4_cache *c, uint32_t heads, uint32_t tokens) {
   const uint64_t rows = (uint64_t)tokens * (heads / c->kv_heads);
   return (rows + kTileRows - 1) / kTileRows * c->kv_heads * c->seqs;
 }
+// Query rows of a (sequence, KV head) from which on the 128-row kernel is taken.
+constexpr uint64_t kTileFrom = 17;
+bool tiled(const vg_kv4_cache *c, uint32_t heads, uint32_t tokens) {
+  return (uint64_t)tokens * (heads / c->kv_heads) >= kTileFrom;
+}
 uint64_t part_bytes(const vg_kv4_cache *c, uint32_t heads, uint32_t tokens) {
+  if (tiled(c, heads, tokens)) return (uint64_t)2 * kTileCtas * 2 * kTileM * (c->head_dim + 2) * 4;
   return most_pieces(segments_of(c, heads, tokens)) * kTileRows * (c->head_dim + 2) * 4;
 }
 
@@ -218,7 +225,9 @@ int vg_k_kv4_attention(const vg_kv4_cache *cache, const void *q, int dtype, uint
   p.heads = heads;
   p.group = heads / cache->kv_heads;
   p.scale = scale * 1.44269504088896340736f;
-  p.row_tiles = (tokens * p.group + kTileRows - 1) / kTileRows;
+  const bool tile = tiled(cache, heads, tokens);
+  const uint32_t block = !tile ? kTileRows : size == 4 ? kTileM : 2 * kTileM;   // query rows that a CTA takes at a time
+  p.row_tiles = (tokens * p.group + block - 1) / block;
   const uint64_t blocks = ((uint64_t)cache->capacity + kWeightWarps - 1) / kWeightWarps * cache->seqs * cache->kv_heads;
   if (track && blocks > kMaxGrid) return VG_ERANGE;
   const cudaStream_t st = (cudaStream_t)cuda_stream;
@@ -226,11 +235,18 @@ int vg_k_kv4_attention(const vg_kv4_cache *cache, const void *q, int dtype, uint
     return by_type(dtype, [&](auto t) {
       using T = decltype(t);
       constexpr int D = decltype(d)::value;
-      const auto fn = kv4_rows_kernel<D, T>;
-      static std::atomic<uint64_t> done{0};
-      const int e = allow_smem((const void *)fn, RowsSmem<D>::kBytes, done);
-      if (e) return e;
-      fn<<<kRowsCtas, kRowsThreads, RowsSmem<D>::kBytes, st>>>(p);
+      static std::atomic<uint64_t> done[2];
+      if (tile) {
+        const auto fn = kv4_tile_kernel<D, T>;
+        const int e = allow_smem((const void *)fn, TileSmem<D>::kBytes, done[0]);
+        if (e) return e;
+        fn<<<kTileCtas, kTileThreads, TileSmem<D>::kBytes, st>>>(p);
+      } else {
+        const auto fn = kv4_rows_kernel<D, T>;
+        const int e = allow_smem((const void *)fn, RowsSmem<D>::kBytes, done[1]);
+        if (e) return e;
+        fn<<<kRowsCtas, kRowsThreads, RowsSmem<D>::kBytes, st>>>(p);
+      }
       if (track) kv4_weights_kernel<D, T><<<(uint32_t)blocks, kWeightWarps * 32, 0, st>>>(p);
       return launched();
     });
