@@ -228,7 +228,7 @@ int vg_k_kv4_attention(const vg_kv4_cache *cache, const void *q, int dtype, uint
   const bool tile = tiled(cache, heads, tokens);
   const uint32_t block = !tile ? kTileRows : size == 4 ? kTileM : 2 * kTileM;   // query rows that a CTA takes at a time
   p.row_tiles = (tokens * p.group + block - 1) / block;
-  const uint64_t blocks = ((uint64_t)cache->capacity + kWeightWarps - 1) / kWeightWarps * cache->seqs * cache->kv_heads;
+  const uint64_t blocks = ((uint64_t)cache->capacity + kWeightRows - 1) / kWeightRows * cache->seqs * cache->kv_heads;
   if (track && blocks > kMaxGrid) return VG_ERANGE;
   const cudaStream_t st = (cudaStream_t)cuda_stream;
   return by_dim(cache->head_dim, [&](auto d) {
@@ -247,7 +247,7 @@ int vg_k_kv4_attention(const vg_kv4_cache *cache, const void *q, int dtype, uint
         if (e) return e;
         fn<<<kRowsCtas, kRowsThreads, RowsSmem<D>::kBytes, st>>>(p);
       }
-      if (track) kv4_weights_kernel<D, T><<<(uint32_t)blocks, kWeightWarps * 32, 0, st>>>(p);
+      if (track) kv4_weights_kernel<D, T><<<(uint32_t)blocks, kWeightThreads, kWeightSmem<D, T>, st>>>(p);
       return launched();
     });
   });

@@ -1,49 +1,116 @@
-// The attention that cache rows draw.
+// The attention that cache rows draw: weights[row] += the sum, over a call's query
+// rows, of exp2(score - log2 of the row's softmax denominator).
+//
+// The denominators come from the attention kernel before it; the scores are
+// computed again, which needs the K codes once more (72 bytes a row, from L2
+// after a decode step) and no room for P. A warp unpacks 32 cache rows to MMA A
+// operands that stay in its registers, and the query rows pass by as B fragments
+// in shared memory, 64 at a time. Every row is summed by one warp in a fixed
+// order and written by one lane.
 #pragma once
 #include "kv4_rows_attention.cuh"
 
 namespace vg {
 
-constexpr uint32_t kWeightWarps = 8;
+constexpr uint32_t kWeightWarps = 8, kWeightThreads = kWeightWarps * 32;
+constexpr uint32_t kWeightRows = kWeightWarps * 32;   // cache rows of a block
+constexpr uint32_t kWeightTiles = 8;                  // of 8 query rows, in shared memory at a time
 
-template <int D>
-__device__ __forceinline__ void row_values(const uint8_t *run, uint32_t row, int v, uint32_t lane, float (&x)[D / 32]) {
-  constexpr int N = D / 32;  // channels of a lane
-  const uint8_t *b = run + Kv4<D>::codes(row, v) + lane * N / 2;
-  uint32_t w = N == 4 ? *(const uint16_t *)b : *b;
-  const float d = __half2float(*(const __half *)(run + Kv4<D>::scales(row, v) + lane * N / 32 * 2));
-#pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = (float)((int)(w >> (4 * i) & 15) - 8) * d;
-}
-
-// weights[row] += the attention that the call's query rows gave to the row: one
-// warp per cache row, recomputing its scores.
 template <int D, typename T>
-__global__ void __launch_bounds__(kWeightWarps * 32) kv4_weights_kernel(const Kv4AttnParams p) {
-  constexpr int N = D / 32;
-  const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const uint32_t blocks = (p.c.capacity + kWeightWarps - 1) / kWeightWarps;
-  const uint32_t lane_row = blockIdx.x / blocks, seq = lane_row / p.c.kv_heads, kv = lane_row % p.c.kv_heads;
-  const uint32_t row = blockIdx.x % blocks * kWeightWarps + warp;
-  if (row >= p.c.capacity || row >= kv4_held(p.c, seq)) return;
-  const uint32_t held = kv4_held(p.c, seq);
-  const int32_t count = kv4_count(p, seq);
-  float k[N], sum = 0.f;
-  row_values<D>(p.c.data + (size_t)lane_row * p.c.tiles * Kv4<D>::kTileBytes, row, 0, lane, k);
-  for (uint32_t t = 0; t < p.tokens; ++t) {
-    if ((int32_t)t >= count || (int64_t)row > (int64_t)held - count + t) continue;
-    for (uint32_t g = 0; g < p.group; ++g) {
-      const uint32_t head = kv * p.group + g;
-      const T *q = (const T *)p.q + (int64_t)seq * p.qs.seq + (int64_t)t * p.qs.token + (int64_t)head * p.qs.head + lane * N;
-      float s = 0.f;
+constexpr uint32_t kWeightSmem = kWeightTiles * (D / 16) * 32 * 2 * 4 * (sizeof(T) == 4 ? 2 : 1);
+
+template <int D, typename T>
+__global__ void __launch_bounds__(kWeightThreads) kv4_weights_kernel(const Kv4AttnParams p) {
+  constexpr bool kSplit = sizeof(T) == 4;
+  constexpr int kSteps = D / 16;
+  constexpr uint32_t kFrag = kSteps * 32 * 2 * (kSplit ? 2 : 1);   // words of a tile's fragments
+  extern __shared__ __align__(16) uint32_t frags[];
+  __shared__ float factors[kWeightTiles * 8], denominators[kWeightTiles * 8];
+  __shared__ uint32_t seens[kWeightTiles * 8];
+  const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
+  const uint32_t blocks = (p.c.capacity + kWeightRows - 1) / kWeightRows;
+  const uint32_t lane_row = blockIdx.x / blocks, seq = lane_row / p.c.kv_heads, kv = lane_row - seq * p.c.kv_heads;
+  const uint32_t held = kv4_held(p.c, seq), block_row = (blockIdx.x - lane_row * blocks) * kWeightRows;
+  if (block_row >= held) return;
+  const uint32_t row0 = block_row + warp * 32, rows = p.tokens * p.group;
+  const uint8_t *run = p.c.data + (size_t)lane_row * p.c.tiles * Kv4<D>::kTileBytes;
+  // ---- K rows row0 + {g, 8 + g, 16 + g, 24 + g} as A fragments ----
+  uint32_t a[2][kSteps][4];
 #pragma unroll
-      for (int i = 0; i < N; ++i) s += (float)q[i] * p.scale * k[i];
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t row = row0 + 8 * i + g;
+    uint32_t w[kSteps / 2] = {};
+    __half2 d = __half2half2(__half(0.f));
+    if (row < held) {
+      const uint8_t *b = run + Kv4<D>::codes(row, 0) + t * (D / 8);
+      if constexpr (D == 128) {
+        const uint4 v = *(const uint4 *)b;
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+      } else {
+        const uint2 v = *(const uint2 *)b;
+        w[0] = v.x, w[1] = v.y;
+      }
+      d = __half2half2(*(const __half *)(run + Kv4<D>::scales(row, 0) + t * (D / 4) / 32 * 2));
+    }
+    const __half2 d72 = minus72(d);
 #pragma unroll
-      for (int b = 16; b; b >>= 1) s += __shfl_xor_sync(~0u, s, b);
-      sum += exp2f(s - p.lse[((size_t)seq * p.tokens + t) * p.heads + head]);
+    for (int k = 0; k < kSteps / 2; ++k) {
+      __half2 h[4];
+      unpack8(w[k], d, d72, h);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) a[i / 2][2 * k + y / 2][y % 2 * 2 + i % 2] = half2_bits(h[y]);
     }
   }
-  if (lane == 0) p.c.weights[(size_t)lane_row * p.c.capacity + row] += sum;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  const uint32_t last_seen = held;   // rows past what every query sees are cut by `seens`
+  for (uint32_t base = 0; base < rows; base += kWeightTiles * 8) {
+    __syncthreads();
+    const uint32_t n = min(kWeightTiles * 8, rows - base), tiles = (n + 7) / 8;
+    for (uint32_t i = warp; i < tiles * 8; i += kWeightWarps) {
+      query_fragment<D, T>(p, seq, kv, base + i, i % 8, held, frags + i / 8 * kFrag, &factors[i], &seens[i]);
+      if (lane == 0) {
+        const uint32_t r = base + i, tok = r / p.group;
+        denominators[i] = r < rows ? p.lse[((size_t)seq * p.tokens + tok) * p.heads + kv * p.group + r - tok * p.group] : INFINITY;
+      }
+    }
+    __syncthreads();
+    if (row0 >= last_seen) continue;
+#pragma unroll 1
+    for (uint32_t j = 0; j < tiles; ++j) {
+      const uint32_t *f = frags + j * kFrag;
+      float c[2][4] = {};
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        uint32_t b[2];
+        *(uint2 *)b = *(const uint2 *)(f + (k * 32 + lane) * 2);
+        mma_f16(c[0], a[0][k], b);
+        mma_f16(c[1], a[1][k], b);
+        if constexpr (kSplit) {
+          *(uint2 *)b = *(const uint2 *)(f + ((kSteps + k) * 32 + lane) * 2);
+          mma_f16(c[0], a[0][k], b);
+          mma_f16(c[1], a[1][k], b);
+        }
+      }
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {   // query rows 8j + 2t + z
+        const uint32_t q = j * 8 + 2 * t + z;
+        const float scale = factors[q], minus = denominators[q];
+        const uint32_t seen = seens[q];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = exp2_fast(fmaf(c[i / 2][i % 2 * 2 + z], scale, -minus));
+          sum[i] += row0 + 8 * i + g < seen ? e : 0.f;
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    sum[i] += __shfl_xor_sync(~0u, sum[i], 1);
+    sum[i] += __shfl_xor_sync(~0u, sum[i], 2);
+    const uint32_t row = row0 + 8 * i + g;
+    if (t == 0 && row < held) p.c.weights[(size_t)lane_row * p.c.capacity + row] += sum[i];
+  }
 }
 
 }  // namespace vg
