@@ -220,6 +220,7 @@ int vg_k_kv4_attention(const vg_kv4_cache *cache, const void *q, int dtype, uint
   p.parts = (float *)(ws + kTicketBytes);
   p.lse = track ? (float *)(ws + kTicketBytes + part_bytes(cache, heads, tokens)) : nullptr;
   p.qs = strides_of(q_strides, tokens, heads, cache->head_dim);
+  p.wide = wide(q, p.qs, size);
   p.counts = counts;
   p.tokens = tokens;
   p.heads = heads;

@@ -47,6 +47,7 @@ struct Kv4AttnParams {
   const int32_t *counts;    // new tokens of each sequence, may be null
   uint32_t tokens, heads, group;
   float scale;              // of the scores, times log2(e)
+  uint32_t wide;            // 16-byte loads of q are aligned
   uint32_t row_tiles;       // tiles of a (sequence, KV head)'s query rows
   uint32_t *tickets;        // [segments], zero between calls
   float *parts;             // [pieces] partial results

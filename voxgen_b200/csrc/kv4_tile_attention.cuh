@@ -21,25 +21,29 @@
 // columns come out in it.
 //
 // The roles. Two softmax warpgroups, each with its own S and O in tensor memory
-// (4 x 128 columns), one warp that issues the products, three that unpack. With
-// more than 128 rows of 16-bit queries the groups hold two query tiles, and an
-// unpacked tile serves 256 rows; otherwise they take every other cache tile of
-// one query tile and their results are added at the end. The products of one
-// group run while the other does its softmax. Bound: at head_dim 128 a tile's two
-// products take as long as its 16,384 exponentials; unpacking hides behind both.
+// (4 x 128 columns), a warpgroup that unpacks, and one warp that issues the
+// products. With more than 128 rows of 16-bit queries the groups hold two query
+// tiles, and an unpacked tile serves 256 rows; otherwise they take every other
+// cache tile of one query tile and their results are added at the end. The
+// products of one group run while the other does its softmax.
 //
-// The split. Units of 128 cache rows, of all (sequence, query rows, KV head)
-// segments in order, are dealt out evenly to one CTA per SM. A segment that spans
-// CTAs leaves a partial result per CTA; the CTA that finishes last (a counter,
-// left at zero) adds them in order.
+// The split. A segment is a block of query rows of a (sequence, KV head) with the
+// cache rows it sees, in units of 128. Few segments are cut into pieces of equal
+// size, about one for each CTA, since changing segments costs several units; many
+// are dealt out evenly to one CTA per SM, in order, unit by unit. A segment that
+// is cut leaves partial results; the CTA that finishes it last (a counter, left
+// at zero) adds them in order.
 #pragma once
 #include "kv4_rows_attention.cuh"
 
 namespace vg {
 
 constexpr uint32_t kTileM = 128, kTileN = 128;
-constexpr uint32_t kTileThreads = 384;          // 8 softmax warps, 1 of products, 3 that unpack
-constexpr uint32_t kUnpackThreads = 96;
+constexpr uint32_t kTileThreads = 512;          // 8 softmax warps, 4 that unpack, 1 of products, 3 idle
+constexpr uint32_t kUnpackThreads = 128;
+// registers of a thread: 512 x 128 at launch, then 2 x 176 + 2 x 80 for the four warpgroups
+constexpr uint32_t kSoftmaxRegs = 176, kOtherRegs = 80;
+constexpr uint32_t kSwitchUnits = 8;            // what changing segments costs, in units
 constexpr uint32_t kTileCtas = 148;
 constexpr uint32_t kRawStages = 3;
 constexpr float kTilePScale = 6.f;              // as kPScale: P below 2^14 with a lead of 2^8
@@ -108,6 +112,14 @@ __device__ __forceinline__ void loaded(float (&x)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+f"(x[i]));
 }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+template <uint32_t N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <uint32_t N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // Shared-memory operand descriptor: 128-byte swizzle; lbo: bytes between panels
@@ -126,6 +138,7 @@ constexpr uint32_t tile_idesc(uint32_t n, bool b_mn) {
 struct TileWork {
   uint32_t seq, block, kv;
   uint32_t first, units, seg_units;   // cache tiles of this piece, and of its segment
+  uint32_t at;                        // place of its first unit, or its number among the pieces
 };
 template <uint32_t kRows>
 __device__ __forceinline__ uint32_t tile_units(const Kv4AttnParams &p, uint32_t seq, uint32_t block) {
@@ -136,69 +149,211 @@ __device__ __forceinline__ uint32_t tile_units(const Kv4AttnParams &p, uint32_t 
   const int32_t seen = (int32_t)held - count + tok + 1;
   return (uint32_t)(max(seen, 1) + (int32_t)kTileN - 1) / kTileN;
 }
-// Total units, and (found) the piece that starts at unit x.
+// Every warp plans for itself, all lanes together.
 template <uint32_t kRows>
-__device__ __forceinline__ uint32_t tile_total(const Kv4AttnParams &p) {
-  uint32_t n = 0;
-#pragma unroll 1
-  for (uint32_t i = threadIdx.x % 32; i < p.c.seqs * p.row_tiles; i += 32)
-    n += tile_units<kRows>(p, i / p.row_tiles, i % p.row_tiles);
-  return __reduce_add_sync(~0u, n) * p.c.kv_heads;
-}
-template <uint32_t kRows>
-__device__ __forceinline__ TileWork tile_find(const Kv4AttnParams &p, uint32_t x) {
-  const uint32_t lane = threadIdx.x % 32, blocks = p.c.seqs * p.row_tiles;
-  uint32_t before = 0;
-#pragma unroll 1
-  for (uint32_t base = 0; base < blocks; base += 32) {
-    const uint32_t i = base + lane;
-    const uint32_t u = i < blocks ? tile_units<kRows>(p, i / p.row_tiles, i % p.row_tiles) : 0;
-    uint32_t sum = u * p.c.kv_heads;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t up = __shfl_up_sync(~0u, sum, o);
-      if (lane >= (uint32_t)o) sum += up;
-    }
-    const uint32_t past = __ballot_sync(~0u, before + sum > x);
-    if (past) {
-      const int at = __ffs(past) - 1;
-      const uint32_t units = __shfl_sync(~0u, u, at);
-      const uint32_t into = x - before - (__shfl_sync(~0u, sum, at) - units * p.c.kv_heads);
-      TileWork w;
-      w.seq = (base + at) / p.row_tiles;
-      w.block = (base + at) % p.row_tiles;
-      w.kv = into / units;
-      w.first = into - w.kv * units;
-      w.units = w.seg_units = units;
-      return w;
-    }
-    before += __shfl_sync(~0u, sum, 31);
+struct TilePlan {
+  const Kv4AttnParams &p;
+  uint32_t blocks, ctas;
+  uint32_t each, more, begin, end;   // dealt out: units of a CTA, the first `more` with one more; this CTA's
+  uint32_t size, pieces;             // cut: units of a piece (0: dealt out), pieces
+
+  __device__ uint32_t pieces_of(uint32_t i, uint32_t of) const {
+    return i < blocks ? (tile_units<kRows>(p, i / p.row_tiles, i % p.row_tiles) + of - 1) / of : 0u;
   }
-  return TileWork{0, 0, 0, 0, 1, 1};
-}
+  __device__ uint32_t sum_of(uint32_t of) const {
+    uint32_t n = 0;
+#pragma unroll 1
+    for (uint32_t i = threadIdx.x % 32; i < blocks; i += 32) n += pieces_of(i, of);
+    return __reduce_add_sync(~0u, n) * p.c.kv_heads;
+  }
+  __device__ explicit TilePlan(const Kv4AttnParams &p) : p(p), blocks(p.c.seqs * p.row_tiles), size(0), pieces(0) {
+    const uint32_t total = sum_of(1), fair = (total + kTileCtas - 1) / kTileCtas;
+    if (blocks * p.c.kv_heads * 4 <= kTileCtas * 3) {
+      uint32_t of = fair;
+#pragma unroll 1
+      for (int i = 0;; ++i) {
+        pieces = sum_of(of);
+        if (pieces <= kTileCtas || i == 3) break;
+        of = max(of + 1, (uint32_t)((uint64_t)of * pieces / kTileCtas));
+      }
+      if (of <= fair + kSwitchUnits) size = of;
+    }
+    ctas = min(gridDim.x, size ? pieces : total);
+    each = total / ctas;
+    more = total - each * ctas;
+    begin = each * blockIdx.x + min(blockIdx.x, more);
+    end = begin + each + (blockIdx.x < more);
+  }
+  __device__ uint32_t owner(uint32_t x) const {
+    return x < more * (each + 1) ? x / (each + 1) : more + (x - more * (each + 1)) / each;
+  }
+  // The segment, and what of it, in which number x of the units (of = 1) or of the pieces lies.
+  __device__ TileWork find(uint32_t x, uint32_t of) const {
+    const uint32_t lane = threadIdx.x % 32;
+    uint32_t before = 0;
+#pragma unroll 1
+    for (uint32_t base = 0; base < blocks; base += 32) {
+      const uint32_t n = pieces_of(base + lane, of);
+      uint32_t sum = n * p.c.kv_heads;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(~0u, sum, o);
+        if (lane >= (uint32_t)o) sum += up;
+      }
+      const uint32_t past = __ballot_sync(~0u, before + sum > x);
+      if (past) {
+        const int at = __ffs(past) - 1;
+        const uint32_t parts = __shfl_sync(~0u, n, at);
+        const uint32_t into = x - before - (__shfl_sync(~0u, sum, at) - parts * p.c.kv_heads);
+        TileWork w;
+        w.seq = (base + at) / p.row_tiles;
+        w.block = (base + at) % p.row_tiles;
+        w.kv = into / parts;
+        w.first = (into - w.kv * parts) * of;
+        w.seg_units = tile_units<kRows>(p, w.seq, w.block);
+        w.units = min(of, w.seg_units - w.first);
+        w.at = x;
+        return w;
+      }
+      before += __shfl_sync(~0u, sum, 31);
+    }
+    return TileWork{0, 0, 0, 0, 0, 1, x};
+  }
+  __device__ TileWork start() const {
+    if (size) return find(blockIdx.x, size);
+    TileWork w = find(begin, 1);
+    w.units = min(end - begin, w.seg_units - w.first);
+    return w;
+  }
+  // The CTA's next piece; false after the last.
+  __device__ bool advance(TileWork &w) const {
+    if (size) {
+      if (w.at + ctas >= pieces) return false;
+      w = find(w.at + ctas, size);
+      return true;
+    }
+    w.at += w.units;
+    if (w.at >= end) return false;
+    w.first = 0;
+    if (++w.kv == p.c.kv_heads) {
+      w.kv = 0;
+      if (++w.block == p.row_tiles) w.block = 0, ++w.seq;
+      w.seg_units = tile_units<kRows>(p, w.seq, w.block);
+    }
+    w.units = min(end - w.at, w.seg_units);
+    return true;
+  }
+  // Partial results of the segment: where this piece's goes, and those of its parts.
+  struct Parts {
+    uint32_t own, first, second, step, count, ticket;
+    __device__ uint32_t slot(uint32_t i) const { return i == 0 ? first : second + (i - 1) * step; }
+  };
+  __device__ Parts parts(const TileWork &w) const {
+    Parts x;
+    if (size) {
+      const uint32_t part = w.first / size;
+      x.own = w.at;
+      x.first = w.at - part;
+      x.second = x.first + 1;
+      x.step = 1;
+      x.count = (w.seg_units + size - 1) / size;
+      x.ticket = (w.seq * p.row_tiles + w.block) * p.c.kv_heads + w.kv;
+    } else {   // a CTA has at most two: of a segment begun before it, and of one that goes on after it
+      const uint32_t c0 = owner(w.at - w.first);
+      x.own = blockIdx.x * 2 + (w.first == 0);
+      x.first = c0 * 2 + 1;
+      x.second = (c0 + 1) * 2;
+      x.step = 2;
+      x.count = owner(w.at - w.first + w.seg_units - 1) - c0 + 1;
+      x.ticket = c0;
+    }
+    return x;
+  }
+};
 
 struct TileBars {
   uint64_t q_full, s_full[2], p_full[2], o_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], raw_full[kRawStages], drained;
 };
 
+// A row of shared memory in 16-byte chunks, turned by the row: a warp that writes
+// one chunk of each of 32 rows, and one that reads a whole row, meet no conflicts.
+template <uint32_t kChunks>
+__device__ __forceinline__ float4 *row_chunk(float *base, uint32_t row, uint32_t chunk) {
+  return (float4 *)base + row * kChunks + (chunk ^ (row % kChunks));
+}
+// Eight columns of O, which hold channels 0 4 1 5 2 6 3 7.
+__device__ __forceinline__ void in_order(const float *o, float4 &low, float4 &high) {
+  low = make_float4(o[0], o[2], o[4], o[6]);
+  high = make_float4(o[1], o[3], o[5], o[7]);
+}
+
 // What the softmax groups do when a piece ends: join the groups' results where
 // they shared a query tile, then finish the rows, or leave a partial result and,
-// last of the segment's CTAs, add them all. 256 threads.
-template <int D, typename T>
-__device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const TileWork &w, uint32_t at, bool pair, uint32_t x,
+// last of the segment's CTAs, add them all. O goes through Q's place in shared
+// memory, so that rows leave in whole lines. 256 threads.
+template <int D, typename T, typename Plan>
+__device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const Plan &plan, const TileWork &w, bool pair, uint32_t x,
                                              uint32_t row, uint32_t row0, float m, float l, bool mine, uint32_t o_addr,
-                                             float *shared_o, float *other_max, float *other_sum, uint32_t *last,
-                                             uint32_t c0, uint32_t c1) {
-  constexpr uint32_t kChunks = D / 4;   // 16-byte chunks of a row
+                                             float *shared_o, float *other_max, float *other_sum, uint32_t *last) {
   const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, rows = p.tokens * p.group;
   const uint32_t block_rows = min(pair ? 2 * kTileM : kTileM, rows - row0);
   const bool whole = w.units == w.seg_units;
-  float w0 = 1.f, w1 = 0.f;
+  const typename Plan::Parts parts = plan.parts(w);
+  auto place = [&](uint32_t i) {
+    const uint32_t tok = (row0 + i) / p.group, head = w.kv * p.group + (row0 + i) - tok * p.group;
+    return ((size_t)w.seq * p.tokens + tok) * p.heads + head;
+  };
+  auto lse = [&](float top, float sum) { return sum == 0.f ? INFINITY : top + log2f(sum) - kTilePScale; };
+  auto slot = [&](uint32_t i) { return p.parts + (size_t)i * kTilePart<D>; };
+  float *part = slot(parts.own);
+  // 4 channels of row r, final or partial
+  auto leave = [&](uint32_t r, uint32_t ch, float4 v) {
+    if (whole) {
+      T y[4] = {from_float<T>(v.x), from_float<T>(v.y), from_float<T>(v.z), from_float<T>(v.w)};
+      T *dst = (T *)p.out + place(r) * D + ch;
+      if constexpr (sizeof(T) == 4) *(float4 *)dst = *(const float4 *)y;
+      else *(uint2 *)dst = *(const uint2 *)y;
+    } else {
+      *(float4 *)(part + r * D + ch) = v;
+    }
+  };
+  auto leave_sums = [&](uint32_t r) {
+    if (!whole) {
+      part[2 * kTileM * D + r] = m;
+      part[2 * kTileM * (D + 1) + r] = l;
+    } else if (p.lse) {
+      p.lse[place(r)] = lse(m, l);
+    }
+  };
   if (!pair) {
+    constexpr uint32_t kChunks = D / 4;
+    float w0 = 1.f, w1 = 0.f;
     if (x == 1) {
       other_max[row] = mine ? m : -INFINITY;
       other_sum[row] = mine ? l : 0.f;
-      if (mine) {
+    }
+    named_bar(2, 256);
+    {
+      const float om = x == 0 ? other_max[row] : m;
+      if (x == 0) {
+        const float top = fmaxf(m, om);
+        w0 = m == -INFINITY ? 0.f : exp2_fast(m - top);
+        w1 = om == -INFINITY ? 0.f : exp2_fast(om - top);
+        l = l * w0 + other_sum[row] * w1;
+        m = top;
+        const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+        w0 *= inv;
+        w1 *= inv;
+        other_max[row] = w1;   // for the other group
+      }
+    }
+    named_bar(2, 256);
+    // group 1 scales and writes its O, group 0 adds its own
+#pragma unroll 1
+    for (uint32_t turn = 0; turn < 2; ++turn) {
+      if (turn == 0 ? x == 1 && mine : x == 0) {
+        const float f = turn ? w0 : other_max[row];
+        const bool add = turn && w.units > 1;
 #pragma unroll 1
         for (uint32_t c = 0; c < D; c += 32) {
           float o[32];
@@ -206,99 +361,128 @@ __device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const TileW
           tmem_wait_load();
           loaded(o);
 #pragma unroll
-          for (uint32_t i = 0; i < 8; ++i)
-            ((float4 *)shared_o)[row * kChunks + ((c / 4 + i) ^ (row % kChunks))] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          for (uint32_t i = 0; i < 32; i += 8) {
+            float4 v[2];
+            in_order(o + i, v[0], v[1]);
+#pragma unroll
+            for (uint32_t k = 0; k < 2; ++k) {
+              float4 *at = row_chunk<kChunks>(shared_o, row, (c + i) / 4 + k);
+              float4 y = add ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
+              // 0 times what an idle or empty group left is not taken
+              if (f != 0.f) y.x = fmaf(v[k].x, f, y.x), y.y = fmaf(v[k].y, f, y.y), y.z = fmaf(v[k].z, f, y.z), y.w = fmaf(v[k].w, f, y.w);
+              *at = y;
+            }
+          }
         }
       }
+      named_bar(2, 256);
     }
-    named_bar(2, 256);
-    if (x == 0) {
-      const float om = other_max[row], top = fmaxf(m, om);
-      w0 = m == -INFINITY ? 0.f : exp2_fast(m - top);
-      w1 = om == -INFINITY ? 0.f : exp2_fast(om - top);
-      l = l * w0 + other_sum[row] * w1;
-      m = top;
-    }
-  }
-  const uint32_t r = pair ? x * kTileM + row : row;   // row of the block
-  const bool writer = (pair || x == 0) && r < block_rows;
-  auto place = [&](uint32_t i) {
-    const uint32_t tok = (row0 + i) / p.group, head = w.kv * p.group + (row0 + i) % p.group;
-    return ((size_t)w.seq * p.tokens + tok) * p.heads + head;
-  };
-  auto lse = [&](float top, float sum) { return sum == 0.f ? INFINITY : top + log2f(sum) - kTilePScale; };
-  auto slot = [&](uint32_t i) { return p.parts + (size_t)i * kTilePart<D>; };
-  float *part = slot(blockIdx.x * 2 + (w.first == 0));
-  const bool joined = !pair && w.units > 1;           // group 1 had a tile
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (pair || x == 0) {   // whole warps: the loads are collective
+    constexpr uint32_t kPer = 32 / kChunks;   // rows of a warp's pass
+#pragma unroll 4
+    for (uint32_t r = warp * kPer + lane / kChunks; r < block_rows; r += 8 * kPer)
+      leave(r, lane % kChunks * 4, *row_chunk<kChunks>(shared_o, r, lane % kChunks));
+    if (x == 0 && row < block_rows) leave_sums(row);
+  } else {
+    // each group in its half of the place, 64 channels at a time
+    constexpr uint32_t kChunks = 16;
+    float *own = shared_o + x * (kTileM * 64);
+    const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+    const uint32_t n = x * kTileM < block_rows ? min(kTileM, block_rows - x * kTileM) : 0;   // rows of this group
 #pragma unroll 1
-    for (uint32_t c = 0; c < D; c += 32) {
-      float o[32];
-      tmem_load32(o_addr + c, o);
-      tmem_wait_load();
-      loaded(o);
-      if (writer && joined) {
+    for (uint32_t c0 = 0; c0 < D; c0 += 64) {
+#pragma unroll 1
+      for (uint32_t c = 0; c < 64; c += 32) {
+        float o[32];
+        tmem_load32(o_addr + c0 + c, o);
+        tmem_wait_load();
+        loaded(o);
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) {
-          const float4 y = ((const float4 *)shared_o)[row * kChunks + ((c / 4 + i) ^ (row % kChunks))];
-          o[4 * i] = o[4 * i] * w0 + y.x * w1, o[4 * i + 1] = o[4 * i + 1] * w0 + y.y * w1;
-          o[4 * i + 2] = o[4 * i + 2] * w0 + y.z * w1, o[4 * i + 3] = o[4 * i + 3] * w0 + y.w * w1;
+        for (uint32_t i = 0; i < 32; i += 8) {
+          float4 v[2];
+          in_order(o + i, v[0], v[1]);
+#pragma unroll
+          for (uint32_t k = 0; k < 2; ++k)
+            *row_chunk<kChunks>(own, row, (c + i) / 4 + k) = make_float4(v[k].x * inv, v[k].y * inv, v[k].z * inv, v[k].w * inv);
         }
       }
-#pragma unroll
-      for (uint32_t i = 0; i < 32; i += 8) {   // columns hold channels 0 4 1 5 2 6 3 7
-        const float z[8] = {o[i], o[i + 2], o[i + 4], o[i + 6], o[i + 1], o[i + 3], o[i + 5], o[i + 7]};
-        if (writer && whole) {
-          float y[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) y[k] = z[k] * inv;
-          store8((T *)p.out + place(r) * D + c + i, y);
-        } else if (writer) {
-          store8(part + r * D + c + i, z);
-        }
-      }
-      __syncwarp();
+      named_bar(3 + x, kTileM);
+#pragma unroll 4
+      for (uint32_t r = warp % 4 * 2 + lane / 16; r < n; r += 8)
+        leave(x * kTileM + r, c0 + lane % 16 * 4, *row_chunk<kChunks>(own, r, lane % 16));
+      named_bar(3 + x, kTileM);
     }
-    if (writer) {
-      if (!whole) {
-        part[2 * kTileM * D + r] = m;
-        part[2 * kTileM * (D + 1) + r] = l;
-      } else if (p.lse) {
-        p.lse[place(r)] = lse(m, l);
-      }
-    }
+    if (row < n) leave_sums(x * kTileM + row);
   }
   if (!whole) {
-    const uint32_t pieces = c1 - c0 + 1;
+    const uint32_t pieces = parts.count;
+    __syncwarp();
     named_bar(2, 256);
     if (threadIdx.x == 0) {
-      *last = atomic_add_acq_rel(p.tickets + c0, 1u) == pieces - 1;   // a CTA begins at most one segment that others finish
-      if (*last) p.tickets[c0] = 0;
+      *last = atomic_add_acq_rel(p.tickets + parts.ticket, 1u) == pieces - 1;
+      if (*last) p.tickets[parts.ticket] = 0;
     }
+    __syncwarp();
     named_bar(2, 256);
     if (*last) {
       constexpr uint32_t N = D / 32;
-      auto piece = [&](uint32_t i) { return (const float *)slot((c0 + i) * 2 + (i == 0)); };
+      auto piece = [&](uint32_t i) { return (const float *)slot(parts.slot(i)); };
+      constexpr uint32_t kBatch = 4;   // rows of a warp in flight; lanes are pieces, then channels
 #pragma unroll 1
-      for (uint32_t i = warp; i < block_rows; i += 8) {
-        float top = -INFINITY, sum = 0.f, y[N] = {};
-#pragma unroll 4
-        for (uint32_t k = 0; k < pieces; ++k) top = fmaxf(top, __ldcg(piece(k) + 2 * kTileM * D + i));
-#pragma unroll 4
-        for (uint32_t k = 0; k < pieces; ++k) {
-          const float pm = __ldcg(piece(k) + 2 * kTileM * D + i), pw = pm == -INFINITY ? 0.f : exp2_fast(pm - top);
-          sum += pw * __ldcg(piece(k) + 2 * kTileM * (D + 1) + i);
+      for (uint32_t i0 = warp; i0 < block_rows; i0 += 8 * kBatch) {
+        float top[kBatch], sum[kBatch], y[kBatch][N];
 #pragma unroll
-          for (uint32_t j = 0; j < N; ++j) y[j] += pw * __ldcg(piece(k) + i * D + j * 32 + lane);
+        for (uint32_t b = 0; b < kBatch; ++b) {
+          top[b] = -INFINITY, sum[b] = 0.f;
+#pragma unroll
+          for (uint32_t j = 0; j < N; ++j) y[b][j] = 0.f;
         }
-        const float f = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll 1
+        for (uint32_t k0 = 0; k0 < pieces; k0 += 32) {
+          const uint32_t n = min(32u, pieces - k0);
+          const float *own = piece(k0 + min(lane, n - 1)) + 2 * kTileM * D;
+          float pw[kBatch];
 #pragma unroll
-        for (uint32_t j = 0; j < N; ++j) ((T *)p.out)[place(i) * D + j * 32 + lane] = from_float<T>(y[j] * f);
-        if (p.lse && lane == 0) p.lse[place(i)] = lse(top, sum);
+          for (uint32_t b = 0; b < kBatch; ++b) {
+            const uint32_t i = min(i0 + 8 * b, block_rows - 1);
+            const float pm = lane < n ? __ldcg(own + i) : -INFINITY, ps = lane < n ? __ldcg(own + 2 * kTileM + i) : 0.f;
+            float up = fmaxf(pm, top[b]);
+#pragma unroll
+            for (int x = 16; x; x >>= 1) up = fmaxf(up, __shfl_xor_sync(~0u, up, x));
+            const float keep = top[b] == -INFINITY ? 0.f : exp2_fast(top[b] - up);
+            pw[b] = pm == -INFINITY ? 0.f : exp2_fast(pm - up);
+            float add = pw[b] * ps;
+#pragma unroll
+            for (int x = 16; x; x >>= 1) add += __shfl_xor_sync(~0u, add, x);
+            sum[b] = sum[b] * keep + add;
+            top[b] = up;
+#pragma unroll
+            for (uint32_t j = 0; j < N; ++j) y[b][j] *= keep;
+          }
+#pragma unroll 2
+          for (uint32_t k = 0; k < n; ++k) {
+            const float *src = piece(k0 + k) + lane;
+#pragma unroll
+            for (uint32_t b = 0; b < kBatch; ++b) {
+              const uint32_t i = min(i0 + 8 * b, block_rows - 1);
+              const float f = __shfl_sync(~0u, pw[b], k);
+#pragma unroll
+              for (uint32_t j = 0; j < N; ++j) y[b][j] += f * __ldcg(src + i * D + j * 32);
+            }
+          }
+        }
+#pragma unroll
+        for (uint32_t b = 0; b < kBatch; ++b) {
+          const uint32_t i = i0 + 8 * b;
+          if (i >= block_rows) break;
+          const float f = sum[b] == 0.f ? 0.f : 1.f / sum[b];
+#pragma unroll
+          for (uint32_t j = 0; j < N; ++j) ((T *)p.out)[place(i) * D + j * 32 + lane] = from_float<T>(y[b][j] * f);
+          if (p.lse && lane == 0) p.lse[place(i)] = lse(top[b], sum[b]);
+        }
       }
     }
   }
+  __syncwarp();
   named_bar(2, 256);   // Q's place and the shared words may change
 }
 
@@ -315,13 +499,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
   __shared__ float factors[2 * kTileM], other_max[kTileM], other_sum[kTileM];
   const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const uint32_t rows = p.tokens * p.group;
-
-  const uint32_t total = tile_total<kRows>(p);
-  const uint32_t ctas = min(gridDim.x, total);
-  if (blockIdx.x >= ctas) return;
-  const uint32_t each = total / ctas, more = total - each * ctas;   // the first `more` CTAs have one unit more
-  const uint32_t begin = each * blockIdx.x + min(blockIdx.x, more), end = begin + each + (blockIdx.x < more);
-  auto owner = [&](uint32_t x) { return x < more * (each + 1) ? x / (each + 1) : more + (x - more * (each + 1)) / each; };
+  const TilePlan<kRows> plan(p);
+  if (blockIdx.x >= plan.ctas) return;
 
   if (threadIdx.x == 0) {
     mbar_init(&bars.q_full, 256);
@@ -339,7 +518,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
     fence_mbar_init();
     aborted = 0;
   }
-  if (warp == 8) tmem_alloc512(&tmem_base);
+  if (warp == 12) tmem_alloc512(&tmem_base);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -351,31 +530,23 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
   };
   // two query tiles, or one whose cache tiles the softmax groups share
   auto paired = [&](const TileWork &w) { return !kSplit && rows - w.block * kRows > kTileM; };
-  // f(work, its place in the CTA's units) for every piece of this CTA
-  const TileWork first_work = tile_find<kRows>(p, begin);   // the whole warp takes part
+  // f(work) for every piece of this CTA; whole warps
+  const TileWork first_work = plan.start();
   auto each_work = [&](auto &&f) {
     TileWork w = first_work;
-#pragma unroll 1
-    for (uint32_t at = begin; at < end;) {
-      w.units = min(end - at, w.seg_units - w.first);
-      f(w, at);
-      at += w.units;
-      w.first = 0;
-      if (at < end && ++w.kv == p.c.kv_heads) {
-        w.kv = 0;
-        if (++w.block == p.row_tiles) w.block = 0, ++w.seq;
-        w.seg_units = tile_units<kRows>(p, w.seq, w.block);
-      }
-    }
+    do f(w);
+    while (plan.advance(w));
   };
 
-  if (warp == 8) {
+  if (warp >= 12) {
+    fewer_registers<kOtherRegs>();
     // ---------------- products ----------------
-    if (lane == 0) {
+    if (warp == 12) {
       const uint32_t q = smem_u32(smem + S::kQ), k = smem_u32(smem + S::kK), v = smem_u32(smem + S::kV);
       constexpr uint32_t kScoreDesc = tile_idesc(kTileN, false), kValueDesc = tile_idesc(D, true);
       uint32_t works = 0, tiles = 0, jobs[2] = {0, 0};   // jobs: of each group
-      each_work([&](const TileWork &w, uint32_t) {
+      each_work([&](const TileWork &w) {
+        if (lane == 0) {
         const bool pair = paired(w);
         const uint32_t n = pair ? 2 * w.units : w.units;
         wait(&bars.q_full, works++ & 1);
@@ -416,134 +587,161 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
           }
         }
         tiles += w.units;
+        }
+        __syncwarp();
       });
-      tc_commit(&bars.drained);   // tensor memory is freed after the last product, even when waits ran out
-      mbar_wait_bounded(&bars.drained, 0);
+      if (lane == 0) {
+        tc_commit(&bars.drained);   // tensor memory is freed after the last product, even when waits ran out
+        mbar_wait_bounded(&bars.drained, 0);
+      }
+      __syncwarp();
     }
-    __syncwarp();
-  } else if (warp > 8) {
+  } else if (warp >= 8) {
+    fewer_registers<kOtherRegs>();
     // ---------------- unpacking ----------------
-    const uint32_t tid = threadIdx.x - 288;
+    const uint32_t tid = threadIdx.x - 256;
     const size_t run_bytes = (size_t)p.c.tiles * Kv4<D>::kTileBytes;
-    // one thread streams the cache's 64-row tiles; a stage is refilled once all have unpacked it
+    // the first warp streams the cache's 64-row tiles; a stage is refilled once all have unpacked it
     TileWork ahead = first_work;
-    uint32_t ahead_raw = 0, ahead_at = begin, fetched = 0;   // raw: 64-row tile of the piece
-    ahead.units = min(end - ahead_at, ahead.seg_units - ahead.first);
+    uint32_t ahead_raw = 0, fetched = 0;   // raw: 64-row tile of the piece
+    bool ahead_on = true;
     auto fetch = [&]() {
-      if (ahead_at >= end || *(volatile uint32_t *)&aborted) return;
+      if (!ahead_on) return;
       const uint32_t raw = ahead.first * 2 + ahead_raw;
-      if (raw < p.c.tiles) {
-        const uint32_t st = fetched % kRawStages;
-        mbar_arrive_expect_tx(&bars.raw_full[st], S::kRawStage);
-        bulk_g2s(smem + S::kRaw + st * S::kRawStage,
-                 p.c.data + ((size_t)ahead.seq * p.c.kv_heads + ahead.kv) * run_bytes + (size_t)raw * S::kRawStage, S::kRawStage,
-                 &bars.raw_full[st]);
+      if (raw < p.c.tiles && !*(volatile uint32_t *)&aborted) {
+        if (lane == 0) {
+          const uint32_t st = fetched % kRawStages;
+          mbar_arrive_expect_tx(&bars.raw_full[st], S::kRawStage);
+          bulk_g2s(smem + S::kRaw + st * S::kRawStage,
+                   p.c.data + ((size_t)ahead.seq * p.c.kv_heads + ahead.kv) * run_bytes + (size_t)raw * S::kRawStage,
+                   S::kRawStage, &bars.raw_full[st]);
+        }
         ++fetched;
       }
       if (++ahead_raw == 2 * ahead.units) {
         ahead_raw = 0;
-        ahead_at += ahead.units;
-        ahead.first = 0;
-        if (ahead_at < end) {
-          if (++ahead.kv == p.c.kv_heads) {
-            ahead.kv = 0;
-            if (++ahead.block == p.row_tiles) ahead.block = 0, ++ahead.seq;
-            ahead.seg_units = tile_units<kRows>(p, ahead.seq, ahead.block);
-          }
-          ahead.units = min(end - ahead_at, ahead.seg_units);
-        }
+        ahead_on = plan.advance(ahead);
       }
     };
-    if (tid == 0) {
-      fetch();
-      fetch();
-      fetch();
-    }
-    __syncwarp();
-    constexpr uint32_t kQuads = D / 32;                 // threads of a row, 32 channels each
+    if (warp == 8)
+      for (uint32_t i = 0; i < kRawStages; ++i) fetch();
+    // a thread unpacks 32 channels of a row, of kPasses rows of K and as many of V
+    constexpr uint32_t kQuads = D / 32, kPassRows = kUnpackThreads / kQuads, kPasses = kKv4Tile / kPassRows;
+    const uint32_t quad = tid % kQuads, r0 = tid / kQuads;
+    // threads of the second panel write their chunks two on, which keeps a row pair's 8 threads off each other
+    const bool turn = quad & 2;
+    uint32_t off[4];
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k)
+      off[k] = quad / 2 * kPanel + r0 * 128 + ((quad % 2 * 4 | ((turn ? 2 : 0) + k & 3)) ^ (r0 & 7)) * 16;
     uint32_t tiles = 0, used = 0;
-    each_work([&](const TileWork &w, uint32_t) {
+    each_work([&](const TileWork &w) {
       const uint32_t held = kv4_held(p.c, w.seq);
 #pragma unroll 1
       for (uint32_t u = 0; u < w.units; ++u, ++tiles) {
-        const uint32_t st = tiles & 1, raw0 = (w.first + u) * 2;
-        const uint32_t have = raw0 + 1 < p.c.tiles ? 2 : 1;    // a run's last tile may have no second half
-        for (uint32_t h = 0; h < have; ++h) wait(&bars.raw_full[(used + h) % kRawStages], (used + h) / kRawStages & 1);
+        const uint32_t st = tiles & 1;
+        if (tiles >= 2) {
+          wait(&bars.k_empty[st], (tiles >> 1) - 1 & 1);
+          wait(&bars.v_empty[st], (tiles >> 1) - 1 & 1);
+        }
+        // one 64-row tile at a time, K and V, so that its stage is free for the third one after it
 #pragma unroll 1
-        for (int v = 0; v < 2; ++v) {
-          if (tiles >= 2) wait(v ? &bars.v_empty[st] : &bars.k_empty[st], (tiles >> 1) - 1 & 1);
-          uint8_t *dst = smem + (v ? S::kV : S::kK) + st * S::kOperand;
-#pragma unroll 1
-          for (uint32_t i = tid; i < kTileN * kQuads; i += kUnpackThreads) {
-            const uint32_t row = i / kQuads, quad = i % kQuads, h = row / kKv4Tile, r = row % kKv4Tile;
-            const uint8_t *src = smem + S::kRaw + (used + (h < have ? h : 0)) % kRawStages * S::kRawStage;
-            const uint4 x = *(const uint4 *)(src + Kv4<D>::codes(r, v) + quad * 16);
-            __half2 d = __half2half2(*(const __half *)(src + Kv4<D>::scales(r, v) + quad * 2));
-            if (raw0 * kKv4Tile + row >= held) d = __half2half2(__half(0.f));   // bytes past the rows held may be anything
-            const __half2 d72 = minus72(d);
-            // threads of the second panel write their chunks two on, which keeps a row pair's 8 threads off each other
-            const bool turn = quad & 2;
-            const uint32_t word[4] = {turn ? x.z : x.x, turn ? x.w : x.y, turn ? x.x : x.z, turn ? x.y : x.w};
-            uint8_t *out = dst + quad / 2 * kPanel + row * 128;
-            const uint32_t chunk = quad % 2 * 4 + (turn ? 2 : 0);
+        for (uint32_t h = 0; h < 2; ++h) {
+          const uint32_t raw = (w.first + u) * 2 + h;
+          const bool have = raw < p.c.tiles;    // a run's last unit may have no second half: it is zeros
+          const uint8_t *src = smem + S::kRaw + used % kRawStages * S::kRawStage;
+          if (have) wait(&bars.raw_full[used % kRawStages], used / kRawStages & 1);
+          uint8_t *dst = smem + S::kK + st * S::kOperand + h * (kKv4Tile * 128);
 #pragma unroll
-            for (uint32_t k = 0; k < 4; ++k) {
-              __align__(16) __half2 y[4];
-              unpack8(word[k], d, d72, y);
-              *(uint4 *)(out + (((chunk & 4) | ((chunk + k) & 3)) ^ (row & 7)) * 16) = *(const uint4 *)y;
+          for (int v = 0; v < 2; ++v) {
+            uint4 x[kPasses];
+            __half d[kPasses];
+#pragma unroll
+            for (uint32_t i = 0; i < kPasses; ++i) {
+              const uint32_t r = r0 + i * kPassRows;
+              x[i] = *(const uint4 *)(src + Kv4<D>::codes(r, v) + quad * 16);
+              d[i] = *(const __half *)(src + Kv4<D>::scales(r, v) + quad * 2);
+              if (raw * kKv4Tile + r >= held) d[i] = __half(0.f);   // bytes past the rows held may be anything
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < kPasses; ++i) {
+              const uint4 y = x[i];
+              const uint32_t word[4] = {turn ? y.z : y.x, turn ? y.w : y.y, turn ? y.x : y.z, turn ? y.y : y.w};
+              const __half2 d2 = __half2half2(d[i]), d72 = minus72(d2);
+              uint8_t *out = dst + v * (S::kV - S::kK) + i * (kPassRows * 128);
+#pragma unroll
+              for (uint32_t k = 0; k < 4; ++k) {
+                __align__(16) __half2 z[4];
+                unpack8(word[k], d2, d72, z);
+                *(uint4 *)(out + off[k]) = *(const uint4 *)z;
+              }
             }
           }
-          fence_async_smem();
-          mbar_arrive(v ? &bars.v_full[st] : &bars.k_full[st]);
+          used += have;
+          if (h == 1) {
+            fence_async_smem();
+            mbar_arrive(&bars.k_full[st]);
+            mbar_arrive(&bars.v_full[st]);
+          }
+          __syncwarp();
+          named_bar(1, kUnpackThreads);   // all have read the stage
+          if (warp == 8) fetch();
         }
-        used += have;
-        __syncwarp();
-        named_bar(1, kUnpackThreads);   // all have read the raw stages
-        if (tid == 0)
-          for (uint32_t h = 0; h < 2; ++h) fetch();
-        __syncwarp();
       }
     });
     // nothing is left in flight but after a wait that ran out
     if (tid == 0)
       for (; used < fetched; ++used) mbar_wait_bounded(&bars.raw_full[used % kRawStages], used / kRawStages & 1);
   } else {
+    more_registers<kSoftmaxRegs>();
     // ---------------- softmax ----------------
     const uint32_t x = warp / 4, row = threadIdx.x % kTileM;       // group, and its row of the tile
     const uint32_t lanes = (warp % 4) << 21;                       // this warp's lanes of tensor memory
     const uint32_t s_addr = tmem + x * 128 + lanes, o_addr = tmem + 256 + x * 128 + lanes;
     uint32_t done = 0, works = 0;   // tiles of this group, pieces in which it had some
-    each_work([&](const TileWork &w, uint32_t at) {
+    each_work([&](const TileWork &w) {
       const bool pair = paired(w);
       const uint32_t row0 = w.block * kRows, held = kv4_held(p.c, w.seq);
       const int32_t count = kv4_count(p, w.seq);
       // ---- Q to shared memory, a warp a row: two tiles, or one (as hi and lo) that both groups load half of ----
       const uint32_t q_rows = pair ? 2 * kTileM : kTileM;
+      constexpr uint32_t L = D / 8, kPer = 32 / L, kBatch = 4;   // lanes of a row, rows of a warp's pass, passes in flight
+      const uint32_t sub = lane % L, lane_row = lane / L;
 #pragma unroll 1
-      for (uint32_t r = warp; r < q_rows; r += 8) {
-        constexpr uint32_t N = D / 32;
-        float y[N];
-        uint32_t top = 0;
-        const bool on = row0 + r < rows;
-        const uint32_t tok = (row0 + r) / p.group, head = w.kv * p.group + (row0 + r) % p.group;
-        const T *src = (const T *)p.q + (int64_t)w.seq * p.qs.seq + (int64_t)tok * p.qs.token + (int64_t)head * p.qs.head + lane * N;
+      for (uint32_t r0 = warp * kPer; r0 < q_rows; r0 += 8 * kPer * kBatch) {
+        float y[kBatch][8];
 #pragma unroll
-        for (uint32_t i = 0; i < N; ++i) {
-          y[i] = on ? (float)src[i] : 0.f;
-          top = max(top, __float_as_uint(y[i]) & 0x7FFFFFFFu);
+        for (uint32_t b = 0; b < kBatch; ++b) {
+          const uint32_t r = row0 + r0 + b * 8 * kPer + lane_row;
+          const uint32_t tok = r / p.group, head = w.kv * p.group + r - tok * p.group;
+          const T *src = (const T *)p.q + (int64_t)w.seq * p.qs.seq + (int64_t)tok * p.qs.token + (int64_t)head * p.qs.head + sub * 8;
+#pragma unroll
+          for (uint32_t i = 0; i < 8; ++i) y[b][i] = 0.f;
+          if (r < rows) {
+            if (p.wide) load8<T, true>(src, y[b]);
+            else load8<T, false>(src, y[b]);
+          }
         }
-        float inverse;
-        const float power = row_power(__uint_as_float(__reduce_max_sync(~0u, top)), inverse);
-        if (lane == 0) factors[r] = fmaxf(p.scale * inverse, 0x1p-126f);
-        uint8_t *dst = smem + S::kQ + r / kTileM * S::kOperand;
 #pragma unroll
-        for (uint32_t i = 0; i < N; ++i) {
-          const uint32_t c = lane * N + i, place = c % 4 * 2 + c % 8 / 4;   // 0 4 1 5 2 6 3 7
-          const uint32_t off = c / 64 * kPanel + r % kTileM * 128 + ((c % 64 / 8) ^ (r & 7)) * 16 + place * 2;
-          const float z = y[i] * power;
-          const __half hi = __float2half_rn(z);
-          *(__half *)(dst + off) = hi;
-          if constexpr (kSplit) *(__half *)(dst + S::kOperand + off) = __float2half_rn(z - __half2float(hi));
+        for (uint32_t b = 0; b < kBatch; ++b) {
+          const uint32_t r = r0 + b * 8 * kPer + lane_row;
+          uint32_t top = 0;
+#pragma unroll
+          for (uint32_t i = 0; i < 8; ++i) top = max(top, __float_as_uint(y[b][i]) & 0x7FFFFFFFu);
+#pragma unroll
+          for (uint32_t o = 1; o < L; o <<= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
+          float inverse;
+          const float power = row_power(__uint_as_float(top), inverse);
+          if (sub == 0) factors[r] = fmaxf(p.scale * inverse, 0x1p-126f);
+          uint8_t *dst = smem + S::kQ + r / kTileM * S::kOperand + sub / 8 * kPanel + r % kTileM * 128 + ((sub % 8) ^ (r & 7)) * 16;
+          __align__(16) uint32_t hi[4], lo[4];   // channels 0 4 1 5 2 6 3 7
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i) {
+            if constexpr (kSplit) split2(y[b][i] * power, y[b][i + 4] * power, hi[i], lo[i]);
+            else hi[i] = half2_bits(__floats2half2_rn(y[b][i] * power, y[b][i + 4] * power));
+          }
+          *(uint4 *)dst = *(const uint4 *)hi;
+          if constexpr (kSplit) *(uint4 *)(dst + S::kOperand) = *(const uint4 *)lo;
         }
       }
       fence_async_smem();
@@ -628,16 +826,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
       if (mine) wait(&bars.o_full[x], works++ & 1);
       __syncwarp();
       tc_fence_after();
-      const uint32_t seg = at - w.first;
-      tile_results<D, T>(p, w, at, pair, x, row, row0, m, l, mine, o_addr, (float *)(smem + S::kQ), other_max, other_sum, &last,
-                         owner(seg), owner(seg + w.seg_units - 1));
+      tile_results<D, T>(p, plan, w, pair, x, row, row0, m, l, mine, o_addr, (float *)(smem + S::kQ), other_max, other_sum, &last);
       tc_fence_before();
     });
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) tmem_free512(tmem);
+  if (warp == 12) tmem_free512(tmem);
   if (threadIdx.x == 0 && aborted) atomicOr(&p.c.state[0].status, kKv4Timeout);
 }
 

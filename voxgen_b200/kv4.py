@@ -176,8 +176,7 @@ class Kv4Cache:
         held read as 0."""
         if dtype not in DTYPES:
             raise VoxGenError(-4, f"{dtype} is not supported")
-        shape = self.seqs, tokens, self.kv_heads, self.head_dim
-        k, v = self.data.new_empty(shape, dtype=dtype), self.data.new_empty(shape, dtype=dtype)
+        k, v = self.data.new_empty((2, self.seqs, tokens, self.kv_heads, self.head_dim), dtype=dtype).unbind()
         rc = self._lib.vg_k_kv4_read(self._ref, _ints(first, self.seqs, self.device, "first"), tokens, DTYPES[dtype],
                                      k.data_ptr(), v.data_ptr(), _stream(stream, self._index))
         if rc:
@@ -283,7 +282,7 @@ def verify_draft(tokens: torch.Tensor, draft: torch.Tensor, target: torch.Tensor
     if torch.cuda.current_device() != device.index:
         with torch.cuda.device(device):
             return verify_draft(tokens, draft, target, u_accept, u_sample, counts=counts, stream=stream)
-    accepted, token = tokens.new_empty(seqs), tokens.new_empty(seqs)
+    accepted, token = tokens.new_empty((2, seqs)).unbind()
     rc = api.lib().vg_k_verify_draft(
         tokens.data_ptr(), draft.data_ptr(), target.data_ptr(), u_accept.data_ptr(), u_sample.data_ptr(),
         _ints(counts, seqs, device, "counts"), seqs, drafted, vocab, accepted.data_ptr(), token.data_ptr(),
