@@ -41,8 +41,8 @@ namespace vg {
 constexpr uint32_t kTileM = 128, kTileN = 128;
 constexpr uint32_t kTileThreads = 512;          // 8 softmax warps, 4 that unpack, 1 of products, 3 idle
 constexpr uint32_t kUnpackThreads = 128;
-// registers of a thread: 512 x 128 at launch, then 2 x 176 + 2 x 80 for the four warpgroups
-constexpr uint32_t kSoftmaxRegs = 176, kOtherRegs = 80;
+// registers of a thread: 512 x 128 at launch, then 2 x 168 + 2 x 88 for the four warpgroups
+constexpr uint32_t kSoftmaxRegs = 168, kOtherRegs = 88;
 constexpr uint32_t kSwitchUnits = 8;            // what changing segments costs, in units
 constexpr uint32_t kTileCtas = 148;
 constexpr uint32_t kRawStages = 3;
@@ -74,16 +74,17 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 __device__ __forceinline__ void tc_commit(uint64_t *bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+// add: whether the product is added to what is there (a constant, or a predicate of the loop).
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
       : "memory");
 }
 __device__ __forceinline__ void tmem_load32(uint32_t addr, float *x) {
@@ -122,10 +123,34 @@ __device__ __forceinline__ void fewer_registers() {
 }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// Shared-memory operand descriptor: 128-byte swizzle; lbo: bytes between panels
-// (MN-major only), 8-row groups are 1024 bytes apart.
-__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lbo) {
-  return (uint64_t)(addr >> 4 & 0x3FFF) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+// Two fp32 operations in one instruction, and the largest of three.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(*(const uint64_t *)&a), "l"(*(const uint64_t *)&b), "l"(*(const uint64_t *)&c));
+  return *(const float2 *)&d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*(const uint64_t *)&a), "l"(*(const uint64_t *)&b));
+  return *(const float2 *)&d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Shared-memory operand descriptor: 128-byte swizzle; panel: bytes between panels
+// (MN-major only), 8-row groups are 1024 bytes apart. The low word holds the
+// address, so a step along the operand is one 32-bit addition to it.
+constexpr uint32_t kOperandHigh = 1024 >> 4 | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t operand_low(uint32_t addr, uint32_t panel) { return addr >> 4 | (panel >> 4) << 16; }
+__device__ __forceinline__ uint64_t operand(uint32_t low, uint32_t bytes_on) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(low + (bytes_on >> 4)), "n"(kOperandHigh));
+  return d;
 }
 // fp16 operands, fp32 accumulator, M = 128; b_mn: B is MN-major.
 constexpr uint32_t tile_idesc(uint32_t n, bool b_mn) {
@@ -272,7 +297,7 @@ struct TilePlan {
 };
 
 struct TileBars {
-  uint64_t q_full, s_full[2], p_full[2], o_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], raw_full[kRawStages], drained;
+  uint64_t q_full, s_full[2], p_half[2], p_full[2], o_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], raw_full[kRawStages], drained;
 };
 
 // A row of shared memory in 16-byte chunks, turned by the row: a warp that writes
@@ -424,7 +449,8 @@ __device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const Plan 
     __syncwarp();
     named_bar(2, 256);
     if (*last) {
-      constexpr uint32_t N = D / 32;
+      constexpr uint32_t N = D / 32;   // channels of a lane
+      using V = typename std::conditional<N == 4, float4, float2>::type;
       auto piece = [&](uint32_t i) { return (const float *)slot(parts.slot(i)); };
       constexpr uint32_t kBatch = 4;   // rows of a warp in flight; lanes are pieces, then channels
 #pragma unroll 1
@@ -460,13 +486,14 @@ __device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const Plan 
           }
 #pragma unroll 2
           for (uint32_t k = 0; k < n; ++k) {
-            const float *src = piece(k0 + k) + lane;
+            const float *src = piece(k0 + k) + lane * N;
 #pragma unroll
             for (uint32_t b = 0; b < kBatch; ++b) {
               const uint32_t i = min(i0 + 8 * b, block_rows - 1);
               const float f = __shfl_sync(~0u, pw[b], k);
+              const V z = __ldcg((const V *)(src + i * D));
 #pragma unroll
-              for (uint32_t j = 0; j < N; ++j) y[b][j] += f * __ldcg(src + i * D + j * 32);
+              for (uint32_t j = 0; j < N; ++j) y[b][j] += f * ((const float *)&z)[j];
             }
           }
         }
@@ -476,7 +503,7 @@ __device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const Plan 
           if (i >= block_rows) break;
           const float f = sum[b] == 0.f ? 0.f : 1.f / sum[b];
 #pragma unroll
-          for (uint32_t j = 0; j < N; ++j) ((T *)p.out)[place(i) * D + j * 32 + lane] = from_float<T>(y[b][j] * f);
+          for (uint32_t j = 0; j < N; ++j) ((T *)p.out)[place(i) * D + lane * N + j] = from_float<T>(y[b][j] * f);
           if (p.lse && lane == 0) p.lse[place(i)] = lse(top[b], sum[b]);
         }
       }
@@ -506,6 +533,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
     mbar_init(&bars.q_full, 256);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.s_full[i], 1);
+      mbar_init(&bars.p_half[i], kTileM);
       mbar_init(&bars.p_full[i], kTileM);
       mbar_init(&bars.o_full[i], 1);
       mbar_init(&bars.k_full[i], kUnpackThreads);
@@ -542,51 +570,58 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
     fewer_registers<kOtherRegs>();
     // ---------------- products ----------------
     if (warp == 12) {
-      const uint32_t q = smem_u32(smem + S::kQ), k = smem_u32(smem + S::kK), v = smem_u32(smem + S::kV);
+      const uint32_t q = operand_low(smem_u32(smem + S::kQ), 0), k = operand_low(smem_u32(smem + S::kK), 0);
+      const uint32_t v = operand_low(smem_u32(smem + S::kV), kPanel);
       constexpr uint32_t kScoreDesc = tile_idesc(kTileN, false), kValueDesc = tile_idesc(D, true);
-      uint32_t works = 0, tiles = 0, jobs[2] = {0, 0};   // jobs: of each group
+      constexpr uint32_t kTileOn = S::kOperand >> 4;   // from one operand to the next, in a descriptor
+      uint32_t works = 0, tiles = 0, jobs0 = 0, jobs1 = 0;   // jobs: of each group
       each_work([&](const TileWork &w) {
         if (lane == 0) {
-        const bool pair = paired(w);
-        const uint32_t n = pair ? 2 * w.units : w.units;
-        wait(&bars.q_full, works++ & 1);
-        tc_fence_after();
+          const bool pair = paired(w);
+          const uint32_t n = pair ? 2 * w.units : w.units;
+          wait(&bars.q_full, works++ & 1);
+          tc_fence_after();
 #pragma unroll 1
-        for (uint32_t j = 0; j <= n; ++j) {
-          if (j < n) {   // scores of job j
-            const uint32_t x = j & 1, tile = tiles + (pair ? j >> 1 : j), st = tile & 1;
-            if (!pair || x == 0) {
-              wait(&bars.k_full[st], tile >> 1 & 1);
-              tc_fence_after();
-            }
-            const uint32_t d = tmem + x * 128, qa = q + (pair ? x * S::kOperand : 0), ka = k + st * S::kOperand;
+          for (uint32_t j = 0; j <= n; ++j) {
+            if (j < n) {   // scores of job j
+              const uint32_t x = j & 1, tile = tiles + (pair ? j >> 1 : j), st = tile & 1;
+              if (!pair || x == 0) {
+                wait(&bars.k_full[st], tile >> 1 & 1);
+                tc_fence_after();
+              }
+              const uint32_t d = tmem + x * 128, qa = q + (pair ? x * kTileOn : 0), ka = k + st * kTileOn;
 #pragma unroll
-            for (uint32_t c = 0; c < D / 16; ++c) {
-              const uint32_t off = c / 4 * kPanel + c % 4 * 32;
-              mma_ss(d, operand(qa + off, 0), operand(ka + off, 0), kScoreDesc, c > 0);
-              if constexpr (kSplit) mma_ss(d, operand(qa + S::kOperand + off, 0), operand(ka + off, 0), kScoreDesc, 1);
+              for (uint32_t c = 0; c < D / 16; ++c) {
+                const uint32_t off = c / 4 * kPanel + c % 4 * 32;
+                mma_ss(d, operand(qa, off), operand(ka, off), kScoreDesc, c > 0);
+                if constexpr (kSplit) mma_ss(d, operand(qa, S::kOperand + off), operand(ka, off), kScoreDesc, true);
+              }
+              tc_commit(&bars.s_full[x]);
+              if (!pair || x == 1) tc_commit(&bars.k_empty[st]);
             }
-            tc_commit(&bars.s_full[x]);
-            if (!pair || x == 1) tc_commit(&bars.k_empty[st]);
-          }
-          if (j > 0) {   // values of job j - 1
-            const uint32_t i = j - 1, x = i & 1, tile = tiles + (pair ? i >> 1 : i), st = tile & 1;
-            wait(&bars.p_full[x], jobs[x] & 1);
-            if (!pair || x == 0) wait(&bars.v_full[st], tile >> 1 & 1);
-            tc_fence_after();
-            const uint32_t d = tmem + 256 + x * 128, pa = tmem + x * 128, va = v + st * S::kOperand;
+            if (j > 0) {   // values of job j - 1
+              const uint32_t i = j - 1, x = i & 1, tile = tiles + (pair ? i >> 1 : i), st = tile & 1;
+              const uint32_t parity = (x ? jobs1 : jobs0) & 1;
+              const uint32_t d = tmem + 256 + x * 128, pa = tmem + x * 128, va = v + st * kTileOn;
+              if (!pair || x == 0) wait(&bars.v_full[st], tile >> 1 & 1);
 #pragma unroll
-            for (uint32_t c = 0; c < kTileN / 16; ++c) {
-              const uint64_t b = operand(va + c * 2048, kPanel);
-              mma_ts(d, pa + c * 8, b, kValueDesc, i > 1 || c > 0);
-              if constexpr (kSplit) mma_ts(d, pa + 64 + c * 8, b, kValueDesc, 1);
+              for (uint32_t half = 0; half < 2; ++half) {
+                wait(half ? &bars.p_full[x] : &bars.p_half[x], parity);
+                tc_fence_after();
+#pragma unroll
+                for (uint32_t c = half * 4; c < half * 4 + 4; ++c) {
+                  const uint64_t b = operand(va, c * 2048);
+                  mma_ts(d, pa + c * 8, b, kValueDesc, c > 0 || i > 1);
+                  if constexpr (kSplit) mma_ts(d, pa + 64 + c * 8, b, kValueDesc, true);
+                }
+              }
+              if (!pair || x == 1) tc_commit(&bars.v_empty[st]);
+              if (i + 2 >= n) tc_commit(&bars.o_full[x]);
+              if (x) ++jobs1;
+              else ++jobs0;
             }
-            if (!pair || x == 1) tc_commit(&bars.v_empty[st]);
-            if (i + 2 >= n) tc_commit(&bars.o_full[x]);
-            ++jobs[x];
           }
-        }
-        tiles += w.units;
+          tiles += w.units;
         }
         __syncwarp();
       });
@@ -705,7 +740,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
       const int32_t count = kv4_count(p, w.seq);
       // ---- Q to shared memory, a warp a row: two tiles, or one (as hi and lo) that both groups load half of ----
       const uint32_t q_rows = pair ? 2 * kTileM : kTileM;
-      constexpr uint32_t L = D / 8, kPer = 32 / L, kBatch = 4;   // lanes of a row, rows of a warp's pass, passes in flight
+      constexpr uint32_t L = D / 8, kPer = 32 / L, kBatch = kTileM / (8 * kPer);   // lanes of a row, rows of a pass, passes in flight
       const uint32_t sub = lane % L, lane_row = lane / L;
 #pragma unroll 1
       for (uint32_t r0 = warp * kPer; r0 < q_rows; r0 += 8 * kPer * kBatch) {
@@ -775,9 +810,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
         }
         float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int c = 4; c < (int)kTileN; c += 4)
+        for (int c = 4; c + 8 <= (int)kTileN; c += 8)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) top[i] = fmaxf(top[i], s[c + i]);
+          for (int i = 0; i < 4; ++i) top[i] = max3(top[i], s[c + i], s[c + 4 + i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top[i] = fmaxf(top[i], s[kTileN - 4 + i]);
         const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f;
         if (__any_sync(~0u, best > m + kLead)) {
           const float up = fmaxf(m, best), r = up == m ? 1.f : exp2_fast(m - up);
@@ -802,21 +839,29 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
           }
         }
         const float base = kTilePScale - (m == -INFINITY ? 0.f : m);
-        float sum[2] = {0.f, 0.f};
+        const float2 f2 = make_float2(f, f), base2 = make_float2(base, base);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int c = 0; c < (int)kTileN; c += 32) {
           uint32_t hi[16], lo[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float a = exp2_fast(fmaf(s[c + 2 * i], f, base)), b = exp2_fast(fmaf(s[c + 2 * i + 1], f, base));
-            sum[0] += a, sum[1] += b;
-            if constexpr (kSplit) split2(a, b, hi[i], lo[i]);
-            else hi[i] = half2_bits(__floats2half2_rn(a, b));
+            float2 e = fma2(make_float2(s[c + 2 * i], s[c + 2 * i + 1]), f2, base2);
+            e.x = exp2_fast(e.x), e.y = exp2_fast(e.y);
+            sum[i % 2] = add2(sum[i % 2], e);
+            if constexpr (kSplit) split2(e.x, e.y, hi[i], lo[i]);
+            else hi[i] = half2_bits(__floats2half2_rn(e.x, e.y));
           }
           tmem_store16(s_addr + c / 2, hi);
           if constexpr (kSplit) tmem_store16(s_addr + 64 + c / 2, lo);
+          if (c == 32) {   // the products of the first 64 rows may start
+            tmem_wait_store();
+            tc_fence_before();
+            mbar_arrive(&bars.p_half[x]);
+          }
         }
-        l += sum[0] + sum[1];
+        sum[0] = add2(sum[0], sum[1]);
+        l += sum[0].x + sum[0].y;
         tmem_wait_store();
         tc_fence_before();
         mbar_arrive(&bars.p_full[x]);
