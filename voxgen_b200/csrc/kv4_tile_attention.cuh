@@ -74,6 +74,14 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 __device__ __forceinline__ void tc_commit(uint64_t *bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// One lane of a converged warp. Unlike a test of the lane number it tells the
+// compiler that what follows runs in one thread, so that descriptors are computed
+// in uniform registers, where the products want them.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t x;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(x));
+  return x != 0;
+}
 // add: whether the product is added to what is there (a constant, or a predicate of the loop).
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
   asm volatile(
@@ -576,7 +584,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
       constexpr uint32_t kTileOn = S::kOperand >> 4;   // from one operand to the next, in a descriptor
       uint32_t works = 0, tiles = 0, jobs0 = 0, jobs1 = 0;   // jobs: of each group
       each_work([&](const TileWork &w) {
-        if (lane == 0) {
+        if (elect_one()) {
           const bool pair = paired(w);
           const uint32_t n = pair ? 2 * w.units : w.units;
           wait(&bars.q_full, works++ & 1);
@@ -625,7 +633,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
         }
         __syncwarp();
       });
-      if (lane == 0) {
+      if (elect_one()) {
         tc_commit(&bars.drained);   // tensor memory is freed after the last product, even when waits ran out
         mbar_wait_bounded(&bars.drained, 0);
       }
