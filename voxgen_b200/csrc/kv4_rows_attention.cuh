@@ -200,31 +200,34 @@ __device__ __forceinline__ Piece find_piece(const Kv4View &c, const Plan &p, uin
 // Cache row of a 16-row tile that MMA row i is (in both halves of the tile).
 __device__ __forceinline__ uint32_t perm8(uint32_t i) { return i % 2 ? 4 + (i / 2 ^ 1) : i / 2; }
 
-// A warp puts query row r of a (sequence, KV head) into column `col` of B fragments
-// [hi, lo][step][lane][2] in shared memory, and says by what its scores are to be
-// multiplied and how many cache rows it sees (0: none, or no such row).
+// A lane's channels of query row r of a (sequence, KV head), and how many cache
+// rows it sees (0: none, or no such row).
 template <int D, typename T>
-__device__ __forceinline__ void query_fragment(const Kv4AttnParams &p, uint32_t seq, uint32_t kv, uint32_t r, uint32_t col,
-                                               uint32_t held, uint32_t *frag, float *factor, uint32_t *sees) {
-  constexpr uint32_t N = D / 32, kLaneChannels = D / 4;   // channels of a lane here, and of a lane of the MMA
+__device__ __forceinline__ uint32_t load_query(const Kv4AttnParams &p, uint32_t seq, uint32_t kv, uint32_t r, uint32_t held,
+                                               float (&x)[D / 32]) {
+  constexpr uint32_t N = D / 32;
   const uint32_t lane = threadIdx.x % 32, tok = r / p.group;
-  float x[N];
 #pragma unroll
   for (uint32_t i = 0; i < N; ++i) x[i] = 0.f;
-  uint32_t seen = 0, top = 0;
-  if (r < p.tokens * p.group) {
-    const int32_t count = kv4_count(p, seq), n = (int32_t)held - count + (int32_t)tok + 1;
-    seen = (int32_t)tok < count && n > 0 ? (uint32_t)n : 0u;
-    const T *q = (const T *)p.q + (int64_t)seq * p.qs.seq + (int64_t)tok * p.qs.token +
-                 (int64_t)(kv * p.group + r - tok * p.group) * p.qs.head + lane * N;
+  if (r >= p.tokens * p.group) return 0;
+  const int32_t count = kv4_count(p, seq), n = (int32_t)held - count + (int32_t)tok + 1;
+  const T *q = (const T *)p.q + (int64_t)seq * p.qs.seq + (int64_t)tok * p.qs.token +
+               (int64_t)(kv * p.group + r - tok * p.group) * p.qs.head + lane * N;
 #pragma unroll
-    for (uint32_t i = 0; i < N; ++i) x[i] = (float)q[i];
-  }
+  for (uint32_t i = 0; i < N; ++i) x[i] = (float)q[i];
+  return (int32_t)tok < count && n > 0 ? (uint32_t)n : 0u;
+}
+// A warp puts a query row into column `col` of B fragments [hi, lo][step][lane][2]
+// in shared memory; what its scores are to be multiplied by.
+template <int D, typename T>
+__device__ __forceinline__ float store_query(const Kv4AttnParams &p, const float (&x)[D / 32], uint32_t col, uint32_t *frag) {
+  constexpr uint32_t N = D / 32, kLaneChannels = D / 4;   // channels of a lane here, and of a lane of the MMA
+  const uint32_t lane = threadIdx.x % 32;
+  uint32_t top = 0;
 #pragma unroll
   for (uint32_t i = 0; i < N; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
   float inverse;
   const float power = row_power(__uint_as_float(__reduce_max_sync(~0u, top)), inverse);
-  if (lane == 0) *factor = fmaxf(p.scale * inverse, 0x1p-126f), *sees = seen;
   // channel c: lane t = c / (D/4) of its column, word (c % (D/4)) / 8, and within the word i = c % 8: pair i % 4 (half
   // i / 4), two pairs a step
 #pragma unroll
@@ -237,6 +240,7 @@ __device__ __forceinline__ void query_fragment(const Kv4AttnParams &p, uint32_t 
     *dst = hi;
     if constexpr (sizeof(T) == 4) dst[D / 16 * 32 * 2 * 2] = __float2half_rn(v - __half2float(hi));
   }
+  return fmaxf(p.scale * inverse, 0x1p-126f);
 }
 
 // T: type of q and out; fp32 operands are hi + lo.
@@ -306,7 +310,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
     const uint32_t held = kv4_held(p.c, seg.seq);
     // ---- the queries as B fragments, a warp a row: column `warp` of the MMA is query row row0 + warp ----
     if (warp < kTileRows) {
-      query_fragment<D, T>(p, seg.seq, kv, row0 + warp, warp, held, &q_frag[0][0][0][0], &factors[warp], &seens[warp]);
+      float x[D / 32];
+      const uint32_t seen = load_query<D, T>(p, seg.seq, kv, row0 + warp, held, x);
+      const float factor = store_query<D, T>(p, x, warp, &q_frag[0][0][0][0]);
+      if (lane == 0) factors[warp] = factor, seens[warp] = seen;
     }
     __syncthreads();
     uint32_t q_hi[kSteps][2], q_lo[kSplit ? kSteps : 1][2];

@@ -327,7 +327,7 @@ __device__ __forceinline__ void in_order(const float *o, float4 &low, float4 &hi
 template <int D, typename T, typename Plan>
 __device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const Plan &plan, const TileWork &w, bool pair, uint32_t x,
                                              uint32_t row, uint32_t row0, float m, float l, bool mine, uint32_t o_addr,
-                                             float *shared_o, float *other_max, float *other_sum, uint32_t *last) {
+                                             float *shared_o, float (*group_max)[kTileM], float (*group_sum)[kTileM], uint32_t *last) {
   const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, rows = p.tokens * p.group;
   const uint32_t block_rows = min(pair ? 2 * kTileM : kTileM, rows - row0);
   const bool whole = w.units == w.seg_units;
@@ -360,54 +360,39 @@ __device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const Plan 
   };
   if (!pair) {
     constexpr uint32_t kChunks = D / 4;
-    float w0 = 1.f, w1 = 0.f;
-    if (x == 1) {
-      other_max[row] = mine ? m : -INFINITY;
-      other_sum[row] = mine ? l : 0.f;
-    }
+    group_max[x][row] = mine ? m : -INFINITY;
+    group_sum[x][row] = mine ? l : 0.f;
     named_bar(2, 256);
-    {
-      const float om = x == 0 ? other_max[row] : m;
-      if (x == 0) {
-        const float top = fmaxf(m, om);
-        w0 = m == -INFINITY ? 0.f : exp2_fast(m - top);
-        w1 = om == -INFINITY ? 0.f : exp2_fast(om - top);
-        l = l * w0 + other_sum[row] * w1;
-        m = top;
-        const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
-        w0 *= inv;
-        w1 *= inv;
-        other_max[row] = w1;   // for the other group
-      }
-    }
-    named_bar(2, 256);
-    // group 1 scales and writes its O, group 0 adds its own
+    const float m0 = group_max[0][row], m1 = group_max[1][row], top = fmaxf(m0, m1);
+    const float w0 = m0 == -INFINITY ? 0.f : exp2_fast(m0 - top), w1 = m1 == -INFINITY ? 0.f : exp2_fast(m1 - top);
+    l = group_sum[0][row] * w0 + group_sum[1][row] * w1;
+    m = top;
+    const float f = (x ? w1 : w0) * (!whole ? 1.f : l == 0.f ? 0.f : 1.f / l);
+    // each group hands over its share of the other's half of the channels, then adds what it was handed to its own half
 #pragma unroll 1
-    for (uint32_t turn = 0; turn < 2; ++turn) {
-      if (turn == 0 ? x == 1 && mine : x == 0) {
-        const float f = turn ? w0 : other_max[row];
-        const bool add = turn && w.units > 1;
+    for (uint32_t pass = 0; pass < 2; ++pass) {
+      const uint32_t from = (x ^ pass ^ 1) * (D / 2);
+      const bool add = pass && (x == 1 || w.units > 1);   // the other group had a tile
 #pragma unroll 1
-        for (uint32_t c = 0; c < D; c += 32) {
-          float o[32];
-          tmem_load32(o_addr + c, o);
-          tmem_wait_load();
-          loaded(o);
+      for (uint32_t c = from; c < from + D / 2; c += 32) {
+        float o[32];
+        tmem_load32(o_addr + c, o);
+        tmem_wait_load();
+        loaded(o);
 #pragma unroll
-          for (uint32_t i = 0; i < 32; i += 8) {
-            float4 v[2];
-            in_order(o + i, v[0], v[1]);
+        for (uint32_t i = 0; i < 32; i += 8) {
+          float4 v[2];
+          in_order(o + i, v[0], v[1]);
 #pragma unroll
-            for (uint32_t k = 0; k < 2; ++k) {
-              float4 *at = row_chunk<kChunks>(shared_o, row, (c + i) / 4 + k);
-              float4 y = add ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
-              // 0 times what an idle or empty group left is not taken
-              if (f != 0.f) y.x = fmaf(v[k].x, f, y.x), y.y = fmaf(v[k].y, f, y.y), y.z = fmaf(v[k].z, f, y.z), y.w = fmaf(v[k].w, f, y.w);
-              *at = y;
-            }
+          for (uint32_t k = 0; k < 2; ++k) {
+            float4 *at = row_chunk<kChunks>(shared_o, row, (c + i) / 4 + k);
+            float4 y = add ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
+            if (mine) y.x = fmaf(v[k].x, f, y.x), y.y = fmaf(v[k].y, f, y.y), y.z = fmaf(v[k].z, f, y.z), y.w = fmaf(v[k].w, f, y.w);
+            *at = y;
           }
         }
       }
+      __syncwarp();
       named_bar(2, 256);
     }
     constexpr uint32_t kPer = 32 / kChunks;   // rows of a warp's pass
@@ -531,7 +516,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
   uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   __shared__ TileBars bars;
   __shared__ uint32_t tmem_base, aborted, last;
-  __shared__ float factors[2 * kTileM], other_max[kTileM], other_sum[kTileM];
+  __shared__ float factors[2 * kTileM], group_max[2][kTileM], group_sum[2][kTileM];
   const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const uint32_t rows = p.tokens * p.group;
   const TilePlan<kRows> plan(p);
@@ -879,7 +864,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
       if (mine) wait(&bars.o_full[x], works++ & 1);
       __syncwarp();
       tc_fence_after();
-      tile_results<D, T>(p, plan, w, pair, x, row, row0, m, l, mine, o_addr, (float *)(smem + S::kQ), other_max, other_sum, &last);
+      tile_results<D, T>(p, plan, w, pair, x, row, row0, m, l, mine, o_addr, (float *)(smem + S::kQ), group_max, group_sum, &last);
       tc_fence_before();
     });
   }

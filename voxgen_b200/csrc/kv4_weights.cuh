@@ -20,7 +20,7 @@ template <int D, typename T>
 constexpr uint32_t kWeightSmem = kWeightTiles * (D / 16) * 32 * 2 * 4 * (sizeof(T) == 4 ? 2 : 1);
 
 template <int D, typename T>
-__global__ void __launch_bounds__(kWeightThreads) kv4_weights_kernel(const Kv4AttnParams p) {
+__global__ void __launch_bounds__(kWeightThreads, 2) kv4_weights_kernel(const Kv4AttnParams p) {
   constexpr bool kSplit = sizeof(T) == 4;
   constexpr int kSteps = D / 16;
   constexpr uint32_t kFrag = kSteps * 32 * 2 * (kSplit ? 2 : 1);   // words of a tile's fragments
@@ -62,19 +62,30 @@ __global__ void __launch_bounds__(kWeightThreads) kv4_weights_kernel(const Kv4At
     }
   }
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  const uint32_t last_seen = held;   // rows past what every query sees are cut by `seens`
   for (uint32_t base = 0; base < rows; base += kWeightTiles * 8) {
     __syncthreads();
     const uint32_t n = min(kWeightTiles * 8, rows - base), tiles = (n + 7) / 8;
-    for (uint32_t i = warp; i < tiles * 8; i += kWeightWarps) {
-      query_fragment<D, T>(p, seq, kv, base + i, i % 8, held, frags + i / 8 * kFrag, &factors[i], &seens[i]);
-      if (lane == 0) {
-        const uint32_t r = base + i, tok = r / p.group;
-        denominators[i] = r < rows ? p.lse[((size_t)seq * p.tokens + tok) * p.heads + kv * p.group + r - tok * p.group] : INFINITY;
+    // a warp takes rows warp, warp + 8, ... (column `warp` of every tile), four loads in flight
+#pragma unroll 1
+    for (uint32_t j0 = 0; j0 < tiles; j0 += 4) {
+      float x[4][D / 32], minus[4];
+      uint32_t seen[4];
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        const uint32_t r = base + (j0 + j) * 8 + warp, tok = r / p.group;
+        seen[j] = load_query<D, T>(p, seq, kv, r, held, x[j]);
+        minus[j] = r < rows ? p.lse[((size_t)seq * p.tokens + tok) * p.heads + kv * p.group + r - tok * p.group] : INFINITY;
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        if (j0 + j >= tiles) break;
+        const float factor = store_query<D, T>(p, x[j], warp, frags + (j0 + j) * kFrag);
+        const uint32_t i = (j0 + j) * 8 + warp;
+        if (lane == 0) factors[i] = factor, seens[i] = seen[j], denominators[i] = minus[j];
       }
     }
     __syncthreads();
-    if (row0 >= last_seen) continue;
+    if (row0 >= held) continue;
 #pragma unroll 1
     for (uint32_t j = 0; j < tiles; ++j) {
       const uint32_t *f = frags + j * kFrag;
