@@ -93,9 +93,9 @@ int allow_smem(const void *fn, size_t bytes, std::atomic<uint64_t> &done) {
 }
 
 // Blocks of a sequence for `items` (token, head) pairs: enough for every SM to be
-// full (8 blocks each), no more than have two passes to make.
+// full (8 blocks each), no more than have a pass to make.
 uint32_t row_blocks(uint64_t items, uint32_t per_block, uint32_t seqs) {
-  const uint64_t most = (items + 2 * per_block - 1) / (2 * per_block), full = (148 * 8 + seqs - 1) / seqs;
+  const uint64_t most = (items + per_block - 1) / per_block, full = (148 * 8 + seqs - 1) / seqs;
   return (uint32_t)std::min(most, full);
 }
 
@@ -106,13 +106,23 @@ uint64_t segments_of(const vg_kv4_cache *c, uint32_t heads, uint32_t tokens) {
   const uint64_t rows = (uint64_t)tokens * (heads / c->kv_heads);
   return (rows + kTileRows - 1) / kTileRows * c->kv_heads * c->seqs;
 }
-// Query rows of a (sequence, KV head) from which on the 128-row kernel is taken.
+// Query rows of a (sequence, KV head) from which on the 128-row kernel is taken: 16 ragged streams with 16 rows each take
+// 14 us with two passes of the few-row kernel, with 24 rows 22 us with the other.
 constexpr uint64_t kTileFrom = 17;
+// Segments of 256 rows from which on they are worth it: with 32 of them a prompt of 512 tokens takes 40 us against 24 with
+// twice as many of 128 rows; with 64, 1024 tokens over 8192 rows take 113 us against 137.
+constexpr uint64_t kPairFrom = 48;
 bool tiled(const vg_kv4_cache *c, uint32_t heads, uint32_t tokens) {
   return (uint64_t)tokens * (heads / c->kv_heads) >= kTileFrom;
 }
+// Whether 16-bit queries are taken 256 rows at a time: an unpacked tile then serves
+// twice as many rows, but there are half as many segments to share out.
+bool paired(const vg_kv4_cache *c, uint32_t heads, uint32_t tokens) {
+  const uint64_t rows = (uint64_t)tokens * (heads / c->kv_heads);
+  return (rows + 2 * kTileM - 1) / (2 * kTileM) * c->kv_heads * c->seqs >= kPairFrom;
+}
 uint64_t part_bytes(const vg_kv4_cache *c, uint32_t heads, uint32_t tokens) {
-  if (tiled(c, heads, tokens)) return (uint64_t)2 * kTileCtas * 2 * kTileM * (c->head_dim + 2) * 4;
+  if (tiled(c, heads, tokens)) return (uint64_t)kTileSlots * 2 * kTileM * (c->head_dim + 2) * 4;
   return most_pieces(segments_of(c, heads, tokens)) * kTileRows * (c->head_dim + 2) * 4;
 }
 
@@ -148,7 +158,7 @@ int vg_k_kv4_append(const vg_kv4_cache *cache, const void *k, const void *v, int
   p.counts = counts;
   p.tokens = tokens;
   const uint64_t items = (uint64_t)tokens * cache->kv_heads;
-  const uint32_t per_block = kRowThreads / (cache->head_dim / 8);
+  const uint32_t per_block = kRowThreads / (cache->head_dim / 16);
   if (items > kMaxGrid) return VG_ERANGE;
   p.blocks = row_blocks(items, per_block, cache->seqs);
   const bool vec = wide(k, p.ks, size) && wide(v, p.vs, size);
@@ -227,7 +237,8 @@ int vg_k_kv4_attention(const vg_kv4_cache *cache, const void *q, int dtype, uint
   p.group = heads / cache->kv_heads;
   p.scale = scale * 1.44269504088896340736f;
   const bool tile = tiled(cache, heads, tokens);
-  const uint32_t block = !tile ? kTileRows : size == 4 ? kTileM : 2 * kTileM;   // query rows that a CTA takes at a time
+  const bool pair = tile && size == 2 && paired(cache, heads, tokens);
+  const uint32_t block = !tile ? kTileRows : pair ? 2 * kTileM : kTileM;   // query rows that a CTA takes at a time
   p.row_tiles = (tokens * p.group + block - 1) / block;
   const uint64_t blocks = ((uint64_t)cache->capacity + kWeightRows - 1) / kWeightRows * cache->seqs * cache->kv_heads;
   if (track && blocks > kMaxGrid) return VG_ERANGE;
@@ -236,19 +247,40 @@ int vg_k_kv4_attention(const vg_kv4_cache *cache, const void *q, int dtype, uint
     return by_type(dtype, [&](auto t) {
       using T = decltype(t);
       constexpr int D = decltype(d)::value;
-      static std::atomic<uint64_t> done[2];
+      static std::atomic<uint64_t> done[3];
       if (tile) {
-        const auto fn = kv4_tile_kernel<D, T>;
-        const int e = allow_smem((const void *)fn, TileSmem<D>::kBytes, done[0]);
+        const auto go = [&](auto fn, std::atomic<uint64_t> &set) {
+          const int e = allow_smem((const void *)fn, TileSmem<D>::kBytes, set);
+          if (!e) fn<<<kTileCtas, kTileThreads, TileSmem<D>::kBytes, st>>>(p);
+          return e;
+        };
+        int e;
+        if constexpr (sizeof(T) == 2) {
+          e = pair ? go(kv4_tile_kernel<D, T, true>, done[2]) : go(kv4_tile_kernel<D, T, false>, done[0]);
+        } else {
+          e = go(kv4_tile_kernel<D, T, false>, done[0]);
+        }
         if (e) return e;
-        fn<<<kTileCtas, kTileThreads, TileSmem<D>::kBytes, st>>>(p);
       } else {
         const auto fn = kv4_rows_kernel<D, T>;
         const int e = allow_smem((const void *)fn, RowsSmem<D>::kBytes, done[1]);
         if (e) return e;
         fn<<<kRowsCtas, kRowsThreads, RowsSmem<D>::kBytes, st>>>(p);
       }
-      if (track) kv4_weights_kernel<D, T><<<(uint32_t)blocks, kWeightThreads, kWeightSmem<D, T>, st>>>(p);
+      if (track) {   // starts as the attention's CTAs leave, and waits for the last of them where it needs their sums
+        cudaLaunchAttribute early{};
+        early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        early.val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((uint32_t)blocks);
+        cfg.blockDim = dim3(kWeightThreads);
+        cfg.dynamicSmemBytes = kWeightSmem<D, T>;
+        cfg.stream = st;
+        cfg.attrs = &early;
+        cfg.numAttrs = 1;
+        const cudaError_t err = cudaLaunchKernelEx(&cfg, kv4_weights_kernel<D, T>, p);
+        if (err != cudaSuccess) return VG_ECUDA;
+      }
       return launched();
     });
   });

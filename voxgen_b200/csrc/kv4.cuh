@@ -67,6 +67,35 @@ enum : int32_t {
   kKv4Timeout = 8,    // a bounded wait inside attention ran out (sequence 0's word)
 };
 
+// Two fp32 operations in one instruction, and the extremes of three.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(*(const uint64_t *)&a), "l"(*(const uint64_t *)&b), "l"(*(const uint64_t *)&c));
+  return *(const float2 *)&d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*(const uint64_t *)&a), "l"(*(const uint64_t *)&b));
+  return *(const float2 *)&d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*(const uint64_t *)&a), "l"(*(const uint64_t *)&b));
+  return *(const float2 *)&d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // d of a block from its extremes.
 __device__ __forceinline__ float kv4_scale(float high, float low) {
   const float d = (high >= -low ? high : low) * -0.125f;

@@ -29,17 +29,18 @@ struct AppendParams {
 
 constexpr uint32_t kRowThreads = 256;
 
-// One lane quantises 8 channels of a K row and of the V row beside it, two rows
-// of each in flight; the four lanes of a block agree on its extremes by shuffles.
-// Bound by the input's bytes: each value is read once, and the stores are 0.56
-// bytes a value.
+// One lane quantises 16 channels of a K row and of the V row beside it; the two
+// lanes of a block agree on its extremes by a shuffle. Bound by the input's bytes
+// and, for 16-bit inputs, nearly as much by the instructions: 16 channels a lane
+// and packed fp32 arithmetic bring them to about 8 a value (8 channels and single
+// operations took 49 us for 28 x 4096 x 2 rows of 128 where the bytes need 23).
 //
 // The rows held are advanced by the last block of a sequence to finish: every
 // block has read them by then, since what it did depended on them. One launch
 // does the whole append.
 template <int D, typename T, bool VEC>
-__global__ void __launch_bounds__(kRowThreads, 4) kv4_append_kernel(const AppendParams p) {
-  constexpr uint32_t L = D / 8;                  // lanes of a row
+__global__ void __launch_bounds__(kRowThreads) kv4_append_kernel(const AppendParams p) {
+  constexpr uint32_t L = D / 16;                 // lanes of a row
   constexpr uint32_t kRows = kRowThreads / L;    // (token, head) pairs per pass
   const uint32_t seq = blockIdx.x / p.blocks, block = blockIdx.x % p.blocks;
   Kv4Seq *st = p.c.state + seq;
@@ -50,71 +51,73 @@ __global__ void __launch_bounds__(kRowThreads, 4) kv4_append_kernel(const Append
   const bool full = !bad && (uint32_t)at + (uint32_t)count > p.c.capacity;
   const uint32_t items = bad || full ? 0 : (uint32_t)count * p.c.kv_heads;
   const uint32_t lane = threadIdx.x % L;
-  const T *k = (const T *)p.k + (int64_t)seq * p.ks.seq + lane * 8;
-  const T *v = (const T *)p.v + (int64_t)seq * p.vs.seq + lane * 8;
+  const T *k = (const T *)p.k + (int64_t)seq * p.ks.seq + lane * 16;
+  const T *v = (const T *)p.v + (int64_t)seq * p.vs.seq + lane * 16;
   bool odd = false;  // met a NaN or an infinity
-  for (uint32_t base = block * kRows * 2; base < items; base += p.blocks * kRows * 2) {
-    float x[2][2][8];
-    uint32_t token[2], head[2];
-    bool on[2];
+  for (uint32_t base = block * kRows; base < items; base += p.blocks * kRows) {
+    const uint32_t item = base + threadIdx.x / L;
+    const bool on = item < items;
+    const uint32_t token = on ? item / p.c.kv_heads : 0, head = on ? item - token * p.c.kv_heads : 0;
+    float x[2][16];
+    const T *src[2] = {k + (int64_t)token * p.ks.token + (int64_t)head * p.ks.head,
+                       v + (int64_t)token * p.vs.token + (int64_t)head * p.vs.head};
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const uint32_t item = base + u * kRows + threadIdx.x / L;
-      on[u] = item < items;
-      token[u] = on[u] ? item / p.c.kv_heads : 0;
-      head[u] = on[u] ? item - token[u] * p.c.kv_heads : 0;
-      load8<T, VEC>(k + (int64_t)token[u] * p.ks.token + (int64_t)head[u] * p.ks.head, x[u][0]);
-      load8<T, VEC>(v + (int64_t)token[u] * p.vs.token + (int64_t)head[u] * p.vs.head, x[u][1]);
+    for (int i = 0; i < 2; ++i) {
+      load8<T, VEC>(src[i], *(float(*)[8])x[i]);
+      load8<T, VEC>(src[i] + 8, *(float(*)[8])(x[i] + 8));
     }
+    const uint32_t row = (uint32_t)at + token;
+    const size_t lane_row = (size_t)seq * p.c.kv_heads + head;
+    uint8_t *run = p.c.data + lane_row * p.c.tiles * Kv4<D>::kTileBytes;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const uint32_t row = (uint32_t)at + token[u];
-      const size_t lane_row = (size_t)seq * p.c.kv_heads + head[u];
-      uint8_t *run = p.c.data + lane_row * p.c.tiles * Kv4<D>::kTileBytes;
+    for (int i = 0; i < 2; ++i) {
+      float(&y)[16] = x[i];
+      const float2 none = make_float2(0.f, 0.f);
+      float high = y[0], low = y[0];
+      float2 zero = none;   // NaN once a value is not finite
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float(&y)[8] = x[u][i];
-        float high = y[0], low = y[0], zero = y[0] * 0.f;
+      for (int j = 0; j < 16; j += 2) {
+        zero = fma2(make_float2(y[j], y[j + 1]), none, zero);
+        high = max3(high, y[j], y[j + 1]);
+        low = min3(low, y[j], y[j + 1]);
+      }
+      const bool wild = !(zero.x + zero.y == 0.f);
+      if (wild || high > kKv4Largest || low < -kKv4Largest) {
+        odd |= on && wild;
+        high = -kKv4Largest, low = kKv4Largest;
 #pragma unroll
-        for (int j = 1; j < 8; ++j) {
+        for (int j = 0; j < 16; ++j) {
+          y[j] = y[j] == y[j] ? fminf(fmaxf(y[j], -kKv4Largest), kKv4Largest) : 0.f;
           high = fmaxf(high, y[j]);
           low = fminf(low, y[j]);
-          zero = fmaf(y[j], 0.f, zero);   // NaN once a value is not finite
-        }
-        if (zero != zero || high > kKv4Largest || low < -kKv4Largest) {
-          odd |= on[u] && zero != zero;
-          high = -kKv4Largest, low = kKv4Largest;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            y[j] = y[j] == y[j] ? fminf(fmaxf(y[j], -kKv4Largest), kKv4Largest) : 0.f;
-            high = fmaxf(high, y[j]);
-            low = fminf(low, y[j]);
-          }
-        }
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-          high = fmaxf(high, __shfl_xor_sync(~0u, high, o));
-          low = fminf(low, __shfl_xor_sync(~0u, low, o));
-        }
-        const float d = kv4_scale(high, low);
-        const float inv = d == 0.f ? 0.f : __frcp_rn(d);
-        // |x * inv| < 8.1, so only 8 has to be brought back to 7. Adding 1.5 * 2^23 rounds to a whole number, ties
-        // to even, as rintf does, and leaves it in the low bits; the codes shift in from the last one on, and the
-        // magic number's own bits leave by one subtraction.
-        uint32_t w = 0;
-#pragma unroll
-        for (int j = 7; j >= 0; --j) w = w * 16 + __float_as_uint(fminf(y[j] * inv, 7.f) + 12582912.f);
-        constexpr uint32_t kMagic = 0x4B400000u - 8u;
-        w -= kMagic * 0x11111111u;
-        if (on[u]) {
-          *(uint32_t *)(run + Kv4<D>::codes(row, i) + lane * 4) = w;
-          if (lane % 4 == 0) *(__half *)(run + Kv4<D>::scales(row, i) + lane / 4 * 2) = __float2half_rn(d);
         }
       }
-      if (on[u] && lane == 0) {
-        if (p.c.weights) p.c.weights[lane_row * p.c.capacity + row] = 0.f;
-        if (p.c.positions) p.c.positions[lane_row * p.c.capacity + row] = s.y - s.x + at + (int32_t)token[u];
+      high = fmaxf(high, __shfl_xor_sync(~0u, high, 1));
+      low = fminf(low, __shfl_xor_sync(~0u, low, 1));
+      const float d = kv4_scale(high, low);
+      const float inv = d == 0.f ? 0.f : __frcp_rn(d);
+      // |x * inv| < 8.1, so only 8 has to be brought back to 7. Adding 1.5 * 2^23 rounds to a whole number, ties to
+      // even, as rintf does, and leaves it in the low bits; the codes shift in from the last one on, and the magic
+      // number's own bits leave by one subtraction.
+      const float2 inv2 = make_float2(inv, inv), magic = make_float2(12582912.f, 12582912.f);
+      uint32_t w[2] = {0, 0};
+#pragma unroll
+      for (int j = 14; j >= 0; j -= 2) {
+        float2 n = mul2(make_float2(y[j], y[j + 1]), inv2);
+        n = add2(make_float2(fminf(n.x, 7.f), fminf(n.y, 7.f)), magic);
+        uint32_t &c = w[j / 8];
+        c = c * 16 + __float_as_uint(n.y);
+        c = c * 16 + __float_as_uint(n.x);
       }
+      constexpr uint32_t kMagic = (0x4B400000u - 8u) * 0x11111111u;
+      if (on) {
+        *(uint2 *)(run + Kv4<D>::codes(row, i) + lane * 8) = make_uint2(w[0] - kMagic, w[1] - kMagic);
+        if (lane % 2 == 0) *(__half *)(run + Kv4<D>::scales(row, i) + lane) = __float2half_rn(d);
+      }
+    }
+    if (on && lane == 0) {
+      if (p.c.weights) p.c.weights[lane_row * p.c.capacity + row] = 0.f;
+      if (p.c.positions) p.c.positions[lane_row * p.c.capacity + row] = s.y - s.x + at + (int32_t)token;
     }
   }
   if (__syncthreads_or(odd) && threadIdx.x == 0) atomicOr(&st->status, kKv4NonFinite);

@@ -260,6 +260,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
   __shared__ __align__(8) float factors[kTileRows];
   __shared__ __align__(8) uint32_t seens[kTileRows];
   const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
+  if (p.lse) pdl_launch_dependents();   // the weights kernel may take the SMs that this one leaves
   const Plan plan = make_plan(p.c, p.c.kv_heads * p.row_tiles);
   if (blockIdx.x >= plan.pieces) return;
   const size_t run_bytes = (size_t)p.c.tiles * Kv4<D>::kTileBytes;

@@ -45,6 +45,7 @@ constexpr uint32_t kUnpackThreads = 128;
 constexpr uint32_t kSoftmaxRegs = 168, kOtherRegs = 88;
 constexpr uint32_t kSwitchUnits = 8;            // what changing segments costs, in units
 constexpr uint32_t kTileCtas = 148;
+constexpr uint32_t kTileSlots = 2 * kTileCtas;  // partial results
 constexpr uint32_t kRawStages = 3;
 constexpr float kTilePScale = 6.f;              // as kPScale: P below 2^14 with a lead of 2^8
 
@@ -131,25 +132,6 @@ __device__ __forceinline__ void fewer_registers() {
 }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// Two fp32 operations in one instruction, and the largest of three.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(d)
-      : "l"(*(const uint64_t *)&a), "l"(*(const uint64_t *)&b), "l"(*(const uint64_t *)&c));
-  return *(const float2 *)&d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*(const uint64_t *)&a), "l"(*(const uint64_t *)&b));
-  return *(const float2 *)&d;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
 // Shared-memory operand descriptor: 128-byte swizzle; panel: bytes between panels
 // (MN-major only), 8-row groups are 1024 bytes apart. The low word holds the
 // address, so a step along the operand is one 32-bit addition to it.
@@ -201,15 +183,18 @@ struct TilePlan {
   }
   __device__ explicit TilePlan(const Kv4AttnParams &p) : p(p), blocks(p.c.seqs * p.row_tiles), size(0), pieces(0) {
     const uint32_t total = sum_of(1), fair = (total + kTileCtas - 1) / kTileCtas;
-    if (blocks * p.c.kv_heads * 4 <= kTileCtas * 3) {
-      uint32_t of = fair;
+    // cut where one or two pieces a CTA share the work about as well as dealing it out does
+    const uint32_t segments = blocks * p.c.kv_heads, rounds = segments * 4 <= kTileCtas * 3 ? 1 : 2;
+    if (segments * 4 <= kTileCtas * 6) {
+      const uint32_t target = kTileCtas * rounds;
+      uint32_t of = max(1u, (total + target - 1) / target);
 #pragma unroll 1
       for (int i = 0;; ++i) {
         pieces = sum_of(of);
-        if (pieces <= kTileCtas || i == 3) break;
-        of = max(of + 1, (uint32_t)((uint64_t)of * pieces / kTileCtas));
+        if (pieces <= target || i == 3) break;
+        of = max(of + 1, (uint32_t)((uint64_t)of * pieces / target));
       }
-      if (of <= fair + kSwitchUnits) size = of;
+      if (of * rounds <= fair + kSwitchUnits && pieces <= kTileSlots) size = of;
     }
     ctas = min(gridDim.x, size ? pieces : total);
     each = total / ctas;
@@ -506,11 +491,13 @@ __device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const Plan 
   named_bar(2, 256);   // Q's place and the shared words may change
 }
 
-template <int D, typename T>
+// PAIR: blocks of 256 query rows, which 16-bit queries have room for.
+template <int D, typename T, bool PAIR>
 __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4AttnParams p) {
   using S = TileSmem<D>;
   constexpr bool kSplit = sizeof(T) == 4;
-  constexpr uint32_t kRows = kSplit ? kTileM : 2 * kTileM;    // query rows of a block
+  static_assert(!(kSplit && PAIR), "hi and lo take the second query tile's place");
+  constexpr uint32_t kRows = PAIR ? 2 * kTileM : kTileM;      // query rows of a block
   constexpr uint32_t kPanel = kTileN * 128;                   // bytes of 64 channels of a tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -519,6 +506,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
   __shared__ float factors[2 * kTileM], group_max[2][kTileM], group_sum[2][kTileM];
   const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const uint32_t rows = p.tokens * p.group;
+  if (p.lse) pdl_launch_dependents();   // the weights kernel may take the SMs that this one leaves
   const TilePlan<kRows> plan(p);
   if (blockIdx.x >= plan.ctas) return;
 
@@ -550,7 +538,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
     if (!mbar_wait_bounded(bar, parity)) *(volatile uint32_t *)&aborted = 1;
   };
   // two query tiles, or one whose cache tiles the softmax groups share
-  auto paired = [&](const TileWork &w) { return !kSplit && rows - w.block * kRows > kTileM; };
+  auto paired = [&](const TileWork &w) { return PAIR && rows - w.block * kRows > kTileM; };
   // f(work) for every piece of this CTA; whole warps
   const TileWork first_work = plan.start();
   auto each_work = [&](auto &&f) {

@@ -31,7 +31,10 @@ __global__ void __launch_bounds__(kWeightThreads, 2) kv4_weights_kernel(const Kv
   const uint32_t blocks = (p.c.capacity + kWeightRows - 1) / kWeightRows;
   const uint32_t lane_row = blockIdx.x / blocks, seq = lane_row / p.c.kv_heads, kv = lane_row - seq * p.c.kv_heads;
   const uint32_t held = kv4_held(p.c, seq), block_row = (blockIdx.x - lane_row * blocks) * kWeightRows;
-  if (block_row >= held) return;
+  if (block_row >= held) {
+    pdl_wait();   // no kernel after this one may start before the attention is done
+    return;
+  }
   const uint32_t row0 = block_row + warp * 32, rows = p.tokens * p.group;
   const uint8_t *run = p.c.data + (size_t)lane_row * p.c.tiles * Kv4<D>::kTileBytes;
   // ---- K rows row0 + {g, 8 + g, 16 + g, 24 + g} as A fragments ----
@@ -68,21 +71,23 @@ __global__ void __launch_bounds__(kWeightThreads, 2) kv4_weights_kernel(const Kv
     // a warp takes rows warp, warp + 8, ... (column `warp` of every tile), four loads in flight
 #pragma unroll 1
     for (uint32_t j0 = 0; j0 < tiles; j0 += 4) {
-      float x[4][D / 32], minus[4];
+      float x[4][D / 32];
       uint32_t seen[4];
 #pragma unroll
-      for (uint32_t j = 0; j < 4; ++j) {
-        const uint32_t r = base + (j0 + j) * 8 + warp, tok = r / p.group;
-        seen[j] = load_query<D, T>(p, seq, kv, r, held, x[j]);
-        minus[j] = r < rows ? p.lse[((size_t)seq * p.tokens + tok) * p.heads + kv * p.group + r - tok * p.group] : INFINITY;
-      }
+      for (uint32_t j = 0; j < 4; ++j) seen[j] = load_query<D, T>(p, seq, kv, base + (j0 + j) * 8 + warp, held, x[j]);
 #pragma unroll
       for (uint32_t j = 0; j < 4; ++j) {
         if (j0 + j >= tiles) break;
         const float factor = store_query<D, T>(p, x[j], warp, frags + (j0 + j) * kFrag);
         const uint32_t i = (j0 + j) * 8 + warp;
-        if (lane == 0) factors[i] = factor, seens[i] = seen[j], denominators[i] = minus[j];
+        if (lane == 0) factors[i] = factor, seens[i] = seen[j];
       }
+    }
+    if (base == 0) pdl_wait();   // what follows needs the attention's sums
+    if (threadIdx.x < tiles * 8) {
+      const uint32_t r = base + threadIdx.x, tok = r / p.group;
+      denominators[threadIdx.x] =
+          r < rows ? p.lse[((size_t)seq * p.tokens + tok) * p.heads + kv * p.group + r - tok * p.group] : INFINITY;
     }
     __syncthreads();
     if (row0 >= held) continue;
