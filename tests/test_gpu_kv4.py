@@ -207,6 +207,10 @@ SHAPES = [
     ([300, 17, 64], 2, 16, 2, 128), ([130, 500], 5, 16, 2, 128), ([90, 700], 3, 6, 3, 64), ([400], 16, 8, 1, 128),
     ([600, 33], 17, 16, 2, 128), ([300], 33, 12, 2, 64), ([129, 450], 100, 4, 2, 128), ([300], 300, 2, 1, 128),
     ([511], 257, 8, 2, 64),
+    # many segments, whole or cut; one long sequence among short ones; pieces of one segment on every SM
+    ([5000] + [3] * 59, 1, 4, 2, 64), ([33] * 70 + [900], 1, 8, 8, 64), ([20000], 1, 1, 1, 64), ([20000], 40, 1, 1, 64),
+    # blocks of 256 query rows (16-bit), the last of them with few; units dealt out over many short segments
+    ([310, 350, 300, 333, 420, 301], 300, 8, 8, 64), ([60, 200, 41] * 10, 40, 8, 8, 64), ([700, 650], 640, 12, 2, 128),
 ]
 
 
@@ -409,6 +413,24 @@ def test_refusals_name_the_fault():
     assert cache.rows().tolist() == [10]
 
 
+def test_more_sequences_than_can_be_cut():
+    """Past 16384 segments every one is a piece; a sample of them is checked."""
+    seqs = 2100
+    rows = [1 + i * 7 % 150 for i in range(seqs)]
+    cache = filled(81, rows, 8, 64, 150)
+    q = normal(82, seqs, 1, 8, 64)
+    out = cache.attention(q)
+    assert torch.equal(out, cache.attention(q))
+    some = list(range(0, seqs, 97)) + [seqs - 1]
+    run = 8 * -(-150 // 64) * 72 * 64
+    raw = cache.data.view(seqs, run)[some].cpu().numpy()
+    k, v = R.unpack(raw, len(some), 8, 64, 150)
+    qn = q[some].double().cpu().numpy()
+    want, _ = R.attention(qn, k, v, [rows[i] for i in some])
+    _, tol = tolerance(qn, k, v, [rows[i] for i in some], "f32")
+    assert np.abs(out[some].double().cpu().numpy() - want).max() <= tol
+
+
 # ---------------------------------------------------------------------------------------------
 # eviction
 # ---------------------------------------------------------------------------------------------
@@ -547,3 +569,55 @@ def test_verify_draws_from_the_target():
     share = torch.bincount(first.long(), minlength=5).double().cpu() / n
     sd = (p * (1 - p) / n).sqrt().double().cpu()
     assert ((share - p.double().cpu()).abs() <= 5 * sd).all(), share
+
+
+# ---------------------------------------------------------------------------------------------
+# the operators together
+# ---------------------------------------------------------------------------------------------
+def example():
+    import importlib.util
+    from pathlib import Path
+    path = Path(__file__).resolve().parents[1] / "examples" / "kv4_session.py"
+    spec = importlib.util.spec_from_file_location("kv4_session", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+def test_a_parked_session_goes_on(tmp_path):
+    """A session's cache in 4 bits and back: the hidden states stay near those of the session that kept fp16.
+    A block's step is 1/8 of its largest magnitude, so a cached value is off by at most 1/16 of it (1/8 for the one
+    opposite the largest); after two layers and a norm the states (of order 1) may differ by a few tenths."""
+    worst, (half, four) = example().park(tmp_path)
+    assert 0 < worst < 1.0
+    assert four * 3 < half * 64 / 48       # 48 rows take a whole tile of 64
+
+
+def test_speculation_over_an_evicting_cache():
+    """The loop against the same loop whose attention is plain torch over the values that the cache stands for."""
+    module = example()
+
+    def plain(cache, q):
+        k, v = (x.permute(0, 2, 1, 3) for x in cache.read(cache.capacity, dtype=torch.float32))
+        streams, n, heads, dim = q.shape
+        group = heads // cache.kv_heads
+        k, v = (x.repeat_interleave(group, 1) for x in (k, v))
+        s = q.permute(0, 2, 1, 3) @ k.transpose(2, 3) / dim ** 0.5
+        seen = cache.rows()[:, None] - n + 1 + torch.arange(n, device="cuda")
+        hidden = torch.arange(cache.capacity, device="cuda") >= seen[..., None]
+        p = s.masked_fill(hidden[:, None], float("-inf")).softmax(-1)
+        cache.weights += p.sum(2).unflatten(1, (cache.kv_heads, group)).sum(2)
+        return (p @ v).permute(0, 2, 1, 3)
+
+    tokens, cache = module.speculate()
+    want, other = module.speculate(attend=plain)
+    assert torch.equal(tokens, want)
+    assert torch.equal(cache.positions[:, :, :48], other.positions[:, :, :48])
+    n = cache.rows().tolist()
+    assert max(n) == 48 and not any(cache.status())
+    # the rows that stay are distinct positions, the last 16 and the first 2 among them
+    last = cache.state[:, 1].tolist()
+    for i in range(4):
+        for h in range(2):
+            held = cache.positions[i, h, :n[i]].tolist()
+            assert len(set(held)) == n[i] and {0, 1} <= set(held) and set(range(last[i] - 16, last[i])) <= set(held)

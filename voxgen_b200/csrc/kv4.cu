@@ -121,6 +121,12 @@ bool paired(const vg_kv4_cache *c, uint32_t heads, uint32_t tokens) {
   const uint64_t rows = (uint64_t)tokens * (heads / c->kv_heads);
   return (rows + 2 * kTileM - 1) / (2 * kTileM) * c->kv_heads * c->seqs >= kPairFrom;
 }
+// The most units of cache rows that a call can have over all its segments.
+uint64_t units_of_call(const vg_kv4_cache *c, uint32_t heads, uint32_t tokens) {
+  const uint64_t rows = (uint64_t)tokens * (heads / c->kv_heads), lanes = (uint64_t)c->kv_heads * c->seqs;
+  if (tiled(c, heads, tokens)) return (rows + kTileM - 1) / kTileM * lanes * ((c->capacity + kTileN - 1) / kTileN);
+  return segments_of(c, heads, tokens) * ((c->capacity + kUnit - 1) / kUnit);
+}
 uint64_t part_bytes(const vg_kv4_cache *c, uint32_t heads, uint32_t tokens) {
   if (tiled(c, heads, tokens)) return (uint64_t)kTileSlots * 2 * kTileM * (c->head_dim + 2) * 4;
   return most_pieces(segments_of(c, heads, tokens)) * kTileRows * (c->head_dim + 2) * 4;
@@ -204,7 +210,7 @@ int vg_k_kv4_attention_bytes(const vg_kv4_cache *cache, uint32_t heads, uint32_t
   if (rc) return rc;
   if (!bytes || !heads || !tokens || heads % cache->kv_heads) return VG_EINVAL;
   if ((uint64_t)heads * tokens > kMaxGrid / cache->seqs) return VG_ERANGE;
-  if (segments_of(cache, heads, tokens) * ((cache->capacity + kUnit - 1) / kUnit) > kMaxGrid) return VG_ERANGE;
+  if (units_of_call(cache, heads, tokens) > kMaxGrid) return VG_ERANGE;   // counted in 32 bits
   *bytes = kTicketBytes + part_bytes(cache, heads, tokens) + (uint64_t)cache->seqs * tokens * heads * 4;
   return VG_OK;
 }
