@@ -5,9 +5,10 @@
 // m16n8k16 MMA: scores are S^T = K Q^T and the output O^T = V^T P^T, with the
 // cache as the A operand. Both K and V come out of the codes with one shift, one
 // lop3 and one fused multiply-add a pair (kv4.cuh), exactly. fp32 queries are
-// fp16 hi + lo, and so is their P, accumulated by a second MMA; 16-bit queries
-// are exact in fp16 (times a power of two) and their P is rounded to 11 bits,
-// like the output. Softmax statistics and sums are fp32.
+// fp16 hi + lo, accumulated by a second MMA; 16-bit queries are exact in fp16
+// (times a power of two). P is hi + lo too, but for bf16, whose output keeps 8
+// bits: rounded to fp16's 11 it would add as much error to an fp16 output as the
+// output's own rounding. Softmax statistics and sums are fp32.
 //
 // The contraction over channels may run in any order as long as both operands
 // agree, so lane (g, t) takes channels [t*D/4, (t+1)*D/4) of its K rows: one wide
@@ -35,6 +36,8 @@
 #pragma once
 #include "kv4_rows.cuh"
 #include "ptx.cuh"
+
+#include <type_traits>
 
 namespace vg {
 
@@ -243,11 +246,11 @@ __device__ __forceinline__ float store_query(const Kv4AttnParams &p, const float
   return fmaxf(p.scale * inverse, 0x1p-126f);
 }
 
-// T: type of q and out; fp32 operands are hi + lo.
+// T: type of q and out.
 template <int D, typename T>
 __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4AttnParams p) {
   using S = RowsSmem<D>;
-  constexpr bool kSplit = sizeof(T) == 4;
+  constexpr bool kSplit = sizeof(T) == 4, kSplitP = !std::is_same<T, __nv_bfloat16>::value;
   constexpr int kSteps = D / 16;                // k-steps of a score, and m-tiles of the output
   constexpr uint32_t kLaneChannels = D / 4;     // of K
   constexpr uint32_t kLaneValues = D / 8;       // channels of V
@@ -402,7 +405,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
         for (int y = 0; y < 2; ++y) {
           const float x0 = exp2_fast(fmaf(c[2 * y], f0, base0)), x1 = exp2_fast(fmaf(c[2 * y + 1], f1, base1));
           l0 += x0, l1 += x1;
-          if constexpr (kSplit) {
+          if constexpr (kSplitP) {
             split2(x0, x1, p_hi[y], p_lo[y]);
             p_lo[y] = transpose8(p_lo[y]);
           } else {
@@ -440,7 +443,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
             for (int z = 0; z < 2; ++z) {
               const uint32_t x[4] = {half2_bits(a[2 * z]), half2_bits(a[2 * z + 1]), half2_bits(b[2 * z]), half2_bits(b[2 * z + 1])};
               mma_f16(o[j * 4 + y * 2 + z], x, p_hi);
-              if constexpr (kSplit) mma_f16(o[j * 4 + y * 2 + z], x, p_lo);
+              if constexpr (kSplitP) mma_f16(o[j * 4 + y * 2 + z], x, p_lo);
             }
           }
         }
