@@ -312,7 +312,7 @@ __device__ __forceinline__ void in_order(const float *o, float4 &low, float4 &hi
 template <int D, typename T, typename Plan>
 __device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const Plan &plan, const TileWork &w, bool pair, uint32_t x,
                                              uint32_t row, uint32_t row0, float m, float l, bool mine, uint32_t o_addr,
-                                             float *shared_o, float (*group_max)[kTileM], float (*group_sum)[kTileM], uint32_t *last) {
+                                             float *shared_o, float (*group_max)[kTileM], float (*group_sum)[kTileM], float *factors, uint32_t *last) {
   const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, rows = p.tokens * p.group;
   const uint32_t block_rows = min(pair ? 2 * kTileM : kTileM, rows - row0);
   const bool whole = w.units == w.seg_units;
@@ -430,60 +430,58 @@ __device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const Plan 
       constexpr uint32_t N = D / 32;   // channels of a lane
       using V = typename std::conditional<N == 4, float4, float2>::type;
       auto piece = [&](uint32_t i) { return (const float *)slot(parts.slot(i)); };
-      constexpr uint32_t kBatch = 4;   // rows of a warp in flight; lanes are pieces, then channels
+      // a thread a row: the weight of each piece, in Q's place, as many rows at a time as it holds
+      const uint32_t some = min(block_rows, 2 * kTileM * D / 2 / pieces);
 #pragma unroll 1
-      for (uint32_t i0 = warp; i0 < block_rows; i0 += 8 * kBatch) {
-        float top[kBatch], sum[kBatch], y[kBatch][N];
-#pragma unroll
-        for (uint32_t b = 0; b < kBatch; ++b) {
-          top[b] = -INFINITY, sum[b] = 0.f;
-#pragma unroll
-          for (uint32_t j = 0; j < N; ++j) y[b][j] = 0.f;
-        }
-#pragma unroll 1
-        for (uint32_t k0 = 0; k0 < pieces; k0 += 32) {
-          const uint32_t n = min(32u, pieces - k0);
-          const float *own = piece(k0 + min(lane, n - 1)) + 2 * kTileM * D;
-          float pw[kBatch];
-#pragma unroll
-          for (uint32_t b = 0; b < kBatch; ++b) {
-            const uint32_t i = min(i0 + 8 * b, block_rows - 1);
-            const float pm = lane < n ? __ldcg(own + i) : -INFINITY, ps = lane < n ? __ldcg(own + 2 * kTileM + i) : 0.f;
-            float up = fmaxf(pm, top[b]);
-#pragma unroll
-            for (int x = 16; x; x >>= 1) up = fmaxf(up, __shfl_xor_sync(~0u, up, x));
-            const float keep = top[b] == -INFINITY ? 0.f : exp2_fast(top[b] - up);
-            pw[b] = pm == -INFINITY ? 0.f : exp2_fast(pm - up);
-            float add = pw[b] * ps;
-#pragma unroll
-            for (int x = 16; x; x >>= 1) add += __shfl_xor_sync(~0u, add, x);
-            sum[b] = sum[b] * keep + add;
-            top[b] = up;
-#pragma unroll
-            for (uint32_t j = 0; j < N; ++j) y[b][j] *= keep;
+      for (uint32_t r0 = 0; r0 < block_rows; r0 += some) {
+        const uint32_t n = min(some, block_rows - r0);
+        if (threadIdx.x < n) {
+          const uint32_t i = r0 + threadIdx.x;
+          float top = -INFINITY, sum = 0.f;
+#pragma unroll 8
+          for (uint32_t k = 0; k < pieces; ++k) {
+            const float pm = __ldcg(piece(k) + 2 * kTileM * D + i);
+            shared_o[k * n + threadIdx.x] = pm;
+            top = fmaxf(top, pm);
           }
-#pragma unroll 2
-          for (uint32_t k = 0; k < n; ++k) {
-            const float *src = piece(k0 + k) + lane * N;
+#pragma unroll 8
+          for (uint32_t k = 0; k < pieces; ++k) {
+            const float ps = __ldcg(piece(k) + 2 * kTileM * (D + 1) + i);
+            const float pm = shared_o[k * n + threadIdx.x], pw = pm == -INFINITY ? 0.f : exp2_fast(pm - top);
+            shared_o[k * n + threadIdx.x] = pw;
+            sum = fmaf(pw, ps, sum);
+          }
+          factors[threadIdx.x] = sum == 0.f ? 0.f : 1.f / sum;
+          if (p.lse) p.lse[place(i)] = lse(top, sum);
+        }
+        __syncwarp();
+        named_bar(2, 256);
+        constexpr uint32_t kBatch = 2;   // rows of a warp in flight
+#pragma unroll 1
+        for (uint32_t i0 = warp; i0 < n; i0 += 8 * kBatch) {
+          float y[kBatch][N] = {};
+#pragma unroll 4
+          for (uint32_t k = 0; k < pieces; ++k) {
 #pragma unroll
             for (uint32_t b = 0; b < kBatch; ++b) {
-              const uint32_t i = min(i0 + 8 * b, block_rows - 1);
-              const float f = __shfl_sync(~0u, pw[b], k);
-              const V z = __ldcg((const V *)(src + i * D));
+              const uint32_t i = min(i0 + 8 * b, n - 1);
+              const V z = __ldcg((const V *)(piece(k) + (r0 + i) * D + lane * N));
+              const float f = shared_o[k * n + i];
 #pragma unroll
-              for (uint32_t j = 0; j < N; ++j) y[b][j] += f * ((const float *)&z)[j];
+              for (uint32_t j = 0; j < N; ++j) y[b][j] = fmaf(f, ((const float *)&z)[j], y[b][j]);
             }
           }
-        }
 #pragma unroll
-        for (uint32_t b = 0; b < kBatch; ++b) {
-          const uint32_t i = i0 + 8 * b;
-          if (i >= block_rows) break;
-          const float f = sum[b] == 0.f ? 0.f : 1.f / sum[b];
+          for (uint32_t b = 0; b < kBatch; ++b) {
+            const uint32_t i = i0 + 8 * b;
+            if (i >= n) break;
+            T *dst = (T *)p.out + place(r0 + i) * D + lane * N;
 #pragma unroll
-          for (uint32_t j = 0; j < N; ++j) ((T *)p.out)[place(i) * D + lane * N + j] = from_float<T>(y[b][j] * f);
-          if (p.lse && lane == 0) p.lse[place(i)] = lse(top[b], sum[b]);
+            for (uint32_t j = 0; j < N; ++j) dst[j] = from_float<T>(y[b][j] * factors[i]);
+          }
         }
+        __syncwarp();
+        named_bar(2, 256);
       }
     }
   }
@@ -852,7 +850,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
       if (mine) wait(&bars.o_full[x], works++ & 1);
       __syncwarp();
       tc_fence_after();
-      tile_results<D, T>(p, plan, w, pair, x, row, row0, m, l, mine, o_addr, (float *)(smem + S::kQ), group_max, group_sum, &last);
+      tile_results<D, T>(p, plan, w, pair, x, row, row0, m, l, mine, o_addr, (float *)(smem + S::kQ), group_max, group_sum, factors, &last);
       tc_fence_before();
     });
   }
