@@ -111,6 +111,9 @@ constexpr uint32_t kMostTickets = 1u << 14;   // segments that may be cut
 // a quarter of a step and a new maximum, however small its lead, is common. P stays below 2^14, and fp16's smallest
 // numbers lie 2^30 below a weight of 1.
 constexpr float kPScale = 6.f, kLead = 8.f;
+// The running maximum of a row that has met no score: finite, so that nothing has to be asked before a subtraction. A row
+// that sees nothing keeps a denominator of 0.
+constexpr float kNoScore = -3e38f;
 
 template <int D>
 constexpr uint32_t kPart = kTileRows * (D + 2);   // floats of a partial result: values, maxima, denominators
@@ -136,7 +139,7 @@ __host__ __device__ __forceinline__ uint64_t most_pieces(uint64_t segments) {
 __device__ __forceinline__ uint32_t units_of(uint32_t rows) { return max(1u, (rows + kUnit - 1) / kUnit); }
 
 // How segments are cut: `lanes` segments a sequence, pieces of `size` units, and
-// how many pieces there are. Every warp plans for itself.
+// how many pieces there are. A warp's work.
 struct Plan {
   uint32_t lanes, size, pieces;
 };
@@ -264,8 +267,16 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
   __shared__ __align__(8) uint32_t seens[kTileRows];
   const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
   if (p.lse) pdl_launch_dependents();   // the weights kernel may take the SMs that this one leaves
-  const Plan plan = make_plan(p.c, p.c.kv_heads * p.row_tiles);
-  if (blockIdx.x >= plan.pieces) return;
+  __shared__ Plan shared_plan;
+  __shared__ Piece shared_piece;
+  if (warp == 0) {
+    const Plan x = make_plan(p.c, p.c.kv_heads * p.row_tiles);
+    if (lane == 0) shared_plan = x;
+    if (blockIdx.x < x.pieces) {
+      const Piece y = find_piece(p.c, x, blockIdx.x);
+      if (lane == 0) shared_piece = y;
+    }
+  }
   const size_t run_bytes = (size_t)p.c.tiles * Kv4<D>::kTileBytes;
   uint8_t *ring = smem + warp * kRowsStages * S::kStage;
   float *merge = (float *)(smem + S::kRing);
@@ -273,7 +284,9 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
   if (lane == 0)
     for (uint32_t i = 0; i < kRowsStages; ++i) mbar_init(&bars[warp][i], 1);
   fence_mbar_init();
-  __syncwarp();
+  __syncthreads();
+  const Plan plan = shared_plan;
+  if (blockIdx.x >= plan.pieces) return;
 
   uint32_t stage = 0, parity = 0, fetch_stage = 0;
   bool timed_out = false;
@@ -299,7 +312,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
     fetch_stage = fetch_stage + 1 == kRowsStages ? 0 : fetch_stage + 1;
   };
 
-  Piece seg = find_piece(p.c, plan, blockIdx.x);
+  Piece seg = shared_piece;
   uint32_t ahead = warp;    // next unit of the piece to fetch
 #pragma unroll 1
   for (uint32_t i = 0; i < kRowsStages && ahead < seg.units; ++i, ahead += kRowsWarps) fetch(seg, ahead);
@@ -331,7 +344,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
     const uint32_t seen0 = seens[2 * t], seen1 = seens[2 * t + 1];
     const uint32_t least = min(seens[0], seens[tile_rows - 1]);   // every row sees these
 
-    float o[kSteps][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    float o[kSteps][4], m0 = kNoScore, m1 = kNoScore, l0 = 0.f, l1 = 0.f;
 #pragma unroll
     for (int j = 0; j < kSteps; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 
@@ -393,13 +406,13 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
             top1 = fmaxf(top1, __shfl_xor_sync(~0u, top1, x));
           }
           top0 = fmaxf(top0, m0), top1 = fmaxf(top1, m1);
-          const float r0 = top0 == m0 ? 1.f : exp2_fast(m0 - top0), r1 = top1 == m1 ? 1.f : exp2_fast(m1 - top1);
+          const float r0 = exp2_fast(m0 - top0), r1 = exp2_fast(m1 - top1);
           m0 = top0, m1 = top1;
           l0 *= r0, l1 *= r1;
 #pragma unroll
           for (int j = 0; j < kSteps; ++j) o[j][0] *= r0, o[j][1] *= r1, o[j][2] *= r0, o[j][3] *= r1;
         }
-        const float base0 = kPScale - (m0 == -INFINITY ? 0.f : m0), base1 = kPScale - (m1 == -INFINITY ? 0.f : m1);
+        const float base0 = kPScale - m0, base1 = kPScale - m1;
         uint32_t p_hi[2], p_lo[2];
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
@@ -465,7 +478,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
       *(float2 *)&w_sum[warp][2 * t] = make_float2(l0, l1);
     }
     __syncthreads();
-    float top0 = -INFINITY, top1 = -INFINITY;
+    float top0 = kNoScore, top1 = kNoScore;
 #pragma unroll
     for (uint32_t w = 0; w < kRowsWarps; ++w) {
       const float2 x = *(const float2 *)&w_max[w][2 * t];
@@ -474,7 +487,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
     // [warp][query row][channel], 16-byte chunks of a lane's channels turned by its query rows: no bank conflicts
     constexpr uint32_t kChunks = kLaneValues / 4;
     {
-      const float e0 = m0 == -INFINITY ? 0.f : exp2_fast(m0 - top0), e1 = m1 == -INFINITY ? 0.f : exp2_fast(m1 - top1);
+      const float e0 = exp2_fast(m0 - top0), e1 = exp2_fast(m1 - top1);
       float4 *dst = (float4 *)(merge + (warp * kTileRows + 2 * t) * D + g * kLaneValues);
 #pragma unroll
       for (uint32_t i = 0; i < kChunks; ++i) {
@@ -488,8 +501,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
       float all = 0.f;
 #pragma unroll
       for (uint32_t w = 0; w < kRowsWarps; ++w) {
-        const float wm = w_max[w][2 * t + g];
-        all += w_sum[w][2 * t + g] * (wm == -INFINITY ? 0.f : exp2_fast(wm - top));
+        all += w_sum[w][2 * t + g] * exp2_fast(w_max[w][2 * t + g] - top);
       }
       f_max[2 * t + g] = top;
       f_sum[2 * t + g] = all;
@@ -542,7 +554,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
         float *weight = merge;   // [pieces][kTileRows]
         auto piece = [&](uint32_t i) { return others + (size_t)i * kPart<D>; };
         if (warp < tile_rows) {   // a warp a query row, its lanes the pieces
-          float top = -INFINITY, all = 0.f;
+          float top = kNoScore, all = 0.f;
 #pragma unroll 1
           for (uint32_t i = lane; i < pieces; i += 32) {
             const float m = __ldcg(piece(i) + kTileRows * D + warp);
@@ -554,7 +566,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
 #pragma unroll 1
           for (uint32_t i = lane; i < pieces; i += 32) {
             const float m = weight[i * kTileRows + warp], sum = __ldcg(piece(i) + kTileRows * (D + 1) + warp);
-            const float w = m == -INFINITY ? 0.f : exp2_fast(m - top);
+            const float w = exp2_fast(m - top);
             all += w * sum;
             weight[i * kTileRows + warp] = w;
           }
