@@ -52,10 +52,13 @@ def _stream(stream, index: int) -> int:
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _on_its_device(call):
     """Runs a method with the cache's device as the current one."""
     def run(self, *args, **kwargs):
-        if torch.cuda.current_device() == self._index:
+        if _current_device() == self._index:
             return call(self, *args, **kwargs)
         with torch.cuda.device(self._index):
             return call(self, *args, **kwargs)
@@ -159,8 +162,8 @@ class Kv4Cache:
         """Stores new K and V rows ``[seqs, tokens, kv_heads, head_dim]`` from row ``at[s]`` on (default: after
         the rows held); ``counts[s]`` says how many of them a sequence has (default: all)."""
         dtype = self._rows_of(k, self.kv_heads, "k")
-        if self._rows_of(v, self.kv_heads, "v") != dtype or v.shape != k.shape:
-            raise _invalid("k and v must agree in shape and type")
+        if v.shape != k.shape or v.dtype is not k.dtype or v.device != self.device:
+            raise _invalid("k and v must agree in shape, type and device")
         tokens = k.shape[1]
         rc = self._lib.vg_k_kv4_append(
             self._ref, k.data_ptr(), v.data_ptr(), dtype, tokens, _strides(k), _strides(v),
@@ -279,7 +282,7 @@ def verify_draft(tokens: torch.Tensor, draft: torch.Tensor, target: torch.Tensor
             raise _invalid(f"verify_draft: {what} must be contiguous {dtype} {list(shape)} on {device}")
     if device.type != "cuda":
         raise _invalid("verify_draft runs on a CUDA device")
-    if torch.cuda.current_device() != device.index:
+    if _current_device() != device.index:
         with torch.cuda.device(device):
             return verify_draft(tokens, draft, target, u_accept, u_sample, counts=counts, stream=stream)
     accepted, token = tokens.new_empty((2, seqs)).unbind()
