@@ -372,6 +372,31 @@ def test_other_streams_and_graphs(tokens):
     assert torch.equal(got.state, want.state)
 
 
+def test_a_stream_as_an_argument():
+    """Each call on a given stream, as a torch stream or its address, from another current stream."""
+    k, v, q = normal(1, 2, 3, 2, 64), normal(2, 2, 3, 2, 64), normal(3, 2, 3, 8, 64)
+    want = filled(91, [70, 20], 2, 64, 128, track=True)
+    want.append(k, v)
+    reference, rows = want.attention(q), want.read(80)
+    want.evict(40, 8, 2)
+    side = torch.cuda.Stream()
+    for stream in (side, side.cuda_stream):
+        got = filled(91, [70, 20], 2, 64, 128, track=True)
+        side.wait_stream(torch.cuda.current_stream())
+        got.append(k, v, stream=stream)
+        out = got.attention(q, stream=stream)
+        read = got.read(80, stream=stream)
+        got.evict(40, 8, 2, stream=stream)
+        p = torch.full((2, 3, 7), 1 / 7, device="cuda")
+        side.wait_stream(torch.cuda.current_stream())
+        accepted, token = kv4.verify_draft(ints(1, 2, 3, 4).view(2, 2), p[:, :2].contiguous(), p,
+                                           torch.zeros(2, 2, device="cuda"), torch.zeros(2, device="cuda"), stream=stream)
+        torch.cuda.synchronize()
+        assert torch.equal(out, reference) and torch.equal(got.state, want.state) and torch.equal(got.weights, want.weights)
+        assert all(torch.equal(a, b) for a, b in zip(read, rows))
+        assert accepted.tolist() == [2, 2] and token.tolist() == [0, 0]
+
+
 def test_one_workspace_serves_calls_of_any_shape():
     cache = filled(61, [500, 90], 2, 128, 512, track=True)
     fresh = filled(61, [500, 90], 2, 128, 512, track=True)

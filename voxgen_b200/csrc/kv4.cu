@@ -80,13 +80,19 @@ int by_dim(uint32_t head_dim, F &&f) {
 }
 
 // Lets fn use up to `bytes` of dynamic shared memory on the current device. `done`
-// belongs to fn: the devices (up to 64) on which that has been set.
-int allow_smem(const void *fn, size_t bytes, std::atomic<uint64_t> &done) {
+// belongs to fn: the devices (up to 64) on which that has been set. `registers`: the
+// fewest registers of a thread that fn may have been compiled to; the tile kernel's
+// warpgroups trade theirs, and if they took more in all than the launch brings, the
+// takers would wait for good.
+int allow_smem(const void *fn, size_t bytes, std::atomic<uint64_t> &done, int registers = 0) {
   if (bytes <= 48 * 1024) return VG_OK;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return VG_ECUDA;
   const uint64_t bit = dev < 64 ? 1ull << dev : 0;
   if (bit && done.load(std::memory_order_acquire) & bit) return VG_OK;
+  cudaFuncAttributes a;
+  if (cudaFuncGetAttributes(&a, fn) != cudaSuccess) return VG_ECUDA;
+  if (a.numRegs < registers) return VG_EUNSUPPORTED;
   if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return VG_ECUDA;
   done.fetch_or(bit, std::memory_order_release);
   return VG_OK;
@@ -256,7 +262,7 @@ int vg_k_kv4_attention(const vg_kv4_cache *cache, const void *q, int dtype, uint
       static std::atomic<uint64_t> done[3];
       if (tile) {
         const auto go = [&](auto fn, std::atomic<uint64_t> &set) {
-          const int e = allow_smem((const void *)fn, TileSmem<D>::kBytes, set);
+          const int e = allow_smem((const void *)fn, TileSmem<D>::kBytes, set, (kSoftmaxRegs + kOtherRegs) / 2);
           if (!e) fn<<<kTileCtas, kTileThreads, TileSmem<D>::kBytes, st>>>(p);
           return e;
         };

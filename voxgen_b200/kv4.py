@@ -46,21 +46,25 @@ _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _stream(stream, index: int) -> int:
-    if stream is None:
-        return _current_stream(index)
-    return stream if isinstance(stream, int) else stream.cuda_stream
-
-
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
+def _on(device, stream):
+    """A context in which ``device`` is current, and ``stream`` (an address or a torch stream) when one is given."""
+    if stream is None:
+        return torch.cuda.device(device)
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device=device)
+    return torch.cuda.stream(stream)
+
+
 def _on_its_device(call):
-    """Runs a method with the cache's device as the current one."""
-    def run(self, *args, **kwargs):
-        if _current_device() == self._index:
+    """Runs a method with the cache's device as the current one, on ``stream`` when one is given: what it allocates
+    then belongs to that stream too."""
+    def run(self, *args, stream=None, **kwargs):
+        if stream is None and _current_device() == self._index:
             return call(self, *args, **kwargs)
-        with torch.cuda.device(self._index):
+        with _on(self.device, stream):
             return call(self, *args, **kwargs)
     return functools.wraps(call)(run)
 
@@ -158,7 +162,7 @@ class Kv4Cache:
 
     @_on_its_device
     def append(self, k: torch.Tensor, v: torch.Tensor, *, at: Optional[torch.Tensor] = None,
-               counts: Optional[torch.Tensor] = None, stream=None) -> None:
+               counts: Optional[torch.Tensor] = None) -> None:
         """Stores new K and V rows ``[seqs, tokens, kv_heads, head_dim]`` from row ``at[s]`` on (default: after
         the rows held); ``counts[s]`` says how many of them a sequence has (default: all)."""
         dtype = self._rows_of(k, self.kv_heads, "k")
@@ -168,27 +172,27 @@ class Kv4Cache:
         rc = self._lib.vg_k_kv4_append(
             self._ref, k.data_ptr(), v.data_ptr(), dtype, tokens, _strides(k), _strides(v),
             _ints(at, self.seqs, self.device, "at"), _ints(counts, self.seqs, self.device, "counts"),
-            _stream(stream, self._index))
+            _current_stream(self._index))
         if rc:
             raise VoxGenError(rc, f"append of {tokens} rows to a cache of {self.capacity}")
 
     @_on_its_device
-    def read(self, tokens: int, *, first: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.float16,
-             stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    def read(self, tokens: int, *, first: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.float16
+             ) -> Tuple[torch.Tensor, torch.Tensor]:
         """Values of rows ``first[s] .. first[s] + tokens - 1`` (default: from row 0), K and V; rows that are not
         held read as 0."""
         if dtype not in DTYPES:
             raise VoxGenError(-4, f"{dtype} is not supported")
         k, v = self.data.new_empty((2, self.seqs, tokens, self.kv_heads, self.head_dim), dtype=dtype).unbind()
         rc = self._lib.vg_k_kv4_read(self._ref, _ints(first, self.seqs, self.device, "first"), tokens, DTYPES[dtype],
-                                     k.data_ptr(), v.data_ptr(), _stream(stream, self._index))
+                                     k.data_ptr(), v.data_ptr(), _current_stream(self._index))
         if rc:
             raise VoxGenError(rc, f"read of {tokens} rows")
         return k, v
 
     # -- attention --------------------------------------------------------------------------
-    def _work(self, heads: int, tokens: int, stream) -> torch.Tensor:
-        """The workspace, large enough for the call; zeroed on the stream that is to use it."""
+    def _work(self, heads: int, tokens: int) -> torch.Tensor:
+        """The workspace, large enough for the call; zeroed on the current stream."""
         need = self._need.get((heads, tokens))
         if need is None:
             n = C.c_uint64()
@@ -196,20 +200,15 @@ class Kv4Cache:
                    f"attention of {heads} heads over {self.kv_heads} KV heads, {tokens} tokens")
             need = self._need[heads, tokens] = n.value
         ws = self._workspace
-        if ws is not None and ws.numel() >= need:
-            return ws
-        on = torch.cuda.current_stream(self._index)
-        if stream is not None:
-            on = torch.cuda.ExternalStream(_stream(stream, self._index), device=self.device)
-        if ws is not None:
-            ws.record_stream(on)
-        with torch.cuda.stream(on):
-            self._workspace = torch.zeros(need, dtype=torch.uint8, device=self.device)
-        return self._workspace
+        if ws is None or ws.numel() < need:
+            if ws is not None:
+                ws.record_stream(torch.cuda.current_stream(self._index))
+            ws = self._workspace = torch.zeros(need, dtype=torch.uint8, device=self.device)
+        return ws
 
     @_on_its_device
     def attention(self, q: torch.Tensor, *, counts: Optional[torch.Tensor] = None, scale: Optional[float] = None,
-                  track: Optional[bool] = None, out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+                  track: Optional[bool] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Attention of the last ``tokens`` rows' queries ``[seqs, tokens, heads, head_dim]``, causal within them.
 
         Adds the attention that each row draws to ``weights`` when the cache tracks it (``track=False`` leaves
@@ -226,24 +225,23 @@ class Kv4Cache:
             track = self.weights is not None
         elif track and self.weights is None:
             raise _invalid("this cache does not track attention")
-        ws = self._work(heads, tokens, stream)
+        ws = self._work(heads, tokens)
         rc = self._lib.vg_k_kv4_attention(
             self._ref, q.data_ptr(), dtype, heads, tokens, _strides(q),
             _ints(counts, self.seqs, self.device, "counts"), self._scale if scale is None else scale, track,
-            out.data_ptr(), ws.data_ptr(), ws.numel(), _stream(stream, self._index))
+            out.data_ptr(), ws.data_ptr(), ws.numel(), _current_stream(self._index))
         if rc:
             raise VoxGenError(rc, f"attention of {tokens} tokens, {heads} heads")
         return out
 
     # -- eviction ---------------------------------------------------------------------------
     @_on_its_device
-    def evict(self, budget: int, recent: int = 0, sinks: int = 0, *, into: Optional["Kv4Cache"] = None,
-              stream=None) -> None:
+    def evict(self, budget: int, recent: int = 0, sinks: int = 0, *, into: Optional["Kv4Cache"] = None) -> None:
         """Cuts sequences that hold more than ``budget`` rows to it: the last ``recent`` and first ``sinks``
         positions stay, and the rest that drew the most attention. ``into``: a cache over the same ``data``
         whose state, weights and positions receive the result instead."""
         rc = self._lib.vg_k_kv4_evict(self._ref, budget, recent, sinks, None if into is None else into._ref,
-                                      _stream(stream, self._index))
+                                      _current_stream(self._index))
         if rc:
             raise VoxGenError(rc, f"eviction to {budget} rows ({recent} recent, {sinks} sinks) of a cache of "
                               f"{self.capacity}" + ("" if self.weights is not None else " that does not track attention"))
@@ -282,14 +280,14 @@ def verify_draft(tokens: torch.Tensor, draft: torch.Tensor, target: torch.Tensor
             raise _invalid(f"verify_draft: {what} must be contiguous {dtype} {list(shape)} on {device}")
     if device.type != "cuda":
         raise _invalid("verify_draft runs on a CUDA device")
-    if _current_device() != device.index:
-        with torch.cuda.device(device):
-            return verify_draft(tokens, draft, target, u_accept, u_sample, counts=counts, stream=stream)
+    if stream is not None or _current_device() != device.index:
+        with _on(device, stream):
+            return verify_draft(tokens, draft, target, u_accept, u_sample, counts=counts)
     accepted, token = tokens.new_empty((2, seqs)).unbind()
     rc = api.lib().vg_k_verify_draft(
         tokens.data_ptr(), draft.data_ptr(), target.data_ptr(), u_accept.data_ptr(), u_sample.data_ptr(),
         _ints(counts, seqs, device, "counts"), seqs, drafted, vocab, accepted.data_ptr(), token.data_ptr(),
-        _stream(stream, device.index))
+        _current_stream(device.index))
     if rc:
         raise VoxGenError(rc, f"verification of {drafted} tokens of a vocabulary of {vocab}")
     return accepted, token
