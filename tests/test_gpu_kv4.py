@@ -456,6 +456,28 @@ def test_more_sequences_than_can_be_cut():
     assert np.abs(out[some].double().cpu().numpy() - want).max() <= tol
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_long_accumulation(dtype):
+    """Dozens of cache tiles in one CTA, some tokens past their count. Tensor-core sums round towards zero, so a long
+    fp32 accumulation would drift: 2^-22 of the result for a tile, of which 4 are summed before a sum that rounds to
+    nearest takes over (2^-20), fp32 sums and 22-bit operands beside it: 2^-18 of the result in the 2-norm. Rounding P
+    and the output to fp16 adds 2^-11."""
+    seqs, tokens = 30, 40
+    counts = [(40, 5, 0)[i % 3] for i in range(seqs)]
+    cache = filled(83, [4000] * seqs, 8, 64, 4000)
+    q = normal(84, seqs, tokens, 8, 64, dtype=TYPES[dtype])
+    out = cache.attention(q, counts=ints(*counts))
+    assert torch.equal(out, cache.attention(q, counts=ints(*counts)))
+    some = [0, 1, 2, 16, 28, 29]
+    raw = cache.data.view(seqs, -1)[some].cpu().numpy()
+    k, v = R.unpack(raw, len(some), 8, 64, 4000)
+    want, _ = R.attention(q[some].double().cpu().numpy(), k, v, [4000] * len(some), [counts[i] for i in some])
+    got = out[some].double().cpu().numpy()
+    assert not got[want == 0].any()
+    tol = 2.0 ** -18 + (2.0 ** -11 if dtype == "f16" else 0)
+    assert np.linalg.norm(got - want) <= tol * np.linalg.norm(want)
+
+
 # ---------------------------------------------------------------------------------------------
 # eviction
 # ---------------------------------------------------------------------------------------------

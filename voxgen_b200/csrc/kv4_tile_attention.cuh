@@ -43,6 +43,11 @@ constexpr uint32_t kTileThreads = 512;          // 8 softmax warps, 4 that unpac
 constexpr uint32_t kUnpackThreads = 128;
 // registers of a thread: 512 x 128 at launch, then 2 x 168 + 2 x 88 for the four warpgroups
 constexpr uint32_t kSoftmaxRegs = 168, kOtherRegs = 88;
+// The products' accumulation rounds towards zero, about 2^-22 of O for a tile of hi and lo. For fp32 queries O therefore
+// starts afresh every kFreshTiles tiles of a group, and what it was is added, with rounding to nearest, to a sum in global
+// memory (it stays in L2): a prompt of 512 tokens over 32768 rows was off by 1.5e-5 of its result, and is by 2e-6 (the
+// plain fp32 form by 3e-6). 16-bit results keep 11 bits or fewer and need none of this.
+constexpr uint32_t kFreshTiles = 4;
 constexpr uint32_t kSwitchUnits = 8;            // what changing segments costs, in units
 constexpr uint32_t kTileCtas = 148;
 constexpr uint32_t kTileSlots = 2 * kTileCtas;  // partial results
@@ -312,6 +317,7 @@ __device__ __forceinline__ void in_order(const float *o, float4 &low, float4 &hi
 template <int D, typename T, typename Plan>
 __device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const Plan &plan, const TileWork &w, bool pair, uint32_t x,
                                              uint32_t row, uint32_t row0, float m, float l, bool mine, uint32_t o_addr,
+                                             const float *kept, float kept_scale,
                                              float *shared_o, float (*group_max)[kTileM], float (*group_sum)[kTileM], float *factors, uint32_t *last) {
   const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, rows = p.tokens * p.group;
   const uint32_t block_rows = min(pair ? 2 * kTileM : kTileM, rows - row0);
@@ -345,11 +351,11 @@ __device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const Plan 
   };
   if (!pair) {
     constexpr uint32_t kChunks = D / 4;
-    group_max[x][row] = mine ? m : -INFINITY;
+    group_max[x][row] = mine ? m : kNoScore;
     group_sum[x][row] = mine ? l : 0.f;
     named_bar(2, 256);
     const float m0 = group_max[0][row], m1 = group_max[1][row], top = fmaxf(m0, m1);
-    const float w0 = m0 == -INFINITY ? 0.f : exp2_fast(m0 - top), w1 = m1 == -INFINITY ? 0.f : exp2_fast(m1 - top);
+    const float w0 = exp2_fast(m0 - top), w1 = exp2_fast(m1 - top);
     l = group_sum[0][row] * w0 + group_sum[1][row] * w1;
     m = top;
     const float f = (x ? w1 : w0) * (!whole ? 1.f : l == 0.f ? 0.f : 1.f / l);
@@ -364,6 +370,10 @@ __device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const Plan 
         tmem_load32(o_addr + c, o);
         tmem_wait_load();
         loaded(o);
+        if (sizeof(T) == 4 && kept) {
+#pragma unroll
+          for (uint32_t i = 0; i < 32; ++i) o[i] = fmaf(kept[(c + i) * kTileM + row], kept_scale, o[i]);
+        }
 #pragma unroll
         for (uint32_t i = 0; i < 32; i += 8) {
           float4 v[2];
@@ -437,7 +447,7 @@ __device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const Plan 
         const uint32_t n = min(some, block_rows - r0);
         if (threadIdx.x < n) {
           const uint32_t i = r0 + threadIdx.x;
-          float top = -INFINITY, sum = 0.f;
+          float top = kNoScore, sum = 0.f;
 #pragma unroll 8
           for (uint32_t k = 0; k < pieces; ++k) {
             const float pm = __ldcg(piece(k) + 2 * kTileM * D + i);
@@ -447,7 +457,7 @@ __device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const Plan 
 #pragma unroll 8
           for (uint32_t k = 0; k < pieces; ++k) {
             const float ps = __ldcg(piece(k) + 2 * kTileM * (D + 1) + i);
-            const float pm = shared_o[k * n + threadIdx.x], pw = pm == -INFINITY ? 0.f : exp2_fast(pm - top);
+            const float pw = exp2_fast(shared_o[k * n + threadIdx.x] - top);
             shared_o[k * n + threadIdx.x] = pw;
             sum = fmaf(pw, ps, sum);
           }
@@ -590,7 +600,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
 #pragma unroll
                 for (uint32_t c = half * 4; c < half * 4 + 4; ++c) {
                   const uint64_t b = operand(va, c * 2048);
-                  mma_ts(d, pa + c * 8, b, kValueDesc, c > 0 || i > 1);
+                  mma_ts(d, pa + c * 8, b, kValueDesc, c > 0 || (kSplit ? i / 2 % kFreshTiles != 0 : i > 1));
                   if constexpr (kSplit) mma_ts(d, pa + 64 + c * 8, b, kValueDesc, true);
                 }
               }
@@ -769,13 +779,36 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
       const bool used_row = row0 + qr < rows;
       uint32_t least = used_row ? seen : 0xFFFFFFFFu;              // fewest of the warp's rows
       least = __reduce_min_sync(~0u, least);
-      float m = -INFINITY, l = 0.f;
+      float m = kNoScore, l = 0.f;
+      // fp32: the sum of earlier O, [channel][row] in the half of a partial result that 128-row blocks do not use, and the
+      // maximum that it is relative to
+      float *const kept = p.parts + (size_t)(blockIdx.x * 2 + x) * kTilePart<D> + kTileM * D;
+      float kept_max = 0.f;
+      bool keeping = false;
       const uint32_t step = pair ? 1 : 2;
 #pragma unroll 1
       for (uint32_t u = pair ? 0 : x; u < w.units; u += step, ++done) {
         wait(&bars.s_full[x], done & 1);
         __syncwarp();
         tc_fence_after();
+        const bool fresh = kSplit ? u / 2 % kFreshTiles == 0 : u < step;   // nothing in O counts
+        if (kSplit && fresh && u >= step) {   // O is whole: the products before these scores are done
+          const float r = exp2_fast(kept_max - m);
+#pragma unroll 1
+          for (uint32_t c = 0; c < D; c += 32) {
+            float o[32];
+            tmem_load32(o_addr + c, o);
+            tmem_wait_load();
+            loaded(o);
+#pragma unroll
+            for (uint32_t i = 0; i < 32; ++i) {
+              float *at = kept + (c + i) * kTileM + row;
+              *at = keeping ? fmaf(*at, r, o[i]) : o[i];
+            }
+          }
+          kept_max = m;
+          keeping = true;
+        }
         float s[kTileN];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_load32(s_addr + c * 32, s + c * 32);
@@ -796,10 +829,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
         for (int i = 0; i < 4; ++i) top[i] = fmaxf(top[i], s[kTileN - 4 + i]);
         const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f;
         if (__any_sync(~0u, best > m + kLead)) {
-          const float up = fmaxf(m, best), r = up == m ? 1.f : exp2_fast(m - up);
+          const float up = fmaxf(m, best), r = exp2_fast(m - up);
           m = up;
           l *= r;
-          if (u >= step) {   // O has something: the products before these scores are done
+          if (!fresh) {   // O has something: the products before these scores are done
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
               uint32_t o[16];
@@ -817,7 +850,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
             }
           }
         }
-        const float base = kTilePScale - (m == -INFINITY ? 0.f : m);
+        const float base = kTilePScale - m;
         const float2 f2 = make_float2(f, f), base2 = make_float2(base, base);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -850,7 +883,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
       if (mine) wait(&bars.o_full[x], works++ & 1);
       __syncwarp();
       tc_fence_after();
-      tile_results<D, T>(p, plan, w, pair, x, row, row0, m, l, mine, o_addr, (float *)(smem + S::kQ), group_max, group_sum, factors, &last);
+      tile_results<D, T>(p, plan, w, pair, x, row, row0, m, l, mine, o_addr, keeping ? kept : nullptr, exp2_fast(kept_max - m),
+                         (float *)(smem + S::kQ), group_max, group_sum, factors, &last);
       tc_fence_before();
     });
   }
