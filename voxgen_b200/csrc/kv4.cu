@@ -98,11 +98,12 @@ int allow_smem(const void *fn, size_t bytes, std::atomic<uint64_t> &done, int re
   return VG_OK;
 }
 
-// Blocks of a sequence for `items` (token, head) pairs: enough for every SM to be
-// full (8 blocks each), no more than have a pass to make.
-uint32_t row_blocks(uint64_t items, uint32_t per_block, uint32_t seqs) {
-  const uint64_t most = (items + per_block - 1) / per_block, full = (148 * 8 + seqs - 1) / seqs;
-  return (uint32_t)std::min(most, full);
+// Blocks of a sequence for `items` (token, head) pairs: no more than have a pass to
+// make, and no more in all than are resident at once (per_sm of them on each SM),
+// so that no second wave runs with a few.
+uint32_t row_blocks(uint64_t items, uint32_t per_block, uint32_t seqs, uint32_t per_sm) {
+  const uint64_t most = (items + per_block - 1) / per_block;
+  return (uint32_t)std::min<uint64_t>(most, std::max(1u, 148 * per_sm / seqs));
 }
 
 // Attention workspace: counters (zero between calls, at the same place for every
@@ -172,7 +173,7 @@ int vg_k_kv4_append(const vg_kv4_cache *cache, const void *k, const void *v, int
   const uint64_t items = (uint64_t)tokens * cache->kv_heads;
   const uint32_t per_block = kRowThreads / (cache->head_dim / 16);
   if (items > kMaxGrid) return VG_ERANGE;
-  p.blocks = row_blocks(items, per_block, cache->seqs);
+  p.blocks = row_blocks(items, per_block, cache->seqs, kAppendBlocks);
   const bool vec = wide(k, p.ks, size) && wide(v, p.vs, size);
   const dim3 grid(p.blocks * cache->seqs);
   const cudaStream_t st = (cudaStream_t)cuda_stream;
@@ -200,7 +201,7 @@ int vg_k_kv4_read(const vg_kv4_cache *cache, const int32_t *first, uint32_t toke
   const uint32_t per_block = kRowThreads / (cache->head_dim / 8);
   const uint64_t items = (uint64_t)tokens * cache->kv_heads;
   if (items > kMaxGrid) return VG_ERANGE;
-  p.blocks = row_blocks(items, per_block, cache->seqs);
+  p.blocks = row_blocks(items, per_block, cache->seqs, 8);
   const dim3 grid(p.blocks * cache->seqs);
   return by_dim(cache->head_dim, [&](auto d) {
     return by_type(dtype, [&](auto t) {

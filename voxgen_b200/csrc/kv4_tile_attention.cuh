@@ -27,6 +27,11 @@
 // cache tile of one query tile and their results are added at the end. The
 // products of one group run while the other does its softmax.
 //
+// Measured: the last 4096 tokens of a prompt over 32768 rows, fp16, 1.03 TFLOP: 987 us,
+// 1.04 PFLOP/s (63% of the measured burst rate). A unit of 256 query rows takes about
+// 4100 cycles, of which the products need 2048 and the softmax's 32768 exponentials as
+// many; the two wait for each other through S, whose place P takes.
+//
 // The split. A segment is a block of query rows of a (sequence, KV head) with the
 // cache rows it sees, in units of 128. Few segments are cut into pieces of equal
 // size, about one for each CTA, since changing segments costs several units; many
