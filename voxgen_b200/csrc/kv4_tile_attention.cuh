@@ -174,13 +174,15 @@ __device__ __forceinline__ uint32_t tile_units(const Kv4AttnParams &p, uint32_t 
   const int32_t seen = (int32_t)held - count + tok + 1;
   return (uint32_t)(max(seen, 1) + (int32_t)kTileN - 1) / kTileN;
 }
-// Every warp plans for itself, all lanes together.
-template <uint32_t kRows>
-struct TilePlan {
-  const Kv4AttnParams &p;
+struct TileDeal {
   uint32_t blocks, ctas;
   uint32_t each, more, begin, end;   // dealt out: units of a CTA, the first `more` with one more; this CTA's
   uint32_t size, pieces;             // cut: units of a piece (0: dealt out), pieces
+};
+// One warp plans for the CTA, all lanes together; the others take the result.
+template <uint32_t kRows>
+struct TilePlan : TileDeal {
+  const Kv4AttnParams &p;
 
   __device__ uint32_t pieces_of(uint32_t i, uint32_t of) const {
     return i < blocks ? (tile_units<kRows>(p, i / p.row_tiles, i % p.row_tiles) + of - 1) / of : 0u;
@@ -191,7 +193,10 @@ struct TilePlan {
     for (uint32_t i = threadIdx.x % 32; i < blocks; i += 32) n += pieces_of(i, of);
     return __reduce_add_sync(~0u, n) * p.c.kv_heads;
   }
-  __device__ explicit TilePlan(const Kv4AttnParams &p) : p(p), blocks(p.c.seqs * p.row_tiles), size(0), pieces(0) {
+  __device__ TilePlan(const Kv4AttnParams &p, const TileDeal &d) : TileDeal(d), p(p) {}
+  __device__ explicit TilePlan(const Kv4AttnParams &p) : p(p) {
+    blocks = p.c.seqs * p.row_tiles;
+    size = pieces = 0;
     const uint32_t total = sum_of(1), fair = (total + kTileCtas - 1) / kTileCtas;
     // cut where one or two pieces a CTA share the work about as well as dealing it out does
     const uint32_t segments = blocks * p.c.kv_heads, rounds = segments * 4 <= kTileCtas * 3 ? 1 : 2;
@@ -520,10 +525,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
   const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const uint32_t rows = p.tokens * p.group;
   if (p.lse) pdl_launch_dependents();   // the weights kernel may take the SMs that this one leaves
-  const TilePlan<kRows> plan(p);
-  if (blockIdx.x >= plan.ctas) return;
-
-  if (threadIdx.x == 0) {
+  __shared__ TileDeal shared_deal;
+  __shared__ TileWork shared_work;
+  if (warp == 0) {
+    const TilePlan<kRows> x(p);
+    if (lane == 0) shared_deal = x;
+    if (blockIdx.x < x.ctas) {
+      const TileWork y = x.start();
+      if (lane == 0) shared_work = y;
+    }
+  }
+  if (threadIdx.x == 32) {
     mbar_init(&bars.q_full, 256);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.s_full[i], 1);
@@ -545,6 +557,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *(volatile uint32_t *)&tmem_base;
+  const TilePlan<kRows> plan(p, shared_deal);
+  if (blockIdx.x >= plan.ctas) {   // nothing for this CTA
+    if (warp == 12) tmem_free512(tmem);
+    return;
+  }
   // a wait that runs out makes every later one return at once: the roles then run to their ends on whatever is there
   auto wait = [&](uint64_t *bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity) || *(volatile uint32_t *)&aborted) return;
@@ -553,7 +570,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
   // two query tiles, or one whose cache tiles the softmax groups share
   auto paired = [&](const TileWork &w) { return PAIR && rows - w.block * kRows > kTileM; };
   // f(work) for every piece of this CTA; whole warps
-  const TileWork first_work = plan.start();
+  const TileWork first_work = shared_work;
   auto each_work = [&](auto &&f) {
     TileWork w = first_work;
     do f(w);
