@@ -33,11 +33,19 @@ __global__ void __launch_bounds__(kWeightThreads, 2) kv4_weights_kernel(const Kv
   const uint32_t lane_row = blockIdx.x / blocks, seq = lane_row / p.c.kv_heads, kv = lane_row - seq * p.c.kv_heads;
   const uint32_t held = kv4_held(p.c, seq), block_row = (blockIdx.x - lane_row * blocks) * kWeightRows;
   if (block_row >= held) {
-    pdl_wait();   // no kernel after this one may start before the attention is done
+    // One block at least waits for the attention, so that no kernel after this one starts before it is done. The other
+    // idle ones make room.
+    if (blockIdx.x == 0) pdl_wait();
     return;
   }
   const uint32_t row0 = block_row + warp * 32, rows = p.tokens * p.group;
   const uint8_t *run = p.c.data + (size_t)lane_row * p.c.tiles * Kv4<D>::kTileBytes;
+  float old[4];   // only this kernel and append write them, and both of those before are done
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t row = row0 + 8 * i + g;
+    old[i] = t == 0 && row < held ? p.c.weights[(size_t)lane_row * p.c.capacity + row] : 0.f;
+  }
   // ---- K rows row0 + {g, 8 + g, 16 + g, 24 + g} as A fragments ----
   uint32_t a[2][kSteps][4];
 #pragma unroll
@@ -126,7 +134,7 @@ __global__ void __launch_bounds__(kWeightThreads, 2) kv4_weights_kernel(const Kv
     sum[i] += __shfl_xor_sync(~0u, sum[i], 1);
     sum[i] += __shfl_xor_sync(~0u, sum[i], 2);
     const uint32_t row = row0 + 8 * i + g;
-    if (t == 0 && row < held) p.c.weights[(size_t)lane_row * p.c.capacity + row] += sum[i];
+    if (t == 0 && row < held) p.c.weights[(size_t)lane_row * p.c.capacity + row] = old[i] + sum[i];
   }
 }
 
