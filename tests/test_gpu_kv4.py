@@ -459,8 +459,8 @@ def test_more_sequences_than_can_be_cut():
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 def test_long_accumulation(dtype):
     """Dozens of cache tiles in one CTA, some tokens past their count. Tensor-core sums round towards zero, so a long
-    fp32 accumulation would drift: 2^-22 of the result for a tile, of which 4 are summed before a sum that rounds to
-    nearest takes over (2^-20), fp32 sums and 22-bit operands beside it: 2^-18 of the result in the 2-norm. Rounding P
+    fp32 accumulation would drift: 2^-22 of the result for a tile, of which a few (at most 4) are summed before a sum
+    that rounds to nearest takes over (2^-20), fp32 sums and 22-bit operands beside it: 2^-18 of the result in the 2-norm. Rounding P
     and the output to fp16 adds 2^-11."""
     seqs, tokens = 30, 40
     counts = [(40, 5, 0)[i % 3] for i in range(seqs)]

@@ -27,9 +27,9 @@
 // cache tile of one query tile and their results are added at the end. The
 // products of one group run while the other does its softmax.
 //
-// Measured: the last 4096 tokens of a prompt over 32768 rows, fp16, 1.03 TFLOP: 987 us,
-// 1.04 PFLOP/s (63% of the measured burst rate). A unit of 256 query rows takes about
-// 4100 cycles, of which the products need 2048 and the softmax's 32768 exponentials as
+// Measured: the last 4096 tokens of a prompt over 32768 rows, fp16, 1.03 TFLOP: 961 us,
+// 1.07 PFLOP/s (65% of the measured burst rate). A unit of 256 query rows takes about
+// 4000 cycles, of which the products need 2048 and the softmax's 32768 exponentials as
 // many; the two wait for each other through S, whose place P takes.
 //
 // The split. A segment is a block of query rows of a (sequence, KV head) with the
@@ -50,9 +50,9 @@ constexpr uint32_t kUnpackThreads = 128;
 constexpr uint32_t kSoftmaxRegs = 168, kOtherRegs = 88;
 // The products' accumulation rounds towards zero, about 2^-22 of O for a tile of hi and lo. For fp32 queries O therefore
 // starts afresh every kFreshTiles tiles of a group, and what it was is added, with rounding to nearest, to a sum in global
-// memory (it stays in L2): a prompt of 512 tokens over 32768 rows was off by 1.5e-5 of its result, and is by 2e-6 (the
-// plain fp32 form by 3e-6). 16-bit results keep 11 bits or fewer and need none of this.
-constexpr uint32_t kFreshTiles = 4;
+// memory (it stays in L2): a prompt of 512 tokens over 32768 rows was off by 1.5e-5 of its result, and is by 1.4e-6 (the
+// plain fp32 form by 3e-6; with 4 tiles 2e-6, and 7% less time). 16-bit results keep 11 bits or fewer and need none of this.
+constexpr uint32_t kFreshTiles = 2;
 constexpr uint32_t kSwitchUnits = 8;            // what changing segments costs, in units
 constexpr uint32_t kTileCtas = 148;
 constexpr uint32_t kTileSlots = 2 * kTileCtas;  // partial results
@@ -822,11 +822,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
             tmem_load32(o_addr + c, o);
             tmem_wait_load();
             loaded(o);
+            float *at = kept + c * kTileM + row;
+            if (keeping) {
+              float before[32];   // all loads before the first store: one latency, not 32
 #pragma unroll
-            for (uint32_t i = 0; i < 32; ++i) {
-              float *at = kept + (c + i) * kTileM + row;
-              *at = keeping ? fmaf(*at, r, o[i]) : o[i];
+              for (uint32_t i = 0; i < 32; ++i) before[i] = at[i * kTileM];
+#pragma unroll
+              for (uint32_t i = 0; i < 32; ++i) o[i] = fmaf(before[i], r, o[i]);
             }
+#pragma unroll
+            for (uint32_t i = 0; i < 32; ++i) at[i * kTileM] = o[i];
           }
           kept_max = m;
           keeping = true;

@@ -5,7 +5,7 @@
 // computed again, which needs the K codes once more (72 bytes a row, from L2
 // after a decode step) and no room for P. A warp unpacks 32 cache rows to MMA A
 // operands that stay in its registers, and the query rows pass by as B fragments
-// in shared memory, 64 at a time. With 5 tokens of 16 ragged streams it adds 8 us to
+// in shared memory, 64 at a time. With 5 tokens of 16 ragged streams it adds 6 us to
 // the attention's 25 (one warp a cache row, scalar, took 200). Every row is summed by one warp in a fixed
 // order and written by one lane.
 #pragma once
