@@ -424,7 +424,8 @@ int vg_k_kv4_bytes(uint32_t seqs, uint32_t kv_heads, uint32_t head_dim,
 /* Stores `tokens` new K and V rows of every sequence from row at[s] on (NULL:
  * after the rows held) and sets the rows held to at[s] + tokens; at[s] below
  * the rows held drops what was appended since, such as rejected draft tokens.
- * counts[s] <= tokens (NULL: tokens) is how many of them sequence s has. k and v
+ * counts[s] <= tokens (NULL: tokens) is how many of them sequence s has (0 with an
+ * earlier at[s] only drops rows). k and v
  * are of type dtype with element strides {sequence, token, head} (host arrays;
  * NULL: [seqs][tokens][kv_heads][head_dim]) and contiguous channels. New rows
  * take the positions that follow and a weight of 0. A sequence whose append is
