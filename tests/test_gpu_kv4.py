@@ -230,6 +230,26 @@ def test_attention(dtype, rows, tokens, heads, kv_heads, dim):
     assert np.abs(out.double().cpu().numpy() - want).max() <= tol
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("rows,tokens,heads,kv_heads,dim", [
+    # cut into pieces, about two a CTA; the last block has 128 query rows
+    ([2048], 2000, 16, 2, 64),
+    # dealt out unit by unit, several segments a CTA
+    ([512, 600, 515, 700, 640, 512, 777, 530], 512, 16, 2, 64), ([530, 400, 777], 400, 24, 2, 128)])
+def test_prompts_whose_blocks_follow_one_another(dtype, rows, tokens, heads, kv_heads, dim):
+    """256 query rows at a time, more blocks than SMs: a CTA's results leave while the next block's cache rows
+    are being unpacked."""
+    cache = filled(len(rows) + tokens, rows, kv_heads, dim, max(rows) + 3)
+    q = (normal(78, len(rows), tokens, heads, dim) * 1.5).to(TYPES[dtype])
+    out = cache.attention(q)
+    assert torch.equal(out, cache.attention(q))
+    k, v = held(cache)
+    qn = q.double().cpu().numpy()
+    want, _ = R.attention(qn, k, v, rows)
+    _, tol = tolerance(qn, k, v, rows, dtype)
+    assert np.abs(out.double().cpu().numpy() - want).max() <= tol
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,tokens,counts", [
     ([0, 5, 3, 64, 200], 1, None), ([2, 0, 70], 5, None), ([10, 10, 90, 0], 6, [0, 3, 6, 2]), ([20, 150], 64, [64, 1]),

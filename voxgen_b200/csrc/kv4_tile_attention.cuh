@@ -67,6 +67,10 @@ struct TileSmem {
   static constexpr uint32_t kRaw = 6 * kOperand;
   static constexpr uint32_t kRawStage = Kv4<D>::kTileBytes;
   static constexpr uint32_t kBytes = kRaw + kRawStages * kRawStage + 1024;   // + alignment
+  // Two query tiles' results: each softmax group stages kStep channels of its O at a time where its own Q tile was.
+  static constexpr uint32_t kStep = D / 2;
+  static constexpr uint32_t kStaged = kTileM * kStep * 4;
+  static_assert(kStaged <= kOperand, "past a group's Q tile lies the other's, or K of the next piece");
 };
 
 template <int D>
@@ -406,15 +410,16 @@ __device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const Plan 
       leave(r, lane % kChunks * 4, *row_chunk<kChunks>(shared_o, r, lane % kChunks));
     if (x == 0 && row < block_rows) leave_sums(row);
   } else {
-    // each group in its half of the place, 64 channels at a time
-    constexpr uint32_t kChunks = 16;
-    float *own = shared_o + x * (kTileM * 64);
+    // each group where its own Q tile was, half of the channels at a time
+    constexpr uint32_t kStep = TileSmem<D>::kStep, kChunks = kStep / 4;
+    constexpr uint32_t kPer = 32 / kChunks;   // rows of a warp's pass
+    float *own = shared_o + x * (TileSmem<D>::kOperand / 4);
     const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
     const uint32_t n = x * kTileM < block_rows ? min(kTileM, block_rows - x * kTileM) : 0;   // rows of this group
 #pragma unroll 1
-    for (uint32_t c0 = 0; c0 < D; c0 += 64) {
+    for (uint32_t c0 = 0; c0 < D; c0 += kStep) {
 #pragma unroll 1
-      for (uint32_t c = 0; c < 64; c += 32) {
+      for (uint32_t c = 0; c < kStep; c += 32) {
         float o[32];
         tmem_load32(o_addr + c0 + c, o);
         tmem_wait_load();
@@ -430,8 +435,8 @@ __device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const Plan 
       }
       named_bar(3 + x, kTileM);
 #pragma unroll 4
-      for (uint32_t r = warp % 4 * 2 + lane / 16; r < n; r += 8)
-        leave(x * kTileM + r, c0 + lane % 16 * 4, *row_chunk<kChunks>(own, r, lane % 16));
+      for (uint32_t r = warp % 4 * kPer + lane / kChunks; r < n; r += 4 * kPer)
+        leave(x * kTileM + r, c0 + lane % kChunks * 4, *row_chunk<kChunks>(own, r, lane % kChunks));
       named_bar(3 + x, kTileM);
     }
     if (row < n) leave_sums(x * kTileM + row);
