@@ -392,6 +392,52 @@ def test_other_streams_and_graphs(tokens):
     assert torch.equal(got.state, want.state)
 
 
+def test_a_graph_replays_after_its_workspace_was_outgrown():
+    """A decode step is captured, then a prompt needs a larger workspace: the graph's stays its own. Buffers of the old
+    one's size, allocated since, are not written to, and nothing that they hold is read."""
+    q, prompt = normal(1, 2, 1, 16, 128), normal(2, 2, 64, 16, 128)
+    cache = filled(55, [900, 700], 2, 128, 1024, track=True)
+    cache.reserve(16, 1)
+    size = cache._workspace.numel()
+    graph, out = torch.cuda.CUDAGraph(), torch.empty_like(q)
+    with torch.cuda.graph(graph):
+        cache.attention(q, out=out)
+    cache.weights.zero_()
+    want = filled(55, [900, 700], 2, 128, 1024, track=True)
+    for _ in range(2):
+        reference = want.attention(q)
+        cache.attention(prompt, track=False)
+        fillers = [torch.full((size,), 255, dtype=torch.uint8, device="cuda") for _ in range(8)]
+        out.fill_(float("nan"))
+        graph.replay()
+        assert torch.equal(out, reference) and torch.equal(cache.weights, want.weights)
+        assert all((x == 255).all() for x in fillers)
+
+
+@pytest.mark.parametrize("tokens", [1, 64])
+def test_a_first_call_in_a_capture(tokens):
+    """Nothing was reserved: the calls of the graph, and those outside it before its first replay, find zeroed
+    workspaces all the same."""
+    q = normal(1, 2, tokens, 16, 128)
+    cache = filled(56, [900, 700], 2, 128, 1024)
+    reference = filled(56, [900, 700], 2, 128, 1024).attention(q)
+    dirty = torch.full((64 << 20,), 255, dtype=torch.uint8, device="cuda")   # what an allocation may find
+    torch.cuda.synchronize()
+    graph, out = torch.cuda.CUDAGraph(), torch.empty_like(q)
+    with torch.cuda.graph(graph):
+        cache.attention(q, out=out)
+        cache.attention(q, out=out)
+        with pytest.raises(VoxGenError, match="captured"):
+            cache.reserve(16, 128)
+    del dirty
+    assert torch.equal(cache.attention(q), reference)
+    for _ in range(2):
+        out.fill_(float("nan"))
+        graph.replay()
+        assert torch.equal(out, reference)
+        assert torch.equal(cache.attention(q), reference)
+
+
 def test_a_stream_as_an_argument():
     """Each call on a given stream, as a torch stream or its address, from another current stream."""
     k, v, q = normal(1, 2, 3, 2, 64), normal(2, 2, 3, 2, 64), normal(3, 2, 3, 8, 64)

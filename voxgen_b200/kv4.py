@@ -13,7 +13,8 @@ how many rows a sequence holds lives in ``cache.state`` on the device::
     cache.evict(budget=2048, recent=256, sinks=4)
 
 A cache is used by one stream at a time; a program that changes streams orders them itself, as for
-any tensor. Errors raise :class:`~voxgen_b200.api.VoxGenError`; what only the device can know (an
+any tensor. The calls can be captured in CUDA graphs; the cache has to outlive them
+(:meth:`Kv4Cache.reserve`). Errors raise :class:`~voxgen_b200.api.VoxGenError`; what only the device can know (an
 append past the capacity, a NaN among the rows) is in ``cache.status()``.
 """
 from __future__ import annotations
@@ -47,6 +48,7 @@ _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
 
 
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None) or torch.cuda.is_current_stream_capturing
 
 
 def _on(device, stream):
@@ -133,6 +135,8 @@ class Kv4Cache:
         self._ref = C.byref(self.desc)
         self._need = {}
         self._workspace = None
+        self._captured = False   # whether a CUDA graph holds the workspace's address
+        self._kept = []          # workspaces outgrown since, which graphs still write to
         self._lib = api.lib()
 
     # -- rows -------------------------------------------------------------------------------
@@ -192,19 +196,38 @@ class Kv4Cache:
 
     # -- attention --------------------------------------------------------------------------
     def _work(self, heads: int, tokens: int) -> torch.Tensor:
-        """The workspace, large enough for the call; zeroed on the current stream."""
+        """A zeroed workspace, large enough for the call. While a graph is being captured the cache's own does not grow:
+        its zero-fill would run with the replay only, after calls that need it. Such a call has one of its own, zeroed
+        by every replay."""
         need = self._need.get((heads, tokens))
         if need is None:
             n = C.c_uint64()
             _check(self._lib.vg_k_kv4_attention_bytes(self._ref, heads, tokens, C.byref(n)),
                    f"attention of {heads} heads over {self.kv_heads} KV heads, {tokens} tokens")
             need = self._need[heads, tokens] = n.value
-        ws = self._workspace
+        ws, capturing = self._workspace, _capturing()
         if ws is None or ws.numel() < need:
+            fresh = torch.zeros(need, dtype=torch.uint8, device=self.device)
+            if capturing:
+                return fresh
             if ws is not None:
                 ws.record_stream(torch.cuda.current_stream(self._index))
-            ws = self._workspace = torch.zeros(need, dtype=torch.uint8, device=self.device)
+                if self._captured:
+                    self._kept.append(ws)
+            self._workspace, self._captured = fresh, False
+            return fresh
+        self._captured |= capturing
         return ws
+
+    @_on_its_device
+    def reserve(self, heads: int, tokens: int) -> None:
+        """Makes the workspace large enough for :meth:`attention` of ``tokens`` tokens and ``heads`` heads, before a
+        CUDA graph of such calls is captured: without it each of the graph's replays zero-fills a workspace of its own."""
+        if _capturing():
+            raise _invalid("reserve: the workspace does not grow while a graph is being captured")
+        if not (0 < heads < 1 << 32 and 0 < tokens < 1 << 32):
+            raise _invalid(f"reserve: {heads} heads, {tokens} tokens")
+        self._work(heads, tokens)
 
     @_on_its_device
     def attention(self, q: torch.Tensor, *, counts: Optional[torch.Tensor] = None, scale: Optional[float] = None,
