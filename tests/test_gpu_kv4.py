@@ -463,6 +463,20 @@ def test_a_stream_as_an_argument():
         assert accepted.tolist() == [2, 2] and token.tolist() == [0, 0]
 
 
+def test_the_default_streams_address():
+    """Address 0 is the default stream, from any current stream."""
+    cache = filled(92, [70, 20], 2, 64, 128)
+    seen = []
+    cache._lib = type("Calls", (), {"vg_k_kv4_append": lambda *a: seen.append(a[-1]) or 0})()
+    k = normal(1, 2, 3, 2, 64)
+    assert torch.cuda.default_stream().cuda_stream == 0
+    with torch.cuda.stream(torch.cuda.Stream()):
+        current = torch.cuda.current_stream().cuda_stream
+        cache.append(k, k, stream=0)
+        cache.append(k, k)
+    assert seen == [0, current]
+
+
 def test_one_workspace_serves_calls_of_any_shape():
     cache = filled(61, [500, 90], 2, 128, 512, track=True)
     fresh = filled(61, [500, 90], 2, 128, 512, track=True)

@@ -55,8 +55,8 @@ def _on(device, stream):
     """A context in which ``device`` is current, and ``stream`` (an address or a torch stream) when one is given."""
     if stream is None:
         return torch.cuda.device(device)
-    if isinstance(stream, int):
-        stream = torch.cuda.ExternalStream(stream, device=device)
+    if isinstance(stream, int):   # torch takes address 0 for a request of a stream from its pool
+        stream = torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)
     return torch.cuda.stream(stream)
 
 
