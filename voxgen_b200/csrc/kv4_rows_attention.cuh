@@ -104,6 +104,38 @@ __device__ __forceinline__ float row_power(float top, float &inverse) {
   return __uint_as_float((uint32_t)(127 + k) << 23);
 }
 
+// The places of a ring of bulk copies, as the thread that issues them counts. Waits are bounded; once one has run out
+// (`stopped`) nothing is issued or waited for any more, places are passed over unread copies, and what was still in
+// flight is waited for once more, again with a limit, before the block ends: a call is held up by a few limits, however
+// many copies it has.
+template <uint32_t kStages>
+struct CopyRing {
+  uint32_t issued = 0, passed = 0, landed = 0;   // landed: copies seen to land, in order
+  bool stopped = false;
+
+  // issue(stage)
+  template <typename F>
+  __host__ __device__ __forceinline__ void fetch(F &&issue) {
+    if (stopped) return;
+    issue(issued % kStages);
+    ++issued;
+  }
+  // The next place is passed; wait(stage, parity) says whether its copy landed in time.
+  template <typename F>
+  __host__ __device__ __forceinline__ void take(F &&wait) {
+    if (!stopped) {
+      stopped = !wait(passed % kStages, passed / kStages & 1);
+      landed += !stopped;
+    }
+    ++passed;
+  }
+  // Once stopped: the copies that were in flight.
+  template <typename F>
+  __host__ __device__ __forceinline__ void drain(F &&wait) {
+    for (; landed < issued; ++landed) wait(landed % kStages, landed / kStages & 1);
+  }
+};
+
 constexpr uint32_t kUnit = 32;        // cache rows of a unit
 constexpr uint32_t kRowsWarps = 16;
 constexpr uint32_t kRowsStages = 2;
@@ -266,7 +298,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
   __shared__ uint64_t bars[kRowsWarps][kRowsStages];
   __shared__ __align__(8) float w_max[kRowsWarps][kTileRows], w_sum[kRowsWarps][kTileRows];
   __shared__ float f_max[kTileRows], f_sum[kTileRows];
-  __shared__ uint32_t last;
+  __shared__ uint32_t last, gave_up;
   __shared__ __align__(8) uint32_t q_frag[kSplit ? 2 : 1][kSteps][32][2];   // B fragments: hi, lo
   __shared__ __align__(8) float factors[kTileRows];
   __shared__ __align__(8) uint32_t seens[kTileRows];
@@ -288,13 +320,13 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
 
   if (lane == 0)
     for (uint32_t i = 0; i < kRowsStages; ++i) mbar_init(&bars[warp][i], 1);
+  if (threadIdx.x == 0) gave_up = 0;
   fence_mbar_init();
   __syncthreads();
   const Plan plan = shared_plan;
   if (blockIdx.x >= plan.pieces) return;
 
-  uint32_t stage = 0, parity = 0, fetch_stage = 0;
-  bool timed_out = false;
+  CopyRing<kRowsStages> copies;
   // this lane's places in a stage
   const uint32_t k_codes = perm8(g) * (D / 2) + t * (D / 8);
   const uint32_t k_scale = 2 * S::kCodes + perm8(g) * (D / 16) + t * kLaneChannels / 32 * 2;
@@ -303,18 +335,19 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
 
   // units of a piece from this warp's `unit` on, one each call, into the next stage of the ring
   auto fetch = [&](const Piece &x, uint32_t unit) {
-    if (lane == 0) {
-      uint8_t *dst = ring + fetch_stage * S::kStage;
-      const uint32_t row = (x.first + unit) * kUnit;
-      const uint8_t *run = p.c.data + ((size_t)x.seq * p.c.kv_heads + x.lane / p.row_tiles) * run_bytes;
-      uint64_t *bar = &bars[warp][fetch_stage];
-      mbar_arrive_expect_tx(bar, S::kStage);
-      bulk_g2s(dst, run + Kv4<D>::codes(row, 0), S::kCodes, bar);
-      bulk_g2s(dst + S::kCodes, run + Kv4<D>::codes(row, 1), S::kCodes, bar);
-      bulk_g2s(dst + 2 * S::kCodes, run + Kv4<D>::scales(row, 0), S::kScales, bar);
-      bulk_g2s(dst + 2 * S::kCodes + S::kScales, run + Kv4<D>::scales(row, 1), S::kScales, bar);
-    }
-    fetch_stage = fetch_stage + 1 == kRowsStages ? 0 : fetch_stage + 1;
+    copies.fetch([&](uint32_t stage) {
+      if (lane == 0) {
+        uint8_t *dst = ring + stage * S::kStage;
+        const uint32_t row = (x.first + unit) * kUnit;
+        const uint8_t *run = p.c.data + ((size_t)x.seq * p.c.kv_heads + x.lane / p.row_tiles) * run_bytes;
+        uint64_t *bar = &bars[warp][stage];
+        mbar_arrive_expect_tx(bar, S::kStage);
+        bulk_g2s(dst, run + Kv4<D>::codes(row, 0), S::kCodes, bar);
+        bulk_g2s(dst + S::kCodes, run + Kv4<D>::codes(row, 1), S::kCodes, bar);
+        bulk_g2s(dst + 2 * S::kCodes, run + Kv4<D>::scales(row, 0), S::kScales, bar);
+        bulk_g2s(dst + 2 * S::kCodes + S::kScales, run + Kv4<D>::scales(row, 1), S::kScales, bar);
+      }
+    });
   };
 
   Piece seg = shared_piece;
@@ -338,6 +371,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
       if (lane == 0) factors[warp] = factor, seens[warp] = seen;
     }
     __syncthreads();
+    copies.stopped |= __any_sync(~0u, *(volatile uint32_t *)&gave_up);   // a wait of any warp in an earlier piece ran out
     uint32_t q_hi[kSteps][2], q_lo[kSplit ? kSteps : 1][2];
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
@@ -355,7 +389,12 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
 
 #pragma unroll 1
     for (uint32_t unit = warp; unit < seg.units; unit += kRowsWarps) {
-      if (!mbar_wait_bounded(&bars[warp][stage], parity)) timed_out = true;
+      const uint32_t stage = copies.passed % kRowsStages;
+      copies.take([&](uint32_t at, uint32_t parity) {
+        const bool in = __all_sync(~0u, mbar_wait_bounded(&bars[warp][at], parity));
+        if (!in && lane == 0) *(volatile uint32_t *)&gave_up = 1;
+        return in;
+      });
       const uint32_t unit_row = (seg.first + unit) * kUnit;
 #pragma unroll 1
       for (uint32_t half = 0; half < kUnit; half += 16) {
@@ -469,7 +508,6 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
       __syncwarp();
       if (ahead < seg.units) fetch(seg, ahead), ahead += kRowsWarps;
       else if (next_ahead < next.units) fetch(next, next_ahead), next_ahead += kRowsWarps;
-      if (++stage == kRowsStages) stage = 0, parity ^= 1;
     }
 
     // ---- the warps' results meet ----
@@ -620,7 +658,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
     seg = next;
     ahead = next_ahead;
   }
-  if (timed_out && lane == 0) atomicOr(&p.c.state[0].status, kKv4Timeout);
+  if (copies.stopped && lane == 0) {
+    copies.drain([&](uint32_t at, uint32_t parity) { mbar_wait_bounded(&bars[warp][at], parity); });
+    atomicOr(&p.c.state[0].status, kKv4Timeout);
+  }
 }
 
 }  // namespace vg
