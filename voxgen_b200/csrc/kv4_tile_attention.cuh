@@ -654,20 +654,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
     const size_t run_bytes = (size_t)p.c.tiles * Kv4<D>::kTileBytes;
     // the first warp streams the cache's 64-row tiles; a stage is refilled once all have unpacked it
     TileWork ahead = first_work;
-    uint32_t ahead_raw = 0, fetched = 0;   // raw: 64-row tile of the piece
+    uint32_t ahead_raw = 0;   // 64-row tile of the piece
+    CopyRing<kRawStages> copies;   // `passed` and `stopped` are the loop's own: `used` below, and `aborted`
     bool ahead_on = true;
     auto fetch = [&]() {
       if (!ahead_on) return;
       const uint32_t raw = ahead.first * 2 + ahead_raw;
       if (raw < p.c.tiles && !*(volatile uint32_t *)&aborted) {
-        if (lane == 0) {
-          const uint32_t st = fetched % kRawStages;
-          mbar_arrive_expect_tx(&bars.raw_full[st], S::kRawStage);
-          bulk_g2s(smem + S::kRaw + st * S::kRawStage,
-                   p.c.data + ((size_t)ahead.seq * p.c.kv_heads + ahead.kv) * run_bytes + (size_t)raw * S::kRawStage,
-                   S::kRawStage, &bars.raw_full[st]);
-        }
-        ++fetched;
+        copies.fetch([&](uint32_t st) {
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&bars.raw_full[st], S::kRawStage);
+            bulk_g2s(smem + S::kRaw + st * S::kRawStage,
+                     p.c.data + ((size_t)ahead.seq * p.c.kv_heads + ahead.kv) * run_bytes + (size_t)raw * S::kRawStage,
+                     S::kRawStage, &bars.raw_full[st]);
+          }
+        });
       }
       if (++ahead_raw == 2 * ahead.units) {
         ahead_raw = 0;
@@ -740,9 +741,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
         }
       }
     });
-    // nothing is left in flight but after a wait that ran out
-    if (tid == 0)
-      for (; used < fetched; ++used) mbar_wait_bounded(&bars.raw_full[used % kRawStages], used / kRawStages & 1);
+    // nothing is left in flight but after a wait that ran out, which passes over copies that have not landed
+    if (tid == 0 && *(volatile uint32_t *)&aborted)
+      copies.drain([&](uint32_t at, uint32_t parity) { mbar_wait_bounded(&bars.raw_full[at], parity); });
   } else {
     more_registers<kSoftmaxRegs>();
     // ---------------- softmax ----------------
