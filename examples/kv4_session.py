@@ -39,6 +39,8 @@ def park(model_dir, preset="pin", prompt=48, more=8):
     k, v = (torch.from_numpy(x.view(np.float16)).cuda().view(layers, prompt, heads, dim) for x in kept.read_kv(prompt))
     cache = kv4.Kv4Cache(layers, heads, dim, prompt)
     cache.append(k, v)
+    if any(cache.status()):   # the engine's fp16 cache holds up to 65504, this one up to 7168
+        raise ValueError("the session holds values that its 4-bit cache would clamp")
 
     back = [x.reshape(layers, prompt, heads * dim).cpu().numpy().view(np.uint16) for x in cache.read(prompt)]
     restored.write_kv(*back)

@@ -385,7 +385,8 @@ int vg_k_attention_noalloc(const float *q, const uint16_t *k_cache,
  * one scale of 7 significant bits, 4.5 bits a value. The scale is -b/8, b being
  * the block's value of largest magnitude (the positive one where two tie); a
  * code is rint(x * (1/scale)), clamped. Values are clamped to +-7168 and a NaN
- * is held as 0 (VG_KV4_NONFINITE reports both), so a cache is always finite;
+ * is held as 0 (VG_KV4_NONFINITE reports both, finite values past 7168 among
+ * them), so a cache is always finite;
  * blocks whose largest magnitude is below 2^-15 are held as zeros. Every value
  * that the cache stands for is an exact fp16 number.
  *
@@ -405,7 +406,7 @@ int vg_k_attention_noalloc(const float *q, const uint16_t *k_cache,
 #define VG_DTYPE_BF16 30
 #define VG_KV4_FULL 1       /* an append would have passed the capacity            */
 #define VG_KV4_BAD_ROW 2    /* an append's first row or count was out of range     */
-#define VG_KV4_NONFINITE 4  /* an append met a NaN or an infinity                  */
+#define VG_KV4_NONFINITE 4  /* an append met a NaN, or a value past +-7168         */
 #define VG_KV4_TIMEOUT 8    /* a bounded wait of an attention ran out (sequence 0)  */
 typedef struct vg_kv4_cache {
   void *data;

@@ -111,6 +111,23 @@ def test_append_special_values():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_append_reports_what_it_clamps(dtype, dim):
+    """A finite value past 7168 in K or V, at either end of a row, sets its own sequence's status; 7168 does not."""
+    step = {"f32": 0.0625, "f16": 4.0, "bf16": 32.0}[dtype]       # 7168 + step is the type's next number, or near it
+    for value, bit in ((7168.0, 0), (7168.0 + step, kv4.STATUS_NONFINITE), (-7168.0 - step, kv4.STATUS_NONFINITE),
+                       (65024.0, kv4.STATUS_NONFINITE)):
+        for place in (0, dim - 1):
+            x = normal(3, 2, 5, 2, dim, dtype=TYPES[dtype])
+            y = x.clone()
+            x[1, 3, 1, place] = value
+            for k, v in ((x, y), (y, x)):
+                cache = kv4.Kv4Cache(2, 2, dim, 64)
+                cache.append(k, v)
+                assert cache.status() == [0, bit], (value, place)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_append_and_read_of_strided_rows(dtype):
     """K and V as parts of a fused projection, on and off 16-byte boundaries, and transposed heads."""
     fused = normal(5, 2, 40, 1 + 2 * 3 * 64, dtype=TYPES[dtype])

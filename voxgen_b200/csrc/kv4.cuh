@@ -63,7 +63,7 @@ struct Kv4Seq {
 enum : int32_t {
   kKv4Full = 1,       // an append went past the capacity
   kKv4BadRow = 2,     // an append started past the rows held, or its count is out of range
-  kKv4NonFinite = 4,  // an append met a NaN or an infinity
+  kKv4NonFinite = 4,  // an append met a NaN, or a value past +-kKv4Largest
   kKv4Timeout = 8,    // a bounded wait inside attention ran out (sequence 0's word)
 };
 

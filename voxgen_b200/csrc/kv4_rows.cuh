@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(kRowThreads, kAppendBlocks) kv4_append_kernel(
   const uint32_t lane = threadIdx.x % L;
   const T *k = (const T *)p.k + (int64_t)seq * p.ks.seq + lane * 16;
   const T *v = (const T *)p.v + (int64_t)seq * p.vs.seq + lane * 16;
-  bool odd = false;  // met a NaN or an infinity
+  bool odd = false;  // met a value that it holds as another: a NaN, an infinity or one past the largest
   for (uint32_t base = block * kRows; base < items; base += p.blocks * kRows) {
     const uint32_t item = base + threadIdx.x / L;
     const bool on = item < items;
@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(kRowThreads, kAppendBlocks) kv4_append_kernel(
       }
       const bool wild = !(zero.x + zero.y == 0.f);
       if (wild || high > kKv4Largest || low < -kKv4Largest) {
-        odd |= on && wild;
+        odd |= on;
         high = -kKv4Largest, low = kKv4Largest;
 #pragma unroll
         for (int j = 0; j < 16; ++j) {

@@ -15,7 +15,7 @@ how many rows a sequence holds lives in ``cache.state`` on the device::
 A cache is used by one stream at a time; a program that changes streams orders them itself, as for
 any tensor. The calls can be captured in CUDA graphs; the cache has to outlive them
 (:meth:`Kv4Cache.reserve`). Errors raise :class:`~voxgen_b200.api.VoxGenError`; what only the device can know (an
-append past the capacity, a NaN among the rows) is in ``cache.status()``.
+append past the capacity, a NaN or a value past 7168 among the rows) is in ``cache.status()``.
 """
 from __future__ import annotations
 
