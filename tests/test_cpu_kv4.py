@@ -1,6 +1,7 @@
 """The 4-bit cache's entry points without a GPU: sizes, and every refusal that the host makes before
 it enqueues anything (addresses are made up; nothing is read)."""
 import ctypes as C
+import re
 
 import pytest
 
@@ -121,3 +122,13 @@ def test_verify_refuses():
         assert api.lib().vg_k_verify_draft(*{**good, name: 0}.values()) == EINVAL, name
     assert api.lib().vg_k_verify_draft(*{**good, "vocab": 1 << 25}.values()) == ERANGE
     assert api.lib().vg_k_verify_draft(*{**good, "counts": A + 1}.values()) == EINVAL
+
+
+def test_dynamic_shared_memory_is_declared_with_the_alignment_of_its_widest_access():
+    """The kernels read and write it 16 bytes at a time; an element type of 1 or 4 bytes promises less."""
+    from voxgen_b200._build import CSRC
+    found = {}
+    for path in CSRC.glob("kv4*.cuh"):
+        for align, name in re.findall(r"extern __shared__ (?:__align__\((\d+)\) )?\w+ (\w+)\[\]", path.read_text()):
+            found[name] = int(align or 0)
+    assert len(found) == 4 and all(a >= 16 for a in found.values()), found

@@ -253,7 +253,7 @@ __device__ __forceinline__ uint32_t warps_before(uint32_t mine, uint32_t *counts
 // rows with ballots, so a pass over the rows has no block barrier.
 template <int D, bool KEYS>
 __global__ void __launch_bounds__(kEvictThreads, 4) kv4_evict_kernel(const EvictParams p) {
-  extern __shared__ uint32_t evict_smem[];   // histogram, keys, holes, movers
+  extern __shared__ __align__(16) uint32_t evict_smem[];   // histogram (read 16 bytes at a time), keys, holes, movers
   __shared__ uint32_t counts[kEvictWarps], chosen[2];
   uint32_t *hist = evict_smem, *keys = hist + kEvictBins;
   uint16_t *holes = (uint16_t *)(keys + (KEYS ? p.c.capacity : 0)), *movers = holes + p.list;

@@ -522,7 +522,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
   static_assert(!(kSplit && PAIR), "hi and lo take the second query tile's place");
   constexpr uint32_t kRows = PAIR ? 2 * kTileM : kTileM;      // query rows of a block
   constexpr uint32_t kPanel = kTileN * 128;                   // bytes of 64 channels of a tile
-  extern __shared__ uint8_t smem_raw[];
+  extern __shared__ __align__(16) uint8_t smem_raw[];
   uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   __shared__ TileBars bars;
   __shared__ uint32_t tmem_base, aborted, last;
