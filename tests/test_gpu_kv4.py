@@ -627,6 +627,16 @@ def test_evict(separate, seqs, kv_heads, dim, capacity, rows, budget, recent, si
             np.testing.assert_array_equal(gk[s, h, budget:], k[s, h, budget:])   # rows past the budget are left
 
 
+@pytest.mark.parametrize("separate", [False, True])
+@pytest.mark.parametrize("seqs,kv_heads,dim,capacity,rows,budget,recent,sinks,ties", [
+    (1, 1, 64, 32768, [32768], 16384, 100, 4, False),                  # the most rows whose keys fit beside the lists
+    (1, 2, 64, 40000, [39999], 20000, 300, 4, True), (2, 1, 128, 65536, [65536, 50001], 32768, 0, 0, False),
+    (1, 1, 64, 65536, [65536], 65535, 0, 1, True), (1, 1, 128, 65536, [65535], 1, 0, 0, True)])
+def test_evict_of_long_caches(separate, seqs, kv_heads, dim, capacity, rows, budget, recent, sinks, ties):
+    """Rows past 32768: 16-bit lists of up to 32768 rows, keys formed anew in every pass."""
+    test_evict(separate, seqs, kv_heads, dim, capacity, rows, budget, recent, sinks, ties)
+
+
 def test_evict_odd_weights():
     """NaN goes first, then -inf, then by value; -0 and +0 tie; +inf and protected rows stay."""
     nan, inf = float("nan"), float("inf")
