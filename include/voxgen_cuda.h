@@ -446,7 +446,9 @@ int vg_k_kv4_read(const vg_kv4_cache *cache, const int32_t *first, uint32_t toke
  * tokens past the count, give zeros. scale multiplies the scores (usually
  * 1/sqrt(head_dim)). With track, the attention that each row draws, summed over
  * the call's tokens and the heads that share the row, is added to the cache's
- * weights. Results do not depend on timing: every sum has a fixed order.
+ * weights. Results do not depend on timing: every sum has a fixed order. out and q
+ * do not overlap, but for a contiguous q that an untracked call may overwrite
+ * (out = q).
  *
  * workspace: vg_k_kv4_attention_bytes() bytes, 16-byte aligned, zero-filled
  * once before its first use; calls leave it ready for the next call of any

@@ -92,6 +92,10 @@ def test_attention_refuses(over, want):
     assert attention(C.byref(desc()), **over) == want
 
 
+def test_attention_refuses_to_track_in_place():
+    assert attention(C.byref(desc()), q=A, out=A, track=1) == EINVAL
+
+
 def test_attention_refuses_to_track_without_weights():
     assert attention(C.byref(desc(weights=None)), track=1) == EINVAL
 

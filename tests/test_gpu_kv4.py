@@ -380,6 +380,18 @@ def test_strided_queries_scale_and_out(tokens):
     assert np.abs(out.double().cpu().numpy() - want).max() <= tol
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("rows,tokens", [([5000, 90], 1), ([3000], 2), ([900, 700], 40), ([2000], 600)])
+def test_queries_may_be_overwritten(dtype, rows, tokens):
+    """out = q where nothing is tracked, with segments cut among CTAs; refused where something is."""
+    cache = filled(43, rows, 2, 64, max(rows), track=True)
+    q = normal(9, len(rows), tokens, 8, 64, dtype=TYPES[dtype])
+    want = cache.attention(q, track=False)
+    with pytest.raises(VoxGenError, match="out cannot be q"):
+        cache.attention(q, out=q)
+    assert torch.equal(cache.attention(q, track=False, out=q), want) and not cache.weights.any()
+
+
 @pytest.mark.parametrize("tokens", [1, 4, 40])
 def test_other_streams_and_graphs(tokens):
     """The calls run on the stream they are given, and a captured loop replays from the device's state."""

@@ -234,7 +234,7 @@ int vg_k_kv4_attention(const vg_kv4_cache *cache, const void *q, int dtype, uint
   if (!size) return VG_EUNSUPPORTED;
   if (!q || !out || !workspace || workspace_bytes < need || !aligned(q, size) || !aligned(out, 16) ||
       !aligned(workspace, 16) || !aligned(counts, 4) || (track && !cache->weights) || !(scale > 0.f) ||
-      !(scale < __builtin_huge_valf()))
+      !(scale < __builtin_huge_valf()) || (track && out == q))   // the tracking kernel reads q while out is written
     return VG_EINVAL;
   uint8_t *ws = (uint8_t *)workspace;
   p.q = q;

@@ -235,7 +235,7 @@ class Kv4Cache:
         """Attention of the last ``tokens`` rows' queries ``[seqs, tokens, heads, head_dim]``, causal within them.
 
         Adds the attention that each row draws to ``weights`` when the cache tracks it (``track=False`` leaves
-        them). ``scale`` is 1/sqrt(head_dim) by default."""
+        them). ``scale`` is 1/sqrt(head_dim) by default. ``out`` may be ``q`` itself where nothing is tracked."""
         if q.dim() != 4:
             raise _invalid("q: expected [seqs, tokens, heads, head_dim]")
         _, tokens, heads, _ = q.shape
@@ -248,6 +248,8 @@ class Kv4Cache:
             track = self.weights is not None
         elif track and self.weights is None:
             raise _invalid("this cache does not track attention")
+        if track and out.data_ptr() == q.data_ptr():
+            raise _invalid("out cannot be q in a call that tracks attention")
         ws = self._work(heads, tokens)
         rc = self._lib.vg_k_kv4_attention(
             self._ref, q.data_ptr(), dtype, heads, tokens, _strides(q),
