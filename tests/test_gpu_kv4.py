@@ -342,6 +342,43 @@ def test_queries_of_extreme_values(dtype, tokens):
     assert np.abs(out[0, 0, 5] - v[0, 0, best]).max() <= (2.0 ** -17 + 2.0 ** -8) * np.abs(v).max()
 
 
+@pytest.mark.parametrize("tokens", [1, 4, 40, 300])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scores_past_2_to_the_24(dtype, tokens):
+    """Scores of 2^25 to 2^40, where fp32 has no fractions left: a row that leads by more than the scores are off by
+    takes all, and every output stays a mean of values."""
+    n, dim = 400, 128
+    for size, scale in ((1e4, 1.0), (1e4, 40.0), (-1e4, 1.0)) if dtype == "f16" else ((1e6, 0.1), (1e7, 1.0), (-1e6, 1.0)):
+        cache = kv4.Kv4Cache(1, 2, dim, n, track=True)
+        k, v = normal(1, 1, n, 2, dim) * 1000, normal(2, 1, n, 2, dim)
+        if size < 0:
+            k, size = k.abs(), -size   # one sign: no score is near 0
+        cache.append(k, v)
+        q = normal(3, 1, tokens, 16, dim, dtype=torch.float32)
+        if (k > 0).all():
+            q = -q.abs()
+        q = (q * size).to(TYPES[dtype])
+        out = cache.attention(q, scale=scale).double().cpu().numpy()[0]
+        assert np.isfinite(out).all()
+        hk, hv = (x[0] for x in held(cache))
+        qn = q[0].double().cpu().numpy()
+        top = np.abs(hv).max()
+        assert np.abs(out).max() <= top * (1 + 2.0 ** -7)
+        off = scale * 2.0 ** -19 * np.einsum("thd,hnd->thn", np.abs(qn), np.repeat(np.abs(hk), 8, 0)).max()
+        score = scale * np.einsum("thd,hnd->thn", qn, np.repeat(hk, 8, 0))
+        seen = n - tokens + 1 + np.arange(tokens)
+        score[np.arange(n) >= np.broadcast_to(seen[:, None, None], score.shape)] = -np.inf
+        order = np.sort(score, -1)
+        clear = order[..., -1] - order[..., -2] > 2 * off + 40
+        assert clear.mean() > 0.9
+        t, h = np.nonzero(clear)
+        best = hv[h // 8, score.argmax(-1)[t, h]]
+        extra = {"f32": 2.0 ** -17, "f16": 2.0 ** -10, "bf16": 2.0 ** -8}[dtype]
+        assert np.abs(out[t, h] - best).max() <= extra * top
+        drawn = cache.weights.cpu().numpy()
+        assert (drawn >= 0).all() and drawn.max() <= 8 * tokens
+
+
 def test_one_row_takes_all_and_the_rest_still_counts():
     """One row of weight 1 against 30000 of weight 2^-20 each: the small ones add up to 3% of the output."""
     n = 30001

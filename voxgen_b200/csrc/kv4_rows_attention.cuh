@@ -147,6 +147,10 @@ constexpr uint32_t kMostTickets = 1u << 14;   // segments that may be cut
 constexpr float kPScale = 6.f, kLead = 8.f;
 // The running maximum of a row that has met no score: finite, so that nothing has to be asked before a subtraction. A row
 // that sees nothing keeps a denominator of 0.
+//
+// The maximum that a block runs is one of the products' sums, not yet scaled: the difference of two sums is scaled, and
+// not two scaled numbers taken from one another, whose rounding passes P's range where scores pass 2^25 (the row of the
+// largest score had a P of infinity or 0).
 constexpr float kNoScore = -3e38f;
 
 template <int D>
@@ -439,25 +443,24 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
             if (r >= seen1) c[2 * y + 1] = -INFINITY;
           }
         }
-        float top0 = fmaxf(c[0], c[2]) * f0, top1 = fmaxf(c[1], c[3]) * f1;
-        if (__any_sync(~0u, top0 > m0 + kLead || top1 > m1 + kLead)) {
+        float top0 = fmaxf(c[0], c[2]), top1 = fmaxf(c[1], c[3]);
+        if (__any_sync(~0u, (top0 - m0) * f0 > kLead || (top1 - m1) * f1 > kLead)) {
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) {
             top0 = fmaxf(top0, __shfl_xor_sync(~0u, top0, x));
             top1 = fmaxf(top1, __shfl_xor_sync(~0u, top1, x));
           }
           top0 = fmaxf(top0, m0), top1 = fmaxf(top1, m1);
-          const float r0 = exp2_fast(m0 - top0), r1 = exp2_fast(m1 - top1);
+          const float r0 = exp2_fast((m0 - top0) * f0), r1 = exp2_fast((m1 - top1) * f1);
           m0 = top0, m1 = top1;
           l0 *= r0, l1 *= r1;
 #pragma unroll
           for (int j = 0; j < kSteps; ++j) o[j][0] *= r0, o[j][1] *= r1, o[j][2] *= r0, o[j][3] *= r1;
         }
-        const float base0 = kPScale - m0, base1 = kPScale - m1;
         uint32_t p_hi[2], p_lo[2];
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-          const float x0 = exp2_fast(fmaf(c[2 * y], f0, base0)), x1 = exp2_fast(fmaf(c[2 * y + 1], f1, base1));
+          const float x0 = exp2_fast(fmaf(c[2 * y] - m0, f0, kPScale)), x1 = exp2_fast(fmaf(c[2 * y + 1] - m1, f1, kPScale));
           l0 += x0, l1 += x1;
           if constexpr (kSplitP) {
             split2(x0, x1, p_hi[y], p_lo[y]);
@@ -513,6 +516,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
       l0 += __shfl_xor_sync(~0u, l0, x);
       l1 += __shfl_xor_sync(~0u, l1, x);
     }
+    m0 = l0 == 0.f ? kNoScore : m0 * f0, m1 = l1 == 0.f ? kNoScore : m1 * f1;   // scaled from here on
     if (g == 0) {
       *(float2 *)&w_max[warp][2 * t] = make_float2(m0, m1);
       *(float2 *)&w_sum[warp][2 * t] = make_float2(l0, l1);

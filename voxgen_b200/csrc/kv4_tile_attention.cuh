@@ -4,14 +4,15 @@
 // r = token * group + head of the group, so a token's whole group shares the
 // cache's rows. A tile is 128 query rows (M) against 128 cache rows (N):
 //   S = Q K^T     128 x 128 x D, both operands in shared memory
-//   P = exp2(S * f - m)          a thread a row, S and P in tensor memory
+//   P = exp2((S - m) * f)        a thread a row, S and P in tensor memory
 //   O += P V      128 x D x 128, P from tensor memory, V in shared memory
 // K and V are unpacked from their codes to fp16 exactly (kv4.cuh), so a 32-bit
 // call needs hi + lo only of its own operands: Q hi and lo against the same K,
 // P hi and lo against the same V, 4 products instead of 2. 16-bit queries are
 // exact in fp16 (times a power of two), and P is rounded to 11 bits, like the
-// output. Statistics and sums are fp32. The running maximum is raised, and O
-// rescaled, only when a score passes it by 2^8.
+// output. Statistics and sums are fp32. The running maximum m is raised, and O
+// rescaled, only when a score passes it by 2^8. It is taken off before the scaling
+// (kNoScore says why), which costs 1% against one multiply-add with S * f - m.
 //
 // The layout. K and V tiles are stored the same way: 128 cache rows of 64
 // channels (128 bytes) a panel, 16-byte chunks turned by the row (the 128-byte
@@ -807,7 +808,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
       const bool used_row = row0 + qr < rows;
       uint32_t least = used_row ? seen : 0xFFFFFFFFu;              // fewest of the warp's rows
       least = __reduce_min_sync(~0u, least);
-      float m = kNoScore, l = 0.f;
+      float m = kNoScore, l = 0.f;   // m: of the products' sums, not yet scaled
       // fp32: the sum of earlier O, [channel][row] in the half of a partial result that 128-row blocks do not use, and the
       // maximum that it is relative to
       float *const kept = p.parts + (size_t)(blockIdx.x * 2 + x) * kTilePart<D> + kTileM * D;
@@ -821,7 +822,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
         tc_fence_after();
         const bool fresh = kSplit ? u / 2 % kFreshTiles == 0 : u < step;   // nothing in O counts
         if (kSplit && fresh && u >= step) {   // O is whole: the products before these scores are done
-          const float r = exp2_fast(kept_max - m);
+          const float r = exp2_fast((kept_max - m) * f);
 #pragma unroll 1
           for (uint32_t c = 0; c < D; c += 32) {
             float o[32];
@@ -860,9 +861,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
           for (int i = 0; i < 4; ++i) top[i] = max3(top[i], s[c + i], s[c + 4 + i]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) top[i] = fmaxf(top[i], s[kTileN - 4 + i]);
-        const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f;
-        if (__any_sync(~0u, best > m + kLead)) {
-          const float up = fmaxf(m, best), r = exp2_fast(m - up);
+        const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        if (__any_sync(~0u, (best - m) * f > kLead)) {
+          const float up = fmaxf(m, best), r = exp2_fast((m - up) * f);
           m = up;
           l *= r;
           if (!fresh) {   // O has something: the products before these scores are done
@@ -883,15 +884,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
             }
           }
         }
-        const float base = kTilePScale - m;
-        const float2 f2 = make_float2(f, f), base2 = make_float2(base, base);
+        const float2 f2 = make_float2(f, f), base2 = make_float2(kTilePScale, kTilePScale), less = make_float2(-m, -m);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int c = 0; c < (int)kTileN; c += 32) {
           uint32_t hi[16], lo[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            float2 e = fma2(make_float2(s[c + 2 * i], s[c + 2 * i + 1]), f2, base2);
+            float2 e = fma2(add2(make_float2(s[c + 2 * i], s[c + 2 * i + 1]), less), f2, base2);
             e.x = exp2_fast(e.x), e.y = exp2_fast(e.y);
             sum[i % 2] = add2(sum[i % 2], e);
             if constexpr (kSplit) split2(e.x, e.y, hi[i], lo[i]);
@@ -916,8 +916,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(const Kv4Attn
       if (mine) wait(&bars.o_full[x], works++ & 1);
       __syncwarp();
       tc_fence_after();
-      tile_results<D, T>(p, plan, w, pair, x, row, row0, m, l, mine, o_addr, keeping ? kept : nullptr, exp2_fast(kept_max - m),
-                         (float *)(smem + S::kQ), group_max, group_sum, factors, &last);
+      tile_results<D, T>(p, plan, w, pair, x, row, row0, l == 0.f ? kNoScore : m * f, l, mine, o_addr, keeping ? kept : nullptr,
+                         exp2_fast((kept_max - m) * f), (float *)(smem + S::kQ), group_max, group_sum, factors, &last);
       tc_fence_before();
     });
   }

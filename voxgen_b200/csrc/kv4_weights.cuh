@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kWeightThreads, 2) kv4_weights_kernel(const Kv
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float e = exp2_fast(fmaf(c[i / 2][i % 2 * 2 + z], scale, -minus));
-          sum[i] += row0 + 8 * i + g < seen ? e : 0.f;
+          sum[i] += row0 + 8 * i + g < seen ? e > 1.f ? 1.f : e : 0.f;   // a share; past 2^24, scores are off by more than 1
         }
       }
     }
