@@ -342,6 +342,32 @@ def test_queries_of_extreme_values(dtype, tokens):
     assert np.abs(out[0, 0, 5] - v[0, 0, best]).max() <= (2.0 ** -17 + 2.0 ** -8) * np.abs(v).max()
 
 
+@pytest.mark.parametrize("rows,tokens,counts", [([1, 700], 1, None), ([5, 700], 5, [5, 3]), ([6000], 2, None), ([40, 900], 40, None),
+                                                ([900], 600, [500])])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scores_that_are_all_minus_infinity(dtype, rows, tokens, counts):
+    """An infinite query whose every score is -infinity has no softmax: NaN, and not the zeros of a query that sees no
+    row. Other heads and tokens, and those past the count, are as they would be."""
+    cache = kv4.Kv4Cache(len(rows), 2, 64, max(rows), track=True)
+    k, v = (normal(i, len(rows), max(rows), 2, 64) for i in (1, 2))
+    k[..., 5] = k[..., 5].abs() + 0.5
+    cache.append(k, v, counts=ints(*rows))
+    q = normal(3, len(rows), tokens, 16, 64, dtype=TYPES[dtype])
+    q[:, 0, 3, 5] = q[:, -1, 9, 5] = -float("inf")
+    clean = q.clone()
+    clean[:, 0, 3] = clean[:, -1, 9] = 0
+    limits = None if counts is None else ints(*counts)
+    out, want = cache.attention(q, counts=limits), cache.attention(clean, counts=limits, track=False)
+    for s, n in enumerate(rows):
+        c = tokens if counts is None else counts[s]
+        for t, h in ((0, 3), (tokens - 1, 9)):
+            sees = t < c and n - c + t + 1 > 0
+            assert out[s, t, h].isnan().all() if sees else not out[s, t, h].any()
+            out[s, t, h] = want[s, t, h] = 0
+        assert cache.weights[s, 0, 0].isnan() and not cache.weights[s, :, n:].any()
+    assert torch.equal(out, want)
+
+
 @pytest.mark.parametrize("tokens", [1, 4, 40, 300])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_scores_past_2_to_the_24(dtype, tokens):

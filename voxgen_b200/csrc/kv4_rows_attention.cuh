@@ -555,15 +555,17 @@ __global__ void __launch_bounds__(kRowsThreads, 1) kv4_rows_kernel(const Kv4Attn
       const uint32_t tok = (row0 + r) / p.group, head = kv * p.group + (row0 + r) % p.group;
       return ((size_t)seg.seq * p.tokens + tok) * p.heads + head;
     };
+    // a row whose softmax sums up to 0: zeros where it sees no cache row, NaN where every score was -infinity
+    auto blank = [&](uint32_t r) { return seens[r] ? NAN : 0.f; };
     auto emit = [&](uint32_t r, uint32_t ch, float4 x, float sum) {   // finished output values
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const float inv = sum == 0.f ? blank(r) : 1.f / sum;
       T y[4] = {from_float<T>(x.x * inv), from_float<T>(x.y * inv), from_float<T>(x.z * inv), from_float<T>(x.w * inv)};
       T *dst = (T *)p.out + place(r) * D + ch;
       if constexpr (sizeof(T) == 4) *(float4 *)dst = *(const float4 *)y;
       else *(uint2 *)dst = *(const uint2 *)y;
     };
     auto emit_lse = [&](uint32_t r, float top, float sum) {
-      p.lse[place(r)] = sum == 0.f ? INFINITY : top + log2f(sum) - kPScale;
+      p.lse[place(r)] = sum == 0.f ? INFINITY + blank(r) : top + log2f(sum) - kPScale;
     };
     float *part = p.parts + (size_t)index * kPart<D>;
     if (threadIdx.x < tile_rows * (D / 4)) {

@@ -342,7 +342,12 @@ __device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const Plan 
     const uint32_t tok = (row0 + i) / p.group, head = w.kv * p.group + (row0 + i) - tok * p.group;
     return ((size_t)w.seq * p.tokens + tok) * p.heads + head;
   };
-  auto lse = [&](float top, float sum) { return sum == 0.f ? INFINITY : top + log2f(sum) - kTilePScale; };
+  // a row whose softmax sums up to 0: zeros where it sees no cache row, NaN where every score was -infinity
+  auto blank = [&](uint32_t i) {
+    const int32_t tok = (int32_t)((row0 + i) / p.group), count = kv4_count(p, w.seq);
+    return i < block_rows && tok < count && (int32_t)kv4_held(p.c, w.seq) - count + tok + 1 > 0 ? NAN : 0.f;
+  };
+  auto lse = [&](uint32_t i, float top, float sum) { return sum == 0.f ? INFINITY + blank(i) : top + log2f(sum) - kTilePScale; };
   auto slot = [&](uint32_t i) { return p.parts + (size_t)i * kTilePart<D>; };
   float *part = slot(parts.own);
   // 4 channels of row r, final or partial
@@ -361,7 +366,7 @@ __device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const Plan 
       part[2 * kTileM * D + r] = m;
       part[2 * kTileM * (D + 1) + r] = l;
     } else if (p.lse) {
-      p.lse[place(r)] = lse(m, l);
+      p.lse[place(r)] = lse(r, m, l);
     }
   };
   if (!pair) {
@@ -373,7 +378,7 @@ __device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const Plan 
     const float w0 = exp2_fast(m0 - top), w1 = exp2_fast(m1 - top);
     l = group_sum[0][row] * w0 + group_sum[1][row] * w1;
     m = top;
-    const float f = (x ? w1 : w0) * (!whole ? 1.f : l == 0.f ? 0.f : 1.f / l);
+    const float f = (x ? w1 : w0) * (!whole ? 1.f : l == 0.f ? blank(row) : 1.f / l);
     // each group hands over its share of the other's half of the channels, then adds what it was handed to its own half
 #pragma unroll 1
     for (uint32_t pass = 0; pass < 2; ++pass) {
@@ -415,7 +420,7 @@ __device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const Plan 
     constexpr uint32_t kStep = TileSmem<D>::kStep, kChunks = kStep / 4;
     constexpr uint32_t kPer = 32 / kChunks;   // rows of a warp's pass
     float *own = shared_o + x * (TileSmem<D>::kOperand / 4);
-    const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+    const float inv = !whole ? 1.f : l == 0.f ? blank(x * kTileM + row) : 1.f / l;
     const uint32_t n = x * kTileM < block_rows ? min(kTileM, block_rows - x * kTileM) : 0;   // rows of this group
 #pragma unroll 1
     for (uint32_t c0 = 0; c0 < D; c0 += kStep) {
@@ -477,8 +482,8 @@ __device__ __forceinline__ void tile_results(const Kv4AttnParams &p, const Plan 
             shared_o[k * n + threadIdx.x] = pw;
             sum = fmaf(pw, ps, sum);
           }
-          factors[threadIdx.x] = sum == 0.f ? 0.f : 1.f / sum;
-          if (p.lse) p.lse[place(i)] = lse(top, sum);
+          factors[threadIdx.x] = sum == 0.f ? blank(i) : 1.f / sum;
+          if (p.lse) p.lse[place(i)] = lse(i, top, sum);
         }
         __syncwarp();
         named_bar(2, 256);
