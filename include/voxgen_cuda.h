@@ -464,7 +464,10 @@ int vg_k_kv4_attention(const vg_kv4_cache *cache, const void *q, int dtype, uint
  * stay, and of the others those with the largest weights (equal weights: the
  * lowest row; a NaN weight goes first). Kept rows past the budget move, in order,
  * into the places of dropped rows; all others stay where they are, and rows past
- * the budget are not written. recent + sinks <= budget; capacity <= 65536.
+ * the budget are not written. Rows are then no longer in the order of their
+ * positions: an append drops only rows that were appended since (at[s] not below
+ * the rows left here), and attention of several tokens follows their own append.
+ * recent + sinks <= budget; capacity <= 65536.
  * into, when not NULL, is a cache of the same shape and data whose state,
  * weights and positions receive the result, and the first cache's are left. */
 int vg_k_kv4_evict(const vg_kv4_cache *cache, uint32_t budget, uint32_t recent,

@@ -5,8 +5,9 @@
 // m16n8k16 MMA: scores are S^T = K Q^T and the output O^T = V^T P^T, with the
 // cache as the A operand. Both K and V come out of the codes with one shift, one
 // lop3 and one fused multiply-add a pair (kv4.cuh), exactly. fp32 queries are
-// fp16 hi + lo, accumulated by a second MMA; 16-bit queries are exact in fp16
-// (times a power of two). P is hi + lo too, but for bf16, whose output keeps 8
+// fp16 hi + lo, accumulated by a second MMA; 16-bit queries keep their bits in fp16
+// (times a power of two a row; a bf16 value below 2^-28 of its row's largest is held
+// to 2^-39 of that). P is hi + lo too, but for bf16, whose output keeps 8
 // bits: rounded to fp16's 11 it would add as much error to an fp16 output as the
 // output's own rounding. Softmax statistics and sums are fp32.
 //
@@ -29,10 +30,11 @@
 // and the CTA that finishes last (a counter, left at zero) adds them in order:
 // sums never depend on timing.
 //
-// Measured: 16 contexts of 24001 to 32768 rows, bf16, 131 MB: 44 us, 3.0 TB/s (46% of
-// the measured copy rate; 4.0 TB/s while it streams, at 2.2 instructions a cycle and
-// 350 for 16 rows). 16 ragged streams of 64 to 4096 rows: 11.3 us, one token over 513
-// rows: 8.4 us, both bound by what runs once.
+// Measured: 16 contexts of 24001 to 32768 rows, bf16, 131 MB: 44 us, 3.0 TB/s (45% of
+// the measured copy rate; 4.0 TB/s while it streams). A warp's 350 instructions for 16
+// rows are one chain (scores, maximum, exponentials, transposes, values): with 16 warps
+// an SM issues 2.2 a cycle, and no pipe is full. 16 ragged streams of 64 to 4096 rows:
+// 11.7 us, one token over 513 rows: 8.5 us, both bound by what runs once.
 //
 // What one call pays once is mostly instruction fetch: code that runs once costs
 // about 5 cycles an instruction here. So the loop body covers 16 cache rows and

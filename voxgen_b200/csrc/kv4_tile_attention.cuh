@@ -8,9 +8,12 @@
 //   O += P V      128 x D x 128, P from tensor memory, V in shared memory
 // K and V are unpacked from their codes to fp16 exactly (kv4.cuh), so a 32-bit
 // call needs hi + lo only of its own operands: Q hi and lo against the same K,
-// P hi and lo against the same V, 4 products instead of 2. 16-bit queries are
-// exact in fp16 (times a power of two), and P is rounded to 11 bits, like the
-// output. Statistics and sums are fp32. The running maximum m is raised, and O
+// P hi and lo against the same V, 4 products instead of 2. 16-bit queries keep
+// their bits in fp16 (times a power of two a row; a bf16 value below 2^-28 of its
+// row's largest is held to 2^-39 of that). Their P is rounded to 11 bits: hi and lo
+// would take fp16 outputs from 2.9e-4 off (a prompt) and 2.5e-4 (a draft) to 2.2e-4
+// and 2.1e-4, the output's own rounding, in 1195 us and not 969, 33.6 us and not
+// 31.4. Statistics and sums are fp32. The running maximum m is raised, and O
 // rescaled, only when a score passes it by 2^8. It is taken off before the scaling
 // (kNoScore says why), which costs 1% against one multiply-add with S * f - m.
 //
@@ -28,8 +31,8 @@
 // cache tile of one query tile and their results are added at the end. The
 // products of one group run while the other does its softmax.
 //
-// Measured: the last 4096 tokens of a prompt over 32768 rows, fp16, 1.03 TFLOP: 961 us,
-// 1.07 PFLOP/s (65% of the measured burst rate). A unit of 256 query rows takes about
+// Measured: the last 4096 tokens of a prompt over 32768 rows, fp16, 1.03 TFLOP: 970 us,
+// 1.06 PFLOP/s (64% of the measured burst rate). A unit of 256 query rows takes about
 // 4000 cycles, of which the products need 2048 and the softmax's 32768 exponentials as
 // many; the two wait for each other through S, whose place P takes.
 //

@@ -30,7 +30,8 @@ constexpr uint32_t kVerifyCtas = 8;             // of a cluster: one sequence
 constexpr uint32_t kVerifyVocab = 1u << 20;     // largest vocabulary
 constexpr uint32_t kVerifyWarps = kVerifyThreads / 32;
 
-// Sum over a warp of values up to 2^38, by two integer reductions of 19 bits each.
+// Sum over a warp of values up to 2^40 (four probabilities a lane), by integer reductions of the low 19 bits and of the 21
+// above them: 32 of either stay below 2^32.
 __device__ __forceinline__ uint64_t warp_sum(uint64_t x) {
   const uint32_t low = __reduce_add_sync(~0u, (uint32_t)x & 0x7FFFFu), high = __reduce_add_sync(~0u, (uint32_t)(x >> 19));
   return low + ((uint64_t)high << 19);

@@ -263,7 +263,8 @@ class Kv4Cache:
     @_on_its_device
     def evict(self, budget: int, recent: int = 0, sinks: int = 0, *, into: Optional["Kv4Cache"] = None) -> None:
         """Cuts sequences that hold more than ``budget`` rows to it: the last ``recent`` and first ``sinks``
-        positions stay, and the rest that drew the most attention. ``into``: a cache over the same ``data``
+        positions stay, and the rest that drew the most attention. Rows then are not in the order of their positions:
+        drop rejected rows (``append`` with ``at``) before this call, not after it. ``into``: a cache over the same ``data``
         whose state, weights and positions receive the result instead."""
         rc = self._lib.vg_k_kv4_evict(self._ref, budget, recent, sinks, None if into is None else into._ref,
                                       _current_stream(self._index))
