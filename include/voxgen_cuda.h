@@ -488,6 +488,129 @@ int vg_k_verify_draft(const int32_t *tokens, const float *draft, const float *ta
                       uint32_t seqs, uint32_t drafted, uint32_t vocab, int32_t *accepted,
                       int32_t *next, void *cuda_stream);
 
+/* ---- a paged KV cache -------------------------------------------------------
+ * No reference counterpart: the reference gives every engine a cache of its own of
+ * max_context rows (src/baselm.rs:451-586). Here K and V rows of many requests lie
+ * in pages of one pool, which requests take as they grow and give back when they
+ * finish. Entry points on the caller's device buffers and stream; a serving loop runs
+ *   step -> append (each layer) -> attention, or select -> attention (each layer).
+ * A table is shared by the layers of a model; each layer has its own pool of the
+ * same pages. A table, its caches and their workspace are used by one stream at a time.
+ *
+ * table: [seqs][seq_pages], the pages of each sequence in order, -1 where it holds none.
+ * rows: [seqs], rows held. status: [seqs], VG_PAGED_* of the last step.
+ * free: [pages], a stack of free pages; pool[0] is its height, pool[1] collects
+ * VG_PAGED_TIMEOUT and VG_PAGED_NONFINITE. For an empty cache: table -1, rows 0, free any order of
+ * 0 .. pages - 1, pool {pages, 0}. Only step changes table, rows, free and pool[0].
+ * page_rows is a power of two from 16 to 256, seqs <= 4096, pages * page_rows < 2^31,
+ * seq_pages * page_rows <= 2^30. */
+#define VG_PAGED_FULL 1       /* the new rows would pass seq_pages                      */
+#define VG_PAGED_NO_PAGES 2   /* the pool had no pages left for them                    */
+#define VG_PAGED_BAD_COUNT 4  /* a count below 0, or past the step's tokens             */
+#define VG_PAGED_TIMEOUT 8    /* a bounded wait of an attention ran out (pool[1])       */
+#define VG_PAGED_NONFINITE 16 /* an append met a NaN or a value that it clamps (pool[1]) */
+typedef struct vg_paged_table {
+  int32_t *table;
+  int32_t *rows;
+  int32_t *status;
+  int32_t *free;
+  int32_t *pool;
+  uint32_t seqs;
+  uint32_t seq_pages;
+  uint32_t pages;
+  uint32_t page_rows;
+} vg_paged_table;
+
+/* What a step leaves for the calls after it, tokens packed in the order of sequences:
+ * starts [seqs + 1]: the first token of each sequence, then the number of all;
+ * slots, positions, sequences [tokens]: where each token's row goes (page * page_rows +
+ * row in the page), its position in its sequence, and the sequence; -1 for tokens past
+ * the last and those of a sequence that was refused;
+ * runs [vg_k_paged_runs()][4]: the new rows page by page: first token, page, first row
+ * in the page, rows (0 past the last run). Each array starts on 16 bytes. */
+typedef struct vg_paged_step {
+  int32_t *starts;
+  int32_t *slots;
+  int32_t *positions;
+  int32_t *sequences;
+  int32_t *runs;
+  uint32_t tokens;
+} vg_paged_step;
+
+/* One layer's pool: data [pages][kv_heads][K, V][page_rows][head_dim] of type dtype
+ * (VG_DTYPE_F16 or VG_DTYPE_BF16), head_dim 64 or 128, 16-byte aligned. summaries: NULL,
+ * or [pages][kv_heads][2][head_dim] of the same type: per channel the smallest and the
+ * largest K of the rows that a page held at its last append, NaN passed over (0 and 0
+ * for a channel of NaN alone). */
+typedef struct vg_paged_cache {
+  const vg_paged_table *table;
+  void *data;
+  void *summaries;
+  int32_t dtype;
+  uint32_t kv_heads;
+  uint32_t head_dim;
+} vg_paged_cache;
+
+/* Bytes of data and of summaries. Host only. */
+int vg_k_paged_bytes(uint32_t pages, uint32_t page_rows, uint32_t kv_heads, uint32_t head_dim,
+                     uint64_t *data_bytes, uint64_t *summary_bytes);
+/* Runs that a step of `tokens` tokens has room for: min(tokens, tokens / page_rows + 2 seqs). Host only. */
+int vg_k_paged_runs(const vg_paged_table *table, uint32_t tokens, uint32_t *runs);
+/* Moves the table on by one step. First sequence s is cut to its first keep[s] rows
+ * (keep[s] < 0 or keep NULL: all stay), and pages that it then does not need go onto the
+ * free stack, in the order of sequences and their entries. Then it gets pages for
+ * counts[s] new rows, and the new rows count as held. Pages come off the stack's top, in
+ * stack order, for the sequences in order; one whose demand and that of all sequences
+ * before it exceed the stack gets none, is left with the rows it kept and says so in its
+ * status, as does one that would pass seq_pages or whose count is out of range. The
+ * tokens of a refused sequence keep their place in the packed order (a count out of
+ * range has none). No call waits for the host. */
+int vg_k_paged_step(const vg_paged_table *table, const int32_t *counts, const int32_t *keep,
+                    const vg_paged_step *step, void *cuda_stream);
+/* Stores the step's new K and V rows, [tokens][kv_heads][head_dim] of type dtype with
+ * element strides {token, head} (host arrays; NULL: contiguous) and contiguous channels,
+ * rounded to the cache's type, and brings the summaries of their pages up to date where
+ * the cache has them. Infinities and values past the type's largest finite number are
+ * held as that one (VG_PAGED_NONFINITE reports them, and NaN). The step must be the
+ * table's last one. */
+int vg_k_paged_append(const vg_paged_cache *cache, const vg_paged_step *step, const void *k,
+                      const void *v, int dtype, const int64_t *k_strides,
+                      const int64_t *v_strides, void *cuda_stream);
+/* The pages that each query is to attend, from the summaries: chosen
+ * [queries][kv_heads][budget], pages of the sequence (not of the pool) in ascending
+ * order, then -1. A query that sees no more pages than budget gets them all. Otherwise
+ * the first `sinks` and the last `recent` pages are chosen and, of the others, those of
+ * the largest scores (equal scores: the lowest page). The score is the sum over channels
+ * and over the heads of the KV head of max(q * smallest, q * largest), in 64 bits; NaN in
+ * q counts as 0, infinities as the largest fp32 number. q, sequences and positions are as
+ * for attention. sinks + recent <= budget; seq_pages <= 24576. */
+int vg_k_paged_select(const vg_paged_cache *cache, const void *q, int dtype, uint32_t queries,
+                      uint32_t heads, const int64_t *q_strides, const int32_t *sequences,
+                      const int32_t *positions, uint32_t budget, uint32_t sinks, uint32_t recent,
+                      int32_t *chosen, void *cuda_stream);
+/* Grouped-query attention of single tokens: q and out [queries][heads][head_dim] of type
+ * dtype, q with element strides {query, head} (NULL: contiguous). Query i is of sequence
+ * sequences[i] (NULL: i) and attends its rows 0 .. positions[i] (NULL: all that are
+ * held), so the tokens of a draft attend causally with the step's sequences and
+ * positions. A position of -1 or a sequence out of range sees no row; a query that sees
+ * no row gives zeros. chosen: NULL, or [queries][kv_heads][budget] as select writes it,
+ * or any pages of the sequence: only rows of these are attended, -1 and pages past the
+ * rows are passed over, a page named twice counts twice. Rows that are not attended may
+ * hold anything; attended ones are finite or NaN, as append leaves them (an infinity put
+ * there some other way may give NaN). Results do not depend on timing: every sum has a
+ * fixed order. out and q do not overlap.
+ *
+ * workspace: vg_k_paged_attention_bytes() bytes (budget 0: no list), 16-byte aligned,
+ * zero-filled once before its first use; calls leave it ready for the next call of any
+ * shape it is large enough for. */
+int vg_k_paged_attention_bytes(const vg_paged_cache *cache, uint32_t queries, uint32_t heads,
+                               uint32_t budget, uint64_t *bytes);
+int vg_k_paged_attention(const vg_paged_cache *cache, const void *q, int dtype, uint32_t queries,
+                         uint32_t heads, const int64_t *q_strides, const int32_t *sequences,
+                         const int32_t *positions, const int32_t *chosen, uint32_t budget,
+                         float scale, void *out, void *workspace, uint64_t workspace_bytes,
+                         void *cuda_stream);
+
 /* ---- failure-detection test hooks (no reference counterpart) -------------- */
 /* One token step (like vg_decode_token without logits) in which every grid-
  * barrier target is one arrival beyond what the grid provides, so the first

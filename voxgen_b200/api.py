@@ -42,6 +42,8 @@ EXPORTS = [
     "vg_test_fake_event_status", "vg_model_batch_columns",
     "vg_k_kv4_bytes", "vg_k_kv4_append", "vg_k_kv4_read", "vg_k_kv4_attention_bytes", "vg_k_kv4_attention",
     "vg_k_kv4_evict", "vg_k_verify_draft",
+    "vg_k_paged_bytes", "vg_k_paged_runs", "vg_k_paged_step", "vg_k_paged_append", "vg_k_paged_select",
+    "vg_k_paged_attention_bytes", "vg_k_paged_attention",
 ]
 
 # which buffer vg_residual_state / vg_residual_copy_state return
@@ -83,6 +85,23 @@ class Kv4CacheDesc(C.Structure):
     """vg_kv4_cache: the device buffers and the shape of a cache held in 4 bits."""
     _fields_ = [(n, C.c_void_p) for n in ("data", "state", "weights", "positions")] + \
         [(n, C.c_uint32) for n in ("seqs", "kv_heads", "head_dim", "capacity")]
+
+
+class PagedTableDesc(C.Structure):
+    """vg_paged_table: the device buffers and the sizes of a paged cache's table."""
+    _fields_ = [(n, C.c_void_p) for n in ("table", "rows", "status", "free", "pool")] + \
+        [(n, C.c_uint32) for n in ("seqs", "seq_pages", "pages", "page_rows")]
+
+
+class PagedStepDesc(C.Structure):
+    """vg_paged_step: the arrays that a step writes."""
+    _fields_ = [(n, C.c_void_p) for n in ("starts", "slots", "positions", "sequences", "runs")] + [("tokens", C.c_uint32)]
+
+
+class PagedCacheDesc(C.Structure):
+    """vg_paged_cache: one layer's pool."""
+    _fields_ = [("table", C.POINTER(PagedTableDesc)), ("data", C.c_void_p), ("summaries", C.c_void_p),
+                ("dtype", C.c_int32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32)]
 
 
 class KernelTime(C.Structure):
@@ -158,6 +177,13 @@ def lib() -> C.CDLL:
         "vg_k_kv4_attention": ([P, P, I, U32, U32, P, P, F, I, P, P, U64, P], I),
         "vg_k_kv4_evict": ([P, U32, U32, U32, P, P], I),
         "vg_k_verify_draft": ([P, P, P, P, P, P, U32, U32, U32, P, P, P], I),
+        "vg_k_paged_bytes": ([U32, U32, U32, U32, C.POINTER(U64), C.POINTER(U64)], I),
+        "vg_k_paged_runs": ([P, U32, C.POINTER(U32)], I),
+        "vg_k_paged_step": ([P, P, P, P, P], I),
+        "vg_k_paged_append": ([P, P, P, P, I, P, P, P], I),
+        "vg_k_paged_select": ([P, P, I, U32, U32, P, P, P, U32, U32, U32, P, P], I),
+        "vg_k_paged_attention_bytes": ([P, U32, U32, U32, C.POINTER(U64)], I),
+        "vg_k_paged_attention": ([P, P, I, U32, U32, P, P, P, P, U32, F, P, P, U64, P], I),
     }
     for name, (args, res) in sig.items():
         f = getattr(L, name)

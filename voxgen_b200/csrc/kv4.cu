@@ -4,9 +4,9 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <atomic>
 
 #include "../../include/voxgen_cuda.h"
+#include "entry.cuh"
 #include "kv4_rows.cuh"
 #include "kv4_rows_attention.cuh"
 #include "kv4_tile_attention.cuh"
@@ -16,15 +16,6 @@
 using namespace vg;
 
 namespace {
-
-constexpr uint64_t kMaxGrid = 0x7FFFFFFFu;
-
-bool aligned(const void *p, size_t a) { return (uintptr_t)p % a == 0; }
-
-int launched() {
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? VG_OK : e == cudaErrorMemoryAllocation ? VG_ENOMEM : VG_ECUDA;
-}
 
 int shape_status(uint64_t seqs, uint64_t kv_heads, uint32_t head_dim, uint32_t capacity) {
   if (!seqs || !kv_heads || !capacity) return VG_EINVAL;
@@ -44,10 +35,6 @@ int view_of(const vg_kv4_cache *c, Kv4View *v) {
   return VG_OK;
 }
 
-size_t type_size(int dtype) {
-  return dtype == VG_DTYPE_F32 ? 4 : dtype == VG_DTYPE_F16 || dtype == VG_DTYPE_BF16 ? 2 : 0;
-}
-
 // Strides in elements {sequence, token, head}; NULL: [seqs][tokens][heads][head_dim].
 Strides strides_of(const int64_t *s, uint32_t tokens, uint32_t heads, uint32_t head_dim) {
   const int64_t row = (int64_t)heads * head_dim;
@@ -58,44 +45,6 @@ Strides strides_of(const int64_t *s, uint32_t tokens, uint32_t heads, uint32_t h
 bool wide(const void *p, const Strides &s, size_t size) {
   const int64_t n = (int64_t)(16 / size);
   return aligned(p, 16) && s.seq % n == 0 && s.token % n == 0 && s.head % n == 0;
-}
-
-template <typename F>
-int by_type(int dtype, F &&f) {
-  switch (dtype) {
-    case VG_DTYPE_F32: return f(float{});
-    case VG_DTYPE_F16: return f(__half{});
-    case VG_DTYPE_BF16: return f(__nv_bfloat16{});
-  }
-  return VG_EUNSUPPORTED;
-}
-
-template <int D>
-struct Dim {
-  static constexpr int value = D;
-};
-template <typename F>
-int by_dim(uint32_t head_dim, F &&f) {
-  return head_dim == 64 ? f(Dim<64>{}) : f(Dim<128>{});
-}
-
-// Lets fn use up to `bytes` of dynamic shared memory on the current device. `done`
-// belongs to fn: the devices (up to 64) on which that has been set. `registers`: the
-// fewest registers of a thread that fn may have been compiled to; the tile kernel's
-// warpgroups trade theirs, and if they took more in all than the launch brings, the
-// takers would wait for good.
-int allow_smem(const void *fn, size_t bytes, std::atomic<uint64_t> &done, int registers = 0) {
-  if (bytes <= 48 * 1024) return VG_OK;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return VG_ECUDA;
-  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-  if (bit && done.load(std::memory_order_acquire) & bit) return VG_OK;
-  cudaFuncAttributes a;
-  if (cudaFuncGetAttributes(&a, fn) != cudaSuccess) return VG_ECUDA;
-  if (a.numRegs < registers) return VG_EUNSUPPORTED;
-  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return VG_ECUDA;
-  done.fetch_or(bit, std::memory_order_release);
-  return VG_OK;
 }
 
 // Blocks of a sequence for `items` (token, head) pairs: no more than have a pass to
