@@ -1,6 +1,7 @@
-"""The paged cache's operators on the CPU (Python and 64-bit numpy), for the tests: written from their
+"""The paged cache's operators in Python and 64-bit arithmetic, for the tests: written from their
 definitions, apart from the kernels and from the forms that the benchmark compares with."""
 import numpy as np
+import torch
 
 FULL, NO_PAGES, BAD_COUNT = 1, 2, 4
 
@@ -71,20 +72,16 @@ class Table:
 
 
 def attention(q, k, v, rows, scale=None):
-    """One query's heads [heads, head_dim] over the rows k, v [kv_heads, rows, head_dim] in 64 bits; rows: which of them
-    each KV head attends, a list of row numbers a head."""
+    """One query's heads [heads, head_dim] over the rows k, v [kv_heads, rows, head_dim] in 64 bits (torch, on any device);
+    rows: which of them each KV head attends, row numbers a head."""
     heads, dim = q.shape
     group = heads // k.shape[0]
-    scale = dim ** -0.5 if scale is None else scale
-    out = np.zeros_like(q, dtype=np.float64)
-    for h in range(heads):
-        mine = rows[h // group]
-        if not len(mine):
-            continue
-        with np.errstate(invalid="ignore"):
-            e = k[h // group, mine] @ q[h] * scale
-            p = np.exp(e - e.max())
-            out[h] = (p / p.sum()) @ v[h // group, mine]
+    out = torch.zeros(heads, dim, dtype=torch.float64, device=q.device)
+    for h, mine in enumerate(rows):
+        if len(mine):
+            e = q[h * group:(h + 1) * group].double() @ k[h, mine].T * (dim ** -0.5 if scale is None else scale)
+            p = (e - e.amax(1, keepdim=True)).exp()
+            out[h * group:(h + 1) * group] = p / p.sum(1, keepdim=True) @ v[h, mine]
     return out
 
 

@@ -273,39 +273,37 @@ def rows_of(cache, seq, layer=0):
     """K and V [kv_heads, rows, dim] that a sequence holds, in 64 bits."""
     n, page = int(cache.table.rows[seq]), cache.table.page_rows
     pages = cache.table.table[seq, :-(-n // page)].long()
-    x = cache.data[layer][pages].double().permute(1, 2, 0, 3, 4).flatten(2, 3)[:, :, :n].cpu().numpy()
+    x = cache.data[layer][pages].double().permute(1, 2, 0, 3, 4).flatten(2, 3)[:, :, :n]
     return x[:, 0], x[:, 1]
 
 
 def check_attention(cache, q, out, dtype, sequences=None, positions=None, chosen=None, scale=None, layer=0):
     page = cache.table.page_rows
     held = {}
-    top, worst, most = 0.0, 0.0, 1e-30
-    x, got = host(q), host(out)
-    want = np.zeros_like(x)
+    top, most = 0.0, 1e-30
+    want = torch.zeros(out.shape, dtype=torch.float64, device="cuda")
     group = q.shape[1] // cache.kv_heads
-    for i in range(len(x)):
+    for i in range(len(q)):
         s = i if sequences is None else sequences[i]
         if not 0 <= s < cache.table.seqs:
             continue
         if s not in held:
             held[s] = rows_of(cache, s, layer)
         k, v = held[s]
-        n = k.shape[1] if positions is None else min(k.shape[1], positions[i] + 1)
+        n = k.shape[1] if positions is None else max(0, min(k.shape[1], positions[i] + 1))
         if chosen is None:
-            mine = [list(range(n))] * cache.kv_heads
+            mine = [torch.arange(n, device="cuda")] * cache.kv_heads
         else:
-            mine = [[r for p in chosen[i][h] if p >= 0 for r in range(p * page, (p + 1) * page) if r < n]
-                    for h in range(cache.kv_heads)]
-        want[i] = R.attention(x[i], k, v, mine, scale)
+            mine = [torch.tensor([r for p in chosen[i][h] if p >= 0 for r in range(p * page, (p + 1) * page) if r < n],
+                                 dtype=torch.long, device="cuda") for h in range(cache.kv_heads)]
+        want[i] = R.attention(q[i], k, v, mine, scale)
         if n > 0:
-            size = (np.abs(x[i])[:, None] * np.abs(np.repeat(k[:, :n], group, 0))).sum(-1).max()
-            top = max(top, size * (q.shape[2] ** -0.5 if scale is None else scale))
-            most = max(most, np.abs(v[:, :n]).max())
+            size = (q[i].double().abs().unflatten(0, (-1, group)) @ k[:, :n].abs().transpose(1, 2)).max()
+            top = max(top, float(size) * (q.shape[2] ** -0.5 if scale is None else scale))
+            most = max(most, float(v[:, :n].abs().max()))
     tol = (top * 2.0 ** -17 + 2.0 ** -17 + EXTRA[dtype]) * most
-    worst = np.abs(got - want).max() if got.size else 0.0
+    worst = float((out.double() - want).abs().max())
     assert worst <= tol, (worst, tol)
-    return worst / tol
 
 
 SHAPES = [
@@ -360,6 +358,52 @@ def test_attention_of_many_sequences(seqs):
     cache = filled(1, rows.tolist(), 16, 2, 64, "f16")
     q = normal(2, seqs, 8, 64)
     check_attention(cache, q, cache.attention(q), "f32")
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 2, 128), (8, 2, 64), (24, 1, 64), (72, 1, 128)])
+@pytest.mark.parametrize("dtype,kind", [("f32", "f16"), ("f32", "bf16"), ("bf16", "bf16")])
+def test_attention_of_long_contexts(heads, kv_heads, dim, dtype, kind):
+    """The ring of copies goes round many times, with teams of 1 to 8 warps in a CTA one after the other."""
+    rows = [20000, 7, 9001, 300]
+    cache = filled(3, rows, 64, kv_heads, dim, kind)
+    q = normal(4, 4, heads, dim, dtype=TYPES[dtype])
+    check_attention(cache, q, cache.attention(q), dtype)
+    rng = np.random.default_rng(heads)
+    sequences = [s for s in rng.integers(0, 4, 14) for _ in range(rng.integers(1, 10))]
+    positions = [int(max(0, rows[s] - 1 - rng.integers(0, 40))) for s in sequences]
+    q = normal(5, len(sequences), heads, dim, dtype=TYPES[dtype])
+    out = cache.attention(q, sequences=ints(sequences), positions=ints(positions))
+    check_attention(cache, q, out, dtype, sequences, positions)
+    again = cache.attention(q, sequences=ints(sequences), positions=ints(positions))
+    assert torch.equal(out, again)
+
+
+def test_attention_of_many_drafts():
+    """More segments than CTAs, so that a CTA's pieces differ in their tiles."""
+    rng = np.random.default_rng(1)
+    rows = rng.integers(1, 900, 40).tolist()
+    cache = filled(3, rows, 16, 2, 64, "f16")
+    sequences = [s for s in range(40) for _ in range(rng.integers(1, 12))]
+    positions = [int(rng.integers(0, rows[s])) for s in sequences]
+    q = normal(5, len(sequences), 16, 64)
+    out = cache.attention(q, sequences=ints(sequences), positions=ints(positions))
+    check_attention(cache, q, out, "f32", sequences, positions)
+
+
+def test_a_row_that_only_later_tokens_see_may_hold_anything():
+    """NaN in the row of a draft's second token leaves its first token's output alone."""
+    cache = filled(3, [40, 33], 16, 1, 64, "f16")
+    table = cache.table
+    q = normal(5, 4, 8, 64)
+    sequences, positions = ints([0, 0, 0, 1]), ints([37, 38, 39, 32])
+    want = cache.attention(q, sequences=sequences, positions=positions)
+    for part in (cache.k(), cache.v()):
+        place = int(table.table[0, 38 // 16]), 0, 38 % 16
+        kept = part[place].clone()
+        part[place] = float("nan")
+        out = cache.attention(q, sequences=sequences, positions=positions)
+        assert torch.equal(out[[0, 3]], want[[0, 3]]) and out[1:3].isnan().all()
+        part[place] = kept
 
 
 def test_attention_of_more_segments_than_are_cut():
@@ -428,8 +472,8 @@ def test_attention_of_scores_past_two_to_the_24():
         q = normal(1, 1, 2, 64) * 1e4
         out = host(cache.attention(q))[0]
         k, v = rows_of(cache, 0)
-        best = (k[0] @ host(q)[0].T).argmax(0)
-        np.testing.assert_allclose(out, v[0, best], rtol=2.0 ** -20, atol=2.0 ** -20)
+        best = (k[0] @ q[0].double().T).argmax(0)
+        np.testing.assert_allclose(out, host(v[0, best]), rtol=2.0 ** -20, atol=2.0 ** -20)
 
 
 def test_damaged_tables_read_no_bad_page():
@@ -594,7 +638,7 @@ def test_a_serving_loop():
                 new = [host(x[starts[s]:starts[s + 1]].half()) if ref.status[s] == 0 else x[:0].cpu().numpy() for x in (k, v)]
                 held[s][layer] = tuple(np.concatenate((a[:cut], b)) for a, b in zip(held[s][layer], new))
                 for mine, theirs in zip(held[s][layer], rows_of(cache, s, layer)):
-                    np.testing.assert_array_equal(mine.transpose(1, 0, 2), theirs)
+                    np.testing.assert_array_equal(mine.transpose(1, 0, 2), host(theirs))
             chosen = cache.select(q, 4, sinks=1, recent=1, sequences=step.sequences, positions=step.positions, layer=layer)
             out = cache.attention(q, sequences=step.sequences, positions=step.positions, chosen=chosen, layer=layer)
             check_attention(cache, q, out, "f32", step.sequences.tolist(), step.positions.tolist(), chosen.tolist(), layer=layer)

@@ -133,7 +133,20 @@ int queries_of(const PagedView &c, uint32_t head_dim, const void *q, int dtype, 
 }
 
 constexpr uint64_t kPagedTicketBytes = kPagedTickets * 4;
-uint32_t head_tiles(const PagedView &c, uint32_t heads) { return (heads / c.kv_heads + kPagedHeads - 1) / kPagedHeads; }
+// How the tiles of 8 heads of a KV head make segments.
+struct Tiling {
+  uint32_t head_tiles, tiles, lanes;   // of a KV head, of a segment (a power of two, 8 at most), segments of a query
+  bool share;                          // consecutive queries of a sequence may make one segment
+};
+Tiling tiling_of(uint32_t kv_heads, uint32_t heads, uint32_t budget) {
+  Tiling x{};
+  x.head_tiles = (heads / kv_heads + kPagedHeads - 1) / kPagedHeads;
+  x.share = x.head_tiles == 1 && !budget;   // lists of pages differ from query to query
+  x.tiles = 1;
+  while (x.tiles < kPagedWarps && x.tiles < x.head_tiles) x.tiles *= 2;
+  x.lanes = kv_heads * ((x.head_tiles + kPagedWarps - 1) / kPagedWarps);
+  return x;
+}
 
 }  // namespace
 
@@ -264,11 +277,14 @@ int vg_k_paged_attention_bytes(const vg_paged_cache *cache, uint32_t queries, ui
   const int rc = cache_of(cache, &c);
   if (rc) return rc;
   if (!bytes || !queries || !heads || heads % cache->kv_heads) return VG_EINVAL;
-  const uint64_t segments = (uint64_t)queries * cache->kv_heads * head_tiles(c, heads);
+  const Tiling x = tiling_of(c.kv_heads, heads, budget);
+  const uint64_t segments = (uint64_t)queries * x.lanes;
   const uint64_t blocks = (uint64_t)(budget ? budget : c.t.seq_pages) << (c.t.shift - 4);   // of a segment, at most
-  if (budget > 0x40000000u || segments > kMaxGrid || blocks > kMaxGrid || segments * blocks > kMaxGrid)
+  const uint64_t cost = segments * blocks * std::max(1u, x.tiles / 2);
+  if (budget > 0x01000000u || segments > kMaxGrid || blocks >= 1u << 29 || cost > kMaxGrid)
     return VG_ERANGE;   // counted in 32 bits
-  *bytes = kPagedTicketBytes + paged_pieces(segments) * kPagedHeads * (cache->head_dim + 2) * 4;
+  *bytes = kPagedTicketBytes +
+           (uint64_t)paged_slots(segments) * (x.share ? kPagedWarps : x.tiles) * kPagedHeads * (cache->head_dim + 2) * 4;
   return VG_OK;
 }
 
@@ -300,7 +316,11 @@ int vg_k_paged_attention(const vg_paged_cache *cache, const void *q, int dtype, 
   p.queries = queries;
   p.heads = heads;
   p.group = x.group;
-  p.head_tiles = head_tiles(c, heads);
+  const Tiling tiling = tiling_of(c.kv_heads, heads, budget);
+  p.head_tiles = tiling.head_tiles;
+  p.share = tiling.share && sequences;   // else every query is of its own sequence
+  p.tiles = p.share ? kPagedWarps : tiling.tiles;
+  p.lanes = tiling.lanes;
   p.scale = scale * 1.44269504088896340736f;
   p.tickets = (uint32_t *)workspace;
   p.parts = (float *)((uint8_t *)workspace + kPagedTicketBytes);

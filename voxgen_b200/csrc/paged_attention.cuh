@@ -11,16 +11,21 @@
 //
 // The bound is bytes: 4 D of them a row for 4 D multiply-adds a head. So one warp
 // does nothing but keep copies in flight: it looks page numbers up 32 at a time and
-// issues tensor copies of 16 rows (K and V; 8 KB at head_dim 128) into the rings of
-// 8 consumer warps, 192 KB in all, through 128-byte swizzled boxes that ldmatrix
-// reads without bank conflicts. A consumer takes every 8th block of 16 rows and
-// keeps its own softmax state; the consumers meet when the piece ends.
+// issues tensor copies of 16 rows (K and V; 8 KB at head_dim 128) into a ring of 128
+// KB, through 128-byte swizzled boxes that ldmatrix reads without bank conflicts.
 //
-// The split. A segment is a (query, KV head, 8 heads of it); it is cut into pieces
-// of at most U blocks of 16 rows, U such that there is about one piece for each of
-// the 148 CTAs (4, where segments are many). A segment of several pieces leaves a
-// partial result for each, and the CTA that finishes last (a counter, left at zero)
-// adds them in order: sums never depend on timing.
+// A tile is (query, 8 heads of a KV head), a warp's work. Up to 8 tiles that read the
+// same rows make a segment: the tiles of more than 8 heads to a KV head, or consecutive
+// queries of one sequence (a draft's tokens). A block of 16 rows is then read once for
+// the T tiles, and the 8 consumer warps are 8 / T teams that take blocks in turn. Tiles
+// never mix queries, so a row that one query sees and another does not is masked warp
+// by warp, whatever it holds.
+//
+// The split. Segments are cut into pieces of at most U blocks, U such that there is
+// about one piece for each of the 148 CTAs (4, where segments are many). The warps of
+// a piece meet in shared memory. A segment of several pieces leaves a partial result
+// for each, and the CTA that finishes last (a counter, left at zero) adds them in
+// order: sums never depend on timing.
 #pragma once
 #include <cuda.h>
 
@@ -40,10 +45,14 @@ struct PagedAttnParams {
   PagedQueries which;
   const int32_t *chosen;     // [queries][kv_heads][budget] pages of each (query, KV head), or null: all
   uint32_t budget;
-  uint32_t queries, heads, group, head_tiles;   // head_tiles: of 8 heads, of a KV head
+  uint32_t queries, heads, group;
+  uint32_t head_tiles;       // of 8 heads, of a KV head
+  uint32_t share;            // consecutive queries of a sequence share what they read
+  uint32_t tiles;            // most tiles of a segment (a power of two); of each segment, where queries do not share
+  uint32_t lanes;            // segments of a query
   float scale;               // of the scores, times log2(e)
-  uint32_t *tickets;         // [segments], zero between calls
-  float *parts;              // [pieces] partial results
+  uint32_t *tickets;         // [queries * lanes], zero between calls
+  float *parts;              // [pieces of cut segments][tiles] partial results
 };
 
 constexpr uint32_t kPagedBlock = 16;     // cache rows of a block: never more than one page's
@@ -53,94 +62,151 @@ constexpr uint32_t kPagedCtas = 148;     // one per SM
 constexpr uint32_t kPagedHeads = 8;      // columns of a tile
 constexpr uint32_t kPagedLeast = 16;     // blocks of a piece: two rounds of the warps
 constexpr uint32_t kPagedTickets = 1u << 14;   // segments that may be cut
+constexpr uint32_t kPagedPlanned = 1024;       // queries whose place in the plan is kept in shared memory
 
 template <int D>
 struct PagedSmem {
   static constexpr uint32_t kHalf = 2 * kPagedBlock * 128;     // one copy: 64 channels of 16 K rows, then of 16 V rows
   static constexpr uint32_t kStage = kHalf * (D / 64);
-  static constexpr uint32_t kStages = 24 / kPagedWarps * 128 / D;   // of a warp's ring
-  static constexpr uint32_t kRing = kPagedWarps * kStages * kStage;
-  static constexpr uint32_t kRow = 68;                         // floats of a row when results meet: 64 and 4 against bank conflicts
-  static constexpr uint32_t kMerge = 20480;                    // results of 64 channels, or the weights of up to 640 pieces
-  static constexpr uint32_t kBytes = kRing + kMerge + 1024;    // the ring starts on a multiple of 1024
-  static_assert(kPagedWarps * kPagedHeads * kRow * 4 <= kMerge, "");
+  static constexpr uint32_t kStages = 16 * 128 / D;
+  // A warp that waits for a stage's next turn has to have waited for the one before (a wait for the turn after one in
+  // flight returns at once): so within a piece a stage is always the same team's, and pieces take whole rounds of 8 stages.
+  static_assert(kStages % kPagedWarps == 0, "");
+  static constexpr uint32_t kRing = kStages * kStage;
+  static constexpr uint32_t kRow = D + 4;                      // floats of a row when results meet: 4 against bank conflicts
+  static constexpr uint32_t kMerge = kPagedWarps * kPagedHeads * kRow * 4;
+  static constexpr uint32_t kTileQ = D / 16 * 32 * 8;          // a tile's queries as B fragments, one term
+  static constexpr uint32_t kShared = kMerge > 3 * kPagedWarps * kTileQ ? kMerge : 3 * kPagedWarps * kTileQ;   // first queries, then results
+  static constexpr uint32_t kBytes = kRing + kShared + 1024;   // the ring starts on a multiple of 1024
 };
 
-// Pieces that a call may be cut into: `segments` plus what the target allows.
+// Pieces that a call is cut into, about, and the partial results that it may leave: a segment that is cut at all has fewer
+// than twice its share of the target in pieces.
 __host__ __device__ __forceinline__ uint32_t paged_target(uint32_t segments) {
   return kPagedCtas * (segments * 4 <= kPagedCtas * 3 ? 1 : 4);
 }
-static_assert((kPagedCtas * 4 + 1) * kPagedHeads * 4 <= PagedSmem<128>::kMerge, "a segment's pieces have their weights there");
-__host__ __device__ __forceinline__ uint64_t paged_pieces(uint64_t segments) {
-  return segments > kPagedTickets ? 0 : segments + paged_target((uint32_t)segments);
+__host__ __device__ __forceinline__ uint32_t paged_slots(uint64_t segments) {
+  return segments > kPagedTickets ? 0 : 2 * paged_target((uint32_t)segments);
 }
 
-// Blocks of 16 rows that a query's segments have: at least one, so that every output is written.
-__device__ __forceinline__ uint32_t paged_blocks(const PagedAttnParams &p, uint32_t query) {
-  if (query >= p.queries) return 0;
-  if (p.chosen) return p.budget << (p.t.shift - 4);
-  return max(1u, (paged_seen(p.t, p.which, query).seen + kPagedBlock - 1) / kPagedBlock);
+// Blocks and tiles of the segments that query i leads, blocks << 2 | log2(tiles); 0 where another query leads. At least one
+// block, so that every output is written. Queries share within aligned eights, in runs of a power of two.
+__device__ __forceinline__ uint32_t paged_entry(const PagedAttnParams &p, uint32_t i) {
+  if (i >= p.queries) return 0;
+  if (p.chosen) return (p.budget << (p.t.shift - 4)) << 2 | (31 - __clz(p.tiles));
+  const auto blocks = [&](uint32_t rows) { return max(1u, (rows + kPagedBlock - 1) / kPagedBlock); };
+  if (!p.share) return blocks(paged_seen(p.t, p.which, i).seen) << 2 | (31 - __clz(p.tiles));
+  const uint32_t from = i & ~7u;
+  const int32_t mine = p.which.sequences[i];
+  uint32_t same = 0;   // of the eight
+#pragma unroll
+  for (uint32_t j = 0; j < 8; ++j)
+    if (from + j < p.queries && p.which.sequences[from + j] == mine) same |= 1u << j;
+  const uint32_t at = i - from;
+  const uint32_t start = 32 - __clz(~same & ((1u << at) - 1)), end = __ffs(~same >> at) - 1 + at;   // of the run around i
+  const uint32_t length = end - start, off = at - start;
+  uint32_t first = 0, size = 8;                      // of the part of the run that i is in
+  if (length < 8) {
+#pragma unroll
+    for (size = 4; size > 1; size >>= 1) {
+      if (!(length & size)) continue;
+      if (off < first + size) break;
+      first += size;
+    }
+  }
+  if (off != first) return 0;
+  uint32_t seen = 0;
+  for (uint32_t j = 0; j < size; ++j) seen = max(seen, paged_seen(p.t, p.which, i + j).seen);
+  return blocks(seen) << 2 | (31 - __clz(size));
 }
-// How segments are cut, as for the 4-bit cache: pieces of `size` blocks, `pieces` of them. A warp's work.
+// What a segment's block costs: a block's bytes take as long as two tiles' arithmetic.
+__device__ __forceinline__ uint32_t paged_cost(uint32_t entry) { return (entry >> 2) << max((int)(entry & 3) - 1, 0); }
+__device__ __forceinline__ uint32_t paged_size(uint32_t entry, uint32_t size) {   // blocks of a piece that costs `size`
+  const uint32_t k = max((int)(entry & 3) - 1, 0);
+  return (size + (1u << k) - 1) >> k;
+}
+__device__ __forceinline__ uint32_t paged_pieces(uint32_t entry, uint32_t size) {
+  const uint32_t n = paged_size(entry, size);
+  return ((entry >> 2) + n - 1) / n;
+}
+
+// How segments are cut: pieces that cost at most `size`, `pieces` of them. A warp's work.
 struct PagedPlan {
-  uint32_t lanes, size, pieces;   // lanes: segments of a query
+  uint32_t size, pieces;
 };
-__device__ __forceinline__ uint32_t paged_pieces_of(uint32_t blocks, uint32_t size) { return (blocks + size - 1) / size; }
-__device__ __forceinline__ PagedPlan paged_plan(const PagedAttnParams &p) {
-  const uint32_t lane = threadIdx.x % 32, lanes = p.kv_heads * p.head_tiles, segments = p.queries * lanes;
-  PagedPlan x{lanes, 1u << 30, segments};   // one piece a segment
-  if (segments > kPagedTickets) return x;
-  uint32_t total = 0;
+template <typename E>
+__device__ __forceinline__ PagedPlan paged_plan(const PagedAttnParams &p, const E &entry) {
+  const uint32_t lane = threadIdx.x % 32;
+  uint32_t total = 0, leads = 0;
 #pragma unroll 1
-  for (uint32_t s = lane; s < p.queries; s += 32) total += paged_blocks(p, s);
-  total = __reduce_add_sync(~0u, total) * lanes;   // the host keeps it below 2^31
+  for (uint32_t s = lane; s < p.queries; s += 32) {
+    const uint32_t e = entry(s);
+    total += paged_cost(e);
+    leads += e != 0;
+  }
+  total = __reduce_add_sync(~0u, total) * p.lanes;   // the host keeps it below 2^31
+  const uint32_t segments = __reduce_add_sync(~0u, leads) * p.lanes;
+  PagedPlan x{1u << 30, segments};   // one piece a segment
+  if (p.queries * p.lanes > kPagedTickets) return x;
   const uint32_t target = paged_target(segments);
   x.size = max(kPagedLeast, (total + target - 1) / target);
 #pragma unroll 1
-  for (int i = 0;; ++i) {
+  for (int i = 0;; ++i) {   // the fewest blocks that make no more pieces than the target, or nearly
     uint32_t n = 0;
 #pragma unroll 1
-    for (uint32_t s = lane; s < p.queries; s += 32) n += paged_pieces_of(paged_blocks(p, s), x.size);
-    x.pieces = __reduce_add_sync(~0u, n) * lanes;
+    for (uint32_t s = lane; s < p.queries; s += 32) n += paged_pieces(entry(s), x.size);
+    x.pieces = __reduce_add_sync(~0u, n) * p.lanes;
     if (x.pieces <= target || i == 3) return x;
-    x.size = max(x.size + 1, (uint32_t)((uint64_t)x.size * x.pieces / target));
+    x.size = max(x.size + 1, (uint32_t)((float)x.size * __fdividef((float)x.pieces, (float)target)));
   }
 }
 
 struct PagedPiece {
-  uint32_t query, lane;         // lane: (KV head, 8 heads of it)
+  uint32_t query, lane;         // lane: (KV head, 8 of its tiles)
   uint32_t part, parts;         // of the segment
+  uint32_t slot;                // of the segment's first partial result
   uint32_t first, blocks;       // of the piece, in the segment
+  uint32_t tiles;               // 1, 2, 4 or 8
 };
-__device__ __forceinline__ PagedPiece paged_piece(const PagedAttnParams &p, const PagedPlan &x, uint32_t index) {
+// Where the search for a CTA's next piece goes on: 32 queries, and the pieces (all, and those of cut segments) before them.
+struct PagedCursor {
+  uint32_t base, before, cut;
+};
+template <typename E>
+__device__ __forceinline__ PagedPiece paged_piece(const PagedAttnParams &p, const PagedPlan &x, uint32_t index, const E &entry,
+                                                  PagedCursor &at32) {
   const uint32_t lane = threadIdx.x % 32;
-  uint32_t before = 0;
 #pragma unroll 1
-  for (uint32_t base = 0; base < p.queries; base += 32) {
-    const uint32_t blocks = paged_blocks(p, base + lane), n = paged_pieces_of(blocks, x.size);
-    uint32_t sum = n * x.lanes;
+  for (; at32.base < p.queries; at32.base += 32) {
+    const uint32_t base = at32.base, before = at32.before, cut_before = at32.cut;
+    const uint32_t e = entry(base + lane), n = paged_pieces(e, x.size);
+    uint32_t sum = n * p.lanes, cut = n > 1 ? sum : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t up = __shfl_up_sync(~0u, sum, o);
-      if (lane >= (uint32_t)o) sum += up;
+      const uint32_t up = __shfl_up_sync(~0u, sum, o), more = __shfl_up_sync(~0u, cut, o);
+      if (lane >= (uint32_t)o) sum += up, cut += more;
     }
     const uint32_t past = __ballot_sync(~0u, before + sum > index);
     if (past) {
       const int at = __ffs(past) - 1;
-      const uint32_t parts = __shfl_sync(~0u, n, at), all = __shfl_sync(~0u, blocks, at);
-      const uint32_t into = index - before - (__shfl_sync(~0u, sum, at) - parts * x.lanes);
+      const uint32_t parts = __shfl_sync(~0u, n, at), all = __shfl_sync(~0u, e, at);
+      const uint32_t into = index - before - (__shfl_sync(~0u, sum, at) - parts * p.lanes);
+      const uint32_t size = paged_size(all, x.size);
       PagedPiece y;
       y.query = base + at;
       y.lane = into / parts;
       y.part = into - y.lane * parts;
       y.parts = parts;
-      y.first = y.part * x.size;
-      y.blocks = min(x.size, all - y.first);
+      y.slot = cut_before + __shfl_sync(~0u, cut, at) - parts * p.lanes + y.lane * parts;
+      y.first = y.part * size;
+      y.blocks = min(size, (all >> 2) - y.first);
+      y.tiles = 1u << (all & 3);
       return y;
     }
-    before += __shfl_sync(~0u, sum, 31);
+    at32.before += __shfl_sync(~0u, sum, 31);
+    at32.cut += __shfl_sync(~0u, cut, 31);
   }
-  return PagedPiece{0, 0, 0, 1, 0, 0};   // past the last piece
+  return PagedPiece{0, 0, 0, 1, 0, 0, 0, 1};   // past the last piece
 }
 
 // ---- MMA operands of either type ----
@@ -199,76 +265,80 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
   constexpr bool kFresh = sizeof(T) == 4;       // O summed afresh
   constexpr uint32_t kFreshSteps = 8;
   extern __shared__ uint8_t paged_smem[];
-  __shared__ uint64_t full[kPagedWarps][S::kStages], empty[kPagedWarps][S::kStages];
-  __shared__ uint32_t valid_rows[kPagedWarps][S::kStages];
+  __shared__ uint64_t full[S::kStages], empty[S::kStages];
+  __shared__ uint32_t first_row[S::kStages];    // of a stage's block in its sequence; past every row: nothing was read
+  __shared__ uint32_t entries[kPagedPlanned];
   __shared__ __align__(8) float w_max[kPagedWarps][kPagedHeads], w_sum[kPagedWarps][kPagedHeads];
-  __shared__ float f_max[kPagedHeads], f_sum[kPagedHeads];
+  __shared__ float f_max[kPagedWarps][kPagedHeads], f_sum[kPagedWarps][kPagedHeads];   // [tile][head]
+  __shared__ __align__(8) float factors[kPagedWarps][kPagedHeads];                    // [tile][head]
   __shared__ uint32_t last, gave_up;
-  __shared__ __align__(8) uint32_t q_frag[kQ][kSteps][32][2];   // B fragments
-  __shared__ __align__(8) float factors[kPagedHeads];
-  __shared__ PagedPlan shared_plan;
   const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
   const uint32_t base = smem_u32(paged_smem), ring = (base + 1023) & ~1023u;
-  float *merge = (float *)(paged_smem + (ring - base) + S::kRing);
+  float *merge = (float *)(paged_smem + (ring - base) + S::kRing);   // [warp][head][kRow]
+  uint32_t *q_frag = (uint32_t *)merge;                             // [tile][term][step][lane][2]
   if (threadIdx.x == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map));
     gave_up = 0;
   }
-  if (warp < kPagedWarps && lane < S::kStages) mbar_init(&full[warp][lane], 1), mbar_init(&empty[warp][lane], 1);
+  if (threadIdx.x < S::kStages) mbar_init(&full[threadIdx.x], 1), mbar_init(&empty[threadIdx.x], kPagedWarps);
   fence_mbar_init();
   pdl_launch_dependents();
   pdl_wait();
-  if (warp == kPagedWarps) {
-    const PagedPlan x = paged_plan(p);
-    if (lane == 0) shared_plan = x;
-  }
+  for (uint32_t i = threadIdx.x; i < min(p.queries, kPagedPlanned); i += kPagedThreads) entries[i] = paged_entry(p, i);
   __syncthreads();
-  const PagedPlan plan = shared_plan;
+  const auto entry = [&](uint32_t i) { return i >= p.queries ? 0 : i < kPagedPlanned ? entries[i] : paged_entry(p, i); };
+  const PagedPlan plan = paged_plan(p, entry);
 
   if (warp == kPagedWarps) {
     // ================= the copying warp =================
-    uint32_t round = 0;        // rounds of 8 blocks, over all pieces
+    uint32_t n0 = 0;           // blocks of the pieces before
+    PagedCursor cursor{};
     bool stopped = false;
 #pragma unroll 1
     for (uint32_t index = blockIdx.x; index < plan.pieces && !stopped; index += gridDim.x) {
-      const PagedPiece x = paged_piece(p, plan, index);
-      const PagedSeen who = paged_seen(p.t, p.which, x.query);
-      const uint32_t kv = x.lane / p.head_tiles, page_rows = p.t.page_rows();
+      const PagedPiece x = paged_piece(p, plan, index, entry, cursor);
+      const uint32_t kv = p.share ? x.lane : x.lane / (p.lanes / p.kv_heads), page_rows = p.t.page_rows();
+      PagedSeen who = paged_seen(p.t, p.which, x.query);
+      if (p.share)
+        for (uint32_t i = 1; i < x.tiles; ++i) who.seen = max(who.seen, paged_seen(p.t, p.which, x.query + i).seen);
       const int32_t *table = p.t.table + (size_t)who.seq * p.t.seq_pages;
       const int32_t *list = p.chosen ? p.chosen + ((size_t)x.query * p.kv_heads + kv) * p.budget : nullptr;
-      // page and rows (1 to 16, 5 bits) of the piece's block i; 0: nothing to read
-      const auto find = [&](uint32_t i) -> uint32_t {
-        if (i >= x.blocks) return 0;
-        const uint32_t row = (x.first + i) * kPagedBlock, entry = row >> p.t.shift, in = row & (page_rows - 1);
-        const uint32_t at = list ? (uint32_t)list[entry] : entry;
-        if (at >= p.t.seq_pages) return 0;
-        const uint32_t first = (at << p.t.shift) + in;
-        if (first >= who.seen) return 0;
-        const uint32_t page = (uint32_t)table[at];
-        return page < p.t.pages ? page << 5 | min(kPagedBlock, who.seen - first) : 0;
+      // page and first row of the piece's block i
+      struct Found {
+        uint32_t page, row;
       };
-      uint32_t next = find(lane);
+      const auto find = [&](uint32_t i) -> Found {
+        const Found none{~0u, ~0u};
+        if (i >= x.blocks) return none;
+        const uint32_t row = (x.first + i) * kPagedBlock, e = row >> p.t.shift, in = row & (page_rows - 1);
+        const uint32_t at = list ? (uint32_t)list[e] : e;
+        if (at >= p.t.seq_pages) return none;
+        const uint32_t first = (at << p.t.shift) + in;
+        if (first >= who.seen) return none;
+        const uint32_t page = (uint32_t)table[at];
+        return page < p.t.pages ? Found{page, first} : none;
+      };
+      Found next = find(lane);
 #pragma unroll 1
       for (uint32_t i = 0; i < x.blocks && !stopped; i += 32) {
-        const uint32_t now = next;
+        const Found now = next;
         next = find(i + 32 + lane);
 #pragma unroll 1
-        for (uint32_t j = 0; j < 4 && i + 8 * j < x.blocks; ++j, ++round) {
-          const uint32_t block = __shfl_sync(~0u, now, 8 * j + lane % 8);
+        for (uint32_t j = 0; j < 32 && i + j < x.blocks; j += 8) {   // whole rounds: stages past the last block hold nothing
+          const uint32_t page = __shfl_sync(~0u, now.page, j + lane % 8), row = __shfl_sync(~0u, now.row, j + lane % 8);
           bool in = true;
-          if (lane < kPagedWarps) {
-            const uint32_t stage = round % S::kStages, turn = round / S::kStages;
-            if (turn) in = mbar_wait_bounded(&empty[lane][stage], (turn - 1) & 1);
+          if (lane < 8) {
+            const uint32_t n = n0 + i + j + lane, stage = n % S::kStages, turn = n / S::kStages;
+            if (turn) in = mbar_wait_bounded(&empty[stage], (turn - 1) & 1);
             if (in) {
-              valid_rows[lane][stage] = block & 31;
-              uint64_t *bar = &full[lane][stage];
-              if (block & 31) {
+              first_row[stage] = row;
+              uint64_t *bar = &full[stage];
+              if (row != ~0u) {
                 mbar_arrive_expect_tx(bar, S::kStage);
-                const int32_t place = (int32_t)((block >> 5) * p.kv_heads + kv);
-                const int32_t row = (int32_t)(((x.first + i + 8 * j + lane) * kPagedBlock) & (page_rows - 1));
-                const uint32_t dst = ring + (lane * S::kStages + stage) * S::kStage;
+                const int32_t place = (int32_t)(page * p.kv_heads + kv);
 #pragma unroll
-                for (int h = 0; h < D / 64; ++h) tensor_g2s(dst + h * S::kHalf, &map, h * 64, row, place, bar);
+                for (int h = 0; h < D / 64; ++h)
+                  tensor_g2s(ring + stage * S::kStage + h * S::kHalf, &map, h * 64, (int32_t)(row & (page_rows - 1)), place, bar);
               } else {
                 mbar_arrive(bar);
               }
@@ -281,33 +351,43 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
           }
         }
       }
+      n0 += (x.blocks + 7) & ~7u;
     }
     if (stopped && lane == 0) atomicOr(&p.t.pool[1], kPagedTimeout);
     return;
   }
 
   // ================= the consumers =================
-  uint32_t round = 0;
+  uint32_t n0 = 0;
+  PagedCursor cursor{};
   bool stopped = false;      // a wait ran out: nothing is waited for any more
-  const uint32_t my_ring = ring + warp * S::kStages * S::kStage;
   // this lane's row of an ldmatrix, and which of the two 16-byte chunks it reads
   const uint32_t k_row = lane % 8 + (lane / 8 % 2) * 8, k_chunk = lane / 16;
   const uint32_t v_row = lane % 8 + (lane / 16) * 8, v_chunk = lane / 8 % 2;
 #pragma unroll 1
   for (uint32_t index = blockIdx.x; index < plan.pieces; index += gridDim.x) {
-    const PagedPiece seg = paged_piece(p, plan, index);
+    const PagedPiece seg = paged_piece(p, plan, index, entry, cursor);
     const bool whole = seg.parts == 1;
-    const uint32_t kv = seg.lane / p.head_tiles, head0 = (seg.lane - kv * p.head_tiles) * kPagedHeads;
-    const uint32_t tile_heads = min(kPagedHeads, p.group - head0);
-    // ---- the queries as B fragments, a warp a head: column `warp` of the MMA ----
-    {
+    const uint32_t chunks = p.lanes / p.kv_heads;   // segments of a KV head, where it has more than 8 tiles
+    const uint32_t kv = p.share ? seg.lane : seg.lane / chunks;
+    const uint32_t tile0 = p.share ? 0 : (seg.lane - kv * chunks) * kPagedWarps;
+    const uint32_t teams = kPagedWarps / seg.tiles, team = warp / seg.tiles, tile = warp & (seg.tiles - 1);
+    // query and first head (of the KV head's) of a tile of the segment
+    const auto query_of = [&](uint32_t k) { return p.share ? seg.query + k : seg.query; };
+    const auto head_of = [&](uint32_t k) { return p.share ? 0 : (tile0 + k) * kPagedHeads; };
+    const uint32_t head0 = head_of(tile);
+    const uint32_t seen = paged_seen(p.t, p.which, query_of(tile)).seen;
+    // ---- the queries as B fragments, a warp a head of every tile: column `warp` of the MMA ----
+#pragma unroll 1
+    for (uint32_t k = 0; k < seg.tiles; ++k) {
       constexpr uint32_t N = D / 32;
+      const uint32_t head = head_of(k) + warp;
+      const T *q = (const T *)p.q + (int64_t)query_of(k) * p.q_query + (int64_t)(kv * p.group + head) * p.q_head + lane * N;
       float x[N];
-      const T *q = (const T *)p.q + (int64_t)seg.query * p.q_query + (int64_t)(kv * p.group + head0 + warp) * p.q_head + lane * N;
       uint32_t top = 0;
 #pragma unroll
       for (uint32_t i = 0; i < N; ++i) {
-        x[i] = warp < tile_heads ? (float)q[i] : 0.f;
+        x[i] = head < p.group ? (float)q[i] : 0.f;
         top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
       }
       // fp16's range is met by a power of two a head; bf16 has fp32's
@@ -318,18 +398,19 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         const uint32_t c = lane * N + i;
         float a = x[i] * power, b = x[i + 1] * power;
 #pragma unroll
-        for (int k = 0; k < kQ; ++k) q_frag[k][c / 16][warp * 4 + c % 8 / 2][c % 16 / 8] = take_pair(a, b, C{});
+        for (int j = 0; j < kQ; ++j)
+          q_frag[(((k * kQ + j) * kSteps + c / 16) * 32 + warp * 4 + c % 8 / 2) * 2 + c % 16 / 8] = take_pair(a, b, C{});
       }
-      if (lane == 0) factors[warp] = fmaxf(p.scale * inverse, 0x1p-126f);
+      if (lane == 0) factors[k][warp] = fmaxf(p.scale * inverse, 0x1p-126f);
     }
     named_bar(1, kPagedWarps * 32);
-    stopped |= __any_sync(~0u, *(volatile uint32_t *)&gave_up);
     uint32_t qf[kQ][kSteps][2];
 #pragma unroll
     for (int k = 0; k < kQ; ++k)
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) *(uint2 *)qf[k][i] = *(const uint2 *)q_frag[k][i][lane];
-    const float f0 = factors[2 * t], f1 = factors[2 * t + 1];   // scores of heads 2t and 2t + 1 are this lane's
+      for (int i = 0; i < kSteps; ++i) *(uint2 *)qf[k][i] = *(const uint2 *)&q_frag[(((tile * kQ + k) * kSteps + i) * 32 + lane) * 2];
+    const float f0 = factors[tile][2 * t], f1 = factors[tile][2 * t + 1];   // scores of heads 2t and 2t + 1 are this lane's
+    stopped |= __any_sync(~0u, *(volatile uint32_t *)&gave_up);
 
     float o[kSteps][4], all_o[kFresh ? kSteps : 1][4], m0 = kNoScore, m1 = kNoScore, l0 = 0.f, l1 = 0.f;
 #pragma unroll
@@ -339,27 +420,34 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       for (int j = 0; j < kSteps; ++j) all_o[j][0] = all_o[j][1] = all_o[j][2] = all_o[j][3] = 0.f;
     }
     uint32_t steps = 0;    // steps that this warp took
-    const uint32_t rounds = (seg.blocks + kPagedWarps - 1) / kPagedWarps;
+    uint32_t stage = (n0 + team) % S::kStages, parity = (n0 + team) / S::kStages & 1;
 #pragma unroll 1
-    for (uint32_t r = 0; r < rounds; ++r, ++round) {
-      const uint32_t stage = round % S::kStages;
-      if (!stopped && !__all_sync(~0u, mbar_wait_bounded(&full[warp][stage], round / S::kStages & 1))) {
+    for (uint32_t b = team; b < ((seg.blocks + 7) & ~7u); b += teams) {
+      if (!stopped && !__all_sync(~0u, mbar_wait_bounded(&full[stage], parity))) {
         stopped = true;
         if (lane == 0) *(volatile uint32_t *)&gave_up = 1;
       }
-      const uint32_t valid = stopped ? 0 : valid_rows[warp][stage];
-      if (valid) {
+      const uint32_t first = first_row[stage];
+      if (!stopped && first < seen && head0 < p.group) {
+        const uint32_t valid = seen - first;   // rows of the block that are seen, when below 16
         ++steps;
-        const uint32_t st = my_ring + stage * S::kStage;
+        const uint32_t st = ring + stage * S::kStage;
         // ---- scores ----
-        float c[4] = {0.f, 0.f, 0.f, 0.f};
+        // even and odd steps (and q's lower terms) in sums of their own: half the chain of dependent products
+        float sums[kQ > 1 ? 3 : 2][4] = {};
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
           uint32_t a[4];
           const uint32_t chunk = (k % 4) * 2 + k_chunk;
           ldmatrix4(a, st + k / 4 * S::kHalf + k_row * 128 + ((chunk ^ (k_row & 7)) << 4));
 #pragma unroll
-          for (int i = 0; i < kQ; ++i) mma_16(c, a, qf[i][k], C{});
+          for (int i = 0; i < kQ; ++i) mma_16(sums[i ? 2 : k % 2], a, qf[i][k], C{});
+        }
+        float c[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          c[i] = sums[0][i] + sums[1][i];
+          if constexpr (kQ > 1) c[i] += sums[2][i];
         }
         // ---- softmax: c[2y + z] is cache row 8y + g, head 2t + z ----
         const bool tail = valid < kPagedBlock;
@@ -419,8 +507,11 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[warp][stage]);
+      if (lane == 0) mbar_arrive_count(&empty[stage], teams);   // the team's T warps make up 8 arrivals
+      stage += teams;
+      if (stage >= S::kStages) stage -= S::kStages, parity ^= 1;
     }
+    n0 += (seg.blocks + 7) & ~7u;
     if constexpr (kFresh) {
 #pragma unroll
       for (int j = 0; j < kSteps; ++j)
@@ -428,7 +519,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         for (int y = 0; y < 4; ++y) o[j][y] += all_o[j][y];
     }
 
-    // ---- the warps' results meet ----
+    // ---- the teams' results meet, tile by tile ----
 #pragma unroll
     for (int x = 4; x < 32; x <<= 1) {
       l0 += __shfl_xor_sync(~0u, l0, x);
@@ -444,123 +535,147 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     }
     named_bar(1, kPagedWarps * 32);
     float top0 = kNoScore, top1 = kNoScore;
-#pragma unroll
-    for (uint32_t w = 0; w < kPagedWarps; ++w) {
+#pragma unroll 1
+    for (uint32_t w = tile; w < kPagedWarps; w += seg.tiles) {
       const float2 x = *(const float2 *)&w_max[w][2 * t];
       top0 = fmaxf(top0, x.x), top1 = fmaxf(top1, x.y);
     }
     const float e0 = exp2_fast(m0 - top0), e1 = exp2_fast(m1 - top1);
-    if (warp == 0 && g < 2) {   // lanes of g = 0 and 1: the denominators of heads 2t and 2t + 1
+    if (team == 0 && g < 2) {   // lanes of g = 0 and 1: the denominators of heads 2t and 2t + 1
       const float top = g ? top1 : top0;
       float all = 0.f;
-      bool seen = false;
-#pragma unroll
-      for (uint32_t w = 0; w < kPagedWarps; ++w) {
+      bool some = false;
+#pragma unroll 1
+      for (uint32_t w = tile; w < kPagedWarps; w += seg.tiles) {
         const float x = w_sum[w][2 * t + g];
-        seen |= x < 0.f;
+        some |= x < 0.f;
         all += (x < 0.f ? 0.f : x) * exp2_fast(w_max[w][2 * t + g] - top);
       }
-      f_max[2 * t + g] = top;
-      f_sum[2 * t + g] = all == 0.f && seen ? -1.f : all;
+      f_max[tile][2 * t + g] = top;
+      f_sum[tile][2 * t + g] = all == 0.f && some ? -1.f : all;
     }
-    float *part = p.parts + (size_t)index * kPart<D>;
-    T *out = (T *)p.out + ((size_t)seg.query * p.heads + kv * p.group + head0) * D;
+    float *part = p.parts + (size_t)(seg.slot + seg.part) * p.tiles * kPart<D>;
+    const auto out_of = [&](uint32_t k, uint32_t head) {   // of a tile's head
+      return (T *)p.out + ((size_t)query_of(k) * p.heads + kv * p.group + head_of(k) + head) * D;
+    };
     const auto inverse_of = [](float sum) {   // zeros where no row was seen, NaN where every score was -infinity
       return sum == 0.f ? 0.f : sum < 0.f ? NAN : 1.f / sum;
     };
 #pragma unroll
-    for (int h = 0; h < D / 64; ++h) {   // 64 channels at a time
-      if (h) named_bar(1, kPagedWarps * 32);
+    for (int j = 0; j < kSteps; ++j) {
+      float *dst = merge + (warp * kPagedHeads + 2 * t) * S::kRow + 16 * j + g;
+      dst[0] = e0 * o[j][0], dst[8] = e0 * o[j][2];
+      dst[S::kRow] = e1 * o[j][1], dst[S::kRow + 8] = e1 * o[j][3];
+    }
+    named_bar(1, kPagedWarps * 32);
+    struct __align__(D / 8) Values {   // a lane's channels of a head
+      float x[D / 32];
+    };
+#pragma unroll 1
+    for (uint32_t k = 0; k < seg.tiles; ++k) {   // a warp a head of every tile
+      if (head_of(k) + warp >= p.group) continue;
+      Values x{};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = 4 * h + i;
-        float *dst = merge + (warp * kPagedHeads + 2 * t) * S::kRow + 16 * i + g;
-        dst[0] = e0 * o[j][0], dst[8] = e0 * o[j][2];
-        dst[S::kRow] = e1 * o[j][1], dst[S::kRow + 8] = e1 * o[j][3];
+      for (uint32_t w = 0; w < kPagedWarps; ++w) {
+        if ((w & (seg.tiles - 1)) != k) continue;
+        const Values y = *(const Values *)(merge + (w * kPagedHeads + warp) * S::kRow + D / 32 * lane);
+#pragma unroll
+        for (uint32_t n = 0; n < D / 32; ++n) x.x[n] += y.x[n];
       }
-      named_bar(1, kPagedWarps * 32);
-      if (warp < tile_heads) {   // a warp a head, two channels a lane
-        float2 x = make_float2(0.f, 0.f);
+      if (whole) {
+        const float inv = inverse_of(f_sum[k][warp]);
+        T *dst = out_of(k, warp) + D / 32 * lane;
 #pragma unroll
-        for (uint32_t w = 0; w < kPagedWarps; ++w) {
-          const float2 y = *(const float2 *)(merge + (w * kPagedHeads + warp) * S::kRow + 2 * lane);
-          x.x += y.x, x.y += y.y;
-        }
-        const uint32_t ch = 64 * h + 2 * lane;
-        if (whole) {
-          const float inv = inverse_of(f_sum[warp]);
-          T *dst = out + warp * D + ch;
-          dst[0] = from_float<T>(x.x * inv), dst[1] = from_float<T>(x.y * inv);
-        } else {
-          *(float2 *)(part + warp * D + ch) = x;
-        }
+        for (uint32_t n = 0; n < D / 32; ++n) dst[n] = from_float<T>(x.x[n] * inv);
+      } else {
+        *(Values *)(part + k * kPart<D> + warp * D + D / 32 * lane) = x;
       }
     }
     if (!whole) {
-      if (threadIdx.x < tile_heads) {
-        part[kPagedHeads * D + threadIdx.x] = f_max[threadIdx.x];
-        part[kPagedHeads * (D + 1) + threadIdx.x] = f_sum[threadIdx.x];
+      if (threadIdx.x < seg.tiles * kPagedHeads) {
+        float *dst = part + threadIdx.x / kPagedHeads * kPart<D> + kPagedHeads * D + threadIdx.x % kPagedHeads;
+        dst[0] = f_max[0][threadIdx.x];
+        dst[kPagedHeads] = f_sum[0][threadIdx.x];
       }
       named_bar(1, kPagedWarps * 32);
       const uint32_t pieces = seg.parts;
-      const float *others = p.parts + (size_t)(index - seg.part) * kPart<D>;
-      uint32_t *ticket = p.tickets + seg.query * plan.lanes + seg.lane;
+      uint32_t *ticket = p.tickets + seg.query * p.lanes + seg.lane;
       if (threadIdx.x == 0) last = atomic_add_acq_rel(ticket, 1u) == pieces - 1;
       named_bar(1, kPagedWarps * 32);
       if (last) {
         if (threadIdx.x == 0) *ticket = 0;
-        float *weight = merge;   // [pieces][kPagedHeads]
-        const auto piece = [&](uint32_t i) { return others + (size_t)i * kPart<D>; };
-        if (warp < tile_heads) {   // a warp a head, its lanes the pieces
-          float top = kNoScore, all = 0.f;
-          bool seen = false;
 #pragma unroll 1
-          for (uint32_t i = lane; i < pieces; i += 32) {
-            const float m = __ldcg(piece(i) + kPagedHeads * D + warp);
-            weight[i * kPagedHeads + warp] = m;
-            top = fmaxf(top, m);
-          }
+        for (uint32_t k = 0; k < seg.tiles; ++k) {   // a warp a head of every tile
+          if (head_of(k) + warp >= p.group) continue;
+          constexpr uint32_t N = D / 32;   // channels of a lane
+          constexpr uint32_t kAhead = 8;   // pieces whose values are loaded before their weights are known
+          const float *from = p.parts + ((size_t)seg.slot * p.tiles + k) * kPart<D>;
+          const size_t stride = (size_t)p.tiles * kPart<D>;
+          const auto values = [&](uint32_t i) {
+            const float *src = from + i * stride + warp * D + lane * N;
+            Values v;
+            if constexpr (N == 4) *(float4 *)v.x = __ldcg((const float4 *)src);
+            else *(float2 *)v.x = __ldcg((const float2 *)src);
+            return v;
+          };
+          // lanes are pieces, 32 at a time
+          const float *stats = from + kPagedHeads * D + warp;
+          float m = lane < pieces ? __ldcg(stats + lane * stride) : kNoScore;
+          float sum = lane < pieces ? __ldcg(stats + lane * stride + kPagedHeads) : 0.f;
+          Values early[kAhead];
+#pragma unroll
+          for (uint32_t i = 0; i < kAhead; ++i) early[i] = values(min(i, pieces - 1));
+          float top = m;
+#pragma unroll 1
+          for (uint32_t i = lane + 32; i < pieces; i += 32) top = fmaxf(top, __ldcg(stats + i * stride));
 #pragma unroll
           for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+          float all = 0.f;
+          bool some = false;
+          Values x{};
 #pragma unroll 1
-          for (uint32_t i = lane; i < pieces; i += 32) {
-            const float sum = __ldcg(piece(i) + kPagedHeads * (D + 1) + warp);
-            const float w = exp2_fast(weight[i * kPagedHeads + warp] - top);
-            seen |= sum < 0.f;
+          for (uint32_t at = 0; at < pieces; at += 32) {
+            if (at) {
+              const uint32_t i = at + lane;
+              m = i < pieces ? __ldcg(stats + i * stride) : kNoScore;
+              sum = i < pieces ? __ldcg(stats + i * stride + kPagedHeads) : 0.f;
+            }
+            const float w = exp2_fast(m - top);
+            some |= sum < 0.f;
             all += w * (sum < 0.f ? 0.f : sum);
-            weight[i * kPagedHeads + warp] = w;
-          }
+            uint32_t i = 0;
+            if (at == 0) {
 #pragma unroll
-          for (int x = 16; x; x >>= 1) all += __shfl_xor_sync(~0u, all, x);
-          seen = __any_sync(~0u, seen);
-          const float inv = inverse_of(all == 0.f && seen ? -1.f : all);
-          __syncwarp();
-          constexpr uint32_t N = D / 32;   // channels of a lane
-          float x[N];
+              for (; i < kAhead; ++i) {
+                const float wi = i < pieces ? __shfl_sync(~0u, w, i) : 0.f;
 #pragma unroll
-          for (uint32_t k = 0; k < N; ++k) x[k] = 0.f;
-#pragma unroll 16
-          for (uint32_t i = 0; i < pieces; ++i) {
-            const float w = weight[i * kPagedHeads + warp];
-            const float *src = piece(i) + warp * D + lane * N;
-            if constexpr (N == 4) {
-              const float4 y = __ldcg((const float4 *)src);
-              x[0] = fmaf(w, y.x, x[0]), x[1] = fmaf(w, y.y, x[1]), x[2] = fmaf(w, y.z, x[2]), x[3] = fmaf(w, y.w, x[3]);
-            } else {
-              const float2 y = __ldcg((const float2 *)src);
-              x[0] = fmaf(w, y.x, x[0]), x[1] = fmaf(w, y.y, x[1]);
+                for (uint32_t n = 0; n < N; ++n)
+                  if (i < pieces) x.x[n] = fmaf(wi, early[i].x[n], x.x[n]);
+              }
+            }
+            const uint32_t end = min(32u, pieces - at);
+#pragma unroll 8
+            for (; i < end; ++i) {
+              const Values v = values(at + i);
+              const float wi = __shfl_sync(~0u, w, i);
+#pragma unroll
+              for (uint32_t n = 0; n < N; ++n) x.x[n] = fmaf(wi, v.x[n], x.x[n]);
             }
           }
 #pragma unroll
-          for (uint32_t k = 0; k < N; ++k) out[warp * D + lane * N + k] = from_float<T>(x[k] * inv);
+          for (int y = 16; y; y >>= 1) all += __shfl_xor_sync(~0u, all, y);
+          const float inv = inverse_of(all == 0.f && __any_sync(~0u, some) ? -1.f : all);
+          T *dst = out_of(k, warp) + lane * N;
+#pragma unroll
+          for (uint32_t n = 0; n < N; ++n) dst[n] = from_float<T>(x.x[n] * inv);
         }
       }
     }
     named_bar(1, kPagedWarps * 32);   // shared results are free for the next piece
   }
-  if (stopped) {   // copies in flight land before the block ends
-    for (uint32_t i = round - min(round, S::kStages); i < round; ++i)
-      mbar_wait_bounded(&full[warp][i % S::kStages], i / S::kStages & 1);
+  if (stopped) {   // copies in flight land before the block ends; the first that does not in time was never issued
+    for (uint32_t i = n0 - min(n0, S::kStages); i < n0; ++i)
+      if (!mbar_wait_bounded(&full[i % S::kStages], i / S::kStages & 1)) break;
     if (lane == 0) atomicOr(&p.t.pool[1], kPagedTimeout);
   }
 }

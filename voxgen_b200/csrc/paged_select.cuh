@@ -11,10 +11,10 @@
 // A cluster of CTAs scores the pages of a (query, KV head); its first CTA then picks
 // from their scores in its shared memory. fp16 and bf16 become doubles by moving
 // bits: a half's bits, shifted, are the double's but for a power of two, which is in
-// the weights. The pick narrows a range of keys (scores as ordered integers): a
-// histogram of 2048 equal parts, then the part that the last chosen key lies in,
-// until its keys are all taken or all equal; two or three rounds unless scores
-// crowd together. Equal keys go to the lowest page.
+// the weights. The pick: a histogram of the keys (scores as ordered integers) over
+// 2048 equal parts of their range finds the part that the last chosen key lies in; the
+// few keys of that part are ranked against each other. Where it has more than 512, it
+// is the next range. Equal keys go to the lowest page.
 #pragma once
 #include <type_traits>
 
@@ -36,7 +36,8 @@ constexpr uint32_t kSelectThreads = 512;
 constexpr uint32_t kSelectWarps = kSelectThreads / 32;
 constexpr uint32_t kSelectBins = 2048;
 constexpr uint32_t kSelectPages = 24576;   // keys that the first CTA has room for
-constexpr uint32_t kSelectChunks = kSelectPages / kSelectThreads;
+constexpr uint32_t kSelectRanked = 512;    // keys that are ranked against each other
+static_assert(kSelectRanked * 12 <= kSelectBins * 4 && kSelectPages / 32 <= 2 * kSelectThreads, "");
 
 // Doubles whose order as unsigned integers is the numbers'.
 __device__ __forceinline__ uint64_t ordered(double x) {
@@ -55,15 +56,24 @@ __device__ __forceinline__ double widened(uint32_t h) {
   return __hiloint2double((int)((h & 0x80000000u) | (h & 0x7FFF0000u) >> (kMantissa<C> - 4)), 0);
 }
 
+// The least and the greatest of a warp.
+__device__ __forceinline__ void reach(unsigned long long &low, unsigned long long &high) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const unsigned long long a = __shfl_xor_sync(~0u, low, o), b = __shfl_xor_sync(~0u, high, o);
+    low = a < low ? a : low, high = b > high ? b : high;
+  }
+}
+
 template <int D, typename T, typename C>
-__global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const PagedSelectParams p) {
+__global__ void __launch_bounds__(kSelectThreads, 2) paged_select_kernel(const PagedSelectParams p) {
   extern __shared__ __align__(16) uint64_t keys[];   // [candidates], of the first CTA
   __shared__ __align__(16) double weights[2][D];     // of the smallest, of the largest
-  __shared__ uint32_t bins[kSelectBins];
-  __shared__ uint32_t counts[kSelectChunks * kSelectWarps];   // greater | equal << 16 of 32 keys
-  __shared__ uint64_t w_low[kSelectWarps], w_high[kSelectWarps];
+  __shared__ __align__(16) uint32_t bins[kSelectBins];
+  __shared__ uint32_t taken[kSelectPages / 32], same[kSelectPages / 32];   // a bit a key
+  __shared__ unsigned long long w_low[8 * kSelectWarps], w_high[8 * kSelectWarps];   // of the warps of the cluster
   __shared__ uint32_t w_sum[kSelectWarps];
-  __shared__ uint32_t found_bin, found_above, found_count;
+  __shared__ uint32_t found_bin, found_above, found_count, listed;
   const PagedTable &t = p.c.t;
   const uint32_t tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const uint32_t ctas = cluster_size(), rank = cluster_rank(), item = blockIdx.x / ctas;
@@ -108,11 +118,16 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const Page
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = ((const double *)weights)[part * 8 + i];
     const int32_t *table = t.table + (size_t)who.seq * t.seq_pages + p.sinks;
-    const uint32_t step = kBatch * kPer;
+    const uint32_t step = kBatch * kPer, stride = ctas * kSelectWarps * step;
     const uint32_t there = remote_smem(keys, 0);
-    for (uint32_t base = (rank * kSelectWarps + warp) * step; base < n; base += ctas * kSelectWarps * step) {
-      const uint32_t mine = base + lane;
-      const uint32_t page = lane < step && mine < n ? (uint32_t)table[mine] : ~0u;
+    unsigned long long low = ~0ull, high = 0;
+    const auto pages_at = [&](uint32_t base) {
+      return lane < step && base + lane < n ? (uint32_t)table[base + lane] : ~0u;
+    };
+    uint32_t base = (rank * kSelectWarps + warp) * step, ahead = pages_at(base);
+    for (; base < n; base += stride) {
+      const uint32_t page = ahead;
+      ahead = pages_at(base + stride);
       uint4 x[kBatch];
 #pragma unroll
       for (uint32_t i = 0; i < kBatch; ++i) {
@@ -154,39 +169,43 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const Page
       for (uint32_t o = 8; o < L; o <<= 1) s[0] += __shfl_xor_sync(~0u, s[0], o);
       // this lane's sum is of batch (lane & 1) * 4 + (lane & 2) + (lane & 4) / 4
       const uint32_t i = base + ((lane & 1) * 4 + (lane & 2) + (lane & 4) / 4) * kPer + sub;
-      if (part < 8 && i < n) st_remote(there + i * 8, ordered(s[0]));
+      if (part < 8 && i < n) {
+        const unsigned long long k = ordered(s[0]);
+        st_remote(there + i * 8, k);
+        low = k < low ? k : low, high = k > high ? k : high;
+      }
+    }
+    reach(low, high);
+    if (lane == 0) {
+      const uint32_t w = rank * kSelectWarps + warp;
+      st_remote(remote_smem(&w_low[w], 0), low);
+      st_remote(remote_smem(&w_high[w], 0), high);
     }
   }
   cluster_sync();
   if (rank) return;
-  // ---- the range of the keys ----
-  uint64_t low = ~0ull, high = 0;
-  const auto widen = [&](uint64_t a, uint64_t b) { low = a < low ? a : low, high = b > high ? b : high; };
-  for (uint32_t i = tid; i < n; i += kSelectThreads) widen(keys[i], keys[i]);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) widen(__shfl_xor_sync(~0u, low, o), __shfl_xor_sync(~0u, high, o));
-  if (lane == 0) w_low[warp] = low, w_high[warp] = high;
-  __syncthreads();
-#pragma unroll
-  for (uint32_t i = 0; i < kSelectWarps; ++i) widen(w_low[i], w_high[i]);
-  // ---- keys from `low` on are taken, but for `equal` == true: of those equal to it only the first `left` ----
+  // ---- the part of the range that the last chosen key lies in ----
+  unsigned long long low = ~0ull, high = 0;
+  for (uint32_t i = lane; i < ctas * kSelectWarps; i += 32) {
+    low = w_low[i] < low ? w_low[i] : low;
+    high = w_high[i] > high ? w_high[i] : high;
+  }
+  reach(low, high);
   uint32_t left = want;   // of the keys in [low, high]; want < n, so some are left out
-  bool equal = false;
+  uint32_t count_in;
   for (;;) {
-    const uint64_t span = high - low;
-    const int bits = 64 - __clzll((long long)span), shift = span ? max(bits - 11, 0) : 0;
-    for (uint32_t i = tid; i < kSelectBins; i += kSelectThreads) bins[i] = 0;
+    const unsigned long long span = high - low;
+    const int bits = 64 - __clzll((long long)span), shift = max(bits - 11, 0);
+    *(uint4 *)(bins + 4 * tid) = make_uint4(0, 0, 0, 0);
     __syncthreads();
     for (uint32_t i = tid; i < n; i += kSelectThreads) {
-      const uint64_t k = keys[i];
+      const unsigned long long k = keys[i];
       if (k >= low && k <= high) atomicAdd(&bins[(uint32_t)((k - low) >> shift)], 1u);
     }
     __syncthreads();
-    // from the top: the bin in which the `left`-th key lies; a thread has 4 bins
-    constexpr uint32_t kEach = kSelectBins / kSelectThreads;
-    uint32_t b[kEach], mine = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < kEach; ++i) b[i] = bins[kSelectBins - 1 - (tid * kEach + i)], mine += b[i];
+    // from the top, four parts a thread
+    const uint4 four = *(const uint4 *)(bins + kSelectBins - 4 - 4 * tid);
+    const uint32_t b[4] = {four.w, four.z, four.y, four.x}, mine = b[0] + b[1] + b[2] + b[3];
     uint32_t sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -195,59 +214,88 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const Page
     }
     if (lane == 31) w_sum[warp] = sum;
     __syncthreads();
-    uint32_t above = sum - mine;
+    const uint32_t others = lane < warp ? w_sum[lane] : 0;   // 16 warps
+    uint32_t above = sum - mine + __reduce_add_sync(~0u, others);
+    if (above < left && above + mine >= left) {
 #pragma unroll
-    for (uint32_t i = 0; i < kSelectWarps; ++i) above += i < warp ? w_sum[i] : 0;
-#pragma unroll
-    for (uint32_t i = 0; i < kEach; ++i) {
-      if (above < left && above + b[i] >= left)
-        found_bin = kSelectBins - 1 - (tid * kEach + i), found_above = above, found_count = b[i];
-      above += b[i];
+      for (uint32_t i = 0; i < 4; ++i) {
+        if (above < left && above + b[i] >= left)
+          found_bin = kSelectBins - 1 - (4 * tid + i), found_above = above, found_count = b[i];
+        above += b[i];
+      }
     }
     __syncthreads();
-    low += (uint64_t)found_bin << shift;
+    low += (unsigned long long)found_bin << shift;
     left -= found_above;
-    if (found_count == left) break;      // all of this part
-    if (shift == 0) {                    // one key, met more often than it is wanted
-      equal = true;
-      break;
-    }
-    const uint64_t end = low + ((1ull << shift) - 1);
+    count_in = found_count;
+    const unsigned long long end = low + ((1ull << shift) - 1);
     high = end < high ? end : high;
+    if (count_in <= kSelectRanked || shift == 0) break;
   }
-  // ---- the chosen ones in order ----
-  const uint32_t chunks = (n + kSelectThreads - 1) / kSelectThreads;
-  for (uint32_t c = 0; c < chunks; ++c) {
-    const uint32_t i = c * kSelectThreads + tid;
-    const uint64_t k = i < n ? keys[i] : 0;   // 0 is below every key
-    const uint32_t more = __ballot_sync(~0u, equal ? k > low : k >= low), same = __ballot_sync(~0u, equal && k == low);
-    if (lane == 0) counts[c * kSelectWarps + warp] = __popc(more) | __popc(same) << 16;
-  }
+  // ---- keys past the part are taken; those in it are listed, or marked where all are equal or all are taken ----
+  const bool rank_them = count_in > left && count_in <= kSelectRanked;
+  unsigned long long *list_keys = (unsigned long long *)bins;
+  uint32_t *list_at = bins + 2 * kSelectRanked;
+  if (tid == 0) listed = 0;
   __syncthreads();
-  // sums before each 32 keys: up to 24576 greater ones and as many equal ones, in 16 bits each
-  if (warp == 0) {
-    uint32_t before = 0;
-    for (uint32_t base = 0; base < chunks * kSelectWarps; base += 32) {
-      const uint32_t i = base + lane, x = i < chunks * kSelectWarps ? counts[i] : 0;
-      uint32_t sum = x;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t up = __shfl_up_sync(~0u, sum, o);
-        if (lane >= (uint32_t)o) sum += up;
-      }
-      if (i < chunks * kSelectWarps) counts[i] = before + sum - x;
-      before += __shfl_sync(~0u, sum, 31);
+  for (uint32_t i = tid; i < (n + 31) / 32 * 32; i += kSelectThreads) {
+    const unsigned long long k = i < n ? keys[i] : 0;   // 0 is below every key
+    const bool in = k >= low && k <= high;
+    const uint32_t more = __ballot_sync(~0u, k > high), equal = __ballot_sync(~0u, in);
+    if (lane == 0) taken[i / 32] = more, same[i / 32] = rank_them ? 0 : equal;
+    if (rank_them && in) {
+      const uint32_t at = atomicAdd(&listed, 1u);
+      list_keys[at] = k, list_at[at] = i;
     }
   }
   __syncthreads();
-  for (uint32_t c = 0; c < chunks; ++c) {
-    const uint32_t i = c * kSelectThreads + tid;
-    const uint64_t k = i < n ? keys[i] : 0;
-    const bool is_more = equal ? k > low : k >= low, is_same = equal && k == low;
-    const uint32_t more = __ballot_sync(~0u, is_more), same = __ballot_sync(~0u, is_same), below = (1u << lane) - 1;
-    const uint32_t before = counts[c * kSelectWarps + warp];
-    const uint32_t a = (before & 0xFFFF) + __popc(more & below), e = (before >> 16) + __popc(same & below);
-    if (is_more || (is_same && e < left)) out[p.sinks + a + min(e, equal ? left : 0u)] = (int32_t)(p.sinks + i);
+  if (rank_them && tid < count_in) {
+    const unsigned long long k = list_keys[tid];
+    const uint32_t at = list_at[tid];
+    uint32_t before = 0;
+#pragma unroll 4
+    for (uint32_t i = 0; i < count_in; ++i) before += list_keys[i] > k || (list_keys[i] == k && list_at[i] < at);
+    if (before < left) atomicOr(&taken[at / 32], 1u << at % 32);
+  }
+  __syncthreads();
+  // ---- the chosen ones in order: a thread has the keys of two words ----
+  const uint32_t words = (n + 31) / 32;
+  const auto sums_before32 = [&](uint32_t mine) {   // of the threads before this one
+    uint32_t sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(~0u, sum, o);
+      if (lane >= (uint32_t)o) sum += up;
+    }
+    if (lane == 31) w_sum[warp] = sum;
+    __syncthreads();
+    const uint32_t others = lane < warp ? w_sum[lane] : 0;
+    sum += __reduce_add_sync(~0u, others) - mine;
+    __syncthreads();
+    return sum;
+  };
+  uint32_t two[2];
+#pragma unroll
+  for (uint32_t i = 0; i < 2; ++i) two[i] = 2 * tid + i < words ? taken[2 * tid + i] : 0;
+  if (!rank_them) {   // the first `left` of the marked ones
+    uint32_t marked[2];
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) marked[i] = 2 * tid + i < words ? same[2 * tid + i] : 0;
+    uint32_t before = sums_before32(__popc(marked[0]) + __popc(marked[1]));
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+      for (; marked[i] && before < left; ++before) {
+        const uint32_t bit = marked[i] & -marked[i];
+        two[i] |= bit;
+        marked[i] ^= bit;
+      }
+      before += __popc(marked[i]);
+    }
+  }
+  uint32_t at = sums_before32(__popc(two[0]) + __popc(two[1]));
+#pragma unroll
+  for (uint32_t i = 0; i < 2; ++i) {
+    for (uint32_t w = two[i]; w; w &= w - 1) out[p.sinks + at++] = (int32_t)(p.sinks + (2 * tid + i) * 32 + __ffs(w) - 1);
   }
   for (uint32_t i = tid; i < p.sinks; i += kSelectThreads) out[i] = (int32_t)i;
   for (uint32_t i = tid; i < p.recent; i += kSelectThreads) out[p.sinks + want + i] = (int32_t)(count - p.recent + i);
