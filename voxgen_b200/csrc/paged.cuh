@@ -55,11 +55,14 @@ struct PagedQueries {
 struct PagedSeen {
   uint32_t seq, seen;
 };
+__device__ __forceinline__ uint32_t paged_held(const PagedTable &t, uint32_t s) {
+  return (uint32_t)min(max(t.rows[s], 0), (int32_t)t.capacity());
+}
 __device__ __forceinline__ PagedSeen paged_seen(const PagedTable &t, const PagedQueries &q, uint32_t i) {
   const int32_t s = q.sequences ? q.sequences[i] : (int32_t)i;
   if ((uint32_t)s >= t.seqs) return {0, 0};
-  uint32_t n = (uint32_t)min(max(t.rows[s], 0), (int32_t)t.capacity());
-  if (q.positions) n = min(n, (uint32_t)(max(q.positions[i], -1) + 1));
+  uint32_t n = paged_held(t, s);
+  if (q.positions) n = min(n, (uint32_t)max(q.positions[i], -1) + 1u);
   return {(uint32_t)s, n};
 }
 

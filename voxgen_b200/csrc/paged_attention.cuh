@@ -10,16 +10,18 @@
 // steps and added with rounding to nearest.
 //
 // The bound is bytes: 4 D of them a row for 4 D multiply-adds a head. So one warp
-// does nothing but keep copies in flight: it looks page numbers up 32 at a time and
-// issues tensor copies of 16 rows (K and V; 8 KB at head_dim 128) into a ring of 128
+// does nothing but keep copies in flight: it looks page numbers up 24 at a time and
+// issues tensor copies of 16 rows (K and V; 8 KB at head_dim 128) into a ring of 192
 // KB, through 128-byte swizzled boxes that ldmatrix reads without bank conflicts.
 //
-// A tile is (query, 8 heads of a KV head), a warp's work. Up to 8 tiles that read the
+// A tile is (query, 8 heads of a KV head), a warp's work. Up to 4 tiles that read the
 // same rows make a segment: the tiles of more than 8 heads to a KV head, or consecutive
 // queries of one sequence (a draft's tokens). A block of 16 rows is then read once for
-// the T tiles, and the 8 consumer warps are 8 / T teams that take blocks in turn. Tiles
-// never mix queries, so a row that one query sees and another does not is masked warp
-// by warp, whatever it holds.
+// the T tiles, and the 12 consumer warps are 12 / T teams that take blocks in turn.
+// Tiles never mix queries, so a row that one query sees and another does not is masked
+// warp by warp, whatever it holds. A warp's step of 16 rows is one chain of dependent
+// instructions (copies awaited, products, maximum, exponentials, transposes, products),
+// so as many warps run as registers allow: 12, with q's terms read from shared memory.
 //
 // The split. Segments are cut into pieces of at most U blocks, U such that there is
 // about one piece for each of the 148 CTAs (4, where segments are many). The warps of
@@ -56,27 +58,30 @@ struct PagedAttnParams {
 };
 
 constexpr uint32_t kPagedBlock = 16;     // cache rows of a block: never more than one page's
-constexpr uint32_t kPagedWarps = 8;      // consumers
+constexpr uint32_t kPagedWarps = 12;     // consumers
 constexpr uint32_t kPagedThreads = (kPagedWarps + 1) * 32;
 constexpr uint32_t kPagedCtas = 148;     // one per SM
 constexpr uint32_t kPagedHeads = 8;      // columns of a tile
-constexpr uint32_t kPagedLeast = 16;     // blocks of a piece: two rounds of the warps
+constexpr uint32_t kPagedTiles = 4;      // most tiles of a segment
+constexpr uint32_t kPagedLeast = 12;     // blocks of a piece: a round of the warps
 constexpr uint32_t kPagedTickets = 1u << 14;   // segments that may be cut
-constexpr uint32_t kPagedPlanned = 1024;       // queries whose place in the plan is kept in shared memory
+constexpr uint32_t kPagedPlanned = 256;        // queries whose place in the plan is kept in shared memory
+constexpr uint32_t kPagedMost = 1u << 26;      // blocks of a segment
+constexpr uint32_t kPagedUncut = ~0u;          // the size of pieces that are whole segments
 
 template <int D>
 struct PagedSmem {
   static constexpr uint32_t kHalf = 2 * kPagedBlock * 128;     // one copy: 64 channels of 16 K rows, then of 16 V rows
   static constexpr uint32_t kStage = kHalf * (D / 64);
-  static constexpr uint32_t kStages = 16 * 128 / D;
+  static constexpr uint32_t kStages = 2 * kPagedWarps * 128 / D;
   // A warp that waits for a stage's next turn has to have waited for the one before (a wait for the turn after one in
-  // flight returns at once): so within a piece a stage is always the same team's, and pieces take whole rounds of 8 stages.
+  // flight returns at once): so within a piece a stage is always the same team's, and pieces take whole rounds of stages.
   static_assert(kStages % kPagedWarps == 0, "");
   static constexpr uint32_t kRing = kStages * kStage;
-  static constexpr uint32_t kRow = D + 4;                      // floats of a row when results meet: 4 against bank conflicts
+  static constexpr uint32_t kRow = 68;                         // floats of a row when results meet: 64 and 4 against bank conflicts
   static constexpr uint32_t kMerge = kPagedWarps * kPagedHeads * kRow * 4;
   static constexpr uint32_t kTileQ = D / 16 * 32 * 8;          // a tile's queries as B fragments, one term
-  static constexpr uint32_t kShared = kMerge > 3 * kPagedWarps * kTileQ ? kMerge : 3 * kPagedWarps * kTileQ;   // first queries, then results
+  static constexpr uint32_t kShared = kMerge > 3 * kPagedTiles * kTileQ ? kMerge : 3 * kPagedTiles * kTileQ;   // first queries, then results
   static constexpr uint32_t kBytes = kRing + kShared + 1024;   // the ring starts on a multiple of 1024
 };
 
@@ -89,97 +94,133 @@ __host__ __device__ __forceinline__ uint32_t paged_slots(uint64_t segments) {
   return segments > kPagedTickets ? 0 : 2 * paged_target((uint32_t)segments);
 }
 
-// Blocks and tiles of the segments that query i leads, blocks << 2 | log2(tiles); 0 where another query leads. At least one
-// block, so that every output is written. Queries share within aligned eights, in runs of a power of two.
-__device__ __forceinline__ uint32_t paged_entry(const PagedAttnParams &p, uint32_t i) {
-  if (i >= p.queries) return 0;
-  if (p.chosen) return (p.budget << (p.t.shift - 4)) << 2 | (31 - __clz(p.tiles));
-  const auto blocks = [&](uint32_t rows) { return max(1u, (rows + kPagedBlock - 1) / kPagedBlock); };
-  if (!p.share) return blocks(paged_seen(p.t, p.which, i).seen) << 2 | (31 - __clz(p.tiles));
+// What the plan needs to know of a query. entry: blocks and tiles of the segments that it leads, blocks << 2 |
+// log2(tiles), at least one block, so that every output is written; 0 where another query leads. Queries share within
+// aligned eights, in runs of 1, 2 or 4. seen: rows that it sees, most: that any query of its segments sees.
+struct PagedLead {
+  uint32_t entry, seq, seen, most;
+};
+__device__ __forceinline__ PagedLead paged_lead(const PagedAttnParams &p, uint32_t i) {
+  const auto entry = [&](uint32_t rows, uint32_t tiles) {
+    return max(1u, (rows + kPagedBlock - 1) / kPagedBlock) << 2 | (31 - __clz(tiles));
+  };
+  if (!p.share) {
+    const PagedSeen who = paged_seen(p.t, p.which, i);
+    const uint32_t e = p.chosen ? entry(p.budget << p.t.shift, p.tiles) : entry(who.seen, p.tiles);
+    return {e, who.seq, who.seen, who.seen};
+  }
   const uint32_t from = i & ~7u;
-  const int32_t mine = p.which.sequences[i];
+  int32_t seqs[8], last[8];
+#pragma unroll
+  for (uint32_t j = 0; j < 8; ++j) {
+    const uint32_t k = min(from + j, p.queries - 1);
+    seqs[j] = p.which.sequences[k];
+    last[j] = p.which.positions ? p.which.positions[k] : 0x7FFFFFFE;
+  }
+  const uint32_t at = i - from;
+  int32_t mine = 0, here = 0;
+#pragma unroll
+  for (uint32_t j = 0; j < 8; ++j)
+    if (j == at) mine = seqs[j], here = last[j];
   uint32_t same = 0;   // of the eight
 #pragma unroll
   for (uint32_t j = 0; j < 8; ++j)
-    if (from + j < p.queries && p.which.sequences[from + j] == mine) same |= 1u << j;
-  const uint32_t at = i - from;
+    if (from + j < p.queries && seqs[j] == mine) same |= 1u << j;
   const uint32_t start = 32 - __clz(~same & ((1u << at) - 1)), end = __ffs(~same >> at) - 1 + at;   // of the run around i
-  const uint32_t length = end - start, off = at - start;
-  uint32_t first = 0, size = 8;                      // of the part of the run that i is in
-  if (length < 8) {
-#pragma unroll
-    for (size = 4; size > 1; size >>= 1) {
-      if (!(length & size)) continue;
-      if (off < first + size) break;
-      first += size;
-    }
+  uint32_t first = start, size = 4;                  // of the part of the run that i is in
+  while (at >= first + size || first + size > end) {
+    if (first + size <= end) first += size;
+    else size /= 2;
   }
-  if (off != first) return 0;
-  uint32_t seen = 0;
-  for (uint32_t j = 0; j < size; ++j) seen = max(seen, paged_seen(p.t, p.which, i + j).seen);
-  return blocks(seen) << 2 | (31 - __clz(size));
+  int32_t top = here;
+#pragma unroll
+  for (uint32_t j = 0; j < 8; ++j)
+    if (j >= first && j < first + size) top = max(top, last[j]);
+  const PagedSeen all = (uint32_t)mine < p.t.seqs ? PagedSeen{(uint32_t)mine, paged_held(p.t, mine)} : PagedSeen{0, 0};
+  const auto seen = [&](int32_t x) { return min(all.seen, (uint32_t)max(x, -1) + 1u); };
+  return {at == first ? entry(seen(top), size) : 0, all.seq, seen(here), seen(top)};
 }
-// What a segment's block costs: a block's bytes take as long as two tiles' arithmetic.
-__device__ __forceinline__ uint32_t paged_cost(uint32_t entry) { return (entry >> 2) << max((int)(entry & 3) - 1, 0); }
+// A little more than a / b.
+__device__ __forceinline__ uint32_t paged_over(uint32_t a, uint32_t b) {
+  return (uint32_t)((float)a * __fdividef(1.f + 0x1p-20f, (float)b)) + 1;
+}
+// What a segment's block costs, in quarters: one tile is bound by the block's bytes, four by their arithmetic.
+__device__ __forceinline__ uint32_t paged_weight(uint32_t entry) { return (entry & 3) == 0 ? 4 : (entry & 3) == 1 ? 6 : 10; }
 __device__ __forceinline__ uint32_t paged_size(uint32_t entry, uint32_t size) {   // blocks of a piece that costs `size`
-  const uint32_t k = max((int)(entry & 3) - 1, 0);
-  return (size + (1u << k) - 1) >> k;
+  if (size == kPagedUncut) return kPagedMost;
+  return (entry & 3) == 0 ? min(size, kPagedMost) : (entry & 3) == 1 ? (2 * size + 2) / 3 : (2 * size + 4) / 5;
 }
-__device__ __forceinline__ uint32_t paged_pieces(uint32_t entry, uint32_t size) {
-  const uint32_t n = paged_size(entry, size);
-  return ((entry >> 2) + n - 1) / n;
+__device__ __forceinline__ uint32_t paged_parts(uint32_t entry, uint32_t size) {   // pieces of a segment
+  const uint32_t b = entry >> 2, each = paged_size(entry, size);
+  uint32_t n = (uint32_t)((float)b * __fdividef(1.f - 0x1p-20f, (float)each));   // a little low
+  n += n * each < b;
+  while (n * each < b) ++n;   // millions of blocks
+  return n;
 }
 
-// How segments are cut: pieces that cost at most `size`, `pieces` of them. A warp's work.
+// How segments are cut: pieces that cost at most `size`, `pieces` of them.
 struct PagedPlan {
   uint32_t size, pieces;
 };
-template <typename E>
-__device__ __forceinline__ PagedPlan paged_plan(const PagedAttnParams &p, const E &entry) {
+struct PagedTally {   // in shared memory, zero before
+  uint32_t total, leads, pieces[8];
+};
+// All threads: leads[] of the first queries, and the plan.
+__device__ __forceinline__ PagedPlan paged_plan(const PagedAttnParams &p, PagedLead *leads, PagedTally &tally) {
   const uint32_t lane = threadIdx.x % 32;
-  uint32_t total = 0, leads = 0;
+  uint32_t total = 0, count = 0;
 #pragma unroll 1
-  for (uint32_t s = lane; s < p.queries; s += 32) {
-    const uint32_t e = entry(s);
-    total += paged_cost(e);
-    leads += e != 0;
+  for (uint32_t i = threadIdx.x; i < p.queries; i += kPagedThreads) {
+    const PagedLead x = paged_lead(p, i);
+    if (i < kPagedPlanned) leads[i] = x;
+    total += ((x.entry >> 2) * paged_weight(x.entry) + 3) / 4;
+    count += x.entry != 0;
   }
-  total = __reduce_add_sync(~0u, total) * p.lanes;   // the host keeps it below 2^31
-  const uint32_t segments = __reduce_add_sync(~0u, leads) * p.lanes;
-  PagedPlan x{1u << 30, segments};   // one piece a segment
-  if (p.queries * p.lanes > kPagedTickets) return x;
+  total = __reduce_add_sync(~0u, total), count = __reduce_add_sync(~0u, count);
+  if (lane == 0 && total) atomicAdd(&tally.total, total), atomicAdd(&tally.leads, count);
+  __syncthreads();
+  total = tally.total * p.lanes;   // the host keeps it below 2^31
+  const uint32_t segments = tally.leads * p.lanes;
+  if (p.queries * p.lanes > kPagedTickets) return PagedPlan{kPagedUncut, segments};   // one piece a segment
   const uint32_t target = paged_target(segments);
-  x.size = max(kPagedLeast, (total + target - 1) / target);
+  // total / target would do if nothing were rounded up; total / (target - segments) makes no more than target pieces. Of eight
+  // sizes from the one to the other the least with no more pieces than the target is taken. Where a CTA has several pieces
+  // anyway, it is the first.
+  const uint32_t least = max(kPagedLeast, paged_over(total, target));
+  const uint32_t more = target == kPagedCtas ? max(least, paged_over(total, target - segments)) - least : 0;
+  const uint32_t k = lane / 4, size = least + (k == 7 ? more : more * k * k / 49);
+  uint32_t n = 0;
 #pragma unroll 1
-  for (int i = 0;; ++i) {   // the fewest blocks that make no more pieces than the target, or nearly
-    uint32_t n = 0;
-#pragma unroll 1
-    for (uint32_t s = lane; s < p.queries; s += 32) n += paged_pieces(entry(s), x.size);
-    x.pieces = __reduce_add_sync(~0u, n) * p.lanes;
-    if (x.pieces <= target || i == 3) return x;
-    x.size = max(x.size + 1, (uint32_t)((float)x.size * __fdividef((float)x.pieces, (float)target)));
-  }
+  for (uint32_t i = threadIdx.x / 32 * 4 + lane % 4; i < p.queries; i += kPagedThreads / 8)
+    n += paged_parts(i < kPagedPlanned ? leads[i].entry : paged_lead(p, i).entry, size);
+  if (n) atomicAdd(&tally.pieces[k], n);
+  __syncthreads();
+  n = tally.pieces[k] * p.lanes;
+  const int found = __ffs(__ballot_sync(~0u, n <= target) | 1u << 31) - 1;
+  return PagedPlan{__shfl_sync(~0u, size, found), __shfl_sync(~0u, n, found)};
 }
 
 struct PagedPiece {
-  uint32_t query, lane;         // lane: (KV head, 8 of its tiles)
+  uint32_t query, lane;         // lane: (KV head, 4 of its tiles)
   uint32_t part, parts;         // of the segment
   uint32_t slot;                // of the segment's first partial result
   uint32_t first, blocks;       // of the piece, in the segment
-  uint32_t tiles;               // 1, 2, 4 or 8
+  uint32_t tiles;               // 1, 2 or 4
+  uint32_t seq, seen;           // of the segment
 };
 // Where the search for a CTA's next piece goes on: 32 queries, and the pieces (all, and those of cut segments) before them.
 struct PagedCursor {
   uint32_t base, before, cut;
 };
 template <typename E>
-__device__ __forceinline__ PagedPiece paged_piece(const PagedAttnParams &p, const PagedPlan &x, uint32_t index, const E &entry,
+__device__ __forceinline__ PagedPiece paged_piece(const PagedAttnParams &p, const PagedPlan &x, uint32_t index, const E &lead,
                                                   PagedCursor &at32) {
   const uint32_t lane = threadIdx.x % 32;
 #pragma unroll 1
   for (; at32.base < p.queries; at32.base += 32) {
     const uint32_t base = at32.base, before = at32.before, cut_before = at32.cut;
-    const uint32_t e = entry(base + lane), n = paged_pieces(e, x.size);
+    const PagedLead who = base + lane < p.queries ? lead(base + lane) : PagedLead{0, 0, 0, 0};
+    const uint32_t e = who.entry, n = paged_parts(e, x.size);
     uint32_t sum = n * p.lanes, cut = n > 1 ? sum : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -194,20 +235,25 @@ __device__ __forceinline__ PagedPiece paged_piece(const PagedAttnParams &p, cons
       const uint32_t size = paged_size(all, x.size);
       PagedPiece y;
       y.query = base + at;
-      y.lane = into / parts;
+      y.lane = (uint32_t)__fdividef((float)into + 0.5f, (float)parts);   // exact: below 2^22
       y.part = into - y.lane * parts;
       y.parts = parts;
       y.slot = cut_before + __shfl_sync(~0u, cut, at) - parts * p.lanes + y.lane * parts;
       y.first = y.part * size;
       y.blocks = min(size, (all >> 2) - y.first);
       y.tiles = 1u << (all & 3);
+      y.seq = __shfl_sync(~0u, who.seq, at);
+      y.seen = __shfl_sync(~0u, who.most, at);
       return y;
     }
     at32.before += __shfl_sync(~0u, sum, 31);
     at32.cut += __shfl_sync(~0u, cut, 31);
   }
-  return PagedPiece{0, 0, 0, 1, 0, 0, 0, 1};   // past the last piece
+  return PagedPiece{0, 0, 0, 1, 0, 0, 0, 1, 0, 0};   // past the last piece
 }
+
+// Stages that a piece takes.
+__device__ __forceinline__ uint32_t paged_rounds(uint32_t blocks) { return (blocks + kPagedWarps - 1) / kPagedWarps * kPagedWarps; }
 
 // ---- MMA operands of either type ----
 __device__ __forceinline__ void mma_16(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2], __half) { mma_f16(c, a, b); }
@@ -229,13 +275,14 @@ __device__ __forceinline__ uint32_t take_pair(float &x, float &y, __nv_bfloat16)
   x -= f.x, y -= f.y;
   return *reinterpret_cast<const uint32_t *>(&h);
 }
+// Volatile keeps these behind the wait for their stage and before its release; products may move among them.
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t address) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(address) : "memory");
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(address));
 }
 __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t address) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(address) : "memory");
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(address));
 }
 // One box of the pool: 64 channels from x on, 16 rows from `row` on, of K and V, of (page, KV head) `place`.
 __device__ __forceinline__ void tensor_g2s(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t row, int32_t place, uint64_t *bar) {
@@ -267,41 +314,41 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
   extern __shared__ uint8_t paged_smem[];
   __shared__ uint64_t full[S::kStages], empty[S::kStages];
   __shared__ uint32_t first_row[S::kStages];    // of a stage's block in its sequence; past every row: nothing was read
-  __shared__ uint32_t entries[kPagedPlanned];
+  __shared__ PagedLead leads[kPagedPlanned];
+  __shared__ PagedTally tally;
   __shared__ __align__(8) float w_max[kPagedWarps][kPagedHeads], w_sum[kPagedWarps][kPagedHeads];
-  __shared__ float f_max[kPagedWarps][kPagedHeads], f_sum[kPagedWarps][kPagedHeads];   // [tile][head]
-  __shared__ __align__(8) float factors[kPagedWarps][kPagedHeads];                    // [tile][head]
+  __shared__ float f_max[kPagedTiles][kPagedHeads], f_sum[kPagedTiles][kPagedHeads];   // [tile][head]
+  __shared__ __align__(8) float factors[kPagedTiles][kPagedHeads];                    // [tile][head]
   __shared__ uint32_t last, gave_up;
   const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
   const uint32_t base = smem_u32(paged_smem), ring = (base + 1023) & ~1023u;
   float *merge = (float *)(paged_smem + (ring - base) + S::kRing);   // [warp][head][kRow]
-  uint32_t *q_frag = (uint32_t *)merge;                             // [tile][term][step][lane][2]
+  uint32_t *q_frag = (uint32_t *)merge;
   if (threadIdx.x == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map));
     gave_up = 0;
   }
   if (threadIdx.x < S::kStages) mbar_init(&full[threadIdx.x], 1), mbar_init(&empty[threadIdx.x], kPagedWarps);
+  if (threadIdx.x < sizeof(PagedTally) / 4) ((uint32_t *)&tally)[threadIdx.x] = 0;
   fence_mbar_init();
+  __syncthreads();
   pdl_launch_dependents();
   pdl_wait();
-  for (uint32_t i = threadIdx.x; i < min(p.queries, kPagedPlanned); i += kPagedThreads) entries[i] = paged_entry(p, i);
-  __syncthreads();
-  const auto entry = [&](uint32_t i) { return i >= p.queries ? 0 : i < kPagedPlanned ? entries[i] : paged_entry(p, i); };
-  const PagedPlan plan = paged_plan(p, entry);
+  const PagedPlan plan = paged_plan(p, leads, tally);
+  const auto lead = [&](uint32_t i) { return i < kPagedPlanned ? leads[i] : paged_lead(p, i); };
+  if (blockIdx.x >= plan.pieces) return;
+  PagedCursor cursor{};
+  PagedPiece piece = paged_piece(p, plan, blockIdx.x, lead, cursor);   // most CTAs have one: what runs once is short
 
   if (warp == kPagedWarps) {
     // ================= the copying warp =================
     uint32_t n0 = 0;           // blocks of the pieces before
-    PagedCursor cursor{};
     bool stopped = false;
 #pragma unroll 1
-    for (uint32_t index = blockIdx.x; index < plan.pieces && !stopped; index += gridDim.x) {
-      const PagedPiece x = paged_piece(p, plan, index, entry, cursor);
+    for (uint32_t index = blockIdx.x; !stopped;) {
+      const PagedPiece x = piece;
       const uint32_t kv = p.share ? x.lane : x.lane / (p.lanes / p.kv_heads), page_rows = p.t.page_rows();
-      PagedSeen who = paged_seen(p.t, p.which, x.query);
-      if (p.share)
-        for (uint32_t i = 1; i < x.tiles; ++i) who.seen = max(who.seen, paged_seen(p.t, p.which, x.query + i).seen);
-      const int32_t *table = p.t.table + (size_t)who.seq * p.t.seq_pages;
+      const int32_t *table = p.t.table + (size_t)x.seq * p.t.seq_pages;
       const int32_t *list = p.chosen ? p.chosen + ((size_t)x.query * p.kv_heads + kv) * p.budget : nullptr;
       // page and first row of the piece's block i
       struct Found {
@@ -314,20 +361,20 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         const uint32_t at = list ? (uint32_t)list[e] : e;
         if (at >= p.t.seq_pages) return none;
         const uint32_t first = (at << p.t.shift) + in;
-        if (first >= who.seen) return none;
+        if (first >= x.seen) return none;
         const uint32_t page = (uint32_t)table[at];
         return page < p.t.pages ? Found{page, first} : none;
       };
       Found next = find(lane);
 #pragma unroll 1
-      for (uint32_t i = 0; i < x.blocks && !stopped; i += 32) {
+      for (uint32_t i = 0; i < x.blocks && !stopped; i += 2 * kPagedWarps) {
         const Found now = next;
-        next = find(i + 32 + lane);
+        next = find(i + 2 * kPagedWarps + lane);
 #pragma unroll 1
-        for (uint32_t j = 0; j < 32 && i + j < x.blocks; j += 8) {   // whole rounds: stages past the last block hold nothing
-          const uint32_t page = __shfl_sync(~0u, now.page, j + lane % 8), row = __shfl_sync(~0u, now.row, j + lane % 8);
+        for (uint32_t j = 0; j < 2 * kPagedWarps && i + j < x.blocks; j += kPagedWarps) {   // whole rounds: stages past the last block hold nothing
+          const uint32_t from = j + lane % kPagedWarps, page = __shfl_sync(~0u, now.page, from), row = __shfl_sync(~0u, now.row, from);
           bool in = true;
-          if (lane < 8) {
+          if (lane < kPagedWarps) {
             const uint32_t n = n0 + i + j + lane, stage = n % S::kStages, turn = n / S::kStages;
             if (turn) in = mbar_wait_bounded(&empty[stage], (turn - 1) & 1);
             if (in) {
@@ -351,7 +398,9 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
           }
         }
       }
-      n0 += (x.blocks + 7) & ~7u;
+      n0 += paged_rounds(x.blocks);
+      if ((index += gridDim.x) >= plan.pieces) break;
+      piece = paged_piece(p, plan, index, lead, cursor);
     }
     if (stopped && lane == 0) atomicOr(&p.t.pool[1], kPagedTimeout);
     return;
@@ -359,29 +408,29 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
 
   // ================= the consumers =================
   uint32_t n0 = 0;
-  PagedCursor cursor{};
   bool stopped = false;      // a wait ran out: nothing is waited for any more
   // this lane's row of an ldmatrix, and which of the two 16-byte chunks it reads
-  const uint32_t k_row = lane % 8 + (lane / 8 % 2) * 8, k_chunk = lane / 16;
-  const uint32_t v_row = lane % 8 + (lane / 16) * 8, v_chunk = lane / 8 % 2;
+  // (swizzled: chunk c of row r lies at c ^ r % 8; chunks 2i and 2i + 1 of step i are those of step 0, ^ 2i)
+  const uint32_t k_row = lane % 8 + (lane / 8 % 2) * 8, k_at = k_row * 128 + ((lane / 16 ^ k_row % 8) << 4);
+  const uint32_t v_row = lane % 8 + (lane / 16) * 8, v_at = kPagedBlock * 128 + v_row * 128 + ((lane / 8 % 2 ^ v_row % 8) << 4);
 #pragma unroll 1
-  for (uint32_t index = blockIdx.x; index < plan.pieces; index += gridDim.x) {
-    const PagedPiece seg = paged_piece(p, plan, index, entry, cursor);
+  for (uint32_t index = blockIdx.x;;) {
+    const PagedPiece seg = piece;
     const bool whole = seg.parts == 1;
-    const uint32_t chunks = p.lanes / p.kv_heads;   // segments of a KV head, where it has more than 8 tiles
+    const uint32_t chunks = p.lanes / p.kv_heads;   // segments of a KV head, where it has more than 4 tiles
     const uint32_t kv = p.share ? seg.lane : seg.lane / chunks;
-    const uint32_t tile0 = p.share ? 0 : (seg.lane - kv * chunks) * kPagedWarps;
+    const uint32_t tile0 = p.share ? 0 : (seg.lane - kv * chunks) * kPagedTiles;
     const uint32_t teams = kPagedWarps / seg.tiles, team = warp / seg.tiles, tile = warp & (seg.tiles - 1);
     // query and first head (of the KV head's) of a tile of the segment
     const auto query_of = [&](uint32_t k) { return p.share ? seg.query + k : seg.query; };
     const auto head_of = [&](uint32_t k) { return p.share ? 0 : (tile0 + k) * kPagedHeads; };
     const uint32_t head0 = head_of(tile);
-    const uint32_t seen = paged_seen(p.t, p.which, query_of(tile)).seen;
-    // ---- the queries as B fragments, a warp a head of every tile: column `warp` of the MMA ----
+    const uint32_t seen = p.share ? lead(query_of(tile)).seen : seg.seen;
+    // ---- the queries as B fragments, a head a warp at a time: column `col` of a tile's MMA ----
 #pragma unroll 1
-    for (uint32_t k = 0; k < seg.tiles; ++k) {
+    for (uint32_t r = warp; r < seg.tiles * kPagedHeads; r += kPagedWarps) {
       constexpr uint32_t N = D / 32;
-      const uint32_t head = head_of(k) + warp;
+      const uint32_t k = r / kPagedHeads, col = r % kPagedHeads, head = head_of(k) + col;
       const T *q = (const T *)p.q + (int64_t)query_of(k) * p.q_query + (int64_t)(kv * p.group + head) * p.q_head + lane * N;
       float x[N];
       uint32_t top = 0;
@@ -394,21 +443,17 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       float inverse = 1.f, power = 1.f;
       if constexpr (std::is_same<C, __half>::value) power = row_power(__uint_as_float(__reduce_max_sync(~0u, top)), inverse);
 #pragma unroll
-      for (uint32_t i = 0; i < N; i += 2) {   // channels c, c + 1: step c / 16, lane 4 warp + c % 8 / 2, register c % 16 / 8
+      for (uint32_t i = 0; i < N; i += 2) {   // channels c, c + 1: step c / 16, lane 4 col + c % 8 / 2, register c % 16 / 8
         const uint32_t c = lane * N + i;
         float a = x[i] * power, b = x[i + 1] * power;
 #pragma unroll
-        for (int j = 0; j < kQ; ++j)
-          q_frag[(((k * kQ + j) * kSteps + c / 16) * 32 + warp * 4 + c % 8 / 2) * 2 + c % 16 / 8] = take_pair(a, b, C{});
+        for (int j = 0; j < kQ; ++j)   // [tile][term][pair of steps][lane][step of the pair][register]
+          q_frag[(((k * kQ + j) * (kSteps / 2) + c / 32) * 32 + col * 4 + c % 8 / 2) * 4 + c % 32 / 8] = take_pair(a, b, C{});
       }
-      if (lane == 0) factors[k][warp] = fmaxf(p.scale * inverse, 0x1p-126f);
+      if (lane == 0) factors[k][col] = fmaxf(p.scale * inverse, 0x1p-126f);
     }
     named_bar(1, kPagedWarps * 32);
-    uint32_t qf[kQ][kSteps][2];
-#pragma unroll
-    for (int k = 0; k < kQ; ++k)
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) *(uint2 *)qf[k][i] = *(const uint2 *)&q_frag[(((tile * kQ + k) * kSteps + i) * 32 + lane) * 2];
+    const uint32_t *my_q = q_frag + (tile * kQ * (kSteps / 2) * 32 + lane) * 4;
     const float f0 = factors[tile][2 * t], f1 = factors[tile][2 * t + 1];   // scores of heads 2t and 2t + 1 are this lane's
     stopped |= __any_sync(~0u, *(volatile uint32_t *)&gave_up);
 
@@ -422,7 +467,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     uint32_t steps = 0;    // steps that this warp took
     uint32_t stage = (n0 + team) % S::kStages, parity = (n0 + team) / S::kStages & 1;
 #pragma unroll 1
-    for (uint32_t b = team; b < ((seg.blocks + 7) & ~7u); b += teams) {
+    for (uint32_t b = team; b < paged_rounds(seg.blocks); b += teams) {
       if (!stopped && !__all_sync(~0u, mbar_wait_bounded(&full[stage], parity))) {
         stopped = true;
         if (lane == 0) *(volatile uint32_t *)&gave_up = 1;
@@ -436,12 +481,20 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         // even and odd steps (and q's lower terms) in sums of their own: half the chain of dependent products
         float sums[kQ > 1 ? 3 : 2][4] = {};
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-          uint32_t a[4];
-          const uint32_t chunk = (k % 4) * 2 + k_chunk;
-          ldmatrix4(a, st + k / 4 * S::kHalf + k_row * 128 + ((chunk ^ (k_row & 7)) << 4));
+        for (int h = 0; h < D / 64; ++h) {   // 64 channels: four loads, then their products
+          uint32_t a[4][4];
 #pragma unroll
-          for (int i = 0; i < kQ; ++i) mma_16(sums[i ? 2 : k % 2], a, qf[i][k], C{});
+          for (int k = 0; k < 4; ++k) ldmatrix4(a[k], (st + k_at + h * S::kHalf) ^ k << 5);
+#pragma unroll
+          for (int i = 0; i < kQ; ++i) {
+#pragma unroll
+            for (int k = 0; k < 4; k += 2) {
+              const uint4 b = *(const uint4 *)(my_q + (i * (kSteps / 2) + 2 * h + k / 2) * 32 * 4);
+              const uint32_t even[2] = {b.x, b.y}, odd[2] = {b.z, b.w};
+              mma_16(sums[i ? 2 : 0], a[k], even, C{});
+              mma_16(sums[i ? 2 : 1], a[k + 1], odd, C{});
+            }
+          }
         }
         float c[4];
 #pragma unroll
@@ -489,13 +542,19 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
             keep[y] = (8 * y + 2 * t < valid ? 0xFFFFu : 0u) | (8 * y + 2 * t + 1 < valid ? 0xFFFF0000u : 0u);
         }
 #pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
-          uint32_t a[4];
-          const uint32_t chunk = (j % 4) * 2 + v_chunk;
-          ldmatrix4_trans(a, st + j / 4 * S::kHalf + kPagedBlock * 128 + v_row * 128 + ((chunk ^ (v_row & 7)) << 4));
-          if (tail) a[0] &= keep[0], a[1] &= keep[0], a[2] &= keep[1], a[3] &= keep[1];
+        for (int h = 0; h < D / 64; ++h) {
+          uint32_t a[4][4];
 #pragma unroll
-          for (int k = 0; k < kP; ++k) mma_16(o[j], a, pf[k], C{});
+          for (int j = 0; j < 4; ++j) ldmatrix4_trans(a[j], (st + v_at + h * S::kHalf) ^ j << 5);
+          if (tail) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a[j][0] &= keep[0], a[j][1] &= keep[0], a[j][2] &= keep[1], a[j][3] &= keep[1];
+          }
+#pragma unroll
+          for (int k = 0; k < kP; ++k) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mma_16(o[4 * h + j], a[j], pf[k], C{});
+          }
         }
         if constexpr (kFresh) {
           if (steps % kFreshSteps == 0) {
@@ -507,11 +566,11 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive_count(&empty[stage], teams);   // the team's T warps make up 8 arrivals
+      if (lane == 0) mbar_arrive_count(&empty[stage], teams);   // the team's T warps make up 12 arrivals
       stage += teams;
       if (stage >= S::kStages) stage -= S::kStages, parity ^= 1;
     }
-    n0 += (seg.blocks + 7) & ~7u;
+    n0 += paged_rounds(seg.blocks);
     if constexpr (kFresh) {
 #pragma unroll
       for (int j = 0; j < kSteps; ++j)
@@ -561,34 +620,41 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     const auto inverse_of = [](float sum) {   // zeros where no row was seen, NaN where every score was -infinity
       return sum == 0.f ? 0.f : sum < 0.f ? NAN : 1.f / sum;
     };
-#pragma unroll
-    for (int j = 0; j < kSteps; ++j) {
-      float *dst = merge + (warp * kPagedHeads + 2 * t) * S::kRow + 16 * j + g;
-      dst[0] = e0 * o[j][0], dst[8] = e0 * o[j][2];
-      dst[S::kRow] = e1 * o[j][1], dst[S::kRow + 8] = e1 * o[j][3];
-    }
-    named_bar(1, kPagedWarps * 32);
-    struct __align__(D / 8) Values {   // a lane's channels of a head
-      float x[D / 32];
-    };
 #pragma unroll 1
-    for (uint32_t k = 0; k < seg.tiles; ++k) {   // a warp a head of every tile
-      if (head_of(k) + warp >= p.group) continue;
-      Values x{};
+    for (int h = 0; h < D / 64; ++h) {   // 64 channels at a time
+      if (h) named_bar(1, kPagedWarps * 32);
+      const auto store = [&](const float(&x)[4], int i) {
+        float *dst = merge + (warp * kPagedHeads + 2 * t) * S::kRow + 16 * i + g;
+        dst[0] = e0 * x[0], dst[8] = e0 * x[2];
+        dst[S::kRow] = e1 * x[1], dst[S::kRow + 8] = e1 * x[3];
+      };
+      if (D == 64 || h == 0) {
 #pragma unroll
-      for (uint32_t w = 0; w < kPagedWarps; ++w) {
-        if ((w & (seg.tiles - 1)) != k) continue;
-        const Values y = *(const Values *)(merge + (w * kPagedHeads + warp) * S::kRow + D / 32 * lane);
-#pragma unroll
-        for (uint32_t n = 0; n < D / 32; ++n) x.x[n] += y.x[n];
-      }
-      if (whole) {
-        const float inv = inverse_of(f_sum[k][warp]);
-        T *dst = out_of(k, warp) + D / 32 * lane;
-#pragma unroll
-        for (uint32_t n = 0; n < D / 32; ++n) dst[n] = from_float<T>(x.x[n] * inv);
+        for (int i = 0; i < 4; ++i) store(o[i], i);
       } else {
-        *(Values *)(part + k * kPart<D> + warp * D + D / 32 * lane) = x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) store(o[kSteps - 4 + i], i);
+      }
+      named_bar(1, kPagedWarps * 32);
+#pragma unroll 1
+      for (uint32_t r = warp; r < seg.tiles * kPagedHeads; r += kPagedWarps) {   // a head a warp at a time, two channels a lane
+        const uint32_t k = r / kPagedHeads, head = r % kPagedHeads;
+        if (head_of(k) + head >= p.group) continue;
+        float2 x = make_float2(0.f, 0.f);
+        const float *src = merge + (k * kPagedHeads + head) * S::kRow + 2 * lane;
+#pragma unroll 3
+        for (uint32_t w = k; w < kPagedWarps; w += seg.tiles, src += seg.tiles * kPagedHeads * S::kRow) {
+          const float2 y = *(const float2 *)src;
+          x.x += y.x, x.y += y.y;
+        }
+        const uint32_t ch = 64 * h + 2 * lane;
+        if (whole) {
+          const float inv = inverse_of(f_sum[k][head]);
+          T *dst = out_of(k, head) + ch;
+          dst[0] = from_float<T>(x.x * inv), dst[1] = from_float<T>(x.y * inv);
+        } else {
+          *(float2 *)(part + k * kPart<D> + head * D + ch) = x;
+        }
       }
     }
     if (!whole) {
@@ -605,21 +671,25 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       if (last) {
         if (threadIdx.x == 0) *ticket = 0;
 #pragma unroll 1
-        for (uint32_t k = 0; k < seg.tiles; ++k) {   // a warp a head of every tile
-          if (head_of(k) + warp >= p.group) continue;
+        for (uint32_t r = warp; r < seg.tiles * kPagedHeads; r += kPagedWarps) {   // a head a warp at a time
+          const uint32_t k = r / kPagedHeads, head = r % kPagedHeads;
+          if (head_of(k) + head >= p.group) continue;
           constexpr uint32_t N = D / 32;   // channels of a lane
           constexpr uint32_t kAhead = 8;   // pieces whose values are loaded before their weights are known
           const float *from = p.parts + ((size_t)seg.slot * p.tiles + k) * kPart<D>;
+          struct __align__(D / 8) Values {   // a lane's channels
+            float x[N];
+          };
           const size_t stride = (size_t)p.tiles * kPart<D>;
           const auto values = [&](uint32_t i) {
-            const float *src = from + i * stride + warp * D + lane * N;
+            const float *src = from + i * stride + head * D + lane * N;
             Values v;
             if constexpr (N == 4) *(float4 *)v.x = __ldcg((const float4 *)src);
             else *(float2 *)v.x = __ldcg((const float2 *)src);
             return v;
           };
           // lanes are pieces, 32 at a time
-          const float *stats = from + kPagedHeads * D + warp;
+          const float *stats = from + kPagedHeads * D + head;
           float m = lane < pieces ? __ldcg(stats + lane * stride) : kNoScore;
           float sum = lane < pieces ? __ldcg(stats + lane * stride + kPagedHeads) : 0.f;
           Values early[kAhead];
@@ -665,12 +735,14 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
 #pragma unroll
           for (int y = 16; y; y >>= 1) all += __shfl_xor_sync(~0u, all, y);
           const float inv = inverse_of(all == 0.f && __any_sync(~0u, some) ? -1.f : all);
-          T *dst = out_of(k, warp) + lane * N;
+          T *dst = out_of(k, head) + lane * N;
 #pragma unroll
           for (uint32_t n = 0; n < N; ++n) dst[n] = from_float<T>(x.x[n] * inv);
         }
       }
     }
+    if ((index += gridDim.x) >= plan.pieces) break;
+    piece = paged_piece(p, plan, index, lead, cursor);
     named_bar(1, kPagedWarps * 32);   // shared results are free for the next piece
   }
   if (stopped) {   // copies in flight land before the block ends; the first that does not in time was never issued

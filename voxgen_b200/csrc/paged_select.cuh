@@ -56,22 +56,13 @@ __device__ __forceinline__ double widened(uint32_t h) {
   return __hiloint2double((int)((h & 0x80000000u) | (h & 0x7FFF0000u) >> (kMantissa<C> - 4)), 0);
 }
 
-// The least and the greatest of a warp.
-__device__ __forceinline__ void reach(unsigned long long &low, unsigned long long &high) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const unsigned long long a = __shfl_xor_sync(~0u, low, o), b = __shfl_xor_sync(~0u, high, o);
-    low = a < low ? a : low, high = b > high ? b : high;
-  }
-}
-
 template <int D, typename T, typename C>
 __global__ void __launch_bounds__(kSelectThreads, 2) paged_select_kernel(const PagedSelectParams p) {
   extern __shared__ __align__(16) uint64_t keys[];   // [candidates], of the first CTA
   __shared__ __align__(16) double weights[2][D];     // of the smallest, of the largest
   __shared__ __align__(16) uint32_t bins[kSelectBins];
   __shared__ uint32_t taken[kSelectPages / 32], same[kSelectPages / 32];   // a bit a key
-  __shared__ unsigned long long w_low[8 * kSelectWarps], w_high[8 * kSelectWarps];   // of the warps of the cluster
+  __shared__ unsigned long long reach[8 * kSelectWarps];   // upper halves of the greatest and the least key of the cluster's warps
   __shared__ uint32_t w_sum[kSelectWarps];
   __shared__ uint32_t found_bin, found_above, found_count, listed;
   const PagedTable &t = p.c.t;
@@ -120,7 +111,7 @@ __global__ void __launch_bounds__(kSelectThreads, 2) paged_select_kernel(const P
     const int32_t *table = t.table + (size_t)who.seq * t.seq_pages + p.sinks;
     const uint32_t step = kBatch * kPer, stride = ctas * kSelectWarps * step;
     const uint32_t there = remote_smem(keys, 0);
-    unsigned long long low = ~0ull, high = 0;
+    uint32_t low = ~0u, high = 0;   // upper halves of the least and the greatest key
     const auto pages_at = [&](uint32_t base) {
       return lane < step && base + lane < n ? (uint32_t)table[base + lane] : ~0u;
     };
@@ -172,25 +163,22 @@ __global__ void __launch_bounds__(kSelectThreads, 2) paged_select_kernel(const P
       if (part < 8 && i < n) {
         const unsigned long long k = ordered(s[0]);
         st_remote(there + i * 8, k);
-        low = k < low ? k : low, high = k > high ? k : high;
+        low = min(low, (uint32_t)(k >> 32)), high = max(high, (uint32_t)(k >> 32));
       }
     }
-    reach(low, high);
-    if (lane == 0) {
-      const uint32_t w = rank * kSelectWarps + warp;
-      st_remote(remote_smem(&w_low[w], 0), low);
-      st_remote(remote_smem(&w_high[w], 0), high);
-    }
+    low = __reduce_min_sync(~0u, low), high = __reduce_max_sync(~0u, high);
+    if (lane == 0) st_remote(remote_smem(&reach[rank * kSelectWarps + warp], 0), (uint64_t)high << 32 | low);
   }
   cluster_sync();
   if (rank) return;
   // ---- the part of the range that the last chosen key lies in ----
-  unsigned long long low = ~0ull, high = 0;
+  uint32_t low_half = ~0u, high_half = 0;
   for (uint32_t i = lane; i < ctas * kSelectWarps; i += 32) {
-    low = w_low[i] < low ? w_low[i] : low;
-    high = w_high[i] > high ? w_high[i] : high;
+    low_half = min(low_half, (uint32_t)reach[i]);
+    high_half = max(high_half, (uint32_t)(reach[i] >> 32));
   }
-  reach(low, high);
+  unsigned long long low = (unsigned long long)__reduce_min_sync(~0u, low_half) << 32;
+  unsigned long long high = (unsigned long long)__reduce_max_sync(~0u, high_half) << 32 | 0xFFFFFFFFu;
   uint32_t left = want;   // of the keys in [low, high]; want < n, so some are left out
   uint32_t count_in;
   for (;;) {
