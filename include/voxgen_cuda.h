@@ -539,7 +539,7 @@ typedef struct vg_paged_step {
 
 /* One layer's pool: data [pages][kv_heads][K, V][page_rows][head_dim] of type dtype
  * (VG_DTYPE_F16 or VG_DTYPE_BF16), head_dim 64 or 128, 16-byte aligned. summaries: NULL,
- * or [pages][kv_heads][2][head_dim] of the same type: per channel the smallest and the
+ * or [pages][kv_heads][2][head_dim] of the same type, 32-byte aligned: per channel the smallest and the
  * largest K of the rows that a page held at its last append, NaN passed over (0 and 0
  * for a channel of NaN alone). */
 typedef struct vg_paged_cache {

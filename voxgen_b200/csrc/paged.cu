@@ -36,7 +36,7 @@ int table_of(const vg_paged_table *t, PagedTable *v) {
 }
 
 int cache_of(const vg_paged_cache *c, PagedView *v) {
-  if (!c || !c->data || !aligned(c->data, 16) || !aligned(c->summaries, 16) || !c->kv_heads) return VG_EINVAL;
+  if (!c || !c->data || !aligned(c->data, 16) || !aligned(c->summaries, 32) || !c->kv_heads) return VG_EINVAL;
   if (c->dtype != VG_DTYPE_F16 && c->dtype != VG_DTYPE_BF16) return VG_EUNSUPPORTED;
   if (c->head_dim != 64 && c->head_dim != 128) return VG_EUNSUPPORTED;
   const int rc = table_of(c->table, &v->t);
@@ -253,9 +253,9 @@ int vg_k_paged_select(const vg_paged_cache *cache, const void *q, int dtype, uin
   p.budget = budget;
   p.sinks = sinks;
   p.recent = recent;
-  // CTAs of a (query, KV head): as many as are resident at once, and have pages to score
+  // CTAs of a (query, KV head): no more than are resident at once, one an SM, and have pages to score
   uint32_t ctas = 8;
-  while (ctas > 1 && (items * ctas > 148 * 4 || (ctas - 1) * kSelectWarps * 8 >= p.c.t.seq_pages)) ctas /= 2;
+  while (ctas > 1 && (items * ctas > 148 || (ctas - 1) * kSelectWarps * 16 >= p.c.t.seq_pages)) ctas /= 2;
   const size_t smem = (size_t)p.c.t.seq_pages * 8;
   return by_dim(cache->head_dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
