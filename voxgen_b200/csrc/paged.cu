@@ -216,7 +216,12 @@ int vg_k_paged_append(const vg_paged_cache *cache, const vg_paged_step *step, co
   // 16-byte loads need the base and every row on a 16-byte boundary
   const bool vec = aligned(k, 16) && aligned(v, 16) && p.ks.token % wide == 0 && p.ks.head % wide == 0 &&
                    p.vs.token % wide == 0 && p.vs.head % wide == 0;
-  const uint32_t grid = (uint32_t)std::min<uint64_t>((uint64_t)p.most_runs * cache->kv_heads, 148 * kPagedRowBlocks);
+  const uint64_t items = (uint64_t)p.most_runs * cache->kv_heads;
+  if (items > kMaxGrid / 2) return VG_ERANGE;
+  // a block an item while all are resident at once, else a warp an item: 65,000 rows of 8 KV heads take 107 us with blocks
+  const bool blocks = items <= 148 * kPagedRowBlocks;
+  const uint32_t warps = kPagedRowThreads / 32;
+  const uint32_t grid = (uint32_t)std::min<uint64_t>(blocks ? items : (items + warps - 1) / warps, 148 * kPagedRowBlocks);
   return by_dim(cache->head_dim, [&](auto d) {
     constexpr int D = decltype(d)::value;
     return by_type(dtype, [&](auto t) {
@@ -224,9 +229,13 @@ int vg_k_paged_append(const vg_paged_cache *cache, const vg_paged_step *step, co
       return by_cache_type(cache->dtype, [&](auto c) {
         using C = decltype(c);
         const auto go = [&](auto fn) { return launch(fn, grid, 1, kPagedRowThreads, 0, cuda_stream, p); };
-        if (cache->summaries)
-          return vec ? go(paged_append_kernel<D, T, C, true, true>) : go(paged_append_kernel<D, T, C, false, true>);
-        return vec ? go(paged_append_kernel<D, T, C, true, false>) : go(paged_append_kernel<D, T, C, false, false>);
+        const auto pick = [&](auto w) {
+          constexpr int W = decltype(w)::value;
+          if (cache->summaries)
+            return vec ? go(paged_append_kernel<D, T, C, true, true, W>) : go(paged_append_kernel<D, T, C, false, true, W>);
+          return vec ? go(paged_append_kernel<D, T, C, true, false, W>) : go(paged_append_kernel<D, T, C, false, false, W>);
+        };
+        return blocks ? pick(Dim<8>{}) : pick(Dim<1>{});
       });
     });
   });

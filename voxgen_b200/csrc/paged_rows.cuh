@@ -1,8 +1,8 @@
 // Append to a paged cache: the step's new rows into their pages, and the summaries
 // of the pages that got rows.
 //
-// A run is what a step adds to one page. A block takes a (run, KV head): lanes of
-// 16 bytes of a cache row, K and V side by side, rows dealt out over the block. The
+// A run is what a step adds to one page. A block, or where there are many a warp,
+// takes a (run, KV head): lanes of 16 bytes of a cache row, K and V side by side. The
 // extremes of K are taken in the cache's own type, two channels an instruction, on
 // the values as they are stored; rows that the page held before are read back for
 // it. Values past the largest finite number of the cache's type are held as that one:
@@ -84,21 +84,27 @@ __device__ __forceinline__ uint4 load_rounded(const T *p, bool &odd) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <int D, typename T, typename C, bool VEC, bool SUM>
+// W: warps of a (run, KV head), 8 or 1. With one there are no block barriers and 4 times as many rows in flight a
+// warp; with 8 a single token's page is read back by a whole block: 2.4 us for a step of 16 streams.
+template <int D, typename T, typename C, bool VEC, bool SUM, int W>
 __global__ void __launch_bounds__(kPagedRowThreads, kPagedRowBlocks) paged_append_kernel(const PagedAppendParams p) {
   constexpr uint32_t L = D / 8;                       // lanes of a row
-  constexpr uint32_t kRows = kPagedRowThreads / L;    // rows a pass
+  constexpr uint32_t kRows = W * 32 / L;              // rows a pass
+  constexpr uint32_t kGroups = kPagedRowThreads / 32 / W;
   using P = Pair<C>;
-  __shared__ uint4 ends[SUM ? kPagedRowThreads / 32 : 1][2][L];
+  __shared__ uint4 ends[SUM && W > 1 ? W : 1][2][L];
   const PagedTable &t = p.c.t;
-  const uint32_t lane = threadIdx.x % L, slot = threadIdx.x / L, page_rows = t.page_rows();
-  const uint64_t items = (uint64_t)p.most_runs * p.c.kv_heads;
+  const uint32_t lane = threadIdx.x % L, slot = threadIdx.x % (W * 32) / L, page_rows = t.page_rows();
+  const uint32_t items = p.most_runs * p.c.kv_heads, stride = gridDim.x * kGroups;   // the host keeps items below 2^31
   bool odd = false;   // met a NaN, or a value past the largest that the cache holds
   pdl_launch_dependents();
   pdl_wait();
-  for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const uint32_t run = (uint32_t)(item / p.c.kv_heads), head = (uint32_t)(item - (uint64_t)run * p.c.kv_heads);
-    const int4 r = p.runs[run];
+  uint32_t item = blockIdx.x * kGroups + threadIdx.x / (W * 32);
+  int4 next = item < items ? p.runs[item / p.c.kv_heads] : make_int4(0, 0, 0, 0);
+  for (; item < items; item += stride) {
+    const int4 r = next;
+    if (item + stride < items) next = p.runs[(item + stride) / p.c.kv_heads];
+    const uint32_t head = item % p.c.kv_heads;
     const uint32_t first = (uint32_t)r.x, page = (uint32_t)r.y, at = (uint32_t)r.z, rows = (uint32_t)r.w;
     if (!rows) break;   // runs past the last are empty
     if (page >= t.pages || at >= page_rows || rows > page_rows - at || first >= p.tokens || rows > p.tokens - first) continue;
@@ -112,13 +118,9 @@ __global__ void __launch_bounds__(kPagedRowThreads, kPagedRowBlocks) paged_appen
 #pragma unroll
       for (int i = 0; i < 4; ++i) low[i] = __hmin2(low[i], pair_of<P>(w[i])), high[i] = __hmax2(high[i], pair_of<P>(w[i]));
     };
-    if constexpr (SUM) {
-#pragma unroll 4
-      for (uint32_t i = slot; i < at; i += kRows) widen(*(const uint4 *)(k_page + (size_t)i * D));
-    }
     const T *k = (const T *)p.k + (int64_t)first * p.ks.token + (int64_t)head * p.ks.head + lane * 8;
     const T *v = (const T *)p.v + (int64_t)first * p.vs.token + (int64_t)head * p.vs.head + lane * 8;
-#pragma unroll 2
+#pragma unroll(W == 1 && sizeof(T) == 2 ? 4 : 2)
     for (uint32_t i = slot; i < rows; i += kRows) {
       const uint4 a = load_rounded<T, C, VEC>(k + (int64_t)i * p.ks.token, odd);
       const uint4 b = load_rounded<T, C, VEC>(v + (int64_t)i * p.vs.token, odd);
@@ -127,6 +129,8 @@ __global__ void __launch_bounds__(kPagedRowThreads, kPagedRowBlocks) paged_appen
       if constexpr (SUM) widen(a);
     }
     if constexpr (SUM) {
+#pragma unroll 4
+      for (uint32_t i = slot; i < at; i += kRows) widen(*(const uint4 *)(k_page + (size_t)i * D));   // rows that it had
       // over the rows of a warp, then over the warps
 #pragma unroll
       for (uint32_t o = L; o < 32; o <<= 1) {
@@ -136,28 +140,37 @@ __global__ void __launch_bounds__(kPagedRowThreads, kPagedRowBlocks) paged_appen
           high[i] = __hmax2(high[i], pair_of<P>(__shfl_xor_sync(~0u, pair_bits(high[i]), o)));
         }
       }
-      const uint32_t warp = threadIdx.x / 32;
-      if (threadIdx.x % 32 < L) {
-        ends[warp][0][lane] = make_uint4(pair_bits(low[0]), pair_bits(low[1]), pair_bits(low[2]), pair_bits(low[3]));
-        ends[warp][1][lane] = make_uint4(pair_bits(high[0]), pair_bits(high[1]), pair_bits(high[2]), pair_bits(high[3]));
-      }
-      __syncthreads();
-      if (threadIdx.x < D / 2) {   // two channels a thread
-        const uint32_t c = threadIdx.x;
-        P a = pair_of<P>(((const uint32_t *)ends[0][0])[c]), b = pair_of<P>(((const uint32_t *)ends[0][1])[c]);
+      uint4 *out = (uint4 *)((C *)p.c.summaries + place * 2 * D);
+      // a channel whose rows are all NaN has kept +inf and -inf: 0 and 0
+      const auto pack = [&](const P(&x)[4]) {
+        uint32_t w[4];
 #pragma unroll
-        for (uint32_t w = 1; w < kPagedRowThreads / 32; ++w) {
-          a = __hmin2(a, pair_of<P>(((const uint32_t *)ends[w][0])[c]));
-          b = __hmax2(b, pair_of<P>(((const uint32_t *)ends[w][1])[c]));
+        for (int i = 0; i < 4; ++i) w[i] = pair_bits(x[i]) & ~__hgt2_mask(low[i], high[i]);
+        return make_uint4(w[0], w[1], w[2], w[3]);
+      };
+      if constexpr (W == 1) {
+        if (threadIdx.x % 32 < L) out[lane] = pack(low), out[L + lane] = pack(high);
+      } else {
+        const uint32_t warp = threadIdx.x / 32;
+        if (threadIdx.x % 32 < L) {
+          ends[warp][0][lane] = make_uint4(pair_bits(low[0]), pair_bits(low[1]), pair_bits(low[2]), pair_bits(low[3]));
+          ends[warp][1][lane] = make_uint4(pair_bits(high[0]), pair_bits(high[1]), pair_bits(high[2]), pair_bits(high[3]));
         }
-        // a channel whose rows are all NaN has kept +inf and -inf: 0 and 0
-        const uint32_t none = __hgt2_mask(a, b);
-        const P top = pair_of<P>(kLargestBits<C>), bottom = pair_of<P>(kLargestBits<C> | 0x80008000u);
-        uint32_t *out = (uint32_t *)((C *)p.c.summaries + place * 2 * D) + c;
-        out[0] = pair_bits(__hmin2(__hmax2(a, bottom), top)) & ~none;
-        out[D / 2] = pair_bits(__hmin2(__hmax2(b, bottom), top)) & ~none;
+        __syncthreads();
+        if (threadIdx.x < D / 2) {   // two channels a thread
+          const uint32_t c = threadIdx.x;
+          P a = pair_of<P>(((const uint32_t *)ends[0][0])[c]), b = pair_of<P>(((const uint32_t *)ends[0][1])[c]);
+#pragma unroll
+          for (uint32_t w = 1; w < W; ++w) {
+            a = __hmin2(a, pair_of<P>(((const uint32_t *)ends[w][0])[c]));
+            b = __hmax2(b, pair_of<P>(((const uint32_t *)ends[w][1])[c]));
+          }
+          const uint32_t none = __hgt2_mask(a, b);
+          ((uint32_t *)out)[c] = pair_bits(a) & ~none;
+          ((uint32_t *)out)[D / 2 + c] = pair_bits(b) & ~none;
+        }
+        __syncthreads();
       }
-      __syncthreads();
     }
   }
   if (odd) atomicOr(&t.pool[1], kPagedNonFinite);
