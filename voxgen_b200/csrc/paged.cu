@@ -76,7 +76,7 @@ int launch(void (*fn)(A...), uint32_t grid, uint32_t cluster, uint32_t threads, 
   cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)stream;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, args...);
   if (e != cudaSuccess) cudaGetLastError();   // reported here, and not by a later call
   return e == cudaSuccess ? VG_OK : e == cudaErrorMemoryAllocation ? VG_ENOMEM : VG_ECUDA;

@@ -65,6 +65,7 @@ constexpr uint32_t kPagedCtas = 148;     // one per SM
 constexpr uint32_t kPagedHeads = 8;      // columns of a tile
 constexpr uint32_t kPagedTiles = 4;      // most tiles of a segment
 constexpr uint32_t kPagedLeast = 12;     // blocks of a piece: a round of the warps
+constexpr uint32_t kPagedWhole = 48;     // blocks of a segment that is not cut: joining takes as long as five rounds
 constexpr uint32_t kPagedTickets = 1u << 14;   // segments that may be cut
 constexpr uint32_t kPagedPlanned = 256;        // queries whose place in the plan is kept in shared memory
 constexpr uint32_t kPagedMost = 1u << 26;      // blocks of a segment
@@ -153,6 +154,7 @@ __device__ __forceinline__ uint32_t paged_size(uint32_t entry, uint32_t size) { 
 }
 __device__ __forceinline__ uint32_t paged_parts(uint32_t entry, uint32_t size) {   // pieces of a segment
   const uint32_t b = entry >> 2, each = paged_size(entry, size);
+  if (b * paged_weight(entry) <= kPagedWhole * 4) return entry != 0;
   uint32_t n = (uint32_t)((float)b * __fdividef(1.f - 0x1p-20f, (float)each));   // a little low
   n += n * each < b;
   while (n * each < b) ++n;   // millions of blocks
@@ -241,7 +243,7 @@ __device__ __forceinline__ PagedPiece paged_piece(const PagedAttnParams &p, cons
       y.parts = parts;
       y.slot = cut_before + __shfl_sync(~0u, cut, at) - parts * p.lanes + y.lane * parts;
       y.first = y.part * size;
-      y.blocks = min(size, (all >> 2) - y.first);
+      y.blocks = parts == 1 ? all >> 2 : min(size, (all >> 2) - y.first);
       y.tiles = 1u << (all & 3);
       y.seq = __shfl_sync(~0u, who.seq, at);
       y.seen = __shfl_sync(~0u, who.most, at);
@@ -574,25 +576,34 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       *(float2 *)&w_sum[warp][2 * t] = make_float2(l0, l1);
     }
     named_bar(1, kPagedWarps * 32);
-    float top0 = kNoScore, top1 = kNoScore;
-#pragma unroll 1
-    for (uint32_t w = tile; w < kPagedWarps; w += seg.tiles) {
-      const float2 x = *(const float2 *)&w_max[w][2 * t];
-      top0 = fmaxf(top0, x.x), top1 = fmaxf(top1, x.y);
-    }
-    const float e0 = exp2_fast(m0 - top0), e1 = exp2_fast(m1 - top1);
-    if (team == 0 && g < 2) {   // lanes of g = 0 and 1: the denominators of heads 2t and 2t + 1
-      const float top = g ? top1 : top0;
-      float all = 0.f;
-      bool some = false;
-#pragma unroll 1
-      for (uint32_t w = tile; w < kPagedWarps; w += seg.tiles) {
-        const float x = w_sum[w][2 * t + g];
-        some |= x < 0.f;
-        all += (x < 0.f ? 0.f : x) * exp2_fast(w_max[w][2 * t + g] - top);
+    // lane (head, s) looks at warps s, s + 4 and s + 8, of which those of this tile count
+    float e0, e1;
+    {
+      const uint32_t h = lane / 4, s = lane % 4;
+      float m[3], l[3], top = kNoScore, all = 0.f;
+#pragma unroll
+      for (uint32_t i = 0; i < 3; ++i) {
+        const uint32_t w = s + 4 * i;
+        const bool mine = (w & (seg.tiles - 1)) == tile;
+        m[i] = mine ? w_max[w][h] : kNoScore, l[i] = mine ? w_sum[w][h] : 0.f;
+        top = fmaxf(top, m[i]);
       }
-      f_max[tile][2 * t + g] = top;
-      f_sum[tile][2 * t + g] = all == 0.f && some ? -1.f : all;
+      top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+      bool some = false;
+#pragma unroll
+      for (uint32_t i = 0; i < 3; ++i) {
+        some |= l[i] < 0.f;
+        all += (l[i] < 0.f ? 0.f : l[i]) * exp2_fast(m[i] - top);
+      }
+      all += __shfl_xor_sync(~0u, all, 1);
+      all += __shfl_xor_sync(~0u, all, 2);
+      some = __ballot_sync(~0u, some) >> (lane & ~3u) & 15;
+      if (team == 0 && s == 0) {
+        f_max[tile][h] = top;
+        f_sum[tile][h] = all == 0.f && some ? -1.f : all;
+      }
+      e0 = exp2_fast(m0 - __shfl_sync(~0u, top, 8 * t)), e1 = exp2_fast(m1 - __shfl_sync(~0u, top, 8 * t + 4));
     }
     float *part = p.parts + (size_t)(seg.slot + seg.part) * p.tiles * kPart<D>;
     const auto out_of = [&](uint32_t k, uint32_t head) {   // of a tile's head

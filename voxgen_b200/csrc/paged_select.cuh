@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kSelectThreads, 1) paged_select_kernel(const P
   if (tid < D) {
     const T *q = (const T *)p.q + (int64_t)query * p.q_query + (int64_t)head * p.group * p.q_head + tid;
     double up = 0, down = 0;
-#pragma unroll 4
+#pragma unroll 8
     for (uint32_t h = 0; h < p.group; ++h) {
       float x = (float)q[(int64_t)h * p.q_head];
       x = x != x ? 0.f : fminf(fmaxf(x, -3.402823466e38f), 3.402823466e38f);

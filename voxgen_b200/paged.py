@@ -71,9 +71,9 @@ class Step:
 
     def __init__(self, table: "PageTable", tokens: int):
         self.tokens, self.seqs, self.device = tokens, table.seqs, table.device
-        self._sizes, total, offsets, _ = table._layout(tokens)
+        total, offsets, self._views = table._layout(tokens)[:3]
         self._buffer = torch.empty(total, dtype=torch.int32, device=table.device)
-        self._parts = None
+        self._parts = [None] * 5
         at = self._buffer.data_ptr()
         self.desc = api.PagedStepDesc(*[at + 4 * o for o in offsets], tokens)
         self._ref = C.byref(self.desc)
@@ -93,10 +93,10 @@ class Step:
         return step
 
     def _part(self, i: int) -> torch.Tensor:
-        if self._parts is None:
-            parts = self._buffer.split_with_sizes(self._sizes)
-            self._parts = [*parts[0:8:2], parts[8].view(-1, 4)]
-        return self._parts[i]
+        x = self._parts[i]
+        if x is None:
+            x = self._parts[i] = self._buffer.as_strided(*self._views[i])
+        return x
 
     starts = property(lambda self: self._part(0))
     slots = property(lambda self: self._part(1))
@@ -142,21 +142,21 @@ class PageTable:
         self._lib = api.lib()
 
     def _layout(self, tokens: int):
-        """Sizes of a step's arrays and of what lies between them, their sum, where each starts, and the runs."""
+        """Of a step's arrays: the sum of their sizes, where each starts, (size, strides, start) of each, and the runs."""
         found = self._layouts.get(tokens)
         if found is None:
             _sizes(tokens=tokens)
             n = C.c_uint32()
             _check(self._lib.vg_k_paged_runs(self._ref, tokens, C.byref(n)), f"a step of {tokens} tokens")
-            sizes, offsets = [], []
+            offsets, total = [], 0
             for x in (self.seqs + 1, tokens, tokens, tokens, 4 * n.value):
-                offsets.append(sum(sizes))
-                sizes += [x, -x % 4]      # each starts on 16 bytes
-            total = sum(sizes)
+                offsets.append(total)
+                total += x + -x % 4      # each starts on 16 bytes
+            views = [((x,), (1,), at) for x, at in zip((self.seqs + 1, tokens, tokens, tokens), offsets)]
+            views.append(((n.value, 4), (4, 1), offsets[4]))
             if len(self._layouts) > 256:
                 self._layouts.clear()
-            found = self._layouts[tokens] = sizes, max(total, 4), offsets, n.value
-            sizes[-1] += found[1] - total
+            found = self._layouts[tokens] = total, offsets, views, n.value
         return found
 
     @_on_its_device
