@@ -791,6 +791,8 @@ def test_refusals():
     refused(lambda: cache.append(step, k[:1], k[:1]))
     refused(lambda: cache.append(step, k, k.half()))
     refused(lambda: cache.append(step, k.double(), k.double()), "VG_EUNSUPPORTED")
+    refused(lambda: cache.append(paged.PageTable(2, 10, 16, 5).step(ints([1, 1]), 2), k, k))     # another table's
+    refused(lambda: table.step(ints([1, 1]), 2, into=paged.PageTable(2, 10, 16, 5).step(ints([1, 1]), 2)))
     refused(lambda: cache.append(step, k, k, layer=1))
     refused(lambda: cache.append(step, k, k, layer=-1))
     refused(lambda: cache.append(step, k.transpose(1, 2).contiguous().transpose(1, 2), k))

@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
   constexpr int kQ = kQTerms<T, C>, kP = kPTerms<T, C>;
   constexpr bool kFresh = sizeof(T) == 4;       // O summed afresh
   constexpr uint32_t kFreshSteps = 8;
-  extern __shared__ uint8_t paged_smem[];
+  extern __shared__ __align__(128) uint8_t paged_smem[];
   __shared__ uint64_t full[S::kStages], empty[S::kStages];
   __shared__ uint32_t first_row[S::kStages];    // of a stage's block in its sequence; past every row: nothing was read
   __shared__ PagedLead leads[kPagedPlanned];

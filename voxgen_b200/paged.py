@@ -70,7 +70,7 @@ class Step:
     _NAMES = ("starts", "slots", "positions", "sequences", "runs")
 
     def __init__(self, table: "PageTable", tokens: int):
-        self.tokens, self.seqs, self.device = tokens, table.seqs, table.device
+        self.table, self.tokens = table, tokens
         total, offsets, self._views = table._layout(tokens)[:3]
         self._buffer = torch.empty(total, dtype=torch.int32, device=table.device)
         self._parts = [None] * 5
@@ -83,8 +83,8 @@ class Step:
            sequences: torch.Tensor, runs: torch.Tensor) -> "Step":
         """A step from arrays in hand, such as copies of an earlier one's (each starts on 16 bytes)."""
         step = cls.__new__(cls)
-        step.tokens = tokens = slots.numel()
-        step.seqs, step.device = table.seqs, table.device
+        step.table, step.tokens = table, slots.numel()
+        tokens = step.tokens
         shapes = (table.seqs + 1,), (tokens,), (tokens,), (tokens,), (table._layout(tokens)[3], 4)
         step._parts = [_expect(x, torch.int32, shape, table.device, what) for x, shape, what in
                        zip((starts, slots, positions, sequences, runs), shapes, cls._NAMES)]
@@ -168,8 +168,8 @@ class PageTable:
         have no slot, and ``status`` says why. ``into``: an earlier step of as many tokens to write over."""
         if into is None:
             into = Step(self, tokens)
-        elif into.tokens != tokens or into.seqs != self.seqs or into.device != self.device:
-            raise _invalid(f"into: a step of {into.tokens} tokens of {into.seqs} sequences for one of {tokens} of {self.seqs}")
+        elif into.table is not self or into.tokens != tokens:
+            raise _invalid(f"into: another table's step, or one of {into.tokens} tokens for one of {tokens}")
         rc = self._lib.vg_k_paged_step(self._ref, _ints(counts, (self.seqs,), self.device, "counts"),
                                        _ints(keep, (self.seqs,), self.device, "keep"), into._ref, _current_stream(self._index))
         if rc:
@@ -266,6 +266,8 @@ class PagedCache:
         one, and ``table.pool[1]`` then has STATUS_NONFINITE, as for NaN."""
         ref = self._layer(layer)
         dtype = self._rows_of(k, self.kv_heads, "k")
+        if step.table is not self.table:
+            raise _invalid("the step is another table's")
         if v.shape != k.shape or v.dtype is not k.dtype or v.device != self.device or k.shape[0] != step.tokens:
             raise _invalid(f"k and v must agree in shape, type and device, and have the step's {step.tokens} rows")
         rc = self._lib.vg_k_paged_append(ref, step._ref, k.data_ptr(), v.data_ptr(), dtype, self._strides(k),
