@@ -167,14 +167,14 @@ def test_ring_stages_are_whole_rounds_of_the_warps():
     """A stage of the attention's ring is always the same team's: the property that its waits need."""
     from voxgen_b200._build import CSRC
     text = (CSRC / "paged_attention.cuh").read_text()
-    warps = int(re.search(r"kPagedWarps = (\d+);", text)[1])
-    assert "kStages % kPagedWarps == 0" in text and all(warps % t == 0 for t in (1, 2, 4))
-    for dim in (64, 128):
-        stages, teams_seen = 2 * warps * 128 // dim, {}
-        for tiles in (1, 2, 4):
-            teams = warps // tiles
-            for block in range(10 * stages):
-                assert teams_seen.setdefault((tiles, block % stages), block % teams) == block % teams
+    assert "kPagedWarps = 12, kPagedFew = 4;" in text and "kStages % W == 0" in text
+    for warps, rounds in ((12, 2), (4, 1)):
+        for dim in (64, 128):
+            stages, team_of = rounds * warps * 128 // dim, {}
+            for tiles in (1, 2, 4):
+                teams = warps // tiles
+                for block in range(10 * stages):
+                    assert team_of.setdefault((tiles, block % stages), block % teams) == block % teams
 
 
 def test_dynamic_shared_memory_is_declared_with_the_alignment_of_its_widest_access():

@@ -136,15 +136,17 @@ constexpr uint64_t kPagedTicketBytes = kPagedTickets * 4;
 // How the tiles of 8 heads of a KV head make segments.
 struct Tiling {
   uint32_t head_tiles, tiles, lanes;   // of a KV head, of a segment (1, 2 or 4), segments of a query
+  uint32_t warps;                      // consumer warps of a CTA
   bool share;                          // consecutive queries of a sequence may make one segment
 };
-Tiling tiling_of(uint32_t kv_heads, uint32_t heads, uint32_t budget) {
+Tiling tiling_of(uint32_t kv_heads, uint32_t heads, uint32_t queries, uint32_t budget) {
   Tiling x{};
   x.head_tiles = (heads / kv_heads + kPagedHeads - 1) / kPagedHeads;
   x.share = x.head_tiles == 1 && !budget;   // lists of pages differ from query to query
   x.tiles = 1;
   while (x.tiles < kPagedTiles && x.tiles < x.head_tiles) x.tiles *= 2;
   x.lanes = kv_heads * ((x.head_tiles + kPagedTiles - 1) / kPagedTiles);
+  x.warps = (uint64_t)queries * x.lanes < kPagedMany ? kPagedWarps : kPagedFew;
   return x;
 }
 
@@ -286,13 +288,13 @@ int vg_k_paged_attention_bytes(const vg_paged_cache *cache, uint32_t queries, ui
   const int rc = cache_of(cache, &c);
   if (rc) return rc;
   if (!bytes || !queries || !heads || heads % cache->kv_heads) return VG_EINVAL;
-  const Tiling x = tiling_of(c.kv_heads, heads, budget);
+  const Tiling x = tiling_of(c.kv_heads, heads, queries, budget);
   const uint64_t segments = (uint64_t)queries * x.lanes;
   const uint64_t blocks = (uint64_t)(budget ? budget : c.t.seq_pages) << (c.t.shift - 4);   // of a segment, at most
   const uint64_t cost = segments * blocks * x.tiles;
   if (x.lanes > 1u << 16 || segments > kMaxGrid || blocks > kPagedMost || cost > kMaxGrid) return VG_ERANGE;   // the plan counts in 32 bits
   *bytes = kPagedTicketBytes +
-           (uint64_t)paged_slots(segments) * (x.share ? kPagedTiles : x.tiles) * kPagedHeads * (cache->head_dim + 2) * 4;
+           (uint64_t)paged_slots(segments, paged_ctas(x.warps)) * (x.share ? kPagedTiles : x.tiles) * kPagedHeads * (cache->head_dim + 2) * 4;
   return VG_OK;
 }
 
@@ -324,7 +326,7 @@ int vg_k_paged_attention(const vg_paged_cache *cache, const void *q, int dtype, 
   p.queries = queries;
   p.heads = heads;
   p.group = x.group;
-  const Tiling tiling = tiling_of(c.kv_heads, heads, budget);
+  const Tiling tiling = tiling_of(c.kv_heads, heads, queries, budget);
   p.head_tiles = tiling.head_tiles;
   p.share = tiling.share && sequences;   // else every query is of its own sequence
   p.tiles = p.share ? kPagedTiles : tiling.tiles;
@@ -339,10 +341,16 @@ int vg_k_paged_attention(const vg_paged_cache *cache, const void *q, int dtype, 
     return by_type(dtype, [&](auto t) {
       using T = decltype(t);
       return by_cache_type(cache->dtype, [&](auto ct) {
-        const auto fn = paged_attention_kernel<D, T, decltype(ct)>;
-        static std::atomic<uint64_t> done;
-        const int e = allow_smem((const void *)fn, PagedSmem<D>::kBytes, done);
-        return e ? e : launch(fn, kPagedCtas, 1, kPagedThreads, PagedSmem<D>::kBytes, cuda_stream, p, map);
+        using C = decltype(ct);
+        const auto go = [&](auto w) {
+          constexpr int W = decltype(w)::value;
+          using S = PagedSmem<D, W, kQTerms<T, C>>;
+          const auto fn = paged_attention_kernel<D, T, C, W>;
+          static std::atomic<uint64_t> done;
+          const int e = allow_smem((const void *)fn, S::kBytes, done);
+          return e ? e : launch(fn, paged_ctas(W), 1, (W + 1) * 32, S::kBytes, cuda_stream, p, map);
+        };
+        return tiling.warps == kPagedWarps ? go(Dim<(int)kPagedWarps>{}) : go(Dim<(int)kPagedFew>{});
       });
     });
   });

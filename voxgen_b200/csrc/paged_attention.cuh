@@ -24,7 +24,7 @@
 // so as many warps run as registers allow: 12, with q's terms read from shared memory.
 //
 // The split. Segments are cut into pieces of at most U blocks, U such that there is
-// about one piece for each of the 148 CTAs (4, where segments are many). The warps of
+// about one piece for each CTA (4, where segments are many). The warps of
 // a piece meet in shared memory. A segment of several pieces leaves a partial result
 // for each, and the CTA that finishes last (a counter, left at zero) adds them in
 // order: sums never depend on timing.
@@ -59,41 +59,44 @@ struct PagedAttnParams {
 };
 
 constexpr uint32_t kPagedBlock = 16;     // cache rows of a block: never more than one page's
-constexpr uint32_t kPagedWarps = 12;     // consumers
-constexpr uint32_t kPagedThreads = (kPagedWarps + 1) * 32;
-constexpr uint32_t kPagedCtas = 148;     // one per SM
+// Consumer warps of a CTA: 12 in one CTA an SM, or 4 in each of two, where segments are many: while the warps of one CTA
+// meet or load the next queries, those of the other go on.
+constexpr uint32_t kPagedWarps = 12, kPagedFew = 4;
+// Segments from which on a CTA has 4 warps. Sequences of 200 to 500 rows, 2 KV heads: 200 of them take 27 us with 12 warps and
+// 28 with 4, 256 take 34 and 30, 1024 take 120 and 94.
+constexpr uint32_t kPagedMany = 444;
+constexpr uint32_t paged_ctas(uint32_t warps) { return 148 * (warps == kPagedWarps ? 1 : 2); }   // resident at once
 constexpr uint32_t kPagedHeads = 8;      // columns of a tile
 constexpr uint32_t kPagedTiles = 4;      // most tiles of a segment
-constexpr uint32_t kPagedLeast = 12;     // blocks of a piece: a round of the warps
 constexpr uint32_t kPagedWhole = 48;     // blocks of a segment that is not cut: joining takes as long as five rounds
 constexpr uint32_t kPagedTickets = 1u << 14;   // segments that may be cut
-constexpr uint32_t kPagedPlanned = 256;        // queries whose place in the plan is kept in shared memory
+constexpr uint32_t paged_planned(uint32_t warps) { return warps == kPagedWarps ? 256 : 1024; }   // queries whose place in the plan is kept
 constexpr uint32_t kPagedMost = 1u << 26;      // blocks of a segment
 constexpr uint32_t kPagedUncut = ~0u;          // the size of pieces that are whole segments
 
-template <int D>
+template <int D, int W, int Q>   // W: consumer warps, Q: terms of a query
 struct PagedSmem {
   static constexpr uint32_t kHalf = 2 * kPagedBlock * 128;     // one copy: 64 channels of 16 K rows, then of 16 V rows
   static constexpr uint32_t kStage = kHalf * (D / 64);
-  static constexpr uint32_t kStages = 2 * kPagedWarps * 128 / D;
+  static constexpr uint32_t kStages = 2 * W * 128 / D;
   // A warp that waits for a stage's next turn has to have waited for the one before (a wait for the turn after one in
   // flight returns at once): so within a piece a stage is always the same team's, and pieces take whole rounds of stages.
-  static_assert(kStages % kPagedWarps == 0, "");
+  static_assert(kStages % W == 0, "");
   static constexpr uint32_t kRing = kStages * kStage;
   static constexpr uint32_t kRow = 68;                         // floats of a row when results meet: 64 and 4 against bank conflicts
-  static constexpr uint32_t kMerge = kPagedWarps * kPagedHeads * kRow * 4;
+  static constexpr uint32_t kMerge = W * kPagedHeads * kRow * 4;
   static constexpr uint32_t kTileQ = D / 16 * 32 * 8;          // a tile's queries as B fragments, one term
-  static constexpr uint32_t kShared = kMerge > 3 * kPagedTiles * kTileQ ? kMerge : 3 * kPagedTiles * kTileQ;   // first queries, then results
+  static constexpr uint32_t kShared = kMerge > Q * kPagedTiles * kTileQ ? kMerge : Q * kPagedTiles * kTileQ;   // first queries, then results
   static constexpr uint32_t kBytes = kRing + kShared + 1024;   // the ring starts on a multiple of 1024
 };
 
 // Pieces that a call is cut into, about, and the partial results that it may leave: a segment that is cut at all has fewer
 // than twice its share of the target in pieces.
-__host__ __device__ __forceinline__ uint32_t paged_target(uint32_t segments) {
-  return kPagedCtas * (segments * 4 <= kPagedCtas * 3 ? 1 : 4);
+__host__ __device__ __forceinline__ uint32_t paged_target(uint32_t segments, uint32_t ctas) {
+  return ctas * (segments * 4 <= ctas * 3 ? 1 : 4);
 }
-__host__ __device__ __forceinline__ uint32_t paged_slots(uint64_t segments) {
-  return segments > kPagedTickets ? 0 : 2 * paged_target((uint32_t)segments);
+__host__ __device__ __forceinline__ uint32_t paged_slots(uint64_t segments, uint32_t ctas) {
+  return segments > kPagedTickets ? 0 : 2 * paged_target((uint32_t)segments, ctas);
 }
 
 // What the plan needs to know of a query. entry: blocks and tiles of the segments that it leads, blocks << 2 |
@@ -169,13 +172,14 @@ struct PagedTally {   // in shared memory, zero before
   uint32_t total, leads, pieces[8];
 };
 // All threads: leads[] of the first queries, and the plan.
-__device__ __forceinline__ PagedPlan paged_plan(const PagedAttnParams &p, PagedLead *leads, PagedTally &tally) {
+template <uint32_t N>
+__device__ __forceinline__ PagedPlan paged_plan(const PagedAttnParams &p, PagedLead (&leads)[N], PagedTally &tally) {
   const uint32_t lane = threadIdx.x % 32;
   uint32_t total = 0, count = 0;
 #pragma unroll 1
-  for (uint32_t i = threadIdx.x; i < p.queries; i += kPagedThreads) {
+  for (uint32_t i = threadIdx.x; i < p.queries; i += blockDim.x) {
     const PagedLead x = paged_lead(p, i);
-    if (i < kPagedPlanned) leads[i] = x;
+    if (i < N) leads[i] = x;
     total += ((x.entry >> 2) * paged_weight(x.entry) + 3) / 4;
     count += x.entry != 0;
   }
@@ -185,17 +189,17 @@ __device__ __forceinline__ PagedPlan paged_plan(const PagedAttnParams &p, PagedL
   total = tally.total * p.lanes;   // the host keeps it below 2^31
   const uint32_t segments = tally.leads * p.lanes;
   if (p.queries * p.lanes > kPagedTickets) return PagedPlan{kPagedUncut, segments};   // one piece a segment
-  const uint32_t target = paged_target(segments);
+  const uint32_t target = paged_target(segments, gridDim.x);
   // total / target would do if nothing were rounded up; total / (target - segments) makes no more than target pieces. Of eight
   // sizes from the one to the other the least with no more pieces than the target is taken. Where a CTA has several pieces
   // anyway, it is the first.
-  const uint32_t least = max(kPagedLeast, paged_over(total, target));
-  const uint32_t more = target == kPagedCtas ? max(least, paged_over(total, target - segments)) - least : 0;
+  const uint32_t least = max(blockDim.x / 32 - 1, paged_over(total, target));   // a round of the warps
+  const uint32_t more = target == gridDim.x ? max(least, paged_over(total, target - segments)) - least : 0;
   const uint32_t k = lane / 4, size = least + (k == 7 ? more : more * k * k / 49);
   uint32_t n = 0;
 #pragma unroll 1
-  for (uint32_t i = threadIdx.x / 32 * 4 + lane % 4; i < p.queries; i += kPagedThreads / 8)
-    n += paged_parts(i < kPagedPlanned ? leads[i].entry : paged_lead(p, i).entry, size);
+  for (uint32_t i = threadIdx.x / 32 * 4 + lane % 4; i < p.queries; i += blockDim.x / 8)
+    n += paged_parts(i < N ? leads[i].entry : paged_lead(p, i).entry, size);
   if (n) atomicAdd(&tally.pieces[k], n);
   __syncthreads();
   n = tally.pieces[k] * p.lanes;
@@ -256,7 +260,8 @@ __device__ __forceinline__ PagedPiece paged_piece(const PagedAttnParams &p, cons
 }
 
 // Stages that a piece takes.
-__device__ __forceinline__ uint32_t paged_rounds(uint32_t blocks) { return (blocks + kPagedWarps - 1) / kPagedWarps * kPagedWarps; }
+template <uint32_t W>
+__device__ __forceinline__ uint32_t paged_rounds(uint32_t blocks) { return (blocks + W - 1) / W * W; }
 
 // Volatile keeps these behind the wait for their stage and before its release; products may move among them.
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t address) {
@@ -286,20 +291,21 @@ constexpr int kPTerms = std::is_same<C, __half>::value ? (std::is_same<T, __nv_b
 template <typename C>
 constexpr float kPagedPScale = std::is_same<C, __half>::value ? kPScale : 0.f;
 
-template <int D, typename T, typename C>
-__global__ void __launch_bounds__(kPagedThreads, 1)
+template <int D, typename T, typename C, int W>
+__global__ void __launch_bounds__((W + 1) * 32, W == kPagedWarps ? 1 : 2)
     paged_attention_kernel(const __grid_constant__ PagedAttnParams p, const __grid_constant__ CUtensorMap map) {
-  using S = PagedSmem<D>;
   constexpr int kSteps = D / 16;                // k-steps of a score, and m-tiles of the output
   constexpr int kQ = kQTerms<T, C>, kP = kPTerms<T, C>;
+  using S = PagedSmem<D, W, kQ>;
+  constexpr uint32_t kLook = 32 / W * W;        // blocks whose pages are looked up at once
   constexpr bool kFresh = sizeof(T) == 4;       // O summed afresh
   constexpr uint32_t kFreshSteps = 8;
   extern __shared__ __align__(128) uint8_t paged_smem[];
   __shared__ uint64_t full[S::kStages], empty[S::kStages];
   __shared__ uint32_t first_row[S::kStages];    // of a stage's block in its sequence; past every row: nothing was read
-  __shared__ PagedLead leads[kPagedPlanned];
+  __shared__ PagedLead leads[paged_planned(W)];
   __shared__ PagedTally tally;
-  __shared__ __align__(8) float w_max[kPagedWarps][kPagedHeads], w_sum[kPagedWarps][kPagedHeads];
+  __shared__ __align__(8) float w_max[(uint32_t)W][kPagedHeads], w_sum[(uint32_t)W][kPagedHeads];
   __shared__ float f_max[kPagedTiles][kPagedHeads], f_sum[kPagedTiles][kPagedHeads];   // [tile][head]
   __shared__ __align__(8) float factors[kPagedTiles][kPagedHeads];                    // [tile][head]
   __shared__ uint32_t last, gave_up;
@@ -311,19 +317,19 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map));
     gave_up = 0;
   }
-  if (threadIdx.x < S::kStages) mbar_init(&full[threadIdx.x], 1), mbar_init(&empty[threadIdx.x], kPagedWarps);
+  if (threadIdx.x < S::kStages) mbar_init(&full[threadIdx.x], 1), mbar_init(&empty[threadIdx.x], (uint32_t)W);
   if (threadIdx.x < sizeof(PagedTally) / 4) ((uint32_t *)&tally)[threadIdx.x] = 0;
   fence_mbar_init();
   __syncthreads();
   pdl_wait();   // and no early start for what comes next: a selection would hold SMs that this call still needs (69 us for
                 // both among 8192 pages of 16 sequences, 77 with it; one short call after another takes 8.2 us, 7.8 with it)
   const PagedPlan plan = paged_plan(p, leads, tally);
-  const auto lead = [&](uint32_t i) { return i < kPagedPlanned ? leads[i] : paged_lead(p, i); };
+  const auto lead = [&](uint32_t i) { return i < paged_planned(W) ? leads[i] : paged_lead(p, i); };
   if (blockIdx.x >= plan.pieces) return;
   PagedCursor cursor{};
   PagedPiece piece = paged_piece(p, plan, blockIdx.x, lead, cursor);   // most CTAs have one: what runs once is short
 
-  if (warp == kPagedWarps) {
+  if (warp == (uint32_t)W) {
     // ================= the copying warp =================
     uint32_t n0 = 0;           // blocks of the pieces before
     bool stopped = false;
@@ -350,14 +356,14 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       };
       Found next = find(lane);
 #pragma unroll 1
-      for (uint32_t i = 0; i < x.blocks && !stopped; i += 2 * kPagedWarps) {
+      for (uint32_t i = 0; i < x.blocks && !stopped; i += kLook) {
         const Found now = next;
-        next = find(i + 2 * kPagedWarps + lane);
+        next = find(i + kLook + lane);
 #pragma unroll 1
-        for (uint32_t j = 0; j < 2 * kPagedWarps && i + j < x.blocks; j += kPagedWarps) {   // whole rounds: stages past the last block hold nothing
-          const uint32_t from = j + lane % kPagedWarps, page = __shfl_sync(~0u, now.page, from), row = __shfl_sync(~0u, now.row, from);
+        for (uint32_t j = 0; j < kLook && i + j < x.blocks; j += (uint32_t)W) {   // whole rounds: stages past the last block hold nothing
+          const uint32_t from = j + lane % (uint32_t)W, page = __shfl_sync(~0u, now.page, from), row = __shfl_sync(~0u, now.row, from);
           bool in = true;
-          if (lane < kPagedWarps) {
+          if (lane < (uint32_t)W) {
             const uint32_t n = n0 + i + j + lane, stage = n % S::kStages, turn = n / S::kStages;
             if (turn) in = mbar_wait_bounded(&empty[stage], (turn - 1) & 1);
             if (in) {
@@ -381,7 +387,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
           }
         }
       }
-      n0 += paged_rounds(x.blocks);
+      n0 += paged_rounds<W>(x.blocks);
       if ((index += gridDim.x) >= plan.pieces) break;
       piece = paged_piece(p, plan, index, lead, cursor);
     }
@@ -403,7 +409,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     const uint32_t chunks = p.lanes / p.kv_heads;   // segments of a KV head, where it has more than 4 tiles
     const uint32_t kv = p.share ? seg.lane : seg.lane / chunks;
     const uint32_t tile0 = p.share ? 0 : (seg.lane - kv * chunks) * kPagedTiles;
-    const uint32_t teams = kPagedWarps / seg.tiles, team = warp / seg.tiles, tile = warp & (seg.tiles - 1);
+    const uint32_t teams = (uint32_t)W / seg.tiles, team = warp / seg.tiles, tile = warp & (seg.tiles - 1);
     // query and first head (of the KV head's) of a tile of the segment
     const auto query_of = [&](uint32_t k) { return p.share ? seg.query + k : seg.query; };
     const auto head_of = [&](uint32_t k) { return p.share ? 0 : (tile0 + k) * kPagedHeads; };
@@ -411,7 +417,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     const uint32_t seen = p.share ? lead(query_of(tile)).seen : seg.seen;
     // ---- the queries as B fragments, a head a warp at a time: column `col` of a tile's MMA ----
 #pragma unroll 1
-    for (uint32_t r = warp; r < seg.tiles * kPagedHeads; r += kPagedWarps) {
+    for (uint32_t r = warp; r < seg.tiles * kPagedHeads; r += (uint32_t)W) {
       constexpr uint32_t N = D / 32;
       const uint32_t k = r / kPagedHeads, col = r % kPagedHeads, head = head_of(k) + col;
       const T *q = (const T *)p.q + (int64_t)query_of(k) * p.q_query + (int64_t)(kv * p.group + head) * p.q_head + lane * N;
@@ -435,7 +441,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       }
       if (lane == 0) factors[k][col] = fmaxf(p.scale * inverse, 0x1p-126f);
     }
-    named_bar(1, kPagedWarps * 32);
+    named_bar(1, (uint32_t)W * 32);
     const uint32_t *my_q = q_frag + (tile * kQ * (kSteps / 2) * 32 + lane) * 4;
     const float f0 = factors[tile][2 * t], f1 = factors[tile][2 * t + 1];   // scores of heads 2t and 2t + 1 are this lane's
     stopped |= __any_sync(~0u, *(volatile uint32_t *)&gave_up);
@@ -450,7 +456,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     uint32_t steps = 0;    // steps that this warp took
     uint32_t stage = (n0 + team) % S::kStages, parity = (n0 + team) / S::kStages & 1;
 #pragma unroll 1
-    for (uint32_t b = team; b < paged_rounds(seg.blocks); b += teams) {
+    for (uint32_t b = team; b < paged_rounds<W>(seg.blocks); b += teams) {
       if (!stopped && !__all_sync(~0u, mbar_wait_bounded(&full[stage], parity))) {
         stopped = true;
         if (lane == 0) *(volatile uint32_t *)&gave_up = 1;
@@ -549,11 +555,11 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive_count(&empty[stage], teams);   // the team's T warps make up 12 arrivals
+      if (lane == 0) mbar_arrive_count(&empty[stage], teams);   // the team's T warps make up W arrivals
       stage += teams;
       if (stage >= S::kStages) stage -= S::kStages, parity ^= 1;
     }
-    n0 += paged_rounds(seg.blocks);
+    n0 += paged_rounds<W>(seg.blocks);
     if constexpr (kFresh) {
 #pragma unroll
       for (int j = 0; j < kSteps; ++j)
@@ -575,14 +581,14 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       *(float2 *)&w_max[warp][2 * t] = make_float2(m0, m1);
       *(float2 *)&w_sum[warp][2 * t] = make_float2(l0, l1);
     }
-    named_bar(1, kPagedWarps * 32);
-    // lane (head, s) looks at warps s, s + 4 and s + 8, of which those of this tile count
+    named_bar(1, (uint32_t)W * 32);
+    // lane (head, s) looks at every fourth warp from s on, of which those of this tile count
     float e0, e1;
     {
       const uint32_t h = lane / 4, s = lane % 4;
-      float m[3], l[3], top = kNoScore, all = 0.f;
+      float m[W / 4], l[W / 4], top = kNoScore, all = 0.f;
 #pragma unroll
-      for (uint32_t i = 0; i < 3; ++i) {
+      for (uint32_t i = 0; i < W / 4; ++i) {
         const uint32_t w = s + 4 * i;
         const bool mine = (w & (seg.tiles - 1)) == tile;
         m[i] = mine ? w_max[w][h] : kNoScore, l[i] = mine ? w_sum[w][h] : 0.f;
@@ -592,7 +598,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
       top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
       bool some = false;
 #pragma unroll
-      for (uint32_t i = 0; i < 3; ++i) {
+      for (uint32_t i = 0; i < W / 4; ++i) {
         some |= l[i] < 0.f;
         all += (l[i] < 0.f ? 0.f : l[i]) * exp2_fast(m[i] - top);
       }
@@ -614,7 +620,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     };
 #pragma unroll 1
     for (int h = 0; h < D / 64; ++h) {   // 64 channels at a time
-      if (h) named_bar(1, kPagedWarps * 32);
+      if (h) named_bar(1, (uint32_t)W * 32);
       const auto store = [&](const float(&x)[4], int i) {
         float *dst = merge + (warp * kPagedHeads + 2 * t) * S::kRow + 16 * i + g;
         dst[0] = e0 * x[0], dst[8] = e0 * x[2];
@@ -627,15 +633,15 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) store(o[kSteps - 4 + i], i);
       }
-      named_bar(1, kPagedWarps * 32);
+      named_bar(1, (uint32_t)W * 32);
 #pragma unroll 1
-      for (uint32_t r = warp; r < seg.tiles * kPagedHeads; r += kPagedWarps) {   // a head a warp at a time, two channels a lane
+      for (uint32_t r = warp; r < seg.tiles * kPagedHeads; r += (uint32_t)W) {   // a head a warp at a time, two channels a lane
         const uint32_t k = r / kPagedHeads, head = r % kPagedHeads;
         if (head_of(k) + head >= p.group) continue;
         float2 x = make_float2(0.f, 0.f);
         const float *src = merge + (k * kPagedHeads + head) * S::kRow + 2 * lane;
 #pragma unroll 3
-        for (uint32_t w = k; w < kPagedWarps; w += seg.tiles, src += seg.tiles * kPagedHeads * S::kRow) {
+        for (uint32_t w = k; w < (uint32_t)W; w += seg.tiles, src += seg.tiles * kPagedHeads * S::kRow) {
           const float2 y = *(const float2 *)src;
           x.x += y.x, x.y += y.y;
         }
@@ -655,15 +661,15 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
         dst[0] = f_max[0][threadIdx.x];
         dst[kPagedHeads] = f_sum[0][threadIdx.x];
       }
-      named_bar(1, kPagedWarps * 32);
+      named_bar(1, (uint32_t)W * 32);
       const uint32_t pieces = seg.parts;
       uint32_t *ticket = p.tickets + seg.query * p.lanes + seg.lane;
       if (threadIdx.x == 0) last = atomic_add_acq_rel(ticket, 1u) == pieces - 1;
-      named_bar(1, kPagedWarps * 32);
+      named_bar(1, (uint32_t)W * 32);
       if (last) {
         if (threadIdx.x == 0) *ticket = 0;
 #pragma unroll 1
-        for (uint32_t r = warp; r < seg.tiles * kPagedHeads; r += kPagedWarps) {   // a head a warp at a time
+        for (uint32_t r = warp; r < seg.tiles * kPagedHeads; r += (uint32_t)W) {   // a head a warp at a time
           const uint32_t k = r / kPagedHeads, head = r % kPagedHeads;
           if (head_of(k) + head >= p.group) continue;
           constexpr uint32_t N = D / 32;   // channels of a lane
@@ -735,7 +741,7 @@ __global__ void __launch_bounds__(kPagedThreads, 1)
     }
     if ((index += gridDim.x) >= plan.pieces) break;
     piece = paged_piece(p, plan, index, lead, cursor);
-    named_bar(1, kPagedWarps * 32);   // shared results are free for the next piece
+    named_bar(1, (uint32_t)W * 32);   // shared results are free for the next piece
   }
   if (stopped) {   // copies in flight land before the block ends; the first that does not in time was never issued
     for (uint32_t i = n0 - min(n0, S::kStages); i < n0; ++i)
