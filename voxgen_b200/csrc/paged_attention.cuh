@@ -4,10 +4,10 @@
 // The mathematics. Up to 8 query heads of a KV head are the columns of m16n8k16
 // MMAs: scores S^T = K Q^T and the output O^T = V^T P^T, cache rows as the A
 // operand. q is held in as many terms of the cache's type as its bits need (fp32:
-// two of fp16, three of bf16), P in two, three for fp32 output over a bf16 cache; so
-// products are as exact as fp32's. Statistics and sums are fp32. The tensor cores
-// add with rounding towards zero, so for fp32 queries O is summed afresh every 8
-// steps and added with rounding to nearest.
+// two of fp16, three of bf16) and P in as many as the output's; so products are as
+// exact as fp32's. Statistics and sums are fp32. The tensor cores add with rounding
+// towards zero, so for fp32 queries O is summed afresh every 8 steps and added with
+// rounding to nearest.
 //
 // The bound is bytes: 4 D of them a row for 4 D multiply-adds a head. So one warp
 // does nothing but keep copies in flight: it looks page numbers up 24 at a time and
@@ -24,10 +24,15 @@
 // so as many warps run as registers allow: 12, with q's terms read from shared memory.
 //
 // The split. Segments are cut into pieces of at most U blocks, U such that there is
-// about one piece for each CTA (4, where segments are many). The warps of
-// a piece meet in shared memory. A segment of several pieces leaves a partial result
-// for each, and the CTA that finishes last (a counter, left at zero) adds them in
-// order: sums never depend on timing.
+// about one piece for each CTA (4, where segments are many). The warps of a piece meet
+// in shared memory. A segment of several pieces leaves a partial result for each, and
+// the CTA that finishes last (a counter, left at zero) adds them in order: sums never
+// depend on timing.
+//
+// Measured: 16 contexts of 24001 to 32768 rows, bf16, 465 MB: 77 us, 6.0 TB/s (93% of
+// the measured copy rate). 16 ragged streams of 64 to 4096 rows, 34 MB: 13.7 us, of
+// which 4 stream: the rest is code that runs once, at about 7 cycles an instruction, and
+// so kept short (loops, not unrolled ones). 5 drafted tokens of those streams: 30 us.
 #pragma once
 #include <cuda.h>
 
