@@ -378,6 +378,40 @@ def test_attention_of_long_contexts(heads, kv_heads, dim, dtype, kind):
     assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("heads,dim", [(16, 128), (40, 64), (48, 128)])
+@pytest.mark.parametrize("dtype,kind", [("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("f16", "bf16"), ("bf16", "bf16")])
+def test_attention_of_hundreds_of_segments(heads, dim, dtype, kind):
+    """Enough of them for CTAs of 4 warps, with long ones that are cut, over all rows and over chosen pages."""
+    rng = np.random.default_rng(heads)
+    rows = rng.integers(0, 70, 230)
+    rows[[3, 100]] = 2500, 1300
+    cache = filled(1, rows.tolist(), 16, 2, dim, kind)
+    q = normal(2, 230, heads, dim, dtype=TYPES[dtype])
+    out = cache.attention(q)
+    check_attention(cache, q, out, dtype)
+    assert torch.equal(out, cache.attention(q))
+    chosen = cache.select(q, 7, sinks=1, recent=2)
+    check_attention(cache, q, cache.attention(q, chosen=chosen), dtype, chosen=chosen.tolist())
+
+
+@pytest.mark.parametrize("kv_heads", [1, 3])
+def test_attention_of_more_queries_than_are_planned_ahead(kv_heads):
+    """Tokens of a few sequences, in runs, past what a CTA keeps in shared memory, with and without cut segments."""
+    rng = np.random.default_rng(kv_heads)
+    rows = [4000, 10, 700]
+    cache = filled(1, rows, 32, kv_heads, 64, "f16")
+    sequences = [s for s in rng.integers(-1, 4, 400) for _ in range(rng.integers(1, 9))]
+    positions = [int(rng.integers(0, rows[s])) if 0 <= s < 3 else 5 for s in sequences]
+    assert len(sequences) > 1100
+    q = normal(3, len(sequences), 8 * kv_heads, 64, dtype=torch.float16)
+    out = cache.attention(q, sequences=ints(sequences), positions=ints(positions))
+    check_attention(cache, q, out, "f16", sequences, positions)
+    some = [i for i, s in enumerate(sequences) if s == 0][:300]     # between the two: 300 queries, CTAs of 12 warps for 1 KV head
+    at = torch.tensor(some, device="cuda")
+    out = cache.attention(q[at], sequences=ints(sequences)[at], positions=ints(positions)[at])
+    check_attention(cache, q[at], out, "f16", [sequences[i] for i in some], [positions[i] for i in some])
+
+
 def test_attention_of_many_drafts():
     """More segments than CTAs, so that a CTA's pieces differ in their tiles."""
     rng = np.random.default_rng(1)

@@ -13,13 +13,13 @@
 // order of channels within a contraction is free), three terms of the weights are
 // columns of B, and a fourth column times |A| is the sum of magnitudes that bounds the
 // error. The cluster's first CTA finds the border by a histogram over 2048 equal parts
-// of the scores' range. Pages above the border by more than the error are taken, those
-// below it by more are not, and the few in between are scored again, in 64 bits, and
-// ranked (fp16 and bf16 become doubles by moving bits: a half's bits, shifted, are the
+// of the scores' range. Pages above the border's part by more than the error are taken,
+// those below it by more are not, and the few in between are listed and ranked; where
+// one of them is nearer to the last taken one than the error, in 64 bits (fp16 and bf16 become doubles by moving bits: a half's bits, shifted, are the
 // double's but for a power of two). Where more than 512 are in between (ties, scores
 // that overflow 32 bits), all pages are scored in 64 bits. Equal scores go to the lowest
 // page. Measured: 8192 pages for 32 heads (134 MB of summaries): 34 us, 49 in 64 bits
-// alone; 2048 pages for one query: 9.4 us, bound by steps that depend on each other and
+// alone; 2048 pages for one query: 7.5 us, bound by steps that depend on each other and
 // by code that runs once.
 #pragma once
 #include <type_traits>
@@ -98,36 +98,16 @@ __global__ void __launch_bounds__(kSelectThreads, 1) paged_select_kernel(const P
   __shared__ unsigned long long list_keys[kSelectRanked];
   __shared__ uint32_t list_at[kSelectRanked];
   __shared__ uint32_t w_sum[kSelectWarps];
-  __shared__ uint32_t found_bin, found_above, found_count, listed, top_weight;
+  __shared__ uint32_t found_bin, found_above, found_count, listed, top_weight, border;
   const PagedTable &t = p.c.t;
   const uint32_t tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const uint32_t ctas = cluster_size(), rank = cluster_rank(), item = blockIdx.x / ctas;
   const uint32_t query = item / p.c.kv_heads, head = item - query * p.c.kv_heads;
   if (tid == 0) top_weight = 0;
   __syncthreads();
+  cluster_arrive();   // waited for where the first CTA's shared memory is first written
   pdl_launch_dependents();
   pdl_wait();
-  const PagedSeen who = paged_seen(t, p.which, query);
-  const uint32_t count = (who.seen + t.page_rows() - 1) >> t.shift;
-  int32_t *out = p.chosen + (size_t)item * p.budget;
-  if (count <= p.budget) {   // all of them; the whole cluster leaves
-    if (rank == 0)
-      for (uint32_t i = tid; i < p.budget; i += kSelectThreads) out[i] = i < count ? (int32_t)i : -1;
-    return;
-  }
-  const uint32_t n = count - p.sinks - p.recent, want = p.budget - p.sinks - p.recent;   // candidates: more than wanted
-  if (want == 0) {   // likewise
-    if (rank == 0) {
-      for (uint32_t i = tid; i < p.sinks; i += kSelectThreads) out[i] = (int32_t)i;
-      for (uint32_t i = tid; i < p.recent; i += kSelectThreads) out[p.sinks + i] = (int32_t)(count - p.recent + i);
-    }
-    return;
-  }
-  // the first pages that this warp scores, asked for early
-  const int32_t *table = t.table + (size_t)who.seq * t.seq_pages + p.sinks;
-  const uint32_t stride = ctas * kSelectWarps * 16;
-  const auto pages_at = [&](uint32_t base) { return lane < 16 && base + lane < n ? (uint32_t)table[base + lane] : ~0u; };
-  uint32_t base = (rank * kSelectWarps + warp) * 16, ahead = pages_at(base);
   // ---- weights ----
   if (tid < D) {
     const T *q = (const T *)p.q + (int64_t)query * p.q_query + (int64_t)head * p.group * p.q_head + tid;
@@ -143,6 +123,29 @@ __global__ void __launch_bounds__(kSelectThreads, 1) paged_select_kernel(const P
     const uint32_t top = __reduce_max_sync(~0u, __float_as_uint(most));
     if (lane == 0) atomicMax(&top_weight, top);
   }
+  const PagedSeen who = paged_seen(t, p.which, query);
+  const uint32_t count = (who.seen + t.page_rows() - 1) >> t.shift;
+  int32_t *out = p.chosen + (size_t)item * p.budget;
+  if (count <= p.budget) {   // all of them; the whole cluster leaves
+    cluster_wait();
+    if (rank == 0)
+      for (uint32_t i = tid; i < p.budget; i += kSelectThreads) out[i] = i < count ? (int32_t)i : -1;
+    return;
+  }
+  const uint32_t n = count - p.sinks - p.recent, want = p.budget - p.sinks - p.recent;   // candidates: more than wanted
+  if (want == 0) {   // likewise
+    cluster_wait();
+    if (rank == 0) {
+      for (uint32_t i = tid; i < p.sinks; i += kSelectThreads) out[i] = (int32_t)i;
+      for (uint32_t i = tid; i < p.recent; i += kSelectThreads) out[p.sinks + i] = (int32_t)(count - p.recent + i);
+    }
+    return;
+  }
+  // the first pages that this warp scores, asked for early
+  const int32_t *table = t.table + (size_t)who.seq * t.seq_pages + p.sinks;
+  const uint32_t stride = ctas * kSelectWarps * 16;
+  const auto pages_at = [&](uint32_t base) { return lane < 16 && base + lane < n ? (uint32_t)table[base + lane] : ~0u; };
+  uint32_t base = (rank * kSelectWarps + warp) * 16, ahead = pages_at(base);
   __syncthreads();
   float inverse;
   const float power = row_power(__uint_as_float(top_weight), inverse);   // brings the largest weight to [2^14, 2^15)
@@ -158,12 +161,13 @@ __global__ void __launch_bounds__(kSelectThreads, 1) paged_select_kernel(const P
 #pragma unroll
     for (int k = 4; k < 8; ++k) frag[at][k * 4 + in][c % 4 / 2] = 0;
   }
-  cluster_sync();   // the fragments are there, and so is the CTA that the keys go to
+  __syncthreads();
   // ---- scores in 32 bits: 16 pages a warp ----
   const uint32_t g = lane / 4, t4 = lane % 4;
   {
     const uint32_t there = remote_smem(keys, 0);
     uint32_t low = ~0u, high = 0, most = 0;
+    cluster_wait();   // the CTA that the keys go to has started
     for (; base < n; base += stride) {
       const uint32_t page = ahead;
       ahead = pages_at(base + stride);
@@ -265,7 +269,7 @@ __global__ void __launch_bounds__(kSelectThreads, 1) paged_select_kernel(const P
       if (lane == 0) taken[i / 32] = more, same[i / 32] = list ? 0 : marked;
       if (list && in) {
         const uint32_t at = atomicAdd(&listed, 1u);
-        if (at < kSelectRanked) list_at[at] = i;
+        if (at < kSelectRanked) list_at[at] = i, list_keys[at] = k;
       }
     }
     __syncthreads();
@@ -299,17 +303,15 @@ __global__ void __launch_bounds__(kSelectThreads, 1) paged_select_kernel(const P
     part(from, to, true, key);
     exact = listed > kSelectRanked;
   }
-  // ---- scores in 64 bits, of the listed ones or of all: a warp takes 8 pages at a time, a lane 16 bytes of a summary ----
-  unsigned long long *wide = exact ? (unsigned long long *)select_smem : list_keys;
-  const uint32_t rescored = exact ? n : listed;
-  __syncthreads();
-  {
+  // Scores in 64 bits, of `count` pages, listed or the first: a warp takes 8 pages at a time, a lane 16 bytes of a summary.
+  const auto score = [&](uint32_t count, const uint32_t *list, unsigned long long *dst) {
+    __syncthreads();
     constexpr uint32_t L = 2 * D / 8, kPer = 32 / L;   // lanes of a summary, summaries of a warp's load
     constexpr uint32_t kBatch = 8, step = kBatch * kPer;
     const uint32_t piece = lane % L, sub = lane / L;
-    for (uint32_t from = warp * step; from < rescored; from += kSelectWarps * step) {
+    for (uint32_t from = warp * step; from < count; from += kSelectWarps * step) {
       uint32_t page = ~0u;
-      if (lane < step && from + lane < rescored) page = (uint32_t)table[exact ? from + lane : list_at[from + lane]];
+      if (lane < step && from + lane < count) page = (uint32_t)table[list ? list[from + lane] : from + lane];
       double s[kBatch];
 #pragma unroll
       for (uint32_t i = 0; i < kBatch; ++i) {
@@ -340,14 +342,15 @@ __global__ void __launch_bounds__(kSelectThreads, 1) paged_select_kernel(const P
       for (uint32_t o = 8; o < L; o <<= 1) s[0] += __shfl_xor_sync(~0u, s[0], o);
       // this lane's sum is of batch (lane & 1) * 4 + (lane & 2) + (lane & 4) / 4
       const uint32_t i = from + ((lane & 1) * 4 + (lane & 2) + (lane & 4) / 4) * kPer + sub;
-      if (piece < 8 && i < rescored) wide[i] = ordered(s[0]);
+      if (piece < 8 && i < count) dst[i] = ordered(s[0]);
     }
-  }
-  __syncthreads();
+    __syncthreads();
+  };
   // ---- without a list: the border in 64 bits ----
-  uint32_t listed_now = listed;
   if (exact) {
-    const auto key = [&](uint32_t i) { return wide[i]; };
+    unsigned long long *all_keys = (unsigned long long *)select_smem;
+    score(n, nullptr, all_keys);
+    const auto key = [&](uint32_t i) { return all_keys[i]; };
     unsigned long long from = 0, to = ~0ull;
     left = want;
     for (;;) {
@@ -355,14 +358,11 @@ __global__ void __launch_bounds__(kSelectThreads, 1) paged_select_kernel(const P
       const uint32_t in = narrow(from, to, left, shift, key);
       if (in <= kSelectRanked || shift == 0) break;
     }
-    __syncthreads();
     if (tid == 0) listed = 0;
     __syncthreads();
     part(from, to, found_count <= kSelectRanked, key);
-    listed_now = listed;
-    if (tid < listed_now) list_keys[tid] = wide[list_at[tid]];
-    __syncthreads();
   }
+  const uint32_t listed_now = listed;
   // ---- how many of the listed or marked ones are taken ----
   const uint32_t words = (n + 31) / 32;   // two a thread
   uint32_t two[2], all;
@@ -370,14 +370,23 @@ __global__ void __launch_bounds__(kSelectThreads, 1) paged_select_kernel(const P
   for (uint32_t i = 0; i < 2; ++i) two[i] = 2 * tid + i < words ? taken[2 * tid + i] : 0;
   sums_before(__popc(two[0]) + __popc(two[1]), all);
   left = want - all;
-  if (tid < listed_now) {
-    const unsigned long long k = list_keys[tid];
-    const uint32_t at = list_at[tid];
-    uint32_t before = 0;
+  // the listed ones are ranked by their scores in 32 bits; where one is nearer to the border than twice the error, in 64
+  uint32_t before = 0;
+  for (bool sure = exact;; sure = true) {
+    const unsigned long long k = tid < listed_now ? list_keys[tid] : 0;
+    const uint32_t at = tid < listed_now ? list_at[tid] : 0;
+    before = 0;
 #pragma unroll 4
     for (uint32_t i = 0; i < listed_now; ++i) before += list_keys[i] > k || (list_keys[i] == k && list_at[i] < at);
-    if (before < left) atomicOr(&taken[at / 32], 1u << at % 32);
+    if (sure) break;
+    const bool is_border = tid < listed_now && before == left - 1;
+    if (is_border) border = (uint32_t)k;
+    __syncthreads();
+    const float away = fabsf(unordered((uint32_t)k) - unordered(border));
+    if (!__syncthreads_or(tid < listed_now && !is_border && away <= 2.001f * error)) break;
+    score(listed_now, list_at, list_keys);
   }
+  if (tid < listed_now && before < left) atomicOr(&taken[list_at[tid] / 32], 1u << list_at[tid] % 32);
   __syncthreads();
 #pragma unroll
   for (uint32_t i = 0; i < 2; ++i) two[i] = 2 * tid + i < words ? taken[2 * tid + i] : 0;
