@@ -280,8 +280,9 @@ class PagedCache:
         if q.dim() != 3:
             raise _invalid("q: expected [queries, heads, head_dim]")
         n, heads, _ = q.shape
-        return (n, heads, self._rows_of(q, heads, "q"), _ints(sequences, (n,), self.device, "sequences"),
-                _ints(positions, (n,), self.device, "positions"))
+        return (n, heads, self._rows_of(q, heads, "q"),
+                None if sequences is None else _ints(sequences, (n,), self.device, "sequences"),
+                None if positions is None else _ints(positions, (n,), self.device, "positions"))
 
     @_on_its_device
     def select(self, q: torch.Tensor, budget: int, *, sinks: int = 0, recent: int = 1,
@@ -353,8 +354,9 @@ class PagedCache:
         rows of these pages of the sequence. ``scale`` is 1/sqrt(head_dim) by default. ``out`` does not overlap ``q``."""
         ref = self._layer(layer)
         n, heads, dtype, sequences, positions = self._queries(q, sequences, positions)
+        strides = self._strides(q)
         if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            out = torch.empty_like(q) if strides is None else torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != self.device or not out.is_contiguous():
             raise _invalid("out must be contiguous and like q")
         budget, pages = 0, None
@@ -365,7 +367,7 @@ class PagedCache:
             return out
         ws = self._work(n, heads, budget)
         rc = self._lib.vg_k_paged_attention(
-            ref, q.data_ptr(), dtype, n, heads, self._strides(q), sequences, positions, pages, budget,
+            ref, q.data_ptr(), dtype, n, heads, strides, sequences, positions, pages, budget,
             self._scale if scale is None else scale, out.data_ptr(), ws.data_ptr(), ws.numel(), _current_stream(self._index))
         if rc:
             raise VoxGenError(rc, f"attention of {n} queries of {heads} heads on {self.kv_heads} KV heads, {self.table.seqs} "
