@@ -24,12 +24,12 @@
 // so as many warps run as registers allow: 12, with q's terms read from shared memory.
 //
 // The split. Segments are cut into pieces of at most U blocks, U such that there is
-// about one piece for each CTA (4, where segments are many). The warps of a piece meet
-// in shared memory. A segment of several pieces leaves a partial result for each, and
+// about one piece for each CTA (up to 4, where segments are many). The warps of a piece
+// meet in shared memory. A segment of several pieces leaves a partial result for each, and
 // the CTA that finishes last (a counter, left at zero) adds them in order: sums never
 // depend on timing.
 //
-// Measured: 16 contexts of 24001 to 32768 rows, bf16, 465 MB: 77 us, 6.0 TB/s (93% of
+// Measured: 16 contexts of 24001 to 32768 rows, bf16, 465 MB: 78 us, 6.0 TB/s (91% of
 // the measured copy rate). 16 ragged streams of 64 to 4096 rows, 34 MB: 13.7 us, of
 // which 4 stream: the rest is code that runs once, at about 7 cycles an instruction, and
 // so kept short (loops, not unrolled ones). 5 drafted tokens of those streams: 30 us.
@@ -95,10 +95,11 @@ struct PagedSmem {
   static constexpr uint32_t kBytes = kRing + kShared + 1024;   // the ring starts on a multiple of 1024
 };
 
-// Pieces that a call is cut into, about, and the partial results that it may leave: a segment that is cut at all has fewer
-// than twice its share of the target in pieces.
+// Pieces that a call is cut into, about: one for each CTA, or up to 4, so that there are a third more than segments. And the
+// partial results that it may leave: a segment that is cut at all has fewer than twice its share of the target in pieces.
 __host__ __device__ __forceinline__ uint32_t paged_target(uint32_t segments, uint32_t ctas) {
-  return ctas * (segments * 4 <= ctas * 3 ? 1 : 4);
+  const uint32_t rounds = (segments * 4 + ctas * 3 - 1) / (ctas * 3);   // segments: no more than kPagedTickets
+  return ctas * (rounds < 1 ? 1 : rounds > 4 ? 4 : rounds);
 }
 __host__ __device__ __forceinline__ uint32_t paged_slots(uint64_t segments, uint32_t ctas) {
   return segments > kPagedTickets ? 0 : 2 * paged_target((uint32_t)segments, ctas);
@@ -196,10 +197,10 @@ __device__ __forceinline__ PagedPlan paged_plan(const PagedAttnParams &p, PagedL
   if (p.queries * p.lanes > kPagedTickets) return PagedPlan{kPagedUncut, segments};   // one piece a segment
   const uint32_t target = paged_target(segments, gridDim.x);
   // total / target would do if nothing were rounded up; total / (target - segments) makes no more than target pieces. Of eight
-  // sizes from the one to the other the least with no more pieces than the target is taken. Where a CTA has several pieces
-  // anyway, it is the first.
+  // sizes from the one to the other the least with no more pieces than the target is taken. Where there are more segments
+  // than that, it is the first.
   const uint32_t least = max(blockDim.x / 32 - 1, paged_over(total, target));   // a round of the warps
-  const uint32_t more = target == gridDim.x ? max(least, paged_over(total, target - segments)) - least : 0;
+  const uint32_t more = target > segments ? max(least, paged_over(total, target - segments)) - least : 0;
   const uint32_t k = lane / 4, size = least + (k == 7 ? more : more * k * k / 49);
   uint32_t n = 0;
 #pragma unroll 1
@@ -727,12 +728,19 @@ __global__ void __launch_bounds__((W + 1) * 32, W == kPagedWarps ? 1 : 2)
               }
             }
             const uint32_t end = min(32u, pieces - at);
-#pragma unroll 8
-            for (; i < end; ++i) {
-              const Values v = values(at + i);
-              const float wi = __shfl_sync(~0u, w, i);
+            constexpr uint32_t kTogether = 8;   // loads in flight; 16 take registers from the steps
+#pragma unroll 1
+            for (; i < end; i += kTogether) {
+              Values v[kTogether];
 #pragma unroll
-              for (uint32_t n = 0; n < N; ++n) x.x[n] = fmaf(wi, v.x[n], x.x[n]);
+              for (uint32_t u = 0; u < kTogether; ++u) v[u] = values(at + min(i + u, end - 1));
+#pragma unroll
+              for (uint32_t u = 0; u < kTogether; ++u) {
+                const float wi = __shfl_sync(~0u, w, (i + u) & 31);
+#pragma unroll
+                for (uint32_t n = 0; n < N; ++n)
+                  if (i + u < end) x.x[n] = fmaf(wi, v[u].x[n], x.x[n]);
+              }
             }
           }
 #pragma unroll
