@@ -600,6 +600,9 @@ int vg_k_paged_select(const vg_paged_cache *cache, const void *q, int dtype, uin
  * there some other way may give NaN). Results do not depend on timing: every sum has a
  * fixed order. out and q do not overlap.
  *
+ * queries * kv_heads * blocks of 16 rows (of seq_pages, or of budget pages) stay below
+ * 2^31 (VG_ERANGE; more than 8 heads to a KV head count 2 or 4 times).
+ *
  * workspace: vg_k_paged_attention_bytes() bytes (budget 0: no list), 16-byte aligned,
  * zero-filled once before its first use; calls leave it ready for the next call of any
  * shape it is large enough for. */

@@ -156,7 +156,7 @@ def test_attention_bytes():
     assert rc == OK and few == 4 * (1 << 14) + 2 * 148 * 4 * 8 * 130 * 4
     # many segments: as many partial results, however many they are; none where no segment is cut
     big = table(seqs=4096)
-    assert attention_bytes(cache(big), queries=300)[1] == attention_bytes(cache(big), queries=4000)[1] > few
+    assert attention_bytes(cache(big), queries=500)[1] == attention_bytes(cache(big), queries=4000)[1] > few
     assert attention_bytes(cache(big), queries=100000)[1] == 4 * (1 << 14)
     assert attention_bytes(queries=0)[0] == EINVAL and attention_bytes(heads=15)[0] == EINVAL
     assert attention_bytes(cache(table(seqs=4096, seq_pages=1 << 24)), queries=4096)[0] == ERANGE

@@ -135,17 +135,17 @@ int queries_of(const PagedView &c, uint32_t head_dim, const void *q, int dtype, 
 constexpr uint64_t kPagedTicketBytes = kPagedTickets * 4;
 // How the tiles of 8 heads of a KV head make segments.
 struct Tiling {
-  uint32_t head_tiles, tiles, lanes;   // of a KV head, of a segment (1, 2 or 4), segments of a query
+  uint32_t tiles, lanes;               // of a segment (1, 2 or 4), segments of a query
   uint32_t warps;                      // consumer warps of a CTA
   bool share;                          // consecutive queries of a sequence may make one segment
 };
 Tiling tiling_of(uint32_t kv_heads, uint32_t heads, uint32_t queries, uint32_t budget) {
   Tiling x{};
-  x.head_tiles = (heads / kv_heads + kPagedHeads - 1) / kPagedHeads;
-  x.share = x.head_tiles == 1 && !budget;   // lists of pages differ from query to query
+  const uint32_t head_tiles = (heads / kv_heads + kPagedHeads - 1) / kPagedHeads;   // of a KV head
+  x.share = head_tiles == 1 && !budget;   // lists of pages differ from query to query
   x.tiles = 1;
-  while (x.tiles < kPagedTiles && x.tiles < x.head_tiles) x.tiles *= 2;
-  x.lanes = kv_heads * ((x.head_tiles + kPagedTiles - 1) / kPagedTiles);
+  while (x.tiles < kPagedTiles && x.tiles < head_tiles) x.tiles *= 2;
+  x.lanes = kv_heads * ((head_tiles + kPagedTiles - 1) / kPagedTiles);
   x.warps = (uint64_t)queries * x.lanes < kPagedMany ? kPagedWarps : kPagedFew;
   return x;
 }
@@ -292,9 +292,10 @@ int vg_k_paged_attention_bytes(const vg_paged_cache *cache, uint32_t queries, ui
   const uint64_t segments = (uint64_t)queries * x.lanes;
   const uint64_t blocks = (uint64_t)(budget ? budget : c.t.seq_pages) << (c.t.shift - 4);   // of a segment, at most
   const uint64_t cost = segments * blocks * x.tiles;
-  if (x.lanes > 1u << 16 || segments > kMaxGrid || blocks > kPagedMost || cost > kMaxGrid) return VG_ERANGE;   // the plan counts in 32 bits
-  *bytes = kPagedTicketBytes +
-           (uint64_t)paged_slots(segments, paged_ctas(x.warps)) * (x.share ? kPagedTiles : x.tiles) * kPagedHeads * (cache->head_dim + 2) * 4;
+  if (x.lanes > 1u << 16 || segments > kMaxGrid || blocks > kPagedMost || cost > kMaxGrid)
+    return VG_ERANGE;   // the plan counts in 32 bits
+  const uint64_t parts = (uint64_t)paged_slots(segments, paged_ctas(x.warps)) * (x.share ? kPagedTiles : x.tiles);
+  *bytes = kPagedTicketBytes + parts * kPagedHeads * (cache->head_dim + 2) * 4;
   return VG_OK;
 }
 
@@ -327,7 +328,6 @@ int vg_k_paged_attention(const vg_paged_cache *cache, const void *q, int dtype, 
   p.heads = heads;
   p.group = x.group;
   const Tiling tiling = tiling_of(c.kv_heads, heads, queries, budget);
-  p.head_tiles = tiling.head_tiles;
   p.share = tiling.share && sequences;   // else every query is of its own sequence
   p.tiles = p.share ? kPagedTiles : tiling.tiles;
   p.lanes = tiling.lanes;

@@ -54,7 +54,6 @@ struct PagedAttnParams {
   const int32_t *chosen;     // [queries][kv_heads][budget] pages of each (query, KV head), or null: all
   uint32_t budget;
   uint32_t queries, heads, group;
-  uint32_t head_tiles;       // of 8 heads, of a KV head
   uint32_t share;            // consecutive queries of a sequence share what they read
   uint32_t tiles;            // most tiles of a segment (a power of two); of each segment, where queries do not share
   uint32_t lanes;            // segments of a query
@@ -366,8 +365,9 @@ __global__ void __launch_bounds__((W + 1) * 32, W == kPagedWarps ? 1 : 2)
         const Found now = next;
         next = find(i + kLook + lane);
 #pragma unroll 1
-        for (uint32_t j = 0; j < kLook && i + j < x.blocks; j += (uint32_t)W) {   // whole rounds: stages past the last block hold nothing
-          const uint32_t from = j + lane % (uint32_t)W, page = __shfl_sync(~0u, now.page, from), row = __shfl_sync(~0u, now.row, from);
+        for (uint32_t j = 0; j < kLook && i + j < x.blocks; j += W) {   // whole rounds: stages past the last block hold nothing
+          const uint32_t from = j + lane % W;
+          const uint32_t page = __shfl_sync(~0u, now.page, from), row = __shfl_sync(~0u, now.row, from);
           bool in = true;
           if (lane < (uint32_t)W) {
             const uint32_t n = n0 + i + j + lane, stage = n % S::kStages, turn = n / S::kStages;

@@ -15,9 +15,10 @@
 // error. The cluster's first CTA finds the border by a histogram over 2048 equal parts
 // of the scores' range. Pages above the border's part by more than the error are taken,
 // those below it by more are not, and the few in between are listed and ranked; where
-// one of them is nearer to the last taken one than the error, in 64 bits (fp16 and bf16 become doubles by moving bits: a half's bits, shifted, are the
-// double's but for a power of two). Where more than 512 are in between (ties, scores
-// that overflow 32 bits), all pages are scored in 64 bits. Equal scores go to the lowest
+// one of them is nearer to the last taken one than the error, in 64 bits (fp16 and bf16
+// become doubles by moving bits: a half's bits, shifted, are the double's but for a power
+// of two). Where more than 512 are in between (ties, scores that overflow 32 bits), all
+// pages are scored in 64 bits. Equal scores go to the lowest
 // page. Measured: 8192 pages for 32 heads (134 MB of summaries): 34 us, 49 in 64 bits
 // alone; 2048 pages for one query: 7.5 us, bound by steps that depend on each other and
 // by code that runs once.
@@ -94,7 +95,7 @@ __global__ void __launch_bounds__(kSelectThreads, 1) paged_select_kernel(const P
   __shared__ __align__(8) uint32_t frag[kSteps][32][2];     // B fragments: three terms and the magnitudes, columns of 0
   __shared__ __align__(16) uint32_t bins[kSelectBins];
   __shared__ uint32_t taken[kSelectPages / 32], same[kSelectPages / 32];   // a bit a key
-  __shared__ unsigned long long reach[8 * kSelectWarps], size[8 * kSelectWarps];   // of the cluster's warps: extremes of keys, magnitudes
+  __shared__ unsigned long long reach[8 * kSelectWarps], size[8 * kSelectWarps];   // of the cluster's warps: keys, magnitudes
   __shared__ unsigned long long list_keys[kSelectRanked];
   __shared__ uint32_t list_at[kSelectRanked];
   __shared__ uint32_t w_sum[kSelectWarps];
