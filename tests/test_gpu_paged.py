@@ -679,6 +679,25 @@ def test_a_serving_loop():
     assert refused
 
 
+@pytest.mark.parametrize("budget", [None, 2])
+@pytest.mark.parametrize("pages", [64, 9])
+def test_the_serving_example(budget, pages):
+    """Every request gets its tokens and all pages come back, also where requests have to wait for pages; with all pages
+    attended, a request's tokens do not depend on what else is served."""
+    import sys
+    from pathlib import Path
+    sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "examples"))
+    import paged_serving
+    rng = np.random.default_rng(3)
+    prompts = [rng.integers(0, 500, n).tolist() for n in (3, 40, 17, 60, 1, 33, 90)]
+    answers, table = paged_serving.serve(prompts, new=9, pages=pages, budget=budget)
+    assert [len(x) for x in answers] == [9] * 7 and table.pool.tolist() == [pages, 0] and not table.rows.any()
+    if budget is None:
+        for i in (0, 3, 6):
+            alone, _ = paged_serving.serve(prompts[i:i + 1], new=9)
+            assert alone[0][:4] == answers[i][:4]      # greedy choices between near scores may part later
+
+
 def test_a_captured_loop_replays():
     """A decode step captured once and replayed gives what eager calls give, bit for bit."""
     def build():
