@@ -53,3 +53,32 @@ def test_weights_are_held_to_32_bits(kind, dtype):
     size = (u[:, None] + w[:, :, None] * v1[:, None].abs() + v2[:, None].abs()) / total
     worst = (((out - want).abs() - half_step(want, dtype)) / size).max()
     assert worst <= 2.0 ** -19, float(worst.log2())
+
+
+@pytest.mark.parametrize("dtype,kind", [("f16", "f16"), ("bf16", "bf16"), ("bf16", "f16"), ("f16", "bf16"), ("f32", "f16")])
+def test_sums_of_long_pieces_have_no_bias(dtype, kind):
+    """More segments than are cut, 4 tokens each, over 131072 rows: one warp adds all of them. The second half of the rows
+    holds the first half's K and its V with the other sign, so outputs are 0, and sums that are cut towards zero on their way up
+    and down again are not.
+
+    Bound, in terms of A = sum(p |v|): a sum is taken afresh after at most 96 products (32 steps of up to three terms), each
+    cut at 2^-22 of what that sum has seen, 2^-15.4 A in all; the 256 sums of an output are added with roundings of 2^-24, 2^-16 A;
+    weights of equal rows are equal. 2^-14.5 is allowed. (Summed in one, the 16384 products of two terms leave 2^-13.7.)"""
+    half, n, heads, dim = 1 << 16, (1 << 14) + 4, 8, 64
+    t = TYPES[kind]
+    b = (uniform(1, half) * 256).floor() / 256
+    u = (1 + uniform(2, half, dim)).to(t).double()
+    k = torch.zeros(2 * half, 1, dim, dtype=torch.float64)
+    k[:, 0, 0] = torch.cat((b, b))
+    v = torch.cat((u, -u))[:, None]
+    table = shuffled(1, 2 * half // 256, 256, 2 * half // 256)
+    cache = paged.PagedCache(table, 1, dim, dtype=t)
+    cache.append(table.step(ints([2 * half]), 2 * half), k.float().cuda(), v.float().cuda())
+    a = 1 + torch.arange(heads).double() / heads
+    q = torch.zeros(n, heads, dim, dtype=TYPES[dtype])
+    q[:, :, 0] = a.to(q.dtype)
+    out = cache.attention(q.cuda(), sequences=ints([0] * n), scale=1.0).double().cpu()
+    p = (a[:, None] * b).exp()
+    size = p @ u / p.sum(1, keepdim=True)
+    worst = (out.abs() / size).max()
+    assert worst <= 2.0 ** -14.5, float(worst.log2())

@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/voxgen_cuda.h"
 #include "entry.cuh"
@@ -150,6 +151,10 @@ Tiling tiling_of(uint32_t kv_heads, uint32_t heads, uint32_t queries, uint32_t b
   return x;
 }
 
+uint64_t blocks_of(const PagedTable &t, uint32_t budget) {   // of a segment, at most
+  return (uint64_t)(budget ? budget : t.seq_pages) << (t.shift - 4);
+}
+
 }  // namespace
 
 extern "C" {
@@ -290,7 +295,7 @@ int vg_k_paged_attention_bytes(const vg_paged_cache *cache, uint32_t queries, ui
   if (!bytes || !queries || !heads || heads % cache->kv_heads) return VG_EINVAL;
   const Tiling x = tiling_of(c.kv_heads, heads, queries, budget);
   const uint64_t segments = (uint64_t)queries * x.lanes;
-  const uint64_t blocks = (uint64_t)(budget ? budget : c.t.seq_pages) << (c.t.shift - 4);   // of a segment, at most
+  const uint64_t blocks = blocks_of(c.t, budget);
   const uint64_t cost = segments * blocks * x.tiles;
   if (x.lanes > 1u << 16 || segments > kMaxGrid || blocks > kPagedMost || cost > kMaxGrid)
     return VG_ERANGE;   // the plan counts in 32 bits
@@ -331,6 +336,7 @@ int vg_k_paged_attention(const vg_paged_cache *cache, const void *q, int dtype, 
   p.share = tiling.share && sequences;   // else every query is of its own sequence
   p.tiles = p.share ? kPagedTiles : tiling.tiles;
   p.lanes = tiling.lanes;
+  const uint64_t blocks = blocks_of(c.t, budget);
   p.scale = scale * 1.44269504088896340736f;
   p.tickets = (uint32_t *)workspace;
   p.parts = (float *)((uint8_t *)workspace + kPagedTicketBytes);
@@ -342,15 +348,22 @@ int vg_k_paged_attention(const vg_paged_cache *cache, const void *q, int dtype, 
       using T = decltype(t);
       return by_cache_type(cache->dtype, [&](auto ct) {
         using C = decltype(ct);
-        const auto go = [&](auto w) {
+        const auto go = [&](auto w, auto fresh) {
           constexpr int W = decltype(w)::value;
           using S = PagedSmem<D, W, kQTerms<T, C>>;
-          const auto fn = paged_attention_kernel<D, T, C, W>;
+          const auto fn = paged_attention_kernel<D, T, C, W, decltype(fresh)::value>;
           static std::atomic<uint64_t> done;
           const int e = allow_smem((const void *)fn, S::kBytes, done);
           return e ? e : launch(fn, paged_ctas(W), 1, (W + 1) * 32, S::kBytes, cuda_stream, p, map);
         };
-        return tiling.warps == kPagedWarps ? go(Dim<(int)kPagedWarps>{}) : go(Dim<(int)kPagedFew>{});
+        const auto sums = [&](auto w) {
+          const uint32_t teams = (uint32_t)decltype(w)::value / p.tiles;   // warps that share a piece's blocks, at least
+          if constexpr (sizeof(T) == 2) {
+            if ((blocks + teams - 1) / teams * kPTerms<C> <= kPagedProducts) return go(w, std::false_type{});
+          }
+          return go(w, std::true_type{});
+        };
+        return tiling.warps == kPagedWarps ? sums(Dim<(int)kPagedWarps>{}) : sums(Dim<(int)kPagedFew>{});
       });
     });
   });

@@ -6,8 +6,8 @@
 // operand. q is held in as many terms of the cache's type as its bits need (fp32:
 // two of fp16, three of bf16), and P in two of fp16 or three of bf16; so products are
 // as exact as fp32's. Statistics and sums are fp32. The tensor cores add with rounding
-// towards zero, so for fp32 queries O is summed afresh every 8 steps and added with
-// rounding to nearest.
+// towards zero, so O is summed afresh every 8 steps (fp32 queries) or 32 (others, where
+// a warp's steps may be many) and added with rounding to nearest.
 //
 // The bound is bytes: 4 D of them a row for 4 D multiply-adds a head. So one warp
 // does nothing but keep copies in flight: it looks page numbers up 24 at a time and
@@ -294,19 +294,25 @@ constexpr int kQTerms = std::is_same<C, __half>::value ? (sizeof(T) == 4 ? 2 : 1
 // bf16 (77.3 us, 77.4 with two) or 4096 chosen rows of each (20.8 us with either).
 template <typename C>
 constexpr int kPTerms = std::is_same<C, __half>::value ? 2 : 3;
+// Products that a warp adds to O for 16-bit queries before it has to be summed afresh: each is cut by 2^-24 of the sum on
+// average, 2^-15 for all of them, where an fp16 output is rounded by up to 2^-12. (One warp that added 131072 rows left 2^-13 of
+// sum(p |v|).) Kernels that sum afresh take as long for long contexts (16 of 32768 rows 76.9 us, 77.2 without), but for drafts
+// of 5 tokens 31.4 us, 30.1 without, and for 64 tokens of 16 streams 396, 374 without: so where no context is that long they
+// are not taken.
+constexpr uint32_t kPagedProducts = 512;
+
 // P is held times 2^6 in fp16, for the range below a weight of 1 (kv4_rows_attention.cuh); bf16 has range enough.
 template <typename C>
 constexpr float kPagedPScale = std::is_same<C, __half>::value ? kPScale : 0.f;
 
-template <int D, typename T, typename C, int W>
+template <int D, typename T, typename C, int W, bool kFresh>   // kFresh: O is summed afresh
 __global__ void __launch_bounds__((W + 1) * 32, W == kPagedWarps ? 1 : 2)
     paged_attention_kernel(const __grid_constant__ PagedAttnParams p, const __grid_constant__ CUtensorMap map) {
   constexpr int kSteps = D / 16;                // k-steps of a score, and m-tiles of the output
   constexpr int kQ = kQTerms<T, C>, kP = kPTerms<C>;
   using S = PagedSmem<D, W, kQ>;
   constexpr uint32_t kLook = 32 / W * W;        // blocks whose pages are looked up at once
-  constexpr bool kFresh = sizeof(T) == 4;       // O summed afresh
-  constexpr uint32_t kFreshSteps = 8;
+  constexpr uint32_t kFreshSteps = sizeof(T) == 4 ? 8 : 32;
   extern __shared__ __align__(128) uint8_t paged_smem[];
   __shared__ uint64_t full[S::kStages], empty[S::kStages];
   __shared__ uint32_t first_row[S::kStages];    // of a stage's block in its sequence; past every row: nothing was read
