@@ -345,6 +345,7 @@ __global__ void __launch_bounds__((W + 1) * 32, W == kPagedWarps ? 1 : 2)
   if (warp == (uint32_t)W) {
     // ================= the copying warp =================
     uint32_t n0 = 0;           // blocks of the pieces before
+    uint32_t issued = lane;    // the number after the last that this lane issued: it issues lane, lane + W, ...
     bool stopped = false;
 #pragma unroll 1
     for (uint32_t index = blockIdx.x; !stopped;) {
@@ -381,6 +382,7 @@ __global__ void __launch_bounds__((W + 1) * 32, W == kPagedWarps ? 1 : 2)
             const uint32_t n = n0 + i + j + lane, stage = n % S::kStages, turn = n / S::kStages;
             if (turn) in = mbar_wait_bounded(&empty[stage], (turn - 1) & 1);
             if (in) {
+              issued = n + W;
               first_row[stage] = row;
               uint64_t *bar = &full[stage];
               if (row != ~0u) {
@@ -405,13 +407,23 @@ __global__ void __launch_bounds__((W + 1) * 32, W == kPagedWarps ? 1 : 2)
       if ((index += gridDim.x) >= plan.pieces) break;
       piece = paged_piece(p, plan, index, lead, cursor);
     }
-    if (stopped && lane == 0) atomicOr(&p.t.pool[1], kPagedTimeout);
+    // The block does not end before its copies have landed. A stage is issued again only after all W arrivals of those who saw its
+    // turn land, so at most the last turn of each of this lane's stages is in flight, whatever consumers do.
+    bool landed = true;
+    if (lane < (uint32_t)W) {
+#pragma unroll 1
+      for (uint32_t k = 1; k <= S::kStages / W && landed && issued >= k * W; ++k) {
+        const uint32_t n = issued - k * W;
+        landed = mbar_wait_bounded(&full[n % S::kStages], n / S::kStages & 1);
+      }
+    }
+    if (!__all_sync(~0u, landed && !stopped) && lane == 0) atomicOr(&p.t.pool[1], kPagedTimeout);
     return;
   }
 
   // ================= the consumers =================
   uint32_t n0 = 0;
-  bool stopped = false;      // a wait ran out: nothing is waited for any more
+  bool stopped = false;      // a wait ran out: nothing is waited for or released any more, and the copying warp's next wait runs out
   // this lane's row of an ldmatrix, and which of the two 16-byte chunks it reads
   // (swizzled: chunk c of row r lies at c ^ r % 8; chunks 2i and 2i + 1 of step i are those of step 0, ^ 2i)
   const uint32_t k_row = lane % 8 + (lane / 8 % 2) * 8, k_at = k_row * 128 + ((lane / 16 ^ k_row % 8) << 4);
@@ -569,7 +581,7 @@ __global__ void __launch_bounds__((W + 1) * 32, W == kPagedWarps ? 1 : 2)
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive_count(&empty[stage], teams);   // the team's T warps make up W arrivals
+      if (lane == 0 && !stopped) mbar_arrive_count(&empty[stage], teams);   // the team's T warps make up W arrivals
       stage += teams;
       if (stage >= S::kStages) stage -= S::kStages, parity ^= 1;
     }
@@ -764,11 +776,7 @@ __global__ void __launch_bounds__((W + 1) * 32, W == kPagedWarps ? 1 : 2)
     piece = paged_piece(p, plan, index, lead, cursor);
     named_bar(1, (uint32_t)W * 32);   // shared results are free for the next piece
   }
-  if (stopped) {   // copies in flight land before the block ends; the first that does not in time was never issued
-    for (uint32_t i = n0 - min(n0, S::kStages); i < n0; ++i)
-      if (!mbar_wait_bounded(&full[i % S::kStages], i / S::kStages & 1)) break;
-    if (lane == 0) atomicOr(&p.t.pool[1], kPagedTimeout);
-  }
+  if (stopped && lane == 0) atomicOr(&p.t.pool[1], kPagedTimeout);
 }
 
 }  // namespace vg
