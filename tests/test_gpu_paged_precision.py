@@ -82,3 +82,68 @@ def test_sums_of_long_pieces_have_no_bias(dtype, kind):
     size = p @ u / p.sum(1, keepdim=True)
     worst = (out.abs() / size).max()
     assert worst <= 2.0 ** -14.5, float(worst.log2())
+
+
+def small_cache(kind, rows, heads=1, dim=64, seed=3, hook=None):
+    """A cache of sequences of rows[s] normal rows, after ``hook(k, v, start)`` has changed them; K and V as they are held, in 64
+    bits (an infinity as the largest number)."""
+    t = TYPES[kind]
+    table = shuffled(len(rows), sum(-(-r // 16) for r in rows), 16, -(-max(rows) // 16))
+    cache = paged.PagedCache(table, heads, dim, dtype=t)
+    g = torch.Generator().manual_seed(seed)
+    k, v = (torch.randn(sum(rows), heads, dim, generator=g) for _ in "kv")
+    starts = [sum(rows[:s]) for s in range(len(rows))]
+    hook(k, v, starts)
+    cache.append(table.step(ints(list(rows)), sum(rows)), k.cuda(), v.cuda())
+    top = torch.finfo(t).max
+    held = [x.clamp(-top, top).to(t).double() for x in (k, v)]
+    return cache, [[x[a:a + n, 0] for x in held] for a, n in zip(starts, rows)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_values_at_the_largest_number(kind, dtype):
+    """Infinities in V, held as the largest number: a mean with some of them in it is finite. Bound: test_gpu_paged.py's for scores
+    (S 2^-17) and sums (2^-15) on sum(p |v|) of the output itself, and half a step of it."""
+    def hook(k, v, starts):
+        for s, places in enumerate(((3, 17, 18, 39), (20, 2000, 2001, 4500))):
+            for r in places:
+                v[starts[s] + r, 0, 5] = float("inf")
+                v[starts[s] + r, 0, 6] = -float("inf")
+    cache, held = small_cache(kind, (40, 5000), hook=hook)
+    q = torch.randn(2, 4, 64, generator=torch.Generator().manual_seed(5)).to(TYPES[dtype])
+    q[:, 0] = 0
+    out = cache.attention(q.cuda()).double().cpu()
+    most = torch.finfo(TYPES[dtype]).max
+    for s, (k, v) in enumerate(held):
+        p = (q[s].double() @ k.T / 8).softmax(1)
+        want, size = p @ v, p @ v.abs()
+        top = float((q[s].double().abs() @ k.T.abs()).max()) / 8
+        near = want.abs() < most
+        assert (out[s][want > most * 1.01] == float("inf")).all() and (out[s][want < -most * 1.01] == -float("inf")).all()
+        good = (out[s] - want).abs() <= half_step(want, dtype) + (top * 2.0 ** -17 + 2.0 ** -15) * size
+        assert (good | ~near).all()
+        assert near.all() or (kind, dtype) == ("bf16", "f16")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_keys_at_the_largest_number(dtype):
+    """Infinities in K of a bf16 cache, held as the largest number: rows with it take all of the weight, or none. Ties (the rest of
+    a score is far below the largest number's last bit) are means of V: bound 2^-20 of it, and half a step."""
+    def hook(k, v, starts):
+        for s, places in enumerate(((3, 17, 30), (20, 2000, 4500))):
+            for r, x in zip(places, (float("inf"), float("inf"), -float("inf"))):
+                k[starts[s] + r, 0, 5] = x
+    cache, held = small_cache("bf16", (40, 5000), hook=hook)
+    q = torch.randn(2, 4, 64, generator=torch.Generator().manual_seed(5)).to(TYPES[dtype])
+    q[:, 0, 5], q[:, 1, 5], q[:, 2, 5], q[:, 3, 5] = 1.5, -1.5, 0.0, 100.0
+    out = cache.attention(q.cuda()).double().cpu()
+    for s, (k, v) in enumerate(held):
+        e = q[s].double() @ k.T / 8
+        p = (e - e.amax(1, keepdim=True)).exp()
+        want = p @ v / p.sum(1, keepdim=True)
+        # where its channel counts for nothing, such a row is like any other
+        slack = torch.full((4, 64), 2.0 ** -20 * float(v.abs().max()), dtype=torch.float64)
+        top = float((q[s, 2].double().abs() @ k.abs().T).max()) / 8
+        slack[2] = (top * 2.0 ** -17 + 2.0 ** -15) * (p[2] @ v.abs()) / p[2].sum()
+        assert ((out[s] - want).abs() <= half_step(want, dtype) + slack).all()

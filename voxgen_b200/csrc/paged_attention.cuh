@@ -301,9 +301,19 @@ constexpr int kPTerms = std::is_same<C, __half>::value ? 2 : 3;
 // are not taken.
 constexpr uint32_t kPagedProducts = 512;
 
-// P is held times 2^6 in fp16, for the range below a weight of 1 (kv4_rows_attention.cuh); bf16 has range enough.
+// P is held times 2^6 in fp16, for the range below a weight of 1 (kv4_rows_attention.cuh), and times 2^-32 in bf16: there V goes
+// up to fp32's largest number (an infinity is held as that), and sums of P V must not.
 template <typename C>
-constexpr float kPagedPScale = std::is_same<C, __half>::value ? kPScale : 0.f;
+constexpr float kPagedPScale = std::is_same<C, __half>::value ? kPScale : -32.f;
+// A power of two for a head's query whose largest magnitude is `top`. fp16's range is met by one that brings it to [2^14, 2^15).
+// bf16 has fp32's range, and so do K's infinities, held as the largest number: no more than 2^-8, and no sum of 128
+// products passes that number.
+__device__ __forceinline__ float query_power(float top, float &inverse, __half) { return row_power(top, inverse); }
+__device__ __forceinline__ float query_power(float top, float &inverse, __nv_bfloat16) {
+  const int e = (int)(__float_as_uint(top) >> 23 & 255) - 127, k = min(max(-9 - e, -114), 0);
+  inverse = __uint_as_float((uint32_t)(127 - k) << 23);
+  return __uint_as_float((uint32_t)(127 + k) << 23);
+}
 
 template <int D, typename T, typename C, int W, bool kFresh>   // kFresh: O is summed afresh
 __global__ void __launch_bounds__((W + 1) * 32, W == kPagedWarps ? 1 : 2)
@@ -454,9 +464,8 @@ __global__ void __launch_bounds__((W + 1) * 32, W == kPagedWarps ? 1 : 2)
         x[i] = head < p.group ? (float)q[i] : 0.f;
         top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
       }
-      // fp16's range is met by a power of two a head; bf16 has fp32's
-      float inverse = 1.f, power = 1.f;
-      if constexpr (std::is_same<C, __half>::value) power = row_power(__uint_as_float(__reduce_max_sync(~0u, top)), inverse);
+      float inverse;
+      const float power = query_power(__uint_as_float(__reduce_max_sync(~0u, top)), inverse, C{});
 #pragma unroll
       for (uint32_t i = 0; i < N; i += 2) {   // channels c, c + 1: step c / 16, lane 4 col + c % 8 / 2, register c % 16 / 8
         const uint32_t c = lane * N + i;
@@ -599,7 +608,9 @@ __global__ void __launch_bounds__((W + 1) * 32, W == kPagedWarps ? 1 : 2)
       l0 += __shfl_xor_sync(~0u, l0, x);
       l1 += __shfl_xor_sync(~0u, l1, x);
     }
-    m0 = l0 == 0.f ? kNoScore : m0 * f0, m1 = l1 == 0.f ? kNoScore : m1 * f1;   // scaled from here on
+    // maxima meet unscaled, as within a warp: a scaled one may pass fp32's range, and rounds by more than differences are
+    if (l0 == 0.f) m0 = kNoScore;
+    if (l1 == 0.f) m1 = kNoScore;
     // a denominator of 0 where rows were seen (every score -infinity) is marked by a -1
     if (steps && l0 == 0.f) l0 = -1.f;
     if (steps && l1 == 0.f) l1 = -1.f;
@@ -612,6 +623,7 @@ __global__ void __launch_bounds__((W + 1) * 32, W == kPagedWarps ? 1 : 2)
     float e0, e1;
     {
       const uint32_t h = lane / 4, s = lane % 4;
+      const float f = factors[tile][h];
       float m[W / 4], l[W / 4], top = kNoScore, all = 0.f;
 #pragma unroll
       for (uint32_t i = 0; i < W / 4; ++i) {
@@ -626,7 +638,7 @@ __global__ void __launch_bounds__((W + 1) * 32, W == kPagedWarps ? 1 : 2)
 #pragma unroll
       for (uint32_t i = 0; i < W / 4; ++i) {
         some |= l[i] < 0.f;
-        all += (l[i] < 0.f ? 0.f : l[i]) * exp2_fast(m[i] - top);
+        all += (l[i] < 0.f ? 0.f : l[i]) * exp2_fast((m[i] - top) * f);
       }
       all += __shfl_xor_sync(~0u, all, 1);
       all += __shfl_xor_sync(~0u, all, 2);
@@ -635,7 +647,7 @@ __global__ void __launch_bounds__((W + 1) * 32, W == kPagedWarps ? 1 : 2)
         f_max[tile][h] = top;
         f_sum[tile][h] = all == 0.f && some ? -1.f : all;
       }
-      e0 = exp2_fast(m0 - __shfl_sync(~0u, top, 8 * t)), e1 = exp2_fast(m1 - __shfl_sync(~0u, top, 8 * t + 4));
+      e0 = exp2_fast((m0 - __shfl_sync(~0u, top, 8 * t)) * f0), e1 = exp2_fast((m1 - __shfl_sync(~0u, top, 8 * t + 4)) * f1);
     }
     float *part = p.parts + (size_t)(seg.slot + seg.part) * p.tiles * kPart<D>;
     const auto out_of = [&](uint32_t k, uint32_t head) {   // of a tile's head
@@ -713,6 +725,7 @@ __global__ void __launch_bounds__((W + 1) * 32, W == kPagedWarps ? 1 : 2)
             return v;
           };
           // lanes are pieces, 32 at a time
+          const float f = factors[k][head];
           const float *stats = from + kPagedHeads * D + head;
           float m = lane < pieces ? __ldcg(stats + lane * stride) : kNoScore;
           float sum = lane < pieces ? __ldcg(stats + lane * stride + kPagedHeads) : 0.f;
@@ -734,7 +747,7 @@ __global__ void __launch_bounds__((W + 1) * 32, W == kPagedWarps ? 1 : 2)
               m = i < pieces ? __ldcg(stats + i * stride) : kNoScore;
               sum = i < pieces ? __ldcg(stats + i * stride + kPagedHeads) : 0.f;
             }
-            const float w = exp2_fast(m - top);
+            const float w = exp2_fast((m - top) * f);
             some |= sum < 0.f;
             all += w * (sum < 0.f ? 0.f : sum);
             uint32_t i = 0;
