@@ -73,7 +73,7 @@ class Step:
         self.table, self.tokens = table, tokens
         total, offsets, self._views = table._layout(tokens)[:3]
         self._buffer = torch.empty(total, dtype=torch.int32, device=table.device)
-        self._parts = [None] * 5
+        self._parts, self._age = [None] * 5, None
         at = self._buffer.data_ptr()
         self.desc = api.PagedStepDesc(*[at + 4 * o for o in offsets], tokens)
         self._ref = C.byref(self.desc)
@@ -81,9 +81,10 @@ class Step:
     @classmethod
     def of(cls, table: "PageTable", starts: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor,
            sequences: torch.Tensor, runs: torch.Tensor) -> "Step":
-        """A step from arrays in hand, such as copies of an earlier one's (each starts on 16 bytes)."""
+        """A step from arrays in hand, such as copies of an earlier one's (each starts on 16 bytes). That they are those of the
+        table's last step is up to the caller."""
         step = cls.__new__(cls)
-        step.table, step.tokens = table, slots.numel()
+        step.table, step.tokens, step._age = table, slots.numel(), None
         tokens = step.tokens
         shapes = (table.seqs + 1,), (tokens,), (tokens,), (tokens,), (table._layout(tokens)[3], 4)
         step._parts = [_expect(x, torch.int32, shape, table.device, what) for x, shape, what in
@@ -139,6 +140,7 @@ class PageTable:
                                        seqs, seq_pages, pages, page_rows)
         self._ref = C.byref(self.desc)
         self._layouts = {}
+        self._age = 0            # steps taken by calls (and resets); those of a graph's replays are not known here
         self._lib = api.lib()
 
     def _layout(self, tokens: int):
@@ -174,10 +176,16 @@ class PageTable:
                                        _ints(keep, (self.seqs,), self.device, "keep"), into._ref, _current_stream(self._index))
         if rc:
             raise VoxGenError(rc, f"a step of {tokens} tokens")
+        if _capturing():
+            into._age = None
+        else:
+            into._age = self._age = self._age + 1
         return into
 
     def reset(self) -> None:
         """Empties every sequence: all pages are free again."""
+        if not _capturing():
+            self._age += 1
         self.table.fill_(-1)
         self.rows.zero_()
         self.status.zero_()
@@ -261,13 +269,15 @@ class PagedCache:
 
     @_on_its_device
     def append(self, step: Step, k: torch.Tensor, v: torch.Tensor, *, layer: int = 0) -> None:
-        """Stores the K and V rows [tokens, kv_heads, head_dim] of the table's last step; rows of tokens without a slot
-        are passed over. Values are rounded to the cache's type; those past its largest finite number are held as that
+        """Stores the K and V rows [tokens, kv_heads, head_dim] of the table's last step (an older one is refused: its pages
+        may be another sequence's by now); rows of tokens without a slot are passed over. Values are rounded to the cache's type; those past its largest finite number are held as that
         one, and ``table.pool[1]`` then has STATUS_NONFINITE, as for NaN."""
         ref = self._layer(layer)
         dtype = self._rows_of(k, self.kv_heads, "k")
         if step.table is not self.table:
             raise _invalid("the step is another table's")
+        if step._age is not None and step._age != self.table._age:
+            raise _invalid("the step is not the table's last one")
         if v.shape != k.shape or v.dtype is not k.dtype or v.device != self.device or k.shape[0] != step.tokens:
             raise _invalid(f"k and v must agree in shape, type and device, and have the step's {step.tokens} rows")
         rc = self._lib.vg_k_paged_append(ref, step._ref, k.data_ptr(), v.data_ptr(), dtype, self._strides(k),
