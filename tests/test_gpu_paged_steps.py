@@ -59,3 +59,22 @@ def test_arrays_in_hand_and_captured_steps_are_not_asked_for_their_age():
     graph.replay()
     cache.append(captured, k, k)                                    # outside of the graph, after its replay
     assert table.rows.tolist() == [5, 5] and captured.positions.tolist()[:2] == [4, 4]
+
+
+def test_a_reserved_workspace_is_not_outgrown_by_a_smaller_batch():
+    """Of 20,000 queries nothing is cut and nothing needs room; of 600 something does."""
+    table = shuffled(2, 40, 16, 20)
+    cache = paged.PagedCache(table, 1, 64)
+    k = normal(1, 300, 1, 64)
+    cache.append(table.step(ints([300, 0]), 300), k, k)
+    cache.reserve(20000, 8)
+    ready = cache._workspace
+    q = normal(2, 600, 8, 64)
+    sequences = ints([0, 1] * 300)
+    want = cache.attention(q, sequences=sequences)
+    assert cache._workspace is ready
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = cache.attention(q, sequences=sequences)
+    graph.replay()
+    assert cache._workspace is ready and torch.equal(out, want)

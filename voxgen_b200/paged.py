@@ -344,14 +344,16 @@ class PagedCache:
 
     @_on_its_device
     def reserve(self, queries: int, heads: int, budget: int = 0) -> None:
-        """Makes the workspace large enough for :meth:`attention` of ``queries`` queries (with a list of ``budget`` pages,
-        if not 0), before a CUDA graph of such calls is captured: without it each of the graph's replays zero-fills a
-        workspace of its own."""
+        """Makes the workspace large enough for :meth:`attention` of up to ``queries`` queries of ``heads`` heads (with lists of
+        up to ``budget`` pages, if not 0), before a CUDA graph of such calls is captured: without it each of the graph's
+        replays zero-fills a workspace of its own."""
         if _capturing():
             raise _invalid("reserve: the workspace does not grow while a graph is being captured")
         if not (0 < heads < 1 << 32 and 0 < queries < 1 << 32 and 0 <= budget < 1 << 32):
             raise _invalid(f"reserve: {queries} queries, {heads} heads, {budget} pages")
-        self._work(queries, heads, budget)
+        while queries:     # fewer queries may need more: very many are not cut into pieces, which the workspace is for
+            self._work(queries, heads, budget)
+            queries //= 2
 
     @_on_its_device
     def attention(self, q: torch.Tensor, *, sequences: Optional[torch.Tensor] = None,
