@@ -78,3 +78,18 @@ def test_a_reserved_workspace_is_not_outgrown_by_a_smaller_batch():
         out = cache.attention(q, sequences=sequences)
     graph.replay()
     assert cache._workspace is ready and torch.equal(out, want)
+
+
+def test_arrays_in_hand_of_no_tokens():
+    table = shuffled(2, 10, 16, 5)
+    cache = paged.PagedCache(table, 1, 64)
+    table.step(ints([30, 20]), 50)
+    step = table.step(ints([0, 0]), 0)
+    copy = paged.Step.of(table, *(x.clone() for x in (step.starts, step.slots, step.positions, step.sequences, step.runs)))
+    none = normal(1, 0, 1, 64)
+    before = cache.data.clone()
+    cache.append(copy, none, none)
+    assert same_bits(cache.data, before)
+    assert table.step(ints([0, 0]), 0, keep=ints([17, 0]), into=copy) is copy
+    cache.append(copy, none, none)
+    assert table.rows.tolist() == [17, 0] and copy.starts.tolist() == [0, 0, 0]

@@ -89,7 +89,8 @@ class Step:
         shapes = (table.seqs + 1,), (tokens,), (tokens,), (tokens,), (table._layout(tokens)[3], 4)
         step._parts = [_expect(x, torch.int32, shape, table.device, what) for x, shape, what in
                        zip((starts, slots, positions, sequences, runs), shapes, cls._NAMES)]
-        step.desc = api.PagedStepDesc(*[x.data_ptr() for x in step._parts], tokens)
+        # an array of no tokens has no address; the entry points want one that is not null, and do not read it
+        step.desc = api.PagedStepDesc(*[x.data_ptr() or 64 for x in step._parts], tokens)
         step._ref = C.byref(step.desc)
         return step
 
