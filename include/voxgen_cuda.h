@@ -541,7 +541,8 @@ typedef struct vg_paged_step {
  * (VG_DTYPE_F16 or VG_DTYPE_BF16), head_dim 64 or 128, 16-byte aligned. summaries: NULL,
  * or [pages][kv_heads][2][head_dim] of the same type, 32-byte aligned: per channel the smallest and the
  * largest K of the rows that a page held at its last append, NaN passed over (0 and 0
- * for a channel of NaN alone). */
+ * for a channel of NaN alone). A step that cuts a page's rows and adds none to it leaves
+ * its summary: a bound for the rows that are left, until the page's next append. */
 typedef struct vg_paged_cache {
   const vg_paged_table *table;
   void *data;

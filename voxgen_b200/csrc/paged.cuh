@@ -5,8 +5,10 @@
 // rows, a power of two, so a block of 16 rows never leaves its page.
 //
 // Summaries. [pages][kv_heads][smallest, largest][head_dim] of the cache's type:
-// per channel the extremes of K over the rows held. NaN is passed over (a channel of
-// NaN alone has 0 and 0), so a summary is always finite.
+// per channel the extremes of K over the rows that the page held at its last append.
+// NaN is passed over (a channel of NaN alone has 0 and 0), and append stores no
+// infinity, so a summary of its rows is finite. A step that cuts rows of a page and adds
+// none there leaves the summary: a bound for the rows left, until the next append.
 //
 // Table. table[seqs][seq_pages] names the pages of a sequence in order, rows[seqs]
 // says how many rows it holds, free[pages] is a stack of free pages whose height

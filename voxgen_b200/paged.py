@@ -200,7 +200,9 @@ class PagedCache:
 
     ``data`` [layers, pages, kv_heads, 2 (K, V), page_rows, head_dim] may be given instead of allocated, with one layer
     without the first dimension; so may ``summaries`` [layers, pages, kv_heads, 2, head_dim] of the same type: per channel
-    the smallest and the largest K of a page's rows, which :meth:`select` needs (True allocates them)."""
+    the smallest and the largest K of the rows that a page held at its last append, which :meth:`select` needs (True
+    allocates them). A step that cuts a page's rows and adds none to it leaves its summary as it was: still a bound for the
+    rows that are left, though perhaps a loose one, until the page's next append."""
 
     def __init__(self, table: PageTable, kv_heads: int, head_dim: int, *, dtype: torch.dtype = torch.float16,
                  layers: int = 1, data: Optional[torch.Tensor] = None,
@@ -271,8 +273,9 @@ class PagedCache:
     @_on_its_device
     def append(self, step: Step, k: torch.Tensor, v: torch.Tensor, *, layer: int = 0) -> None:
         """Stores the K and V rows [tokens, kv_heads, head_dim] of the table's last step (an older one is refused: its pages
-        may be another sequence's by now); rows of tokens without a slot are passed over. Values are rounded to the cache's type; those past its largest finite number are held as that
-        one, and ``table.pool[1]`` then has STATUS_NONFINITE, as for NaN."""
+        may be another sequence's by now); rows of tokens without a slot are passed over. Values are rounded to the cache's
+        type; those past its largest finite number are held as that one, and ``table.pool[1]`` then has STATUS_NONFINITE, as
+        for NaN."""
         ref = self._layer(layer)
         dtype = self._rows_of(k, self.kv_heads, "k")
         if step.table is not self.table:
