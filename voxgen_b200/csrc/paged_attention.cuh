@@ -21,7 +21,8 @@
 // Tiles never mix queries, so a row that one query sees and another does not is masked
 // warp by warp, whatever it holds. A warp's step of 16 rows is one chain of dependent
 // instructions (copies awaited, products, maximum, exponentials, transposes, products),
-// so as many warps run as registers allow: 12, with q's terms read from shared memory.
+// so as many warps run as registers allow: 12 at 128 each (at head_dim 128 most kernels
+// spill 20 bytes, fp32 queries over bf16 96), with q's terms read from shared memory.
 //
 // The split. Segments are cut into pieces of at most U blocks, U such that there is
 // about one piece for each CTA (up to 4, where segments are many). The warps of a piece
@@ -29,7 +30,7 @@
 // the CTA that finishes last (a counter, left at zero) adds them in order: sums never
 // depend on timing.
 //
-// Measured: 16 contexts of 24001 to 32768 rows, bf16, 465 MB: 78 us, 6.0 TB/s (91% of
+// Measured: 16 contexts of 24001 to 32768 rows, bf16, 465 MB: 77 us, 6.0 TB/s (93% of
 // the measured copy rate). 16 ragged streams of 64 to 4096 rows, 34 MB: 13.7 us, of
 // which 4 stream: the rest is code that runs once, at about 7 cycles an instruction, and
 // so kept short (loops, not unrolled ones). 5 drafted tokens of those streams: 30 us.
