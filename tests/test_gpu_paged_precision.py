@@ -147,3 +147,21 @@ def test_keys_at_the_largest_number(dtype):
         top = float((q[s, 2].double().abs() @ k.abs().T).max()) / 8
         slack[2] = (top * 2.0 ** -17 + 2.0 ** -15) * (p[2] @ v.abs()) / p[2].sum()
         assert ((out[s] - want).abs() <= half_step(want, dtype) + slack).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("power", [-100, -110])
+def test_values_near_the_smallest_number(power, dtype):
+    """Weights are held scaled, so products of a bf16 cache's smallest values are subnormal: each of the up to three products of a
+    block, and each of 48 joined warps and pieces, is off by 2^-149 at most, which the weights' sum (2^-20 at least) makes 2^-129 in
+    the output: 2^-120 for the 160 of them here. To it test_gpu_paged.py's bound for scores and sums."""
+    def hook(k, v, starts):
+        v.copy_((1 + v.abs()) * 2.0 ** power)
+    cache, held = small_cache("bf16", (40, 100), hook=hook)
+    q = torch.randn(2, 4, 64, generator=torch.Generator().manual_seed(5)).to(TYPES[dtype])
+    out = cache.attention(q.cuda()).double().cpu()
+    for s, (k, v) in enumerate(held):
+        want = (q[s].double() @ k.T / 8).softmax(1) @ v
+        top = float((q[s].double().abs() @ k.T.abs()).max()) / 8
+        bound = half_step(want, dtype) + (top * 2.0 ** -17 + 2.0 ** -15) * want + 2.0 ** -120
+        assert ((out[s] - want).abs() <= bound).all()

@@ -22,7 +22,7 @@
 // warp by warp, whatever it holds. A warp's step of 16 rows is one chain of dependent
 // instructions (copies awaited, products, maximum, exponentials, transposes, products),
 // so as many warps run as registers allow: 12 at 128 each (at head_dim 128 most kernels
-// spill 20 bytes, fp32 queries over bf16 96), with q's terms read from shared memory.
+// spill 8 to 44 bytes, fp32 queries over bf16 96), with q's terms read from shared memory.
 //
 // The split. Segments are cut into pieces of at most U blocks, U such that there is
 // about one piece for each CTA (up to 4, where segments are many). The warps of a piece
@@ -302,10 +302,11 @@ constexpr int kPTerms = std::is_same<C, __half>::value ? 2 : 3;
 // are not taken.
 constexpr uint32_t kPagedProducts = 512;
 
-// P is held times 2^6 in fp16, for the range below a weight of 1 (kv4_rows_attention.cuh), and times 2^-32 in bf16: there V goes
-// up to fp32's largest number (an infinity is held as that), and sums of P V must not.
+// P is held times 2^6 in fp16, for the range below a weight of 1 (kv4_rows_attention.cuh), and times 2^-20 in bf16: there V goes
+// up to fp32's largest number (an infinity is held as that), and sums of P V over a million rows must not pass it. At the other
+// end outputs below 2^-104 lose bits, as products become subnormal (2^-32 would cost those below 2^-92).
 template <typename C>
-constexpr float kPagedPScale = std::is_same<C, __half>::value ? kPScale : -32.f;
+constexpr float kPagedPScale = std::is_same<C, __half>::value ? kPScale : -20.f;
 // A power of two for a head's query whose largest magnitude is `top`. fp16's range is met by one that brings it to [2^14, 2^15).
 // bf16 has fp32's range, and so do K's infinities, held as the largest number: no more than 2^-8, and no sum of 128
 // products passes that number.
